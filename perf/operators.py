@@ -188,7 +188,7 @@ def prepare(case, seed):
     elif k == "embed":
         s.update(out=_new(c["n"], c["dim"]), dw=_new(c["vocab"], c["dim"]))
     else:
-        s.update(loss=_new(1), stats=_new(c["n"] + 1), dz=_new(c["n"], c["vocab"]))
+        s.update(loss=_new(1), stats=_new(2 * c["n"] + 1), dz=_new(c["n"], c["vocab"]))
     return s
 
 
