@@ -48,6 +48,7 @@ LIB_NAME = "libaar_hip.so"
 # in AGPRs.
 HIP_FILE_FLAGS = {
     "flash_attn": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "cross_attn": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "gemm_small": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

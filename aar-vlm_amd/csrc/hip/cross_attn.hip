@@ -1,0 +1,805 @@
+// Cross attention: queries against an encoder's keys and values of another
+// length, forward and backward, in fp32.
+//
+// For every batch b and query head h, with the keys j < len[b] and the shared
+// key/value head hk = h / G, G = H / Hkv:
+//   s_ij = scale q_i . k_j,  m_i = max_j s_ij,  l_i = sum_j exp(s_ij - m_i),
+//   O_i = sum_j exp(s_ij - m_i) v_j / l_i,      lse_i = m_i + ln l_i
+// and a row without keys has O = 0, lse = -inf.  Backward, with P = exp(s - lse),
+// D_i = dO_i . O_i and dS = P (dO V^T - D):
+//   dQ = scale dS K,  dV = P^T dO,  dK = scale dS^T Q, both summed over the G
+//   heads that share the key.
+//
+// The query heads of a shared key/value head are one list of G * Tq query rows, so
+// a workgroup's K and V tiles serve whatever heads its rows belong to, and the
+// sums over the group happen in the accumulators that dK and dV have anyway.
+// Rows of K and V from len[b] on are never read; their gradients are zero.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <initializer_list>
+
+#include "bf16x3.hpp"
+#include "common.hpp"
+#include "flash_offsets.hpp"
+#include "flash_tile.hpp"
+
+namespace aar {
+namespace {
+
+struct CaArgs {
+  FaIn q, k, v, o_in, dout;
+  FaOut o, dq, dk, dv;
+  const int64_t* lens;
+  float* lse;     // [B * Hkv][R]
+  float* D;       // [B * Hkv][R], backward
+  float* part_o;  // [B * Hkv][splits][R][DP] normalised partial O
+  float* part_l;  // [B * Hkv][splits][R] m + log2(l) of it
+  int Tq, Tk, d, G, Hkv, R, BH;  // R = G * Tq rows of each of the BH = B * Hkv key/value heads
+  int splits, chunk;             // key ranges, and their keys
+  float scale, scale_log2;
+};
+
+// Keys of batch b.
+__device__ __forceinline__ int ca_len(const CaArgs& a, int bh) {
+  if (!a.lens) return a.Tk;
+  const int64_t n = a.lens[bh / a.Hkv];
+  return n < 0 ? 0 : (n > a.Tk ? a.Tk : (int)n);
+}
+
+// Element offset of query row r of key/value head bh in a query-shaped operand.
+template <typename T>
+__device__ __forceinline__ int64_t ca_row(const T& x, const CaArgs& a, int bh, int r) {
+  const int g = a.G == 1 ? 0 : r / a.Tq;
+  const int t = a.G == 1 ? r : r - g * a.Tq;
+  return (int64_t)(bh / a.Hkv) * x.sb + ((int64_t)(bh % a.Hkv) * a.G + g) * x.sh + (int64_t)t * x.st;
+}
+
+template <typename T>
+__device__ __forceinline__ auto ca_head(const T& x, const CaArgs& a, int bh) {
+  return x.p + (int64_t)(bh / a.Hkv) * x.sb + (int64_t)(bh % a.Hkv) * x.sh;
+}
+
+// -------------------------------------------------------------- few query rows
+
+// Up to RQ query rows a key/value head (single tokens): bound by the bytes of K
+// and V.  LPK lanes hold a key's row, four floats each, and walk the keys with
+// their own online softmax, U keys' loads in flight; the groups' and waves'
+// states meet once at the end.  The key range is split over enough workgroups to
+// fill the GPU, joined by cross_combine_kernel.
+template <int RQ, int LPK, bool VEC>
+__global__ void __launch_bounds__(256)
+cross_rows_kernel(const CaArgs a) {
+  constexpr int U = RQ >= 8 ? 2 : 4;
+  constexpr int kGroups = kWave / LPK;
+  constexpr int kWaves = 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int sub = lane / LPK, c = 4 * (lane % LPK);
+  const int bh = blockIdx.x % a.BH, part = blockIdx.x / a.BH;
+  const int len = ca_len(a, bh);
+  const int k0 = part * a.chunk, k1 = min(len, k0 + a.chunk);
+  const float* __restrict__ K = ca_head(a.k, a, bh);
+  const float* __restrict__ V = ca_head(a.v, a, bh);
+
+  f32x4 q[RQ], acc[RQ];
+  float m[RQ], l[RQ];
+#pragma unroll
+  for (int r = 0; r < RQ; ++r) {
+    q[r] = acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (r < a.R && c < a.d) q[r] = load4<VEC>(a.q.p + ca_row(a.q, a, bh, r) + c, a.d - c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[r][e] *= a.scale_log2;
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+  }
+  for (int b = k0 + wave * U * kGroups; b < k1; b += kWaves * U * kGroups) {
+    f32x4 kf[U], vf[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = b + u * kGroups + sub;
+      kf[u] = vf[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (key < k1 && c < a.d) {
+        kf[u] = load4<VEC>(K + (int64_t)key * a.k.st + c, a.d - c);
+        vf[u] = load4<VEC>(V + (int64_t)key * a.v.st + c, a.d - c);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RQ; ++r) {
+      float s[U], mn = m[r];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float x = kf[u][0] * q[r][0] + kf[u][1] * q[r][1] + kf[u][2] * q[r][2] + kf[u][3] * q[r][3];
+        x += dpp_quad_xor1(x);
+        x += dpp_quad_xor2(x);
+        x += dpp_half_mirror(x);
+        if (LPK >= 16) x += dpp_row_mirror(x);
+        if (LPK >= 32) x += swizzle_xor16(x);
+        s[u] = b + u * kGroups + sub < k1 ? x : -INFINITY;
+        mn = fmaxf(mn, s[u]);
+      }
+      const float mu = mn == -INFINITY ? 0.f : mn;
+      const float alpha = fast_exp2(m[r] - mu);
+      l[r] *= alpha;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[r][e] *= alpha;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float p = fast_exp2(s[u] - mu);
+        l[r] += p;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[r][e] += p * vf[u][e];
+      }
+      m[r] = mn;
+    }
+  }
+
+  // The wave's groups, then the waves.
+  __shared__ f32x4 sacc[kWaves][RQ][LPK];
+  __shared__ float sm[kWaves][RQ], sl[kWaves][RQ];
+#pragma unroll
+  for (int r = 0; r < RQ; ++r) {
+    float mw = m[r];
+#pragma unroll
+    for (int o = LPK; o < kWave; o *= 2) mw = fmaxf(mw, __shfl_xor(mw, o, kWave));
+    const float f = fast_exp2(m[r] - (mw == -INFINITY ? 0.f : mw));
+    float lw = l[r] * f;
+    f32x4 aw;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) aw[e] = acc[r][e] * f;
+#pragma unroll
+    for (int o = LPK; o < kWave; o *= 2) {
+      lw += __shfl_xor(lw, o, kWave);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) aw[e] += __shfl_xor(aw[e], o, kWave);
+    }
+    if (sub == 0) sacc[wave][r][lane] = aw;
+    if (lane == 0) {
+      sm[wave][r] = mw;
+      sl[wave][r] = lw;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < RQ * LPK; i += 256) {
+    const int r = i / LPK, cc = 4 * (i % LPK);
+    if (r >= a.R) continue;
+    float mx = sm[0][r];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) mx = fmaxf(mx, sm[w][r]);
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    float ls = 0.f;
+    f32x4 os = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = fast_exp2(sm[w][r] - mu);
+      ls += sl[w][r] * f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) os[e] += sacc[w][r][i % LPK][e] * f;
+    }
+    const float inv = ls == 0.f ? 0.f : 1.0f / ls;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) os[e] *= inv;
+    if (a.splits > 1) {
+      const int64_t row = ((int64_t)bh * a.splits + part) * a.R + r;
+      *reinterpret_cast<f32x4*>(a.part_o + row * (4 * LPK) + cc) = os;
+      if (cc == 0) a.part_l[row] = mx + log2f(ls);
+    } else {
+      if (cc < a.d) store4<VEC>(a.o.p + ca_row(a.o, a, bh, r) + cc, os, a.d - cc);
+      if (cc == 0) a.lse[(int64_t)bh * a.R + r] = (mx + log2f(ls)) * kLn2;
+    }
+  }
+}
+
+// The parts of every query row: with L_p = m_p + log2(l_p) and M their largest,
+//   O = sum_p 2^(L_p - M) O_p / W,  lse = (M + log2 W) ln 2,  W = sum_p 2^(L_p - M);
+// a row without keys has M = -inf.  DP / 4 lanes a row.
+template <int DP, bool VEC>
+__global__ void __launch_bounds__(256)
+cross_combine_kernel(const CaArgs a) {
+  constexpr int kLanes = DP / 4;
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = u / kLanes;
+  if (row >= (int64_t)a.BH * a.R) return;
+  const int c = (int)(u % kLanes) * 4;
+  const int bh = (int)(row / a.R), r = (int)(row % a.R);
+  const float* L = a.part_l + (int64_t)bh * a.splits * a.R + r;
+  const float* O = a.part_o + ((int64_t)bh * a.splits * a.R + r) * DP + c;
+  float mx = -INFINITY;
+  for (int p = 0; p < a.splits; ++p) mx = fmaxf(mx, L[(int64_t)p * a.R]);
+  const float mu = mx == -INFINITY ? 0.f : mx;
+  float w = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = 0; p < a.splits; ++p) {
+    const float f = fast_exp2(L[(int64_t)p * a.R] - mu);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(O + (int64_t)p * a.R * DP);
+    w += f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += f * x[e];
+  }
+  const float inv = w == 0.f ? 0.f : 1.0f / w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] *= inv;
+  if (c < a.d) store4<VEC>(a.o.p + ca_row(a.o, a, bh, r) + c, o, a.d - c);
+  if (c == 0) a.lse[row] = (mx + log2f(w)) * kLn2;
+}
+
+// ------------------------------------------------------------------- forward
+
+// A workgroup takes 128 query rows (32 a wave, a lane its row) and its key range,
+// 32 keys at a time: S^T = K Q^T leaves a lane 16 keys of its row, whose online
+// softmax is in registers but for one exchange with lane ^ 32, and P feeds
+// O^T += V^T P^T from the registers it is left in.  K is staged a tile ahead of V.
+template <int DP, bool VEC>
+__global__ void __launch_bounds__(kFaThreads)
+cross_fwd_kernel(const CaArgs a) {
+  constexpr int NC = DP / 8;
+  constexpr int NB = DP / 32;
+  constexpr int LD = DP + 4;
+  __shared__ __attribute__((aligned(16))) float ks[2][kTile * LD];
+  __shared__ __attribute__((aligned(16))) float vts[2][DP * kLdt];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lr = lane & 31, h = lane >> 5;
+  const int bh = blockIdx.x % a.BH;
+  const int rest = blockIdx.x / a.BH;
+  const int part = rest % a.splits, qb = rest / a.splits;
+  const int len = ca_len(a, bh);
+  const int k0 = part * a.chunk, k1 = min(len, k0 + a.chunk);
+  const float* __restrict__ K = ca_head(a.k, a, bh);
+  const float* __restrict__ V = ca_head(a.v, a, bh);
+  const int qi = qb * kBlock + wave * kTile + lr;  // this lane's row
+
+  f32x4 qr[NC];
+  const float* Q = a.q.p + (qi < a.R ? ca_row(a.q, a, bh, qi) : 0);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int dd = 8 * c + 4 * h;
+    qr[c] = qi < a.R ? load4<VEC>(Q + dd, a.d - dd) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  f32x16 o[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) o[b] = zero16();
+  float m = -INFINITY, l = 0.f;
+  const int ntiles = k1 > k0 ? (k1 - k0 + kTile - 1) / kTile : 0;
+  const bool work = qb * kBlock + wave * kTile < a.R;
+
+  TileCopy<DP, VEC> kc, vc;
+  if (ntiles > 0) {
+    kc.load(K, a.k.st, k0, k1, a.d, tid);
+    vc.load(V, a.v.st, k0, k1, a.d, tid);
+    kc.template store<LD>(ks[0], tid);
+    vc.template store_t<kLdt, true>(vts[0], tid);
+  }
+  __syncthreads();
+  for (int t = 0; t < ntiles; ++t) {
+    const int kv0 = k0 + t * kTile;
+    const bool has_next = t + 1 < ntiles;
+    if (has_next) {
+      kc.load(K, a.k.st, kv0 + kTile, k1, a.d, tid);
+      vc.load(V, a.v.st, kv0 + kTile, k1, a.d, tid);
+    }
+    if (work) {
+      const float* kt = ks[t & 1];
+      const float* vt = vts[t & 1];
+      f32x16 s = zero16();
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const f32x4 kf = *reinterpret_cast<const f32x4*>(kt + lr * LD + 8 * c + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = mfma32(kf[e], qr[c][e], s);
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = kv0 + acc_row(r, h) < k1 ? s[r] * a.scale_log2 : -INFINITY;
+        mx = fmaxf(mx, s[r]);
+      }
+      mx = half_swap_max(mx);
+      const float mn = fmaxf(m, mx);
+      const float mu = mn == -INFINITY ? 0.f : mn;
+      const float alpha = fast_exp2(m - mu);
+      float ps = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = fast_exp2(s[r] - mu);
+        ps += s[r];
+      }
+      l = l * alpha + half_swap_sum(ps);
+      m = mn;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[b][r] *= alpha;
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int col = b * 32 + lr;
+          const f32x4 vf = *reinterpret_cast<const f32x4*>(vt + col * kLdt + vt_swz<true>(col, 8 * g + 4 * h));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[b] = mfma32(vf[e], s[4 * g + e], o[b]);
+        }
+      }
+    }
+    if (has_next) {
+      kc.template store<LD>(ks[(t + 1) & 1], tid);
+      vc.template store_t<kLdt, true>(vts[(t + 1) & 1], tid);
+    }
+    __syncthreads();
+  }
+  if (qi >= a.R) return;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const float l2 = m + log2f(l);
+  const int64_t prow = ((int64_t)bh * a.splits + part) * a.R + qi;
+  float* orow = a.splits > 1 ? a.part_o + prow * DP : a.o.p + ca_row(a.o, a, bh, qi);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int dd = b * 32 + 8 * g + 4 * h;
+      const f32x4 v = {o[b][4 * g] * inv, o[b][4 * g + 1] * inv, o[b][4 * g + 2] * inv, o[b][4 * g + 3] * inv};
+      if (a.splits > 1) *reinterpret_cast<f32x4*>(orow + dd) = v;
+      else if (dd < a.d) store4<VEC>(orow + dd, v, a.d - dd);
+    }
+  }
+  if (h == 0) {
+    if (a.splits > 1) a.part_l[prow] = l2;
+    else a.lse[(int64_t)bh * a.R + qi] = l2 * kLn2;
+  }
+}
+
+// ------------------------------------------------------------------ backward
+
+// dQ, and D of the rows for the dK/dV pass: a workgroup takes 128 query rows with
+// q and dO in registers and walks the keys: S^T, dP^T (lane = row), dS, dQ^T +=
+// K^T dS^T.
+template <int DP, bool VEC>
+__global__ void __launch_bounds__(kFaThreads)
+cross_bwd_dq_kernel(const CaArgs a) {
+  constexpr int NC = DP / 8;
+  constexpr int NB = DP / 32;
+  constexpr int LD = DP + 4;
+  __shared__ __attribute__((aligned(16))) float ks[2][kTile * LD];
+  __shared__ __attribute__((aligned(16))) float vs[2][kTile * LD];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lr = lane & 31, h = lane >> 5;
+  const int bh = blockIdx.x % a.BH, qb = blockIdx.x / a.BH;
+  const int len = ca_len(a, bh);
+  const float* __restrict__ K = ca_head(a.k, a, bh);
+  const float* __restrict__ V = ca_head(a.v, a, bh);
+  const int qi = qb * kBlock + wave * kTile + lr;
+  const bool row_ok = qi < a.R;
+
+  f32x4 qr[NC], dor[NC];
+  float dsum = 0.f;
+  {
+    const float* Q = a.q.p + (row_ok ? ca_row(a.q, a, bh, qi) : 0);
+    const float* dO = a.dout.p + (row_ok ? ca_row(a.dout, a, bh, qi) : 0);
+    const float* O = a.o_in.p + (row_ok ? ca_row(a.o_in, a, bh, qi) : 0);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int dd = 8 * c + 4 * h;
+      const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+      qr[c] = row_ok ? load4<VEC>(Q + dd, a.d - dd) : z;
+      dor[c] = row_ok ? load4<VEC>(dO + dd, a.d - dd) : z;
+      const f32x4 of = row_ok ? load4<VEC>(O + dd, a.d - dd) : z;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dsum += dor[c][e] * of[e];
+    }
+  }
+  dsum = half_swap_sum(dsum);
+  // A row without keys, or past the end, has P = 0.
+  float l2 = row_ok ? a.lse[(int64_t)bh * a.R + qi] * kLog2e : INFINITY;
+  if (l2 == -INFINITY) l2 = INFINITY;
+  if (row_ok && h == 0) a.D[(int64_t)bh * a.R + qi] = dsum;
+  f32x16 dq[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) dq[b] = zero16();
+  const int ntiles = (len + kTile - 1) / kTile;
+  const bool work = qb * kBlock + wave * kTile < a.R;
+
+  TileCopy<DP, VEC> kc, vc;
+  if (ntiles > 0) {
+    kc.load(K, a.k.st, 0, len, a.d, tid);
+    vc.load(V, a.v.st, 0, len, a.d, tid);
+    kc.template store<LD>(ks[0], tid);
+    vc.template store<LD>(vs[0], tid);
+  }
+  __syncthreads();
+  for (int t = 0; t < ntiles; ++t) {
+    const int kv0 = t * kTile;
+    const bool has_next = t + 1 < ntiles;
+    if (has_next) {
+      kc.load(K, a.k.st, kv0 + kTile, len, a.d, tid);
+      vc.load(V, a.v.st, kv0 + kTile, len, a.d, tid);
+    }
+    if (work) {
+      const float* kt = ks[t & 1];
+      const float* vt = vs[t & 1];
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const f32x4 kf = *reinterpret_cast<const f32x4*>(kt + lr * LD + 8 * c + 4 * h);
+        const f32x4 vf = *reinterpret_cast<const f32x4*>(vt + lr * LD + 8 * c + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s = mfma32(kf[e], qr[c][e], s);
+          dp = mfma32(vf[e], dor[c][e], dp);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const bool in = kv0 + acc_row(r, h) < len;
+        const float p = fast_exp2(s[r] * a.scale_log2 - l2);
+        dp[r] = in ? p * (dp[r] - dsum) : 0.f;
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int st = 0; st < 16; ++st) dq[b] = mfma32(kt[acc_row(st, h) * LD + b * 32 + lr], dp[st], dq[b]);
+      }
+    }
+    if (has_next) {
+      kc.template store<LD>(ks[(t + 1) & 1], tid);
+      vc.template store<LD>(vs[(t + 1) & 1], tid);
+    }
+    __syncthreads();
+  }
+  if (!row_ok) return;
+  float* row = a.dq.p + ca_row(a.dq, a, bh, qi);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int dd = b * 32 + 8 * g + 4 * h;
+      if (dd >= a.d) continue;
+      const f32x4 v = {dq[b][4 * g] * a.scale, dq[b][4 * g + 1] * a.scale, dq[b][4 * g + 2] * a.scale,
+                       dq[b][4 * g + 3] * a.scale};
+      store4<VEC>(row + dd, v, a.d - dd);
+    }
+  }
+}
+
+// A [32][DP] tile of query rows (TileCopy over rows that may cross heads).
+template <int DP, bool VEC>
+struct CaRowTile : TileCopy<DP, VEC> {
+  using Base = TileCopy<DP, VEC>;
+  __device__ __forceinline__ void load_rows(const FaIn& x, const CaArgs& a, int bh, int row0, int tid) {
+#pragma unroll
+    for (int i = 0; i < Base::kPer; ++i) {
+      const int u = tid + i * kFaThreads;
+      const int r = row0 + u / (DP / 4);
+      const int c = (u % (DP / 4)) * 4;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      if (u < Base::kUnits && r < a.R) v = load4<VEC>(x.p + ca_row(x, a, bh, r) + c, a.d - c);
+      Base::reg[i] = v;
+    }
+  }
+};
+
+// dK and dV: a workgroup takes 128 keys (32 a wave, a lane its key, k and v in
+// registers) and walks the query rows: S, dP (lane = key), P, dS, dV^T += dO^T P,
+// dK^T += Q^T dS.
+template <int DP, bool VEC>
+__global__ void __launch_bounds__(kFaThreads, DP <= 64 ? 2 : 1)
+cross_bwd_dkdv_kernel(const CaArgs a) {
+  constexpr int NC = DP / 8;
+  constexpr int NB = DP / 32;
+  constexpr int LD = DP + 4;
+  __shared__ __attribute__((aligned(16))) float qs[2][kTile * LD];
+  __shared__ __attribute__((aligned(16))) float dos[2][kTile * LD];
+  __shared__ __attribute__((aligned(16))) float ls[2][kTile];
+  __shared__ __attribute__((aligned(16))) float ds[2][kTile];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lr = lane & 31, h = lane >> 5;
+  const int kb = blockIdx.x / a.BH, bh = blockIdx.x % a.BH;
+  const int len = ca_len(a, bh);
+  const int kw = kb * kBlock + wave * kTile;  // the wave's first key
+  const int kj = kw + lr;
+  const bool key_ok = kj < len;
+  const float* __restrict__ K = ca_head(a.k, a, bh);
+  const float* __restrict__ V = ca_head(a.v, a, bh);
+
+  f32x4 kr[NC], vr[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int dd = 8 * c + 4 * h;
+    kr[c] = key_ok ? load4<VEC>(K + (int64_t)kj * a.k.st + dd, a.d - dd) : f32x4{0.f, 0.f, 0.f, 0.f};
+    vr[c] = key_ok ? load4<VEC>(V + (int64_t)kj * a.v.st + dd, a.d - dd) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  f32x16 dk[NB], dv[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) dk[b] = dv[b] = zero16();
+  // a workgroup whose keys are all masked only writes zeros
+  const int ntiles = kb * kBlock < len ? (a.R + kTile - 1) / kTile : 0;
+
+  CaRowTile<DP, VEC> qc, dc;
+  float lreg = 0.f, dreg = 0.f;
+  auto load_tile = [&](int t) {
+    qc.load_rows(a.q, a, bh, t * kTile, tid);
+    dc.load_rows(a.dout, a, bh, t * kTile, tid);
+    if (tid < kTile) {
+      const int r = t * kTile + tid;
+      lreg = r < a.R ? a.lse[(int64_t)bh * a.R + r] * kLog2e : INFINITY;
+      if (lreg == -INFINITY) lreg = INFINITY;
+      dreg = r < a.R ? a.D[(int64_t)bh * a.R + r] : 0.f;
+    }
+  };
+  auto store_tile = [&](int buf) {
+    qc.template store<LD>(qs[buf], tid);
+    dc.template store<LD>(dos[buf], tid);
+    if (tid < kTile) {
+      ls[buf][tid] = lreg;
+      ds[buf][tid] = dreg;
+    }
+  };
+  if (ntiles > 0) {
+    load_tile(0);
+    store_tile(0);
+  }
+  __syncthreads();
+  for (int t = 0; t < ntiles; ++t) {
+    const int cur = t & 1;
+    const bool has_next = t + 1 < ntiles;
+    if (has_next) load_tile(t + 1);
+    if (kw < len) {
+      const float* qt = qs[cur];
+      const float* dot = dos[cur];
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const f32x4 qf = *reinterpret_cast<const f32x4*>(qt + lr * LD + 8 * c + 4 * h);
+        const f32x4 df = *reinterpret_cast<const f32x4*>(dot + lr * LD + 8 * c + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s = mfma32(qf[e], kr[c][e], s);
+          dp = mfma32(df[e], vr[c][e], dp);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 l4 = *reinterpret_cast<const f32x4*>(&ls[cur][8 * g + 4 * h]);
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(&ds[cur][8 * g + 4 * h]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          const float p = key_ok ? fast_exp2(s[r] * a.scale_log2 - l4[e]) : 0.f;
+          s[r] = p;
+          dp[r] = key_ok ? p * (dp[r] - d4[e]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int st = 0; st < 16; ++st) {
+          const int q = acc_row(st, h);
+          dv[b] = mfma32(dot[q * LD + b * 32 + lr], s[st], dv[b]);
+          dk[b] = mfma32(qt[q * LD + b * 32 + lr], dp[st], dk[b]);
+        }
+      }
+    }
+    if (has_next) store_tile(cur ^ 1);
+    __syncthreads();
+  }
+  if (kj >= a.Tk) return;
+  float* krow = ca_head(a.dk, a, bh) + (int64_t)kj * a.dk.st;
+  float* vrow = ca_head(a.dv, a, bh) + (int64_t)kj * a.dv.st;
+  // (a masked key's zero is written as such: its sums may hold 0 * inf)
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int dd = b * 32 + 8 * g + 4 * h;
+      if (dd >= a.d) continue;
+      f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
+      if (key_ok) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = dk[b][4 * g + e] * a.scale;
+          y[e] = dv[b][4 * g + e];
+        }
+      }
+      store4<VEC>(krow + dd, x, a.d - dd);
+      store4<VEC>(vrow + dd, y, a.d - dd);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host side
+
+constexpr int kFewRows = 8;    // query rows a key/value head up to which cross_rows_kernel runs
+constexpr int kMaxSplits = 64;
+
+int pad_dim(int64_t d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
+
+// Key ranges a forward is split into, and their keys.  Enough workgroups to fill
+// the GPU (four to a CU for the few-row kernel, which lives on loads in flight,
+// two for the tiled one), ranges of at least 64 (128) keys.
+void ca_plan(int64_t bh, int64_t R, int64_t Tk, int* splits, int* chunk) {
+  const int64_t cus = device_cu_count();
+  const bool few = R <= kFewRows;
+  const int64_t grid = bh * (few ? 1 : ceil_div(R, kBlock));
+  const int64_t want = few ? 4 * cus : 2 * cus, least = few ? 64 : 128;
+  int64_t s = grid * 3 / 2 >= want ? 1 : ceil_div(want, grid);
+  s = std::max<int64_t>(1, std::min<int64_t>({s, Tk / least, (int64_t)kMaxSplits}));
+  const int64_t c = ceil_div(ceil_div(std::max<int64_t>(Tk, 1), s), kTile) * kTile;
+  *chunk = (int)c;
+  *splits = (int)std::max<int64_t>(1, ceil_div(Tk, c));
+}
+
+bool ca_shape_ok(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk) {
+  const int64_t most = int64_t(1) << 24;
+  if (B > most || H > most || Tq > most || Tk > most) return false;
+  if (H / Hkv * Tq > most || B * Hkv > most) return false;
+  // a dispatch holds its work items in 32 bits
+  const int64_t q = B * Hkv * ceil_div(H / Hkv * Tq, kBlock), k = B * Hkv * ceil_div(Tk, kBlock);
+  return q * kFaThreads <= (int64_t)UINT32_MAX && k * kFaThreads <= (int64_t)UINT32_MAX &&
+         B * H * Tq <= (int64_t)UINT32_MAX / 32;
+}
+
+bool ca_vec_ok(int64_t d, std::initializer_list<const void*> ptrs, const int64_t* strides, int n) {
+  if (d % 4 != 0) return false;
+  for (const void* p : ptrs)
+    if (!aligned16(p)) return false;
+  for (int i = 0; i < n; ++i)
+    if (strides[i] % 4 != 0) return false;
+  return true;
+}
+
+FaIn ca_in(const float* p, const int64_t* s) { return FaIn{p, s[0], s[1], s[2]}; }
+FaOut ca_out(float* p, const int64_t* s) { return FaOut{p, s[0], s[1], s[2]}; }
+
+template <int RQ, bool VEC>
+void launch_few(const CaArgs& a, int dp, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)a.BH * a.splits)), block(256);
+  if (dp == 32) cross_rows_kernel<RQ, 8, VEC><<<grid, block, 0, st>>>(a);
+  else if (dp == 64) cross_rows_kernel<RQ, 16, VEC><<<grid, block, 0, st>>>(a);
+  else cross_rows_kernel<RQ, 32, VEC><<<grid, block, 0, st>>>(a);
+}
+
+template <int DP, bool VEC>
+int launch_fwd(const CaArgs& a, hipStream_t st) {
+  if (a.R <= kFewRows) {
+    if (a.R == 1) launch_few<1, VEC>(a, DP, st);
+    else if (a.R == 2) launch_few<2, VEC>(a, DP, st);
+    else if (a.R <= 4) launch_few<4, VEC>(a, DP, st);
+    else launch_few<8, VEC>(a, DP, st);
+  } else {
+    const int64_t nqb = ceil_div(a.R, kBlock);
+    cross_fwd_kernel<DP, VEC><<<dim3((unsigned)(nqb * a.BH * a.splits)), dim3(kFaThreads), 0, st>>>(a);
+  }
+  const int rc = launch_status();
+  if (rc != AAR_OK || a.splits == 1) return rc;
+  const int64_t lanes = (int64_t)a.BH * a.R * (DP / 4);
+  cross_combine_kernel<DP, VEC><<<dim3((unsigned)ceil_div(lanes, (int64_t)256)), dim3(256), 0, st>>>(a);
+  return launch_status();
+}
+
+template <int DP, bool VEC>
+int launch_bwd(const CaArgs& a, hipStream_t st) {
+  if (a.R > 0) {
+    cross_bwd_dq_kernel<DP, VEC><<<dim3((unsigned)(ceil_div(a.R, kBlock) * a.BH)), dim3(kFaThreads), 0, st>>>(a);
+    const int rc = launch_status();
+    if (rc != AAR_OK) return rc;
+  }
+  if (a.Tk == 0) return AAR_OK;
+  cross_bwd_dkdv_kernel<DP, VEC><<<dim3((unsigned)(ceil_div(a.Tk, kBlock) * a.BH)), dim3(kFaThreads), 0, st>>>(a);
+  return launch_status();
+}
+
+template <bool FWD>
+int ca_dispatch(const CaArgs& a, bool vec, hipStream_t st) {
+  const int dp = pad_dim(a.d);
+  if constexpr (FWD) {
+    if (dp == 32) return vec ? launch_fwd<32, true>(a, st) : launch_fwd<32, false>(a, st);
+    if (dp == 64) return vec ? launch_fwd<64, true>(a, st) : launch_fwd<64, false>(a, st);
+    return vec ? launch_fwd<128, true>(a, st) : launch_fwd<128, false>(a, st);
+  } else {
+    if (dp == 32) return vec ? launch_bwd<32, true>(a, st) : launch_bwd<32, false>(a, st);
+    if (dp == 64) return vec ? launch_bwd<64, true>(a, st) : launch_bwd<64, false>(a, st);
+    return vec ? launch_bwd<128, true>(a, st) : launch_bwd<128, false>(a, st);
+  }
+}
+
+int ca_check(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d) {
+  if (B < 0 || H < 0 || Hkv < 0 || Tq < 0 || Tk < 0 || d <= 0 || d > 128) return AAR_EINVAL;
+  if ((H == 0) != (Hkv == 0) || (H > 0 && H % Hkv != 0)) return AAR_EINVAL;
+  if (H > 0 && !ca_shape_ok(B, H, Hkv, Tq, Tk)) return AAR_EUNSUPPORTED;
+  return AAR_OK;
+}
+
+size_t part_o_bytes(int64_t bh, int64_t R, int64_t d, int splits) {
+  return (size_t)bh * splits * (size_t)R * pad_dim(d) * sizeof(float);
+}
+
+CaArgs ca_args(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d, const int64_t* lens, float* lse,
+               float scale) {
+  CaArgs a{};
+  a.lens = lens;
+  a.lse = lse;
+  a.Tq = (int)Tq;
+  a.Tk = (int)Tk;
+  a.d = (int)d;
+  a.G = (int)(H / Hkv);
+  a.Hkv = (int)Hkv;
+  a.R = (int)(H / Hkv * Tq);
+  a.BH = (int)(B * Hkv);
+  a.scale = scale;
+  a.scale_log2 = scale * kLog2e;
+  return a;
+}
+
+}  // namespace
+}  // namespace aar
+
+using namespace aar;
+
+extern "C" {
+
+size_t aar_cross_attn_fwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d) {
+  if (ca_check(B, H, Hkv, Tq, Tk, d) != AAR_OK || B == 0 || H == 0 || Tq == 0 || Tk == 0) return 0;
+  int splits, chunk;
+  ca_plan(B * Hkv, H / Hkv * Tq, Tk, &splits, &chunk);
+  if (splits == 1) return 0;
+  return part_o_bytes(B * Hkv, H / Hkv * Tq, d, splits) + (size_t)B * H * Tq * splits * sizeof(float);
+}
+
+int aar_cross_attn_fwd_f32(const float* q, const float* k, const float* v, const int64_t* kv_lens, float* o, float* lse,
+                           int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d,
+                           const int64_t* strides, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = ca_check(B, H, Hkv, Tq, Tk, d);
+  if (rc != AAR_OK) return rc;
+  if (B == 0 || H == 0 || Tq == 0) return AAR_OK;
+  if (!q || !o || !lse || !strides || (Tk > 0 && (!k || !v))) return AAR_EINVAL;
+  CaArgs a = ca_args(B, H, Hkv, Tq, Tk, d, kv_lens, lse, scale);
+  a.q = ca_in(q, strides);
+  a.k = ca_in(k, strides + 3);
+  a.v = ca_in(v, strides + 6);
+  a.o = ca_out(o, strides + 9);
+  ca_plan(a.BH, a.R, Tk, &a.splits, &a.chunk);
+  if (a.splits > 1) {
+    const size_t need = aar_cross_attn_fwd_workspace_bytes(B, H, Hkv, Tq, Tk, d);
+    if (!workspace || !aligned16(workspace) || workspace_bytes < need) return AAR_EWORKSPACE;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_l = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_o_bytes(a.BH, a.R, d, a.splits));
+  }
+  return ca_dispatch<true>(a, ca_vec_ok(d, {q, k, v, o}, strides, 12), as_stream(stream));
+}
+
+// D of every query row
+size_t aar_cross_attn_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d) {
+  if (ca_check(B, H, Hkv, Tq, Tk, d) != AAR_OK) return 0;
+  return (size_t)B * H * Tq * sizeof(float);
+}
+
+int aar_cross_attn_bwd_f32(const float* q, const float* k, const float* v, const int64_t* kv_lens, const float* o,
+                           const float* lse, const float* dout, float* dq, float* dk, float* dv, int64_t B, int64_t H,
+                           int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d, const int64_t* strides, float scale,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = ca_check(B, H, Hkv, Tq, Tk, d);
+  if (rc != AAR_OK) return rc;
+  if (B == 0 || H == 0) return AAR_OK;
+  if (!strides) return AAR_EINVAL;
+  if (Tq > 0 && (!q || !o || !lse || !dout || !dq)) return AAR_EINVAL;
+  if (Tk > 0 && (!k || !v || !dk || !dv)) return AAR_EINVAL;
+  if (Tq == 0 && Tk == 0) return AAR_OK;
+  if (Tq > 0 &&
+      (!workspace || workspace_bytes < aar_cross_attn_bwd_workspace_bytes(B, H, Hkv, Tq, Tk, d)))
+    return AAR_EWORKSPACE;
+  CaArgs a = ca_args(B, H, Hkv, Tq, Tk, d, kv_lens, const_cast<float*>(lse), scale);
+  a.q = ca_in(q, strides);
+  a.k = ca_in(k, strides + 3);
+  a.v = ca_in(v, strides + 6);
+  a.o_in = ca_in(o, strides + 9);
+  a.dout = ca_in(dout, strides + 12);
+  a.dq = ca_out(dq, strides + 15);
+  a.dk = ca_out(dk, strides + 18);
+  a.dv = ca_out(dv, strides + 21);
+  a.D = static_cast<float*>(workspace);
+  a.splits = 1;
+  return ca_dispatch<false>(a, ca_vec_ok(d, {q, k, v, o, dout, dq, dk, dv}, strides, 24), as_stream(stream));
+}
+
+}  // extern "C"

@@ -551,6 +551,103 @@ int aar_dropout_f32(const float* x, float* out, float* mask, int64_t n, float p,
 int aar_causal_mask_f32(const float* x, float* y, int64_t mats, int64_t T, float fill,
                         void* stream);
 
+/* ------------------------ operators of a decoder that reads an encoder ----
+ * No counterparts in the reference, whose model is a decoder alone. */
+
+/* Cross attention: queries [B, H, Tq, d] against keys and values [B, Hkv, Tk, d]
+ * of another length; H a multiple of Hkv, and query head h reads key/value head
+ * h / (H / Hkv).  kv_lens (int64 [B] on the device, NULL: all Tk) hides the keys
+ * j >= kv_lens[b] of batch b (a value below 0 counts as 0, one above Tk as Tk):
+ * they are not read, whatever they hold.
+ *   O = softmax(scale * Q K^T) V,  lse = m + ln(l) per query row ([B, H, Tq]);
+ * a row without keys has O = 0 and lse = -inf.  `strides` lists (sb, sh, st) in
+ * elements of q, k, v, o (12 values; head dim contiguous), as in
+ * aar_flash_fwd_strided_f32; 128-bit paths need 16-byte aligned pointers and d
+ * and all strides multiples of 4.  d <= 128.  Where the query rows are too few to
+ * fill the GPU the key range is split and joined through the workspace (0 bytes
+ * otherwise; 16-byte aligned, AAR_EWORKSPACE). */
+size_t aar_cross_attn_fwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d);
+int aar_cross_attn_fwd_f32(const float* q, const float* k, const float* v, const int64_t* kv_lens, float* o,
+                           float* lse, int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d,
+                           const int64_t* strides, float scale, void* workspace, size_t workspace_bytes,
+                           void* stream);
+/* dq, dk, dv (fully overwritten; keys hidden by kv_lens get zeros), summed over
+ * the query heads that share a key/value head; no float atomics, the same bits
+ * on every run.  24 strides: q, k, v, o, dout, dq, dk, dv. */
+size_t aar_cross_attn_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d);
+int aar_cross_attn_bwd_f32(const float* q, const float* k, const float* v, const int64_t* kv_lens, const float* o,
+                           const float* lse, const float* dout, float* dq, float* dk, float* dv, int64_t B,
+                           int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d, const int64_t* strides,
+                           float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* out[i][:] = scale * w[ids[i]][:] (w [vocab, dim], ids int64 [n]): an
+ * embedding lookup whose rows are scaled, as where the table is shared with the
+ * vocabulary head.  An id outside [0, vocab) yields a zero row and sets
+ * *err = 1 (err may be NULL). */
+int aar_embedding_scaled_fwd_f32(const float* w, const int64_t* ids, float* out, int64_t n, int64_t vocab,
+                                 int64_t dim, float scale, int* err, void* stream);
+/* dw[v][:] = scale * sum of g[i][:] over the i with ids[i] == v (dw [vocab, dim]
+ * fully overwritten; rows without a token are zero; ids outside [0, vocab) give
+ * nothing).  The tokens are sorted by id and summed in their order, chunk by
+ * chunk: no float atomics, the same bits on every run.  Any vocabulary (unlike
+ * aar_embedding_bwd_f32, whose one-hot product is limited to n * vocab <= 2^30);
+ * n and vocab below 2^31 (AAR_EUNSUPPORTED).  The workspace holds the sorted
+ * tokens and the partial sums of rows that cross chunks; 16-byte aligned
+ * (AAR_EWORKSPACE). */
+size_t aar_embedding_sorted_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t dim);
+int aar_embedding_sorted_bwd_f32(const float* g, const int64_t* ids, float* dw, int64_t n, int64_t vocab,
+                                 int64_t dim, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Root-mean-square norm of every query and key head with the rotary position
+ * embedding in the same pass.  Row i of x holds q_heads + k_heads heads of d
+ * floats at x + i * x_row (a packed projection's row may hold more after them);
+ * y likewise at y + i * y_row.  Per head, with w = wq[d] or wk[d]:
+ *   u = x * rsqrt(mean(x^2) + eps) * w
+ *   y[c]         = u[c] cos a - u[c + r/2] sin a      c < r/2, r = rotary_dim,
+ *   y[c + r/2]   = u[c + r/2] cos a + u[c] sin a      a = position * base^(-2c / r)
+ *   y[c]         = u[c]                               c >= r
+ * position of row i = positions[i % n_positions] (int64, on the device; rows a
+ * multiple of n_positions: one list for a batch of equally long sequences, or
+ * one position a row).  The angle is formed in 64 bits, so far positions lose
+ * nothing.  2 <= d <= 256; r even, 0 <= r <= d (0: norms only, positions may be
+ * NULL); base > 0; eps >= 0; x_row and y_row of at least (q_heads + k_heads) * d
+ * where rows > 1.  y may be x (y_row == x_row). */
+int aar_qk_norm_rope_fwd_f32(const float* x, int64_t x_row, const float* wq, const float* wk,
+                             const int64_t* positions, int64_t n_positions, float* y, int64_t y_row,
+                             int64_t rows, int64_t q_heads, int64_t k_heads, int64_t d, int64_t rotary_dim,
+                             double base, float eps, void* stream);
+/* The gradients: dx at dx + i * dx_row (only the heads' columns are written),
+ * dwq and dwk [d] (fully overwritten, fixed-order sums through the workspace;
+ * the gradient of a weight without heads is zero).  dx may be gy with
+ * dx_row == gy_row. */
+size_t aar_qk_norm_rope_bwd_workspace_bytes(int64_t rows, int64_t q_heads, int64_t k_heads, int64_t d);
+int aar_qk_norm_rope_bwd_f32(const float* gy, int64_t gy_row, const float* x, int64_t x_row, const float* wq,
+                             const float* wk, const int64_t* positions, int64_t n_positions, float* dx,
+                             int64_t dx_row, float* dwq, float* dwk, int64_t rows, int64_t q_heads,
+                             int64_t k_heads, int64_t d, int64_t rotary_dim, double base, float eps,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* Distillation from a teacher's top logits: logits [n, vocab] (the student's),
+ * t_logits and t_ids [n, top] (the teacher's best entries of each row and where
+ * they stand).  An id of -1 marks an absent entry; a row without entries is
+ * left out (no loss, zero gradient, not counted).  With tau = temperature,
+ *   p = softmax(t_logits / tau) over the row's entries, q = softmax(logits / tau)
+ *   loss = tau^2 * mean over the counted rows of sum_k p_k (ln p_k - ln q[t_ids_k])
+ * Entries may name the same id twice: their p add up.  An id below -1 or >= vocab
+ * sets *err = 1 (err may be NULL) and leaves its row out.
+ * stats [2 n + 1] keeps what the backward needs: each row's largest logit and
+ * its sum of exp((z - max) / tau) (+inf for a row that is left out), then the
+ * number of counted rows.  1 <= top <= 1024, vocab below 2^31 (AAR_EUNSUPPORTED),
+ * temperature > 0. */
+size_t aar_distill_workspace_bytes(int64_t n);
+int aar_distill_fwd_f32(const float* logits, const float* t_logits, const int64_t* t_ids, float* loss,
+                        float* stats, int64_t n, int64_t vocab, int64_t top, float temperature, int* err,
+                        void* workspace, size_t workspace_bytes, void* stream);
+/* dlogits [n, vocab] = grad[0] * tau / counted * (q - p), grad a device scalar. */
+int aar_distill_bwd_f32(const float* grad, const float* logits, const float* t_logits, const int64_t* t_ids,
+                        const float* stats, float* dlogits, int64_t n, int64_t vocab, int64_t top,
+                        float temperature, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
