@@ -53,6 +53,10 @@ from ._core import (  # noqa: E402
     scaled_add_inplace,
     adamw_step,
     flash_attention,
+    cross_attention,
+    qk_norm_rope,
+    embedding_scaled,
+    distill_loss,
     cuda_synchronize,
 )
 
@@ -95,6 +99,10 @@ __all__ = [
     "scaled_add_inplace",
     "adamw_step",
     "flash_attention",
+    "cross_attention",
+    "qk_norm_rope",
+    "embedding_scaled",
+    "distill_loss",
     "cuda_synchronize",
     "nn",
     "optim",

@@ -109,15 +109,20 @@ def _rng_or_default(rng):
 
 
 class Embedding(Module):
-    """Lookup table, weight [num_embeddings, embedding_dim] ~ N(0, 1)."""
+    """Lookup table, weight [num_embeddings, embedding_dim] ~ N(0, 1).  With a
+    `scale` the rows are multiplied by it, and the weight's gradient sums the
+    tokens sorted by id (any vocabulary size)."""
 
-    def __init__(self, num_embeddings, embedding_dim, *, rng=None):
+    def __init__(self, num_embeddings, embedding_dim, *, rng=None, scale=None):
         super().__init__()
         table = _rng_or_default(rng).standard_normal((num_embeddings, embedding_dim))
         self.weight = _new_parameter(table)
+        self.scale = scale
 
     def forward(self, ids):
-        return _core.embedding(self.weight.tensor, ids)
+        if self.scale is None:
+            return _core.embedding(self.weight.tensor, ids)
+        return _core.embedding_scaled(self.weight.tensor, ids, self.scale)
 
 
 class CrossEntropyLoss(Module):
@@ -134,6 +139,26 @@ class CrossEntropyLoss(Module):
             logits = _core.reshape(logits, [rows, logits.shape[-1]])
             targets = _core.reshape(targets, [rows])
         return _core.cross_entropy(logits, targets, self.ignore_index)
+
+
+class DistillationLoss(Module):
+    """temperature^2 * mean KL(teacher || student) over the teacher's top
+    entries: teacher_logits and teacher_ids [..., K] for logits [..., V].  An id
+    of -1 marks an absent entry; rows without entries above -inf do not count."""
+
+    def __init__(self, temperature=1.0):
+        super().__init__()
+        if not 0.0 < temperature < math.inf:
+            raise ValueError("DistillationLoss: temperature must be positive")
+        self.temperature = temperature
+
+    def forward(self, logits, teacher_logits, teacher_ids):
+        if len(logits.shape) > 2:
+            rows = math.prod(logits.shape[:-1])
+            logits = _core.reshape(logits, [rows, logits.shape[-1]])
+            teacher_logits = _core.reshape(teacher_logits, [rows, teacher_logits.shape[-1]])
+            teacher_ids = _core.reshape(teacher_ids, [rows, teacher_ids.shape[-1]])
+        return _core.distill_loss(logits, teacher_logits, teacher_ids, self.temperature)
 
 
 class Linear(Module):
@@ -229,9 +254,15 @@ class MultiHeadAttention(Module):
     as one op (_core._flash_attention_qkv): q, k and v are read in place from
     the [B, T, 3*D] projection and the output is written as [B, T, D].
     ``forward_views`` is the same computation through explicit per-head
-    [B, H, T, d] views and flash_attention (used to check the fused path)."""
+    [B, H, T, d] views and flash_attention (used to check the fused path).
 
-    def __init__(self, d_model, n_heads, *, causal=False, bias=True, rng=None):
+    With ``qk_norm`` every query and key head is RMS-normed (weights ``q_norm``
+    and ``k_norm``) and the first ``rotary_dim`` columns of each (None: all, 0:
+    none) are rotated by the position, in one pass before the attention;
+    positions are 0 .. T-1 unless ``forward`` is given others ([T] or [B, T])."""
+
+    def __init__(self, d_model, n_heads, *, causal=False, bias=True, rng=None, qk_norm=False, rotary_dim=None,
+                 rope_base=10000.0, norm_eps=1e-6):
         super().__init__()
         if d_model % n_heads != 0:
             raise ValueError("d_model must be divisible by n_heads")
@@ -242,9 +273,33 @@ class MultiHeadAttention(Module):
         rng = _rng_or_default(rng)
         self.qkv_proj = Linear(d_model, 3 * d_model, bias=bias, rng=rng)
         self.out_proj = Linear(d_model, d_model, bias=bias, rng=rng)
+        self.qk_norm = qk_norm
+        if qk_norm:
+            self.rotary_dim = self.d_head if rotary_dim is None else rotary_dim
+            self.rope_base = rope_base
+            self.norm_eps = norm_eps
+            self.q_norm = _new_parameter(np.ones(self.d_head))
+            self.k_norm = _new_parameter(np.ones(self.d_head))
+            self._positions = {}
 
-    def forward(self, x):
-        heads = _core._flash_attention_qkv(self.qkv_proj(x), self.n_heads, self.causal)
+    def _positions_or_default(self, positions, x):
+        if positions is not None or self.rotary_dim == 0:
+            return positions
+        key = (x.shape[-2], x.device)
+        if key not in self._positions:
+            self._positions[key] = _core.from_numpy(np.arange(key[0], dtype=np.int64)).to(x.device)
+        return self._positions[key]
+
+    def forward(self, x, positions=None):
+        qkv = self.qkv_proj(x)
+        if self.qk_norm:
+            heads = _core._flash_attention_qkv_rope(
+                qkv, self.q_norm.tensor, self.k_norm.tensor, self._positions_or_default(positions, x), self.n_heads,
+                self.causal, self.rotary_dim, self.rope_base, self.norm_eps)
+        elif positions is not None:
+            raise ValueError("MultiHeadAttention: positions need qk_norm")
+        else:
+            heads = _core._flash_attention_qkv(qkv, self.n_heads, self.causal)
         return self.out_proj(heads)
 
     def _split_heads(self, packed):
@@ -257,8 +312,60 @@ class MultiHeadAttention(Module):
             views.append(_core.transpose(one, 1, 2))
         return views
 
-    def forward_views(self, x):
+    def _rotate_heads(self, q, k, positions):
+        """[B, H, T, d] queries and keys -> normed and rotated views."""
+        B, H, T, d = q.shape
+        out = []
+        for one, heads in ((q, (H, 0)), (k, (0, H))):
+            rows = _core.reshape(_core.transpose(one, 1, 2), [B, T, H * d])
+            rows = _core.qk_norm_rope(rows, self.q_norm.tensor, self.k_norm.tensor, positions, *heads, self.rotary_dim,
+                                      self.rope_base, self.norm_eps)
+            out.append(_core.transpose(_core.reshape(rows, [B, T, H, d]), 1, 2))
+        return out
+
+    def forward_views(self, x, positions=None):
         B, T, _ = x.shape
         q, k, v = self._split_heads(self.qkv_proj(x))
+        if self.qk_norm:
+            q, k = self._rotate_heads(q, k, self._positions_or_default(positions, x))
+        elif positions is not None:
+            raise ValueError("MultiHeadAttention: positions need qk_norm")
         merged = _core.transpose(_core.flash_attention(q, k, v, self.causal), 1, 2)  # [B, T, H, d]
         return self.out_proj(_core.reshape(merged, [B, T, self.d_model]))
+
+
+class CrossAttention(Module):
+    """Attention of x [B, Tq, d_model] to a context [B, Tk, d_context] (an
+    encoder's states): query projection, packed key/value projection with
+    ``n_kv_heads`` heads (n_heads a multiple of it), attention over projections
+    read in place, output projection.  ``context_lens`` (Int64 [B]) hides a padded
+    context's rows from context_lens[b] on.
+
+    Serving projects the context once and attends to it for every new token:
+    ``kv = m.project_context(context)``, then ``m.attend(x, kv, context_lens)``."""
+
+    def __init__(self, d_model, n_heads, *, d_context=None, n_kv_heads=None, bias=True, rng=None):
+        super().__init__()
+        if d_model % n_heads != 0:
+            raise ValueError("d_model must be divisible by n_heads")
+        self.d_model = d_model
+        self.n_heads = n_heads
+        self.n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
+        if self.n_kv_heads <= 0 or n_heads % self.n_kv_heads != 0:
+            raise ValueError("n_heads must be divisible by n_kv_heads")
+        self.d_head = d_model // n_heads
+        rng = _rng_or_default(rng)
+        self.q_proj = Linear(d_model, d_model, bias=bias, rng=rng)
+        self.kv_proj = Linear(d_model if d_context is None else d_context, 2 * self.n_kv_heads * self.d_head, bias=bias,
+                              rng=rng)
+        self.out_proj = Linear(d_model, d_model, bias=bias, rng=rng)
+
+    def project_context(self, context):
+        return self.kv_proj(context)
+
+    def attend(self, x, kv, context_lens=None):
+        heads = _core._cross_attention_packed(self.q_proj(x), kv, self.n_heads, self.n_kv_heads, context_lens)
+        return self.out_proj(heads)
+
+    def forward(self, x, context, context_lens=None):
+        return self.attend(x, self.project_context(context), context_lens)

@@ -153,6 +153,14 @@ distill_row_kernel(const float* __restrict__ Z, const float* __restrict__ Tl, co
   const int64_t* ids = Ti + row * top;
   float tm, ts;
   teacher_sum(t, ids, top, k, lane, tm, ts);
+  if (ts == 0.f) {  // nothing above -inf: left out like a row without entries
+    if (lane == 0) {
+      row_loss[row] = 0.f;
+      stats[2 * row] = 0.f;
+      stats[2 * row + 1] = INFINITY;
+    }
+    return;
+  }
   const float ln_s = logf(a.s);
   // sum_k p_k (ln p_k - ln q_k) = sum_k e_k ((t_k - tm) / tau - ln q_k) / ts - ln ts
   float acc = 0.f;
@@ -165,7 +173,7 @@ distill_row_kernel(const float* __restrict__ Z, const float* __restrict__ Tl, co
   }
   acc = wave_sum(acc);
   if (lane == 0) {
-    row_loss[row] = ts == 0.f ? 0.f : tau2 * (acc / ts - logf(ts));
+    row_loss[row] = tau2 * (acc / ts - logf(ts));
     stats[2 * row] = a.m;
     stats[2 * row + 1] = a.s;
   }
@@ -243,7 +251,7 @@ distill_bwd_kernel(const float* __restrict__ grad, const float* __restrict__ Z, 
     const int64_t* ids = Ti + row * top;
     float tm, ts;
     teacher_sum(t, ids, top, k, lane, tm, ts);
-    const float inv = ts == 0.f ? 0.f : 1.0f / ts;
+    const float inv = 1.0f / ts;
     for (int i = lane; i < top; i += kWave) {
       const int id = (int)ids[i];
       sid[i] = id;

@@ -288,6 +288,133 @@ flash_fwd_kernel(FaIn Qv, FaIn Kv, FaIn Vv, FaOut Ov, float* __restrict__ Lse, i
   }
 }
 
+// A [32][DP] tile staged transposed for the split products whose reduced-over
+// dimension is the tile's rows (V^T P^T): a thread takes 8 rows of one
+// column, which is one lane's operand of the matrix op.  Planes are
+// [part][octet][column] in 16-byte units.
+template <int DP>
+struct FaKtSplit {
+  static constexpr int kUnits = DP * 4;  // (column, octet of rows)
+  static constexpr int kPer = kUnits / kFaThreads;
+  static_assert(kUnits % kFaThreads == 0, "whole units per thread");
+  static constexpr int kPlanes = 3 * kUnits;  // 16-byte units of a stage
+  float f[kPer][8];
+  float top = 0.f;  // largest magnitude of this thread's elements
+
+  // Key e of octet o = 2s + h within the tile: acc_row(8s + e, h).
+  __device__ __forceinline__ static int key(int o, int e) {
+    return 16 * (o >> 1) + 8 * (e >> 2) + 4 * (o & 1) + (e & 3);
+  }
+  // Rows past T are clamped onto row T - 1 (their P is 0; an infinite element
+  // sends the wave to the fp32 instruction) and columns past d onto column d - 1 (they
+  // feed outputs that are not stored), so no load is predicated.  Offsets
+  // within a tile fit 32 bits (`small`) or take the clamped form, whose
+  // addresses are 64-bit and signed.
+  uint32_t off[kPer];
+  int64_t row4;  // bytes per row
+  bool small;
+  __device__ __forceinline__ void init(int64_t st, int d, int tid) {
+    row4 = st * 4;
+    small = tile_offsets_fit(st);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int u = tid + i * kFaThreads;
+      off[i] = tile_offset(key(u / DP, 0), st, min(u % DP, d - 1));
+    }
+  }
+  __device__ __forceinline__ void load(const float* __restrict__ K, int64_t st, int row0, int T, int d, int tid) {
+    if (row0 + kTile <= T && small) {
+      const char* base = reinterpret_cast<const char*>(K + (int64_t)row0 * st);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)  // key(o, e) = key(o, 0) + key(0, e)
+          f[i][e] = *reinterpret_cast<const float*>(base + key(0, e) * row4 + off[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int u = tid + i * kFaThreads;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int row = min(row0 + key(u / DP, e), T - 1);
+          f[i][e] = K[(int64_t)row * st + min(u % DP, d - 1)];
+        }
+      }
+    }
+  }
+  // rem: what the splits left over (bf16_split_pair).
+  __device__ __forceinline__ void store(u32x4* s, int tid, uint32_t& rem) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int u = tid + i * kFaThreads;
+      u32x4 parts[3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t w[3];
+        top = fmaxf(fmaxf(top, fabsf(f[i][2 * e])), fabsf(f[i][2 * e + 1]));
+        bf16_split_pair(f[i][2 * e], f[i][2 * e + 1], w, rem);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) parts[p][e] = w[p];
+      }
+#pragma unroll
+      for (int p = 0; p < 3; ++p) s[p * kUnits + u] = parts[p];
+    }
+  }
+};
+
+// The same for products over the columns (K Q^T): a thread takes 8 columns of
+// one row; planes are [part][octet of columns][row], the octets one unit
+// further apart so that the eight threads of a row store to distinct banks.
+template <int DP>
+struct FaRowSplit {
+  static constexpr int kOcts = DP / 8;
+  static constexpr int kUnits = kTile * kOcts;
+  static_assert(kUnits == kFaThreads, "one unit per thread");
+  static constexpr int kOs = kTile + 1;
+  static constexpr int kPlane = kOcts * kOs;
+  f32x4 f[2];
+  float top = 0.f;
+
+  // Rows past T are clamped onto row T - 1 (the caller masks them), columns
+  // past d onto earlier ones (Q is zero there).
+  uint32_t off[2];
+  bool small;
+  __device__ __forceinline__ static int column(int tid, int g, int d) {
+    return min(8 * (tid % kOcts) + 4 * g, d - 4);  // d is a multiple of 4
+  }
+  __device__ __forceinline__ void init(int64_t st, int d, int tid) {
+    small = tile_offsets_fit(st);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) off[g] = tile_offset(tid / kOcts, st, column(tid, g, d));
+  }
+  __device__ __forceinline__ void load(const float* __restrict__ K, int64_t st, int row0, int T, int d, int tid) {
+    if (row0 + kTile <= T && small) {
+      const char* base = reinterpret_cast<const char*>(K + (int64_t)row0 * st);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) f[g] = *reinterpret_cast<const f32x4*>(base + off[g]);
+    } else {
+      const float* row = K + (int64_t)min(row0 + tid / kOcts, T - 1) * st;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) f[g] = *reinterpret_cast<const f32x4*>(row + column(tid, g, d));
+    }
+  }
+  __device__ __forceinline__ void store(u32x4* s, int tid, uint32_t& rem) {
+    u32x4 parts[3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = f[e >> 1][2 * (e & 1)], y = f[e >> 1][2 * (e & 1) + 1];
+      uint32_t w[3];
+      top = fmaxf(fmaxf(top, fabsf(x)), fabsf(y));
+      bf16_split_pair(x, y, w, rem);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) parts[p][e] = w[p];
+    }
+#pragma unroll
+    for (int p = 0; p < 3; ++p) s[p * kPlane + (tid % kOcts) * kOs + tid / kOcts] = parts[p];
+  }
+};
+
 // Forward on the bf16 matrix cores, every operand in three bf16 parts
 // (bf16x3.hpp): Q is split once into registers, K and V tiles once per workgroup
 // on their way into LDS (double-buffered planes, one barrier per tile), P in the

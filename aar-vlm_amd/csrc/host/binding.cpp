@@ -157,7 +157,31 @@ PYBIND11_MODULE(_core, m) {
   m.def("bmm_at_b", &bmm_at_b, gil_release());
   m.def("dropout", &dropout, py::arg("x"), py::arg("p"), gil_release());
 
+  // Operators of a decoder that reads an encoder and learns from a teacher.
+  m.def("cross_attention", &cross_attention, py::arg("q"), py::arg("k"), py::arg("v"),
+        py::arg("kv_lens") = std::shared_ptr<Tensor>(), gil_release(),
+        "softmax(q k^T / sqrt(d)) v of q [B, H, Tq, d] over k, v [B, Hkv, Tk, d] (H a multiple of Hkv); kv_lens "
+        "(Int64 [B]) hides the keys from kv_lens[b] on, and a row without keys gives zeros.");
+  m.def("qk_norm_rope", &qk_norm_rope, py::arg("x"), py::arg("q_weight"), py::arg("k_weight"), py::arg("positions"),
+        py::arg("n_q_heads"), py::arg("n_k_heads"), py::arg("rotary_dim") = -1, py::arg("base") = 10000.0,
+        py::arg("eps") = 1e-6f, gil_release(),
+        "RMS norm of every query and key head of x [..., T, (n_q_heads + n_k_heads) * d] and the rotary position "
+        "embedding of its first rotary_dim columns (-1: all, 0: none); positions Int64, [T] or one per row.");
+  m.def("embedding_scaled", &embedding_scaled, py::arg("weight"), py::arg("ids"), py::arg("scale"), gil_release(),
+        "scale * weight[ids]; the weight's gradient sums sorted tokens (any vocabulary, reproducible).");
+  m.def("distill_loss", &distill_loss, py::arg("logits"), py::arg("teacher_logits"), py::arg("teacher_ids"),
+        py::arg("temperature") = 1.0f, gil_release(),
+        "temperature^2 * mean KL of softmax(teacher / temperature), over each row's K entries, from "
+        "softmax(logits / temperature); an id of -1 marks an absent entry, a row without entries above -inf does not count.");
+
   // Extensions of this build (not in the reference API).
+  m.def("_cross_attention_packed", &cross_attention_packed, py::arg("q"), py::arg("kv"), py::arg("n_heads"),
+        py::arg("n_kv_heads"), py::arg("kv_lens") = std::shared_ptr<Tensor>(), gil_release(),
+        "cross_attention over projections read in place: q [B, Tq, H*d], kv [B, Tk, 2*Hkv*d] -> [B, Tq, H*d].");
+  m.def("_flash_attention_qkv_rope", &flash_attention_qkv_rope, py::arg("qkv"), py::arg("q_weight"),
+        py::arg("k_weight"), py::arg("positions"), py::arg("n_heads"), py::arg("causal"), py::arg("rotary_dim") = -1,
+        py::arg("base") = 10000.0, py::arg("eps") = 1e-6f, gil_release(),
+        "_flash_attention_qkv with queries and keys normed and rotated as by qk_norm_rope.");
   m.def("_flash_attention_fwd", &flash_attention_fwd_lse, py::arg("q"), py::arg("k"), py::arg("v"),
         py::arg("causal"), gil_release(),
         "Forward flash attention returning (O, lse); lse = m + ln(l) per query row.");

@@ -182,21 +182,26 @@ class SumAllFunction : public Function {
   const char* name() const override { return "SumAllFunction"; }
 };
 
+// dW of a lookup: the one-hot product, or by sorted tokens where that product
+// is refused (n * vocab above 2^30).
+Tensor table_grad(const Tensor& gc, const Tensor& ids, int64_t V) {
+  const int64_t D = gc.shape.back();
+  const int64_t n = n_of(ids);
+  if (static_cast<double>(n) * static_cast<double>(V) > static_cast<double>(1ll << 30)) {
+    return embedding_sorted_grad(gc, ids, V, 1.0f);
+  }
+  Tensor dW = Tensor::empty({V, D}, DType::Fp32, Device::CUDA);
+  Workspace ws(aar_embedding_bwd_workspace_bytes(n, V, D));
+  check_status(aar_embedding_bwd_f32(fp(gc), ip(ids), fp(dW), n, V, D, ws.data(), ws.bytes(), current_stream()),
+               "embedding backward");
+  return dW;
+}
+
 class EmbeddingFunction : public Function {
  public:
   Tensor saved_ids;
   int64_t vocab_size = 0;
-  std::vector<Tensor> backward(const Tensor& g) override {
-    Tensor gc = as_contig(g);
-    const int64_t D = gc.shape.back();
-    const int64_t n = n_of(saved_ids);
-    Tensor dW = Tensor::empty({vocab_size, D}, DType::Fp32, Device::CUDA);
-    Workspace ws(aar_embedding_bwd_workspace_bytes(n, vocab_size, D));
-    check_status(aar_embedding_bwd_f32(fp(gc), ip(saved_ids), fp(dW), n, vocab_size, D, ws.data(), ws.bytes(),
-                                       current_stream()),
-                 "embedding backward");
-    return {dW};
-  }
+  std::vector<Tensor> backward(const Tensor& g) override { return {table_grad(as_contig(g), saved_ids, vocab_size)}; }
   const char* name() const override { return "EmbeddingFunction"; }
 };
 
@@ -208,16 +213,7 @@ class EmbeddingAddFunction : public Function {
   int64_t vocab1 = 0, vocab2 = 0;
   std::vector<Tensor> backward(const Tensor& g) override {
     Tensor gc = as_contig(g);
-    const int64_t D = gc.shape.back();
-    auto table_grad = [&](const Tensor& ids, int64_t V) {
-      const int64_t n = n_of(ids);
-      Tensor dW = Tensor::empty({V, D}, DType::Fp32, Device::CUDA);
-      Workspace ws(aar_embedding_bwd_workspace_bytes(n, V, D));
-      check_status(aar_embedding_bwd_f32(fp(gc), ip(ids), fp(dW), n, V, D, ws.data(), ws.bytes(), current_stream()),
-                   "embedding backward");
-      return dW;
-    };
-    return {table_grad(saved_ids1, vocab1), table_grad(saved_ids2, vocab2)};
+    return {table_grad(gc, saved_ids1, vocab1), table_grad(gc, saved_ids2, vocab2)};
   }
   const char* name() const override { return "EmbeddingAddFunction"; }
 };

@@ -631,6 +631,51 @@ class FlashQKVFunction : public Function {
   const char* name() const override { return "FlashQKVFunction"; }
 };
 
+// The same with queries and keys normed and rotated first: the rotated pair is
+// kept as one [..., T, 2*D] tensor, v stays in the packed projection.  Backward:
+// dv goes straight into the packed gradient, dq and dk through the rotation's
+// backward into its other columns.
+class FlashQKVRopeFunction : public Function {
+ public:
+  Tensor saved_qkv, saved_qk, saved_o, saved_lse, wq, wk, positions;
+  int64_t B = 0, H = 0, T = 0, d = 0, rotary = 0;
+  bool causal = false;
+  float scale_factor = 1.0f, eps = 0.0f;
+  double base = 0.0;
+  std::vector<Tensor> backward(const Tensor& grad_output) override {
+    Tensor go = as_contig(grad_output);
+    Tensor dqkv = Tensor::empty(saved_qkv.shape, saved_qkv.dtype, saved_qkv.device);
+    Tensor dqk = Tensor::empty(saved_qk.shape, saved_qk.dtype, saved_qk.device);
+    Tensor dwq = Tensor::empty({d}, wq.dtype, wq.device), dwk = Tensor::empty({d}, wk.dtype, wk.device);
+    const int64_t D = H * d, rows = B * T;
+    int64_t st[24];
+    strides(st, D);
+    if (rows > 0) {
+      Workspace ws = flash_bwd_workspace(B * H, T, d, causal);
+      check_status(aar_flash_bwd_strided_f32(fp(saved_qk), fp(saved_qk) + D, fp(saved_qkv) + 2 * D, fp(saved_o),
+                                             fp(saved_lse), fp(go), fp(dqk), fp(dqk) + D, fp(dqkv) + 2 * D, B, H, T, d,
+                                             st, causal ? 1 : 0, scale_factor, ws.data(), ws.bytes(), current_stream()),
+                   "flash_attention_qkv_rope backward");
+    }
+    Workspace ws(aar_qk_norm_rope_bwd_workspace_bytes(rows, H, H, d));
+    check_status(aar_qk_norm_rope_bwd_f32(fp(dqk), 2 * D, fp(saved_qkv), 3 * D, fp(wq), fp(wk),
+                                          rotary ? static_cast<const int64_t*>(positions.data()) : nullptr,
+                                          rotary ? static_cast<int64_t>(positions.numel()) : 0, fp(dqkv), 3 * D, fp(dwq),
+                                          fp(dwk), rows, H, H, d, rotary, base, eps, ws.data(), ws.bytes(),
+                                          current_stream()),
+                 "flash_attention_qkv_rope backward");
+    return {dqkv, dwq, dwk};
+  }
+  const char* name() const override { return "FlashQKVRopeFunction"; }
+
+  // q, k, v, o, dout, dq, dk, dv
+  void strides(int64_t* st, int64_t D) const {
+    const int64_t two[3] = {T * 2 * D, d, 2 * D}, three[3] = {T * 3 * D, d, 3 * D}, one[3] = {T * D, d, D};
+    const int64_t* all[8] = {two, two, three, one, one, two, two, three};
+    for (int i = 0; i < 8; ++i) put3(st + 3 * i, all[i]);
+  }
+};
+
 
 // ------------------------------------------------------------------ add
 
@@ -1210,6 +1255,61 @@ Tensor flash_attention_qkv(const Tensor& qkv, int64_t n_heads, bool causal) {
   fn->d = d;
   fn->causal = causal;
   fn->scale_factor = s;
+  out.requires_grad = true;
+  out.grad_fn = fn;
+  return out;
+}
+
+Tensor flash_attention_qkv_rope(const Tensor& qkv, const Tensor& q_weight, const Tensor& k_weight,
+                                const std::shared_ptr<Tensor>& positions, int64_t n_heads, bool causal,
+                                int64_t rotary_dim, double base, float eps) {
+  const char* op = "flash_attention_qkv_rope";
+  const int64_t d = check_rope(qkv, q_weight, k_weight, positions, 3 * n_heads, rotary_dim, base, eps, op);
+  if (d > 128) throw std::invalid_argument("flash_attention: d_head exceeds D_MAX (128)");
+  if (qkv.device == Device::CPU) throw_cpu_compute(op);
+  auto fn = std::make_shared<FlashQKVRopeFunction>();
+  Tensor x = as_contig(qkv), wq = as_contig(q_weight), wk = as_contig(k_weight);
+  const int64_t D = n_heads * d, T = x.shape[x.shape.size() - 2];
+  const int64_t rows = static_cast<int64_t>(x.numel()) / (3 * D);
+  fn->B = T > 0 ? rows / T : 0;
+  fn->H = n_heads;
+  fn->T = T;
+  fn->d = d;
+  fn->rotary = rotary_dim;
+  fn->causal = causal;
+  fn->scale_factor = 1.0f / std::sqrt(static_cast<float>(d));
+  fn->eps = eps;
+  fn->base = base;
+  if (rotary_dim > 0) fn->positions = as_contig(*positions);
+  std::vector<int64_t> qk_shape(x.shape), o_shape(x.shape);
+  qk_shape.back() = 2 * D;
+  o_shape.back() = D;
+  Tensor qk = Tensor::empty(qk_shape, x.dtype, x.device);
+  Tensor out = Tensor::empty(o_shape, x.dtype, x.device);
+  Tensor lse = Tensor::empty({fn->B * n_heads, T}, x.dtype, x.device);
+  if (rows > 0) {
+    check_status(aar_qk_norm_rope_fwd_f32(fp(x), 3 * D, fp(wq), fp(wk),
+                                          rotary_dim ? static_cast<const int64_t*>(fn->positions.data()) : nullptr,
+                                          rotary_dim ? static_cast<int64_t>(fn->positions.numel()) : 0, fp(qk), 2 * D,
+                                          rows, n_heads, n_heads, d, rotary_dim, base, eps, current_stream()),
+                 op);
+    int64_t st[24];
+    fn->strides(st, D);
+    Workspace ws = flash_fwd_workspace(fn->B * n_heads, T, d, causal);
+    check_status(aar_flash_fwd_strided_f32(fp(qk), fp(qk) + D, fp(x) + 2 * D, fp(out), fp(lse), fn->B, n_heads, T, d, st,
+                                           causal ? 1 : 0, fn->scale_factor, ws.data(), ws.bytes(), current_stream()),
+                 op);
+  }
+  if (!x.requires_grad && !wq.requires_grad && !wk.requires_grad) return out;
+  fn->record_input(x);
+  fn->record_input(wq);
+  fn->record_input(wk);
+  fn->saved_qkv = x;
+  fn->saved_qk = qk;
+  fn->saved_o = out;
+  fn->saved_lse = lse;
+  fn->wq = wq;
+  fn->wk = wk;
   out.requires_grad = true;
   out.grad_fn = fn;
   return out;

@@ -2,6 +2,7 @@
 // the reference's namespace-vlm functions bound in cppsrc/python/binding.cpp).
 #pragma once
 
+#include <memory>
 #include <tuple>
 
 #include "tensor.hpp"
@@ -83,6 +84,34 @@ Tensor bmm_at_b(const Tensor& a, const Tensor& b);
 Tensor apply_causal_mask(const Tensor& x);
 Tensor dropout(const Tensor& x, float p);
 void manual_seed(uint64_t seed);
+
+// Operators of a decoder that reads an encoder and learns from a teacher (no
+// counterparts in the reference; lm_ops.cpp, flash_attention_qkv_rope in ops.cpp).
+// Cross attention of q [B, H, Tq, d] over k, v [B, Hkv, Tk, d], H a multiple of
+// Hkv; kv_lens (Int64 [B], null: all keys) hides the keys from kv_lens[b] on.
+Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::shared_ptr<Tensor>& kv_lens);
+// The same over projections read in place: q [B, Tq, H*d], kv [B, Tk, 2*Hkv*d].
+Tensor cross_attention_packed(const Tensor& q, const Tensor& kv, int64_t n_heads, int64_t n_kv_heads,
+                              const std::shared_ptr<Tensor>& kv_lens);
+// Per-head RMS norm and rotary position embedding of x [..., T, (Hq + Hk) * d];
+// rotary_dim < 0 means d; positions [T] or one per row (unused at rotary_dim 0).
+Tensor qk_norm_rope(const Tensor& x, const Tensor& q_weight, const Tensor& k_weight,
+                    const std::shared_ptr<Tensor>& positions, int64_t n_q_heads, int64_t n_k_heads, int64_t rotary_dim,
+                    double base, float eps);
+// Its argument checks (rotary_dim < 0 becomes d); returns d.
+int64_t check_rope(const Tensor& x, const Tensor& q_weight, const Tensor& k_weight,
+                   const std::shared_ptr<Tensor>& positions, int64_t heads, int64_t& rotary_dim, double base, float eps,
+                   const char* op);
+// flash_attention_qkv with queries and keys normed and rotated first.
+Tensor flash_attention_qkv_rope(const Tensor& qkv, const Tensor& q_weight, const Tensor& k_weight,
+                                const std::shared_ptr<Tensor>& positions, int64_t n_heads, bool causal,
+                                int64_t rotary_dim, double base, float eps);
+// scale * embedding(weight, ids), its gradient by sorted tokens.
+Tensor embedding_scaled(const Tensor& weight, const Tensor& ids, float scale);
+// dW [vocab, D] = scale * sums of g's rows by their ids (contiguous operands).
+Tensor embedding_sorted_grad(const Tensor& g, const Tensor& ids, int64_t vocab, float scale);
+// Distillation of logits [N, V] from a teacher's top entries [N, K] (id -1: absent).
+Tensor distill_loss(const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_ids, float temperature);
 
 // Token-window batch (x, y) of shape [starts, seq_len] gathered on the device
 // from an int64 token stream (python/shakespeare/scripts/data.py:38-53).

@@ -629,8 +629,8 @@ int aar_qk_norm_rope_bwd_f32(const float* gy, int64_t gy_row, const float* x, in
 
 /* Distillation from a teacher's top logits: logits [n, vocab] (the student's),
  * t_logits and t_ids [n, top] (the teacher's best entries of each row and where
- * they stand).  An id of -1 marks an absent entry; a row without entries is
- * left out (no loss, zero gradient, not counted).  With tau = temperature,
+ * they stand).  An id of -1 marks an absent entry; a row without entries, or
+ * with none above -inf, is left out (no loss, zero gradient, not counted).  With tau = temperature,
  *   p = softmax(t_logits / tau) over the row's entries, q = softmax(logits / tau)
  *   loss = tau^2 * mean over the counted rows of sum_k p_k (ln p_k - ln q[t_ids_k])
  * Entries may name the same id twice: their p add up.  An id below -1 or >= vocab

@@ -1,0 +1,270 @@
+"""Cross attention (aar_cross_attn_*, ag.cross_attention, nn.CrossAttention) on
+the GPU against its definition in 64 bits: lengths from none to long, odd sizes,
+padded contexts (rows without keys, garbage behind the lengths), shared heads,
+strided and unaligned operands, other streams and captured graphs."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import lmops as M
+from devutil import dev, host
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def L(gpu):
+    return M.lib()
+
+
+def rand(seed, *shape, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).cuda()
+
+
+def run(L, q, k, v, lens, do=None, scale=None):
+    B, H, Tq, d = q.shape
+    o, lse = torch.full_like(q, 7.0, memory_format=torch.contiguous_format), torch.full((B, H, Tq), 7.0, device="cuda")
+    M.cross_fwd(L, q, k, v, lens, o, lse, scale)
+    if do is None:
+        return o, lse
+    dq, dk, dv = (torch.full(t.shape, 7.0, device="cuda") for t in (q, k, v))
+    M.cross_bwd(L, q, k, v, lens, o, lse, do, dq, dk, dv, scale)
+    return o, lse, dq, dk, dv
+
+
+def check(L, q, k, v, lens, do, scale=None, smax=6.0):
+    got = run(L, q, k, v, lens, do, scale)
+    ref = M.cross_exact(q, k, v, lens, do, scale)
+    tol = M.attn_tol(q.shape[-1], max(k.shape[2], q.shape[2] * q.shape[1] // k.shape[1]), smax)
+    mass = M.cross_mass(q, k, v, lens, do, scale)
+    for name, g, r in zip(("o", "lse", "dq", "dk", "dv"), got, ref):
+        # dS is a difference of two sums of their own: twice the roundings
+        M.near(g, r, tol * (2 if name[0] == "d" else 1), name, mass.get(name))
+
+
+# B, H, Hkv, Tq, Tk, d
+SHAPES = [
+    (1, 1, 1, 1, 1, 64), (2, 3, 3, 1, 5, 64), (3, 2, 2, 1, 300, 64), (2, 4, 1, 1, 777, 128), (1, 8, 1, 1, 65, 32),
+    (2, 6, 2, 2, 129, 40), (1, 2, 2, 7, 1000, 64), (1, 2, 2, 8, 31, 30), (2, 3, 3, 9, 33, 64), (1, 5, 5, 31, 64, 128),
+    (2, 2, 2, 32, 32, 64), (1, 3, 3, 33, 31, 96), (2, 4, 2, 100, 65, 64), (1, 2, 1, 129, 200, 36), (1, 1, 1, 300, 1, 64),
+    (1, 2, 2, 257, 577, 64), (2, 8, 4, 65, 300, 128), (1, 3, 3, 50, 70, 1), (1, 2, 2, 40, 90, 3), (1, 2, 2, 64, 2049, 64),
+    (4, 12, 12, 130, 260, 64), (1, 1, 1, 2000, 40, 64), (1, 1, 1, 1, 8192, 64), (16, 16, 16, 140, 140, 64),
+]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_against_the_definition(L, shape):
+    B, H, Hkv, Tq, Tk, d = shape
+    q, do = rand(1, B, H, Tq, d), rand(2, B, H, Tq, d)
+    k, v = rand(3, B, Hkv, Tk, d), rand(4, B, Hkv, Tk, d)
+    check(L, q, k, v, None, do)
+
+
+@pytest.mark.parametrize("shape", [(5, 2, 2, 1, 200, 64), (5, 4, 2, 3, 100, 128), (5, 2, 2, 40, 200, 64),
+                                   (5, 4, 1, 70, 333, 36), (5, 3, 3, 200, 130, 30), (5, 2, 2, 33, 900, 64)])
+def test_padded_contexts(L, shape):
+    """Lengths none, one, a tile's border, some and all; what stands behind them is
+    never read: infinities and NaN there change nothing."""
+    B, H, Hkv, Tq, Tk, d = shape
+    q, do = rand(1, B, H, Tq, d), rand(2, B, H, Tq, d)
+    k, v = rand(3, B, Hkv, Tk, d), rand(4, B, Hkv, Tk, d)
+    lens = torch.tensor([0, 1, 32, Tk // 2 + 1, Tk], device="cuda")
+    check(L, q, k, v, lens, do)
+    clean = run(L, q, k, v, lens, do)
+    for b in range(B):
+        n = int(lens[b])
+        k[b, :, n:] = math.nan
+        v[b, :, n:] = math.inf
+    dirty = run(L, q, k, v, lens, do)
+    for a, b in zip(clean, dirty):
+        assert torch.equal(a, b)
+    o, lse, dq, dk, dv = dirty
+    assert (o[0] == 0).all() and (lse[0] == -math.inf).all() and (dq[0] == 0).all()
+    for b in range(B):
+        assert (dk[b, :, int(lens[b]):] == 0).all() and (dv[b, :, int(lens[b]):] == 0).all()
+    # lengths outside [0, Tk] count as its ends
+    odd = torch.tensor([-5, 1, 32, Tk // 2 + 1, Tk + 1000], device="cuda")
+    for a, b in zip(dirty, run(L, q, k, v, odd, do)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("Tq", [1, 5, 40])
+def test_no_keys_and_no_queries(L, Tq):
+    q, do = rand(1, 2, 4, Tq, 64), rand(2, 2, 4, Tq, 64)
+    k = torch.empty(2, 2, 0, 64, device="cuda")
+    o, lse, dq, dk, dv = run(L, q, k, k, None, do)
+    assert (o == 0).all() and (lse == -math.inf).all() and (dq == 0).all() and dk.numel() == 0
+    k = rand(3, 2, 2, 50, 64)
+    none = torch.empty(2, 4, 0, 64, device="cuda")
+    o, lse, dq, dk, dv = run(L, none, k, k, None, none)
+    assert (dk == 0).all() and (dv == 0).all()
+
+
+@pytest.mark.parametrize("Tq", [1, 6, 90])
+@pytest.mark.parametrize("d", [64, 128, 36])
+def test_strided_operands(L, Tq, d):
+    """Packed projections, rows and heads in other orders, unaligned bases."""
+    B, H, Hkv, Tk = 2, 4, 2, 150
+    qp, kv = rand(1, B, Tq, H, d), rand(2, B, Tk, 2, Hkv, d)
+    do = rand(3, B, Tq, H, d)
+    q, k, v = qp.permute(0, 2, 1, 3), kv[:, :, 0].permute(0, 2, 1, 3), kv[:, :, 1].permute(0, 2, 1, 3)
+    ref = M.cross_exact(q, k, v, None, do.permute(0, 2, 1, 3))
+    tol = 2 * M.attn_tol(d, Tk)
+    dense = run(L, q.contiguous(), k.contiguous(), v.contiguous(), None, do.permute(0, 2, 1, 3).contiguous())
+    for offset in (0, 1):  # unaligned by one float: the element-wise path
+        def at(t):
+            buf = torch.empty(t.numel() + 8, device="cuda")
+            got = torch.as_strided(buf, t.shape, t.stride(), offset)
+            got.copy_(t)
+            return got
+        q1, do1 = at(qp).permute(0, 2, 1, 3), at(do).permute(0, 2, 1, 3)
+        kv1 = at(kv)
+        k1, v1 = kv1[:, :, 0].permute(0, 2, 1, 3), kv1[:, :, 1].permute(0, 2, 1, 3)
+        o, dq = at(torch.zeros_like(qp)).permute(0, 2, 1, 3), at(torch.zeros_like(qp)).permute(0, 2, 1, 3)
+        dkv = at(torch.zeros_like(kv))
+        dk, dv = dkv[:, :, 0].permute(0, 2, 1, 3), dkv[:, :, 1].permute(0, 2, 1, 3)
+        lse = torch.empty(B, H, Tq, device="cuda")
+        M.cross_fwd(L, q1, k1, v1, None, o, lse)
+        M.cross_bwd(L, q1, k1, v1, None, o, lse, do1, dq, dk, dv)
+        for name, g, r, x in zip(("o", "lse", "dq", "dk", "dv"), (o, lse, dq, dk, dv), ref, dense):
+            M.near(g, r, tol, name)
+            if offset == 0:
+                assert torch.equal(g, x), name
+
+
+@pytest.mark.parametrize("Tq", [1, 50])
+def test_extreme_scores(L, Tq):
+    """Scores of +-1000 (one key takes all), all keys equal, a negative scale, and
+    keys of -inf that leave a row nothing."""
+    q, k, v = rand(1, 1, 2, Tq, 64), rand(2, 1, 2, 100, 64), rand(3, 1, 2, 100, 64)
+    o, lse = run(L, q, k, v, None, scale=100.0)
+    ro, rl = M.cross_exact(q, k, v, None, scale=100.0)
+    M.near(lse, rl, M.attn_tol(64, 100, 1.0), "lse")  # of the size of its scores
+    # P moves by the scores' own rounding: sqrt(64) half steps of scores up to 6 * 8 * 100
+    M.near(o, ro, M.attn_tol(64, 100, 4800.0), "o")
+    check(L, q, torch.zeros_like(k), v, None, rand(4, 1, 2, Tq, 64))
+    check(L, q, k, v, None, rand(4, 1, 2, Tq, 64), scale=-0.125)
+    # queries with a positive first column against keys of -inf there: every score is -inf
+    q[..., 0] = q[..., 0].abs() + 1
+    k[..., 0] = -math.inf
+    o, lse = run(L, q, k, v, None)
+    assert (o == 0).all() and (lse == -math.inf).all()
+
+
+def test_gradients_against_differences(L):
+    """d/dh of sum(do * O) along random directions, from forwards alone, in steps
+    whose own error is of order h^2."""
+    q, k, v = rand(1, 1, 4, 5, 64), rand(2, 1, 2, 60, 64), rand(3, 1, 2, 60, 64)
+    do = rand(4, 1, 4, 5, 64)
+    lens = torch.tensor([47], device="cuda")
+    _, _, dq, dk, dv = run(L, q, k, v, lens, do)
+    h = 2.0 ** -6
+    for i, (x, g) in enumerate(((q, dq), (k, dk), (v, dv))):
+        w = rand(10 + i, *x.shape)
+        args = [q, k, v]
+        vals = []
+        for s in (h, -h):
+            args[i] = x + s * w
+            vals.append((run(L, *args, lens)[0].double() * do.double()).sum().item())
+        want = (g.double() * w.double()).sum().item()
+        # third derivative about |w|^3 ~ 1 per score; outputs' roundings over 2 h
+        bound = (h * h + M.attn_tol(64, 60) / h) * (do.norm() * w.norm()).item() / 4
+        assert abs((vals[0] - vals[1]) / (2 * h) - want) <= bound
+
+
+def test_reproducible_and_on_other_streams(L):
+    q, k, v, do = rand(1, 3, 4, 70, 64), rand(2, 3, 2, 500, 64), rand(3, 3, 2, 500, 64), rand(4, 3, 4, 70, 64)
+    lens = torch.tensor([500, 3, 77], device="cuda")
+    first = run(L, q, k, v, lens, do)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = run(L, q, k, v, lens, do)
+    side.synchronize()
+    for a, b in zip(first, second):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("Tq", [1, 40])
+def test_captured_graph(L, Tq):
+    """A captured forward and backward replayed with new inputs, with eager work
+    between the replays."""
+    q, k, v, do = rand(1, 2, 4, Tq, 64), rand(2, 2, 2, 600, 64), rand(3, 2, 2, 600, 64), rand(4, 2, 4, Tq, 64)
+    lens = torch.tensor([600, 30], device="cuda")
+    o, lse = torch.empty_like(q), torch.empty(2, 4, Tq, device="cuda")
+    dq, dk, dv = (torch.empty_like(t) for t in (q, k, v))
+    dims = (2, 4, 2, Tq, 600, 64)
+    wf, wb = M.scratch(L.aar_cross_attn_fwd_workspace_bytes(*dims)), M.scratch(L.aar_cross_attn_bwd_workspace_bytes(*dims))
+
+    def both():
+        M.cross_fwd(L, q, k, v, lens, o, lse, ws=wf)
+        M.cross_bwd(L, q, k, v, lens, o, lse, do, dq, dk, dv, ws=wb)
+
+    both()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        both()
+    for i in range(3):
+        for j, t in enumerate((q, k, v, do)):
+            t.copy_(rand(20 + 4 * i + j, *t.shape))
+        lens.copy_(torch.tensor([600 - 100 * i, 31 * i]))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (o, lse, dq, dk, dv)]
+        for a, b in zip(got, run(L, q, k, v, lens, do)):
+            assert torch.equal(a, b)
+
+
+def test_ops_and_module(gpu):
+    """ag.cross_attention on views, and nn.CrossAttention whole, projected once for
+    single tokens, and with the context's gradient."""
+    rng = np.random.default_rng(5)
+    B, Tq, Tk, D, C, H, Hkv = 3, 9, 40, 96, 56, 6, 2
+    d = D // H
+    lens = np.array([40, 0, 17], np.int64)
+    tl = gpu.from_numpy(lens).to(gpu.Device.CUDA)
+    x, ctx = rng.standard_normal((B, Tq, D)).astype(np.float32), rng.standard_normal((B, Tk, C)).astype(np.float32)
+    gy = rng.standard_normal((B, Tq, D)).astype(np.float32)
+    m = gpu.nn.CrossAttention(D, H, d_context=C, n_kv_heads=Hkv, rng=rng).to(gpu.Device.CUDA)
+    tx, tc = dev(gpu, x, True), dev(gpu, ctx, True)
+    y = m(tx, tc, tl)
+    y.backward(dev(gpu, gy))
+    w = [torch.from_numpy(host(gpu, p.tensor)).double().requires_grad_() for p in m.parameters()]
+    X, Cx = (torch.from_numpy(t).double().requires_grad_() for t in (x, ctx))
+    q = (X @ w[0].t() + w[1]).view(B, Tq, H, d).transpose(1, 2)
+    kv = (Cx @ w[2].t() + w[3]).view(B, Tk, 2, Hkv, d)
+    k, v = (kv[:, :, i].transpose(1, 2).repeat_interleave(H // Hkv, 1) for i in (0, 1))
+    seen = torch.arange(Tk) < torch.from_numpy(lens).view(B, 1, 1, 1)
+    s = (q @ k.transpose(2, 3) / math.sqrt(d)).masked_fill(~seen, -1e300)
+    p = torch.softmax(s, -1) * seen
+    ref = (p @ v).transpose(1, 2).reshape(B, Tq, D) @ w[4].t() + w[5]
+    ref.backward(torch.from_numpy(gy).double())
+    # products of up to 96 terms on both sides of the attention
+    tol = 4 * M.attn_tol(96, 40)
+    M.near(host(gpu, y), ref, tol, "y")
+    M.near(host(gpu, tx.grad), X.grad, tol, "dx")
+    M.near(host(gpu, tc.grad), Cx.grad, tol, "dcontext")
+    for i, (a, b) in enumerate(zip(m.parameters(), w)):
+        M.near(host(gpu, a.tensor.grad), b.grad, tol, f"parameter {i}")
+    kvp = m.project_context(dev(gpu, ctx))
+    for t in range(Tq):
+        one = m.attend(dev(gpu, x[:, t:t + 1]), kvp, tl)
+        M.near(host(gpu, one)[:, 0], ref.detach()[:, t], tol, f"token {t}")
+    # the op itself over transposed views
+    tq, tk = dev(gpu, rng.standard_normal((B, Tq, H, d)), True), dev(gpu, rng.standard_normal((B, Tk, Hkv, d)), True)
+    tv = dev(gpu, rng.standard_normal((B, Tk, Hkv, d)), True)
+    o = gpu.cross_attention(*(gpu.transpose(t, 1, 2) for t in (tq, tk, tv)), tl)
+    g = rng.standard_normal((B, H, Tq, d)).astype(np.float32)
+    o.backward(dev(gpu, g))
+    hq, hk, hv = (torch.from_numpy(host(gpu, t)).transpose(1, 2) for t in (tq, tk, tv))
+    ro, _, dq, dk, dv = M.cross_exact(hq, hk, hv, torch.from_numpy(lens), torch.from_numpy(g))
+    for name, a, b in (("o", host(gpu, o), ro), ("dq", host(gpu, tq.grad), dq.transpose(1, 2)),
+                       ("dk", host(gpu, tk.grad), dk.transpose(1, 2)), ("dv", host(gpu, tv.grad), dv.transpose(1, 2))):
+        M.near(a, b, 2 * M.attn_tol(d, Tk), name)
