@@ -62,6 +62,58 @@ __device__ __forceinline__ auto ca_head(const T& x, const CaArgs& a, int bh) {
   return x.p + (int64_t)(bh / a.Hkv) * x.sb + (int64_t)(bh % a.Hkv) * x.sh;
 }
 
+// A lane's row of a forward: O and lse, or the normalised part and its log2 sum.
+template <int DP, bool VEC>
+__device__ __forceinline__ void ca_store_row(const CaArgs& a, int bh, int part, int qi, int h,
+                                             const f32x16 (&o)[DP / 32], float m, float l) {
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const float l2 = m + log2f(l);
+  const int64_t prow = ((int64_t)bh * a.splits + part) * a.R + qi;
+  float* orow = a.splits > 1 ? a.part_o + prow * DP : a.o.p + ca_row(a.o, a, bh, qi);
+#pragma unroll
+  for (int b = 0; b < DP / 32; ++b) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int dd = b * 32 + 8 * g + 4 * h;
+      const f32x4 v = {o[b][4 * g] * inv, o[b][4 * g + 1] * inv, o[b][4 * g + 2] * inv, o[b][4 * g + 3] * inv};
+      if (a.splits > 1) *reinterpret_cast<f32x4*>(orow + dd) = v;
+      else if (dd < a.d) store4<VEC>(orow + dd, v, a.d - dd);
+    }
+  }
+  if (h == 0) {
+    if (a.splits > 1) a.part_l[prow] = l2;
+    else a.lse[(int64_t)bh * a.R + qi] = l2 * kLn2;
+  }
+}
+
+// A lane's row of accumulators times f.
+template <int DP, bool VEC>
+__device__ __forceinline__ void ca_store_scaled(float* row, const f32x16 (&x)[DP / 32], float f, int d, int h) {
+#pragma unroll
+  for (int b = 0; b < DP / 32; ++b) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int dd = b * 32 + 8 * g + 4 * h;
+      if (dd >= d) continue;
+      const f32x4 v = {x[b][4 * g] * f, x[b][4 * g + 1] * f, x[b][4 * g + 2] * f, x[b][4 * g + 3] * f};
+      store4<VEC>(row + dd, v, d - dd);
+    }
+  }
+}
+
+// A lane's key: dK and dV.  A masked key's zero is written as such (its sums may
+// hold 0 * inf).
+template <int DP, bool VEC>
+__device__ __forceinline__ void ca_store_key(const CaArgs& a, int bh, int kj, bool key_ok, f32x16 (&dk)[DP / 32],
+                                             f32x16 (&dv)[DP / 32], int h) {
+  if (!key_ok) {
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) dk[b] = dv[b] = zero16();
+  }
+  ca_store_scaled<DP, VEC>(ca_head(a.dk, a, bh) + (int64_t)kj * a.dk.st, dk, a.scale, a.d, h);
+  ca_store_scaled<DP, VEC>(ca_head(a.dv, a, bh) + (int64_t)kj * a.dv.st, dv, 1.0f, a.d, h);
+}
+
 // -------------------------------------------------------------- few query rows
 
 // Up to RQ query rows a key/value head (single tokens): bound by the bytes of K
@@ -329,25 +381,7 @@ cross_fwd_kernel(const CaArgs a) {
     }
     __syncthreads();
   }
-  if (qi >= a.R) return;
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  const float l2 = m + log2f(l);
-  const int64_t prow = ((int64_t)bh * a.splits + part) * a.R + qi;
-  float* orow = a.splits > 1 ? a.part_o + prow * DP : a.o.p + ca_row(a.o, a, bh, qi);
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int dd = b * 32 + 8 * g + 4 * h;
-      const f32x4 v = {o[b][4 * g] * inv, o[b][4 * g + 1] * inv, o[b][4 * g + 2] * inv, o[b][4 * g + 3] * inv};
-      if (a.splits > 1) *reinterpret_cast<f32x4*>(orow + dd) = v;
-      else if (dd < a.d) store4<VEC>(orow + dd, v, a.d - dd);
-    }
-  }
-  if (h == 0) {
-    if (a.splits > 1) a.part_l[prow] = l2;
-    else a.lse[(int64_t)bh * a.R + qi] = l2 * kLn2;
-  }
+  if (qi < a.R) ca_store_row<DP, VEC>(a, bh, part, qi, h, o, m, l);
 }
 
 // ------------------------------------------------------------------ backward
@@ -447,19 +481,7 @@ cross_bwd_dq_kernel(const CaArgs a) {
     }
     __syncthreads();
   }
-  if (!row_ok) return;
-  float* row = a.dq.p + ca_row(a.dq, a, bh, qi);
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int dd = b * 32 + 8 * g + 4 * h;
-      if (dd >= a.d) continue;
-      const f32x4 v = {dq[b][4 * g] * a.scale, dq[b][4 * g + 1] * a.scale, dq[b][4 * g + 2] * a.scale,
-                       dq[b][4 * g + 3] * a.scale};
-      store4<VEC>(row + dd, v, a.d - dd);
-    }
-  }
+  if (row_ok) ca_store_scaled<DP, VEC>(a.dq.p + ca_row(a.dq, a, bh, qi), dq, a.scale, a.d, h);
 }
 
 // A [32][DP] tile of query rows (TileCopy over rows that may cross heads).
@@ -583,28 +605,610 @@ cross_bwd_dkdv_kernel(const CaArgs a) {
     if (has_next) store_tile(cur ^ 1);
     __syncthreads();
   }
-  if (kj >= a.Tk) return;
-  float* krow = ca_head(a.dk, a, bh) + (int64_t)kj * a.dk.st;
-  float* vrow = ca_head(a.dv, a, bh) + (int64_t)kj * a.dv.st;
-  // (a masked key's zero is written as such: its sums may hold 0 * inf)
+  if (kj < a.Tk) ca_store_key<DP, VEC>(a, bh, kj, key_ok, dk, dv, h);
+}
+
+// ---------------------------------------------------- on the bf16 matrix cores
+// The same passes with every operand in three bf16 parts (bf16x3.hpp): six matrix
+// ops per 16 steps at 14 times the fp32 instruction's rate.  What a wave keeps in
+// registers for all tiles (q; q and dO; k and v) is split once; a tile is split on
+// its way into LDS, once a workgroup, as three row-major planes.  Products over
+// the head dim read rows of them; products over the tile's rows (V^T P^T, K^T
+// dS^T, dO^T P, Q^T dS) read columns through the transposing LDS read, so a tile
+// that serves both is split and stored once.  P and dS are split in the registers
+// the softmax leaves them in.
+
+// A [32][DP] tile in three planes of 32 rows; a row's 16 spare bytes put 16
+// consecutive rows' 128-bit reads on distinct banks.
+template <int DP>
+struct SplitTile {
+  static constexpr int kRow = 2 * DP + 16;  // bytes
+  static constexpr int kPlane = kTile * kRow;
+  static constexpr int kBytes = 3 * kPlane;
+  static constexpr int kOcts = DP / 8;
+  static constexpr int kPer = kTile * kOcts / kFaThreads;  // 8-column units a thread stages
+  static_assert(kPer * kFaThreads == kTile * kOcts, "whole units");
+  f32x4 f[kPer][2];
+  float top = 0.f;   // largest magnitude of this thread's elements
+  uint32_t rem = 0;  // what the splits left over (bf16_split_pair)
+
+  // Row of unit i of thread tid, and its first column.
+  __device__ __forceinline__ static int row(int i, int tid) { return (tid + i * kFaThreads) / kOcts; }
+  __device__ __forceinline__ static int col(int i, int tid) { return 8 * (tid % kOcts); }
+  // `at(r)` is the pointer to row r of the tile, null for a row that is not read.
+  template <typename At>
+  __device__ __forceinline__ void load(int d, int tid, At at) {
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
+    for (int i = 0; i < kPer; ++i) {
+      const float* p = at(row(i, tid));
+      const int c = col(i, tid);
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int dd = b * 32 + 8 * g + 4 * h;
-      if (dd >= a.d) continue;
-      f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
-      if (key_ok) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] = dk[b][4 * g + e] * a.scale;
-          y[e] = dv[b][4 * g + e];
-        }
+      for (int g = 0; g < 2; ++g) {
+        f[i][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (p && c + 4 * g < d) f[i][g] = *reinterpret_cast<const f32x4*>(p + c + 4 * g);
       }
-      store4<VEC>(krow + dd, x, a.d - dd);
-      store4<VEC>(vrow + dd, y, a.d - dd);
     }
   }
+  __device__ __forceinline__ void store(char* s, int tid) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      u32x4 parts[3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = f[i][e >> 1][2 * (e & 1)], y = f[i][e >> 1][2 * (e & 1) + 1];
+        uint32_t w[3];
+        top = fmaxf(fmaxf(top, fabsf(x)), fabsf(y));
+        bf16_split_pair(x, y, w, rem);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) parts[p][e] = w[p];
+      }
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+        *reinterpret_cast<u32x4*>(s + p * kPlane + row(i, tid) * kRow + 2 * col(i, tid)) = parts[p];
+    }
+  }
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// ds_read_b64_tr_b16: 16 lanes read four rows of 16 bf16 each (lane j the four
+// from column 4 (j % 4) of row j / 4) and lane j receives column j of the rows.
+__device__ __forceinline__ void read_columns(const char* p, uint32_t& lo, uint32_t& hi) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  const u32x2 w = __builtin_bit_cast(u32x2, v);
+  lo = w[0];
+  hi = w[1];
+#endif
+}
+
+// acc += tile . B over the head dim: the tile's 32 rows are the output's rows,
+// B's columns (b[c][part], lane = column) the output's.
+template <int DP>
+__device__ __forceinline__ f32x16 split_rows(const char* s, const u32x4 (&b)[DP / 16][3], int lr, int h) {
+  f32x16 acc = zero16();
+  const char* p = s + lr * SplitTile<DP>::kRow + 16 * h;
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) {
+    u32x4 x[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) x[i] = *reinterpret_cast<const u32x4*>(p + i * SplitTile<DP>::kPlane + 32 * c);
+#pragma unroll
+    for (int i = 0; i < kSplitProducts; ++i) acc = mfma_bf16(x[kSplitA[i]], b[c][kSplitB[i]], acc);
+  }
+  return acc;
+}
+
+// The three parts of accumulator registers 8 k .. 8 k + 7, the right operand of
+// the products over the tile's rows.
+__device__ __forceinline__ void split_regs(const f32x16& s, int k, u32x4 (&pp)[3], uint32_t& rem) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t w[3];
+    bf16_split_pair(s[8 * k + 2 * e], s[8 * k + 2 * e + 1], w, rem);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) pp[p][e] = w[p];
+  }
+}
+
+// acc[b] += tile^T . (rows 16 k .. 16 k + 15 of P): column 32 b + lr of the tile,
+// its rows in the order of the accumulator registers that pp was made of.
+template <int DP>
+__device__ __forceinline__ void split_cols(const char* s, const u32x4 (&pp)[3], int k, int lane, f32x16 (&acc)[DP / 32]) {
+  using T = SplitTile<DP>;
+  const int h = lane >> 5, j = lane & 15;
+  const char* p = s + (16 * k + 4 * h + (j >> 2)) * T::kRow + 2 * (16 * ((lane >> 4) & 1) + 4 * (j & 3));
+#pragma unroll
+  for (int b = 0; b < DP / 32; ++b) {
+    u32x4 x[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      uint32_t w[4];
+      read_columns(p + i * T::kPlane + 64 * b, w[0], w[1]);
+      read_columns(p + i * T::kPlane + 64 * b + 8 * T::kRow, w[2], w[3]);
+      x[i] = u32x4{w[0], w[1], w[2], w[3]};
+    }
+#pragma unroll
+    for (int i = 0; i < kSplitProducts; ++i) acc[b] = mfma_bf16(x[kSplitA[i]], pp[kSplitB[i]], acc[b]);
+  }
+}
+
+// A lane's row (its half's octets of each 16 columns) times f, in parts.
+template <int DP>
+__device__ __forceinline__ void split_row(const float* p, int d, float f, int h, u32x4 (&out)[DP / 16][3], float& top,
+                                          uint32_t& rem) {
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int dd = 16 * c + 8 * h + 4 * g;
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+      if (p && dd < d) x = *reinterpret_cast<const f32x4*>(p + dd);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float u = x[2 * e] * f, v = x[2 * e + 1] * f;
+        // rounded here: fused into the split's first subtraction, a product would
+        // leave bits that three parts do not hold
+        asm volatile("" : "+v"(u), "+v"(v));
+        uint32_t w[3];
+        top = fmaxf(fmaxf(top, fabsf(u)), fabsf(v));
+        bf16_split_pair(u, v, w, rem);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) out[c][i][2 * g + e] = w[i];
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ float wave_top(float v) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_max(v))));
+}
+
+// Forward.  The running maximum m of a row follows its scores only when they pass
+// it by 2^8 (the sums stay far from fp32's end), so O is rarely rescaled.
+template <int DP, int STAGES>
+__global__ void __launch_bounds__(kFaThreads, 2)
+cross_fwd_split_kernel(const CaArgs a) {
+  using Tile = SplitTile<DP>;
+  constexpr int NB = DP / 32;
+  __shared__ __attribute__((aligned(16))) char ks[STAGES][Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) char vs[STAGES][Tile::kBytes];
+  __shared__ uint32_t range[3];  // largest magnitude of K, of V (as bits), what their splits left over
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lr = lane & 31, h = lane >> 5;
+  const int bh = blockIdx.x % a.BH;
+  const int rest = blockIdx.x / a.BH;
+  const int part = rest % a.splits, qb = rest / a.splits;
+  const int len = ca_len(a, bh);
+  const int k0 = part * a.chunk, k1 = min(len, k0 + a.chunk);
+  const float* __restrict__ K = ca_head(a.k, a, bh);
+  const float* __restrict__ V = ca_head(a.v, a, bh);
+  const int qi = qb * kBlock + wave * kTile + lr;  // this lane's row
+  const bool work = qb * kBlock + wave * kTile < a.R;
+  const float* Q = qi < a.R ? a.q.p + ca_row(a.q, a, bh, qi) : nullptr;
+  if (tid < 3) range[tid] = 0u;
+
+  u32x4 qp[DP / 16][3];
+  float q_top = 0.f;
+  uint32_t q_rem = 0, p_rem = 0;
+  split_row<DP>(Q, a.d, a.scale_log2, h, qp, q_top, q_rem);
+  const bool q_exact = !__any((q_rem & kSplitRemBits) != 0);
+  q_top = wave_top(q_top);
+  f32x16 o[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) o[b] = zero16();
+  float m = -INFINITY, l = 0.f;
+
+  // Online softmax of a tile of log2 scores: s becomes P, O is rescaled where m moves.
+  auto soft = [&](f32x16& s, int kv0) {
+    if (kv0 + kTile > k1) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (kv0 + acc_row(r, h) >= k1) s[r] = -INFINITY;
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    mx = half_swap_max(mx);
+    if (__any(mx > m + 8.f)) {
+      const float mn = mx > m + 8.f ? mx : m;
+      const float alpha = fast_exp2(m - (mn == -INFINITY ? 0.f : mn));
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[b][r] *= alpha;
+      }
+    }
+    const float mu = m == -INFINITY ? 0.f : m;
+    float ps = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] = fast_exp2(s[r] - mu);
+      ps += s[r];
+    }
+    l += half_swap_sum(ps);
+  };
+  auto compute = [&](const char* kt, const char* vt, int kv0) {
+    f32x16 s = split_rows<DP>(kt, qp, lr, h);
+    soft(s, kv0);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      u32x4 pp[3];
+      split_regs(s, k, pp, p_rem);
+      split_cols<DP>(vt, pp, k, lane, o);
+    }
+  };
+
+  const int ntiles = k1 > k0 ? (k1 - k0 + kTile - 1) / kTile : 0;
+  Tile kc, vc;
+  auto load = [&](int t) {
+    const int row0 = k0 + t * kTile;
+    kc.load(a.d, tid, [&](int r) { return row0 + r < k1 ? K + (int64_t)(row0 + r) * a.k.st : nullptr; });
+    vc.load(a.d, tid, [&](int r) { return row0 + r < k1 ? V + (int64_t)(row0 + r) * a.v.st : nullptr; });
+  };
+  if (ntiles > 0) load(0);
+  if (STAGES == 2 && ntiles > 0) {
+    kc.store(ks[0], tid);
+    vc.store(vs[0], tid);
+  }
+  lds_barrier();
+  for (int t = 0; t < ntiles; ++t) {
+    const bool has_next = t + 1 < ntiles;
+    if (STAGES == 1) {
+      kc.store(ks[0], tid);
+      vc.store(vs[0], tid);
+      lds_barrier();
+    }
+    if (has_next) load(t + 1);
+    if (work) compute(ks[STAGES == 2 ? t & 1 : 0], vs[STAGES == 2 ? t & 1 : 0], k0 + t * kTile);
+    if (STAGES == 2 && has_next) {
+      kc.store(ks[(t + 1) & 1], tid);
+      vc.store(vs[(t + 1) & 1], tid);
+    }
+    lds_barrier();
+  }
+
+  // What the split does not cover: sums that might overflow, an element of q, K or
+  // V that is not held exactly, and probabilities below 2^-110 where O is so
+  // small that it feels them.  Such a wave's rows are redone with the fp32
+  // instruction, straight from HBM.
+  atomicMax(&range[0], __float_as_uint(kc.top));  // >= 0: ordered as their bits
+  atomicMax(&range[1], __float_as_uint(vc.top));
+  atomicOr(&range[2], kc.rem | vc.rem);
+  __syncthreads();
+  const float v_top = __uint_as_float(range[1]), n = (float)(k1 - k0);
+  bool redo = !q_exact || (range[2] & kSplitRemBits) != 0 ||
+              split_overflows(q_top, __uint_as_float(range[0]), (float)a.d) || split_overflows(256.f, v_top, n);
+  if (__any((p_rem & kSplitRemBits) != 0)) {
+    const float floor = split_loss_floor(v_top, 0.f, n);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) redo = redo || fabsf(o[b][r]) < floor;
+  }
+  if (work && ntiles > 0 && __any(redo)) {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) o[b] = zero16();
+    for (int t = 0; t < ntiles; ++t) {
+      const int kv0 = k0 + t * kTile;
+      f32x16 s = zero16();
+      for (int c = 0; c < a.d; c += 2) {
+        const bool on = c + h < a.d;
+        const float kf = on && kv0 + lr < k1 ? K[(int64_t)(kv0 + lr) * a.k.st + c + h] : 0.f;
+        const float qf = on && Q ? Q[c + h] * a.scale_log2 : 0.f;
+        s = mfma32(kf, qf, s);
+      }
+      soft(s, kv0);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int col = b * 32 + lr;
+#pragma unroll
+        for (int st = 0; st < 16; ++st) {
+          const int row = kv0 + acc_row(st, h);
+          const float v = row < k1 && col < a.d ? V[(int64_t)row * a.v.st + col] : 0.f;
+          o[b] = mfma32(v, s[st], o[b]);
+        }
+      }
+    }
+  }
+  if (qi < a.R) ca_store_row<DP, true>(a, bh, part, qi, h, o, m, l);
+}
+
+// dQ (and D).
+__global__ void __launch_bounds__(kFaThreads, 2)
+cross_bwd_dq_split_kernel(const CaArgs a) {
+  constexpr int DP = 64, NB = 2;
+  using Tile = SplitTile<DP>;
+  __shared__ __attribute__((aligned(16))) char ks[2][Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) char vs[2][Tile::kBytes];
+  __shared__ uint32_t range[3];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lr = lane & 31, h = lane >> 5;
+  const int bh = blockIdx.x % a.BH, qb = blockIdx.x / a.BH;
+  const int len = ca_len(a, bh);
+  const float* __restrict__ K = ca_head(a.k, a, bh);
+  const float* __restrict__ V = ca_head(a.v, a, bh);
+  const int qi = qb * kBlock + wave * kTile + lr;
+  const bool row_ok = qi < a.R, work = qb * kBlock + wave * kTile < a.R;
+  const float* Q = row_ok ? a.q.p + ca_row(a.q, a, bh, qi) : nullptr;
+  const float* dO = row_ok ? a.dout.p + ca_row(a.dout, a, bh, qi) : nullptr;
+  if (tid < 3) range[tid] = 0u;
+
+  float dsum = 0.f;
+  if (row_ok) {
+    const float* O = a.o_in.p + ca_row(a.o_in, a, bh, qi);
+#pragma unroll
+    for (int c = 0; c < DP / 8; ++c) {
+      const int dd = 8 * c + 4 * h;
+      if (dd < a.d) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(dO + dd), y = *reinterpret_cast<const f32x4*>(O + dd);
+        dsum += x[0] * y[0] + x[1] * y[1] + x[2] * y[2] + x[3] * y[3];
+      }
+    }
+  }
+  dsum = half_swap_sum(dsum);
+  float l2 = row_ok ? a.lse[(int64_t)bh * a.R + qi] * kLog2e : INFINITY;
+  if (l2 == -INFINITY) l2 = INFINITY;  // a row without keys has P = 0
+  if (row_ok && h == 0) a.D[(int64_t)bh * a.R + qi] = dsum;
+
+  u32x4 qp[DP / 16][3], dop[DP / 16][3];
+  float q_top = 0.f, do_top = 0.f, ds_top = 0.f;
+  uint32_t in_rem = 0, ds_rem = 0;
+  split_row<DP>(Q, a.d, a.scale_log2, h, qp, q_top, in_rem);
+  split_row<DP>(dO, a.d, 1.f, h, dop, do_top, in_rem);
+  const bool exact = !__any((in_rem & kSplitRemBits) != 0);
+  q_top = wave_top(q_top);
+  do_top = wave_top(do_top);
+  f32x16 dq[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) dq[b] = zero16();
+
+  // dS of a tile from its log2 scores and dP.
+  auto dscore = [&](const f32x16& s, f32x16& dp, int kv0) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float x = fast_exp2(s[r] - l2) * (dp[r] - dsum);
+      dp[r] = kv0 + acc_row(r, h) < len ? x : 0.f;
+    }
+  };
+  const int ntiles = (len + kTile - 1) / kTile;
+  Tile kc, vc;
+  auto load = [&](int t) {
+    const int row0 = t * kTile;
+    kc.load(a.d, tid, [&](int r) { return row0 + r < len ? K + (int64_t)(row0 + r) * a.k.st : nullptr; });
+    vc.load(a.d, tid, [&](int r) { return row0 + r < len ? V + (int64_t)(row0 + r) * a.v.st : nullptr; });
+  };
+  if (ntiles > 0) {
+    load(0);
+    kc.store(ks[0], tid);
+    vc.store(vs[0], tid);
+  }
+  lds_barrier();
+  for (int t = 0; t < ntiles; ++t) {
+    const bool has_next = t + 1 < ntiles;
+    if (has_next) load(t + 1);
+    if (work) {
+      const f32x16 s = split_rows<DP>(ks[t & 1], qp, lr, h);
+      f32x16 dp = split_rows<DP>(vs[t & 1], dop, lr, h);
+      dscore(s, dp, t * kTile);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ds_top = fmaxf(ds_top, fabsf(dp[r]));
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        u32x4 pp[3];
+        split_regs(dp, k, pp, ds_rem);
+        split_cols<DP>(ks[t & 1], pp, k, lane, dq);
+      }
+    }
+    if (has_next) {
+      kc.store(ks[(t + 1) & 1], tid);
+      vc.store(vs[(t + 1) & 1], tid);
+    }
+    lds_barrier();
+  }
+
+  // As in the forward: a wave whose operands or sums the parts do not hold is redone.
+  atomicMax(&range[0], __float_as_uint(kc.top));
+  atomicMax(&range[1], __float_as_uint(vc.top));
+  atomicOr(&range[2], kc.rem | vc.rem);
+  __syncthreads();
+  const float k_top = __uint_as_float(range[0]), d = (float)a.d;
+  ds_top = wave_top(ds_top);
+  bool redo = !exact || (range[2] & kSplitRemBits) != 0 || split_overflows(q_top, k_top, d) ||
+              split_overflows(do_top, __uint_as_float(range[1]), d) || split_overflows(ds_top, k_top, (float)len);
+  if (__any((ds_rem & kSplitRemBits) != 0)) {
+    const float floor = split_loss_floor(k_top, 0.f, (float)len);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) redo = redo || fabsf(dq[b][r]) < floor;
+  }
+  if (work && ntiles > 0 && __any(redo)) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) dq[b] = zero16();
+    for (int t = 0; t < ntiles; ++t) {
+      const int kv0 = t * kTile;
+      f32x16 s = zero16(), dp = zero16();
+      for (int c = 0; c < a.d; c += 2) {
+        const bool in = c + h < a.d, key = in && kv0 + lr < len;
+        s = mfma32(key ? K[(int64_t)(kv0 + lr) * a.k.st + c + h] : 0.f, in && Q ? Q[c + h] * a.scale_log2 : 0.f, s);
+        dp = mfma32(key ? V[(int64_t)(kv0 + lr) * a.v.st + c + h] : 0.f, in && dO ? dO[c + h] : 0.f, dp);
+      }
+      dscore(s, dp, kv0);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int col = b * 32 + lr;
+#pragma unroll
+        for (int st = 0; st < 16; ++st) {
+          const int row = kv0 + acc_row(st, h);
+          dq[b] = mfma32(row < len && col < a.d ? K[(int64_t)row * a.k.st + col] : 0.f, dp[st], dq[b]);
+        }
+      }
+    }
+  }
+  if (row_ok) ca_store_scaled<DP, true>(a.dq.p + ca_row(a.dq, a, bh, qi), dq, a.scale, a.d, h);
+}
+
+// dK and dV.
+__global__ void __launch_bounds__(kFaThreads, 2)
+cross_bwd_dkdv_split_kernel(const CaArgs a) {
+  constexpr int DP = 64, NB = 2;
+  using Tile = SplitTile<DP>;
+  __shared__ __attribute__((aligned(16))) char qs[2][Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) char dos[2][Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) float ls[2][kTile];
+  __shared__ __attribute__((aligned(16))) float ds[2][kTile];
+  __shared__ uint32_t range[3];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lr = lane & 31, h = lane >> 5;
+  const int kb = blockIdx.x / a.BH, bh = blockIdx.x % a.BH;
+  const int len = ca_len(a, bh);
+  const int kw = kb * kBlock + wave * kTile;
+  const int kj = kw + lr;
+  const bool key_ok = kj < len, work = kw < len;
+  const float* K = key_ok ? ca_head(a.k, a, bh) + (int64_t)kj * a.k.st : nullptr;
+  const float* V = key_ok ? ca_head(a.v, a, bh) + (int64_t)kj * a.v.st : nullptr;
+  if (tid < 3) range[tid] = 0u;
+
+  u32x4 kp[DP / 16][3], vp[DP / 16][3];
+  float k_top = 0.f, v_top = 0.f, ds_top = 0.f;
+  uint32_t in_rem = 0, p_rem = 0, ds_rem = 0;
+  split_row<DP>(K, a.d, a.scale_log2, h, kp, k_top, in_rem);
+  split_row<DP>(V, a.d, 1.f, h, vp, v_top, in_rem);
+  const bool exact = !__any((in_rem & kSplitRemBits) != 0);
+  k_top = wave_top(k_top);
+  v_top = wave_top(v_top);
+  f32x16 dk[NB], dv[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) dk[b] = dv[b] = zero16();
+  const int ntiles = kb * kBlock < len ? (a.R + kTile - 1) / kTile : 0;
+
+  // P (in s) and dS (in dp) of a tile; `stat(g, l4, d4)` gives the lse and D of rows 8 g + 4 h ..
+  auto dscore = [&](f32x16& s, f32x16& dp, auto stat) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4 l4, d4;
+      stat(g, l4, d4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * g + e;
+        const float p = key_ok ? fast_exp2(s[r] - l4[e]) : 0.f;
+        s[r] = p;
+        dp[r] = key_ok ? p * (dp[r] - d4[e]) : 0.f;
+      }
+    }
+  };
+  Tile qc, dc;
+  float lreg = 0.f, dreg = 0.f;
+  auto lse_of = [&](int r) {
+    const float x = r < a.R ? a.lse[(int64_t)bh * a.R + r] * kLog2e : INFINITY;
+    return x == -INFINITY ? INFINITY : x;  // a row without keys, or past the end, has P = 0
+  };
+  auto d_of = [&](int r) { return r < a.R ? a.D[(int64_t)bh * a.R + r] : 0.f; };
+  auto load = [&](int t) {
+    const int row0 = t * kTile;
+    qc.load(a.d, tid, [&](int r) { return row0 + r < a.R ? a.q.p + ca_row(a.q, a, bh, row0 + r) : nullptr; });
+    dc.load(a.d, tid, [&](int r) { return row0 + r < a.R ? a.dout.p + ca_row(a.dout, a, bh, row0 + r) : nullptr; });
+    if (tid < kTile) {
+      lreg = lse_of(row0 + tid);
+      dreg = d_of(row0 + tid);
+    }
+  };
+  auto store = [&](int buf) {
+    qc.store(qs[buf], tid);
+    dc.store(dos[buf], tid);
+    if (tid < kTile) {
+      ls[buf][tid] = lreg;
+      ds[buf][tid] = dreg;
+    }
+  };
+  if (ntiles > 0) {
+    load(0);
+    store(0);
+  }
+  lds_barrier();
+  for (int t = 0; t < ntiles; ++t) {
+    const int cur = t & 1;
+    const bool has_next = t + 1 < ntiles;
+    if (has_next) load(t + 1);
+    if (work) {
+      f32x16 s = split_rows<DP>(qs[cur], kp, lr, h);
+      f32x16 dp = split_rows<DP>(dos[cur], vp, lr, h);
+      dscore(s, dp, [&](int g, f32x4& l4, f32x4& d4) {
+        l4 = *reinterpret_cast<const f32x4*>(&ls[cur][8 * g + 4 * h]);
+        d4 = *reinterpret_cast<const f32x4*>(&ds[cur][8 * g + 4 * h]);
+      });
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ds_top = fmaxf(ds_top, fabsf(dp[r]));
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        u32x4 pp[3];
+        split_regs(s, k, pp, p_rem);
+        split_cols<DP>(dos[cur], pp, k, lane, dv);
+        split_regs(dp, k, pp, ds_rem);
+        split_cols<DP>(qs[cur], pp, k, lane, dk);
+      }
+    }
+    if (has_next) store(cur ^ 1);
+    lds_barrier();
+  }
+
+  atomicMax(&range[0], __float_as_uint(qc.top));
+  atomicMax(&range[1], __float_as_uint(dc.top));
+  atomicOr(&range[2], qc.rem | dc.rem);
+  __syncthreads();
+  const float q_top = __uint_as_float(range[0]), do_top = __uint_as_float(range[1]), d = (float)a.d, n = (float)a.R;
+  ds_top = wave_top(ds_top);
+  bool redo = !exact || (range[2] & kSplitRemBits) != 0 || split_overflows(k_top, q_top, d) ||
+              split_overflows(v_top, do_top, d) || split_overflows(1.f, do_top, n) || split_overflows(ds_top, q_top, n);
+  if (__any((p_rem & kSplitRemBits) != 0 || (ds_rem & kSplitRemBits) != 0)) {
+    const float fv = split_loss_floor(do_top, 0.f, n), fk = split_loss_floor(q_top, 0.f, n);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) redo = redo || fabsf(dv[b][r]) < fv || fabsf(dk[b][r]) < fk;
+  }
+  if (work && ntiles > 0 && __any(redo)) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) dk[b] = dv[b] = zero16();
+    for (int t = 0; t < ntiles; ++t) {
+      const int row0 = t * kTile;
+      const bool mine = row0 + lr < a.R;
+      const float* Q = mine ? a.q.p + ca_row(a.q, a, bh, row0 + lr) : nullptr;
+      const float* dO = mine ? a.dout.p + ca_row(a.dout, a, bh, row0 + lr) : nullptr;
+      f32x16 s = zero16(), dp = zero16();
+      for (int c = 0; c < a.d; c += 2) {
+        const bool in = c + h < a.d;
+        s = mfma32(in && Q ? Q[c + h] : 0.f, in && K ? K[c + h] * a.scale_log2 : 0.f, s);
+        dp = mfma32(in && dO ? dO[c + h] : 0.f, in && V ? V[c + h] : 0.f, dp);
+      }
+      dscore(s, dp, [&](int g, f32x4& l4, f32x4& d4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          l4[e] = lse_of(row0 + 8 * g + 4 * h + e);
+          d4[e] = d_of(row0 + 8 * g + 4 * h + e);
+        }
+      });
+#pragma unroll
+      for (int st = 0; st < 16; ++st) {
+        const int r = row0 + acc_row(st, h);
+        const int64_t qo = r < a.R ? ca_row(a.q, a, bh, r) : 0, oo = r < a.R ? ca_row(a.dout, a, bh, r) : 0;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const int col = b * 32 + lr;
+          const bool in = r < a.R && col < a.d;
+          dv[b] = mfma32(in ? a.dout.p[oo + col] : 0.f, s[st], dv[b]);
+          dk[b] = mfma32(in ? a.q.p[qo + col] : 0.f, dp[st], dk[b]);
+        }
+      }
+    }
+  }
+  if (kj < a.Tk) ca_store_key<DP, true>(a, bh, kj, key_ok, dk, dv, h);
 }
 
 // ------------------------------------------------------------------ host side
@@ -628,6 +1232,10 @@ void ca_plan(int64_t bh, int64_t R, int64_t Tk, int* splits, int* chunk) {
   *chunk = (int)c;
   *splits = (int)std::max<int64_t>(1, ceil_div(Tk, c));
 }
+
+// Whether the tiled passes run on the bf16 matrix cores.
+bool ca_fwd_split(const CaArgs& a) { return a.Tk > 64; }
+bool ca_bwd_split(const CaArgs& a) { return a.Tk > 64; }
 
 bool ca_shape_ok(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk) {
   const int64_t most = int64_t(1) << 24;
@@ -667,8 +1275,13 @@ int launch_fwd(const CaArgs& a, hipStream_t st) {
     else if (a.R <= 4) launch_few<4, VEC>(a, DP, st);
     else launch_few<8, VEC>(a, DP, st);
   } else {
-    const int64_t nqb = ceil_div(a.R, kBlock);
-    cross_fwd_kernel<DP, VEC><<<dim3((unsigned)(nqb * a.BH * a.splits)), dim3(kFaThreads), 0, st>>>(a);
+    const dim3 grid((unsigned)(ceil_div(a.R, kBlock) * a.BH * a.splits));
+    bool split = false;
+    if constexpr (VEC && DP >= 64) {
+      split = ca_fwd_split(a);
+      if (split) cross_fwd_split_kernel<DP, DP == 64 ? 2 : 1><<<grid, dim3(kFaThreads), 0, st>>>(a);
+    }
+    if (!split) cross_fwd_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
   }
   const int rc = launch_status();
   if (rc != AAR_OK || a.splits == 1) return rc;
@@ -679,13 +1292,18 @@ int launch_fwd(const CaArgs& a, hipStream_t st) {
 
 template <int DP, bool VEC>
 int launch_bwd(const CaArgs& a, hipStream_t st) {
+  const bool split = VEC && DP == 64 && ca_bwd_split(a);
   if (a.R > 0) {
-    cross_bwd_dq_kernel<DP, VEC><<<dim3((unsigned)(ceil_div(a.R, kBlock) * a.BH)), dim3(kFaThreads), 0, st>>>(a);
+    const dim3 grid((unsigned)(ceil_div(a.R, kBlock) * a.BH));
+    if (split) cross_bwd_dq_split_kernel<<<grid, dim3(kFaThreads), 0, st>>>(a);
+    else cross_bwd_dq_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
     const int rc = launch_status();
     if (rc != AAR_OK) return rc;
   }
   if (a.Tk == 0) return AAR_OK;
-  cross_bwd_dkdv_kernel<DP, VEC><<<dim3((unsigned)(ceil_div(a.Tk, kBlock) * a.BH)), dim3(kFaThreads), 0, st>>>(a);
+  const dim3 grid((unsigned)(ceil_div(a.Tk, kBlock) * a.BH));
+  if (split) cross_bwd_dkdv_split_kernel<<<grid, dim3(kFaThreads), 0, st>>>(a);
+  else cross_bwd_dkdv_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
   return launch_status();
 }
 
