@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <initializer_list>
+#include <type_traits>
 
 #include "bf16x3.hpp"
 #include "common.hpp"
@@ -38,7 +39,9 @@ struct CaArgs {
   float* part_o;  // [B * Hkv][splits][R][DP] normalised partial O
   float* part_l;  // [B * Hkv][splits][R] m + log2(l) of it
   int Tq, Tk, d, G, Hkv, R, BH;  // R = G * Tq rows of each of the BH = B * Hkv key/value heads
-  int splits, chunk;             // key ranges, and their keys
+  int splits, chunk;             // key ranges of the forward or of dQ, and their keys
+  float *dq_part, *dk_part, *dv_part;  // backward: [splits][BH][R][DP], [kv_splits][BH][Tk][DP] partial sums
+  int kv_splits, kv_tiles;             // ranges of query rows of dK and dV, and their tiles
   float scale, scale_log2;
 };
 
@@ -101,14 +104,31 @@ __device__ __forceinline__ void ca_store_scaled(float* row, const f32x16 (&x)[DP
   }
 }
 
+// A lane's row of dQ: to its place, or its part's.
+template <int DP, bool VEC>
+__device__ __forceinline__ void ca_store_dq(const CaArgs& a, int bh, int part, int qi, const f32x16 (&dq)[DP / 32],
+                                            int h) {
+  if (a.splits > 1) {
+    ca_store_scaled<DP, true>(a.dq_part + (((int64_t)part * a.BH + bh) * a.R + qi) * DP, dq, a.scale, DP, h);
+  } else {
+    ca_store_scaled<DP, VEC>(a.dq.p + ca_row(a.dq, a, bh, qi), dq, a.scale, a.d, h);
+  }
+}
+
 // A lane's key: dK and dV.  A masked key's zero is written as such (its sums may
 // hold 0 * inf).
 template <int DP, bool VEC>
-__device__ __forceinline__ void ca_store_key(const CaArgs& a, int bh, int kj, bool key_ok, f32x16 (&dk)[DP / 32],
-                                             f32x16 (&dv)[DP / 32], int h) {
+__device__ __forceinline__ void ca_store_key(const CaArgs& a, int bh, int part, int kj, bool key_ok,
+                                             f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP / 32], int h) {
   if (!key_ok) {
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) dk[b] = dv[b] = zero16();
+  }
+  if (a.kv_splits > 1) {
+    const int64_t at = (((int64_t)part * a.BH + bh) * a.Tk + kj) * DP;
+    ca_store_scaled<DP, true>(a.dk_part + at, dk, a.scale, DP, h);
+    ca_store_scaled<DP, true>(a.dv_part + at, dv, 1.0f, DP, h);
+    return;
   }
   ca_store_scaled<DP, VEC>(ca_head(a.dk, a, bh) + (int64_t)kj * a.dk.st, dk, a.scale, a.d, h);
   ca_store_scaled<DP, VEC>(ca_head(a.dv, a, bh) + (int64_t)kj * a.dv.st, dv, 1.0f, a.d, h);
@@ -399,8 +419,9 @@ cross_bwd_dq_kernel(const CaArgs a) {
   __shared__ __attribute__((aligned(16))) float vs[2][kTile * LD];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lr = lane & 31, h = lane >> 5;
-  const int bh = blockIdx.x % a.BH, qb = blockIdx.x / a.BH;
-  const int len = ca_len(a, bh);
+  const int bh = blockIdx.x % a.BH, rest = blockIdx.x / a.BH;
+  const int part = rest % a.splits, qb = rest / a.splits;
+  const int k0 = part * a.chunk, k1 = min(ca_len(a, bh), k0 + a.chunk);
   const float* __restrict__ K = ca_head(a.k, a, bh);
   const float* __restrict__ V = ca_head(a.v, a, bh);
   const int qi = qb * kBlock + wave * kTile + lr;
@@ -427,27 +448,27 @@ cross_bwd_dq_kernel(const CaArgs a) {
   // A row without keys, or past the end, has P = 0.
   float l2 = row_ok ? a.lse[(int64_t)bh * a.R + qi] * kLog2e : INFINITY;
   if (l2 == -INFINITY) l2 = INFINITY;
-  if (row_ok && h == 0) a.D[(int64_t)bh * a.R + qi] = dsum;
+  if (row_ok && h == 0 && part == 0) a.D[(int64_t)bh * a.R + qi] = dsum;
   f32x16 dq[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) dq[b] = zero16();
-  const int ntiles = (len + kTile - 1) / kTile;
+  const int ntiles = k1 > k0 ? (k1 - k0 + kTile - 1) / kTile : 0;
   const bool work = qb * kBlock + wave * kTile < a.R;
 
   TileCopy<DP, VEC> kc, vc;
   if (ntiles > 0) {
-    kc.load(K, a.k.st, 0, len, a.d, tid);
-    vc.load(V, a.v.st, 0, len, a.d, tid);
+    kc.load(K, a.k.st, k0, k1, a.d, tid);
+    vc.load(V, a.v.st, k0, k1, a.d, tid);
     kc.template store<LD>(ks[0], tid);
     vc.template store<LD>(vs[0], tid);
   }
   __syncthreads();
   for (int t = 0; t < ntiles; ++t) {
-    const int kv0 = t * kTile;
+    const int kv0 = k0 + t * kTile;
     const bool has_next = t + 1 < ntiles;
     if (has_next) {
-      kc.load(K, a.k.st, kv0 + kTile, len, a.d, tid);
-      vc.load(V, a.v.st, kv0 + kTile, len, a.d, tid);
+      kc.load(K, a.k.st, kv0 + kTile, k1, a.d, tid);
+      vc.load(V, a.v.st, kv0 + kTile, k1, a.d, tid);
     }
     if (work) {
       const float* kt = ks[t & 1];
@@ -465,7 +486,7 @@ cross_bwd_dq_kernel(const CaArgs a) {
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const bool in = kv0 + acc_row(r, h) < len;
+        const bool in = kv0 + acc_row(r, h) < k1;
         const float p = fast_exp2(s[r] * a.scale_log2 - l2);
         dp[r] = in ? p * (dp[r] - dsum) : 0.f;
       }
@@ -481,7 +502,7 @@ cross_bwd_dq_kernel(const CaArgs a) {
     }
     __syncthreads();
   }
-  if (row_ok) ca_store_scaled<DP, VEC>(a.dq.p + ca_row(a.dq, a, bh, qi), dq, a.scale, a.d, h);
+  if (row_ok) ca_store_dq<DP, VEC>(a, bh, part, qi, dq, h);
 }
 
 // A [32][DP] tile of query rows (TileCopy over rows that may cross heads).
@@ -516,7 +537,8 @@ cross_bwd_dkdv_kernel(const CaArgs a) {
   __shared__ __attribute__((aligned(16))) float ds[2][kTile];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lr = lane & 31, h = lane >> 5;
-  const int kb = blockIdx.x / a.BH, bh = blockIdx.x % a.BH;
+  const int bh = blockIdx.x % a.BH, rest = blockIdx.x / a.BH;
+  const int part = rest % a.kv_splits, kb = rest / a.kv_splits;
   const int len = ca_len(a, bh);
   const int kw = kb * kBlock + wave * kTile;  // the wave's first key
   const int kj = kw + lr;
@@ -535,7 +557,8 @@ cross_bwd_dkdv_kernel(const CaArgs a) {
 #pragma unroll
   for (int b = 0; b < NB; ++b) dk[b] = dv[b] = zero16();
   // a workgroup whose keys are all masked only writes zeros
-  const int ntiles = kb * kBlock < len ? (a.R + kTile - 1) / kTile : 0;
+  const int t0 = part * a.kv_tiles;
+  const int t1 = kb * kBlock < len ? min((a.R + kTile - 1) / kTile, t0 + a.kv_tiles) : t0;
 
   CaRowTile<DP, VEC> qc, dc;
   float lreg = 0.f, dreg = 0.f;
@@ -557,14 +580,14 @@ cross_bwd_dkdv_kernel(const CaArgs a) {
       ds[buf][tid] = dreg;
     }
   };
-  if (ntiles > 0) {
-    load_tile(0);
+  if (t0 < t1) {
+    load_tile(t0);
     store_tile(0);
   }
   __syncthreads();
-  for (int t = 0; t < ntiles; ++t) {
-    const int cur = t & 1;
-    const bool has_next = t + 1 < ntiles;
+  for (int t = t0; t < t1; ++t) {
+    const int cur = (t - t0) & 1;
+    const bool has_next = t + 1 < t1;
     if (has_next) load_tile(t + 1);
     if (kw < len) {
       const float* qt = qs[cur];
@@ -605,7 +628,7 @@ cross_bwd_dkdv_kernel(const CaArgs a) {
     if (has_next) store_tile(cur ^ 1);
     __syncthreads();
   }
-  if (kj < a.Tk) ca_store_key<DP, VEC>(a, bh, kj, key_ok, dk, dv, h);
+  if (kj < a.Tk) ca_store_key<DP, VEC>(a, bh, part, kj, key_ok, dk, dv, h);
 }
 
 // ---------------------------------------------------- on the bf16 matrix cores
@@ -617,6 +640,19 @@ cross_bwd_dkdv_kernel(const CaArgs a) {
 // dS^T, dO^T P, Q^T dS) read columns through the transposing LDS read, so a tile
 // that serves both is split and stored once.  P and dS are split in the registers
 // the softmax leaves them in.
+
+// A third of a pair's split (bf16_split_pair in three pieces): a and b become what
+// is left over, w[piece] the part.
+__device__ __forceinline__ void split_piece(int piece, float& a, float& b, uint32_t& w, uint32_t& rem) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  if (piece == 2) rem = __builtin_amdgcn_bitop3_b32(rem, __float_as_uint(a), __float_as_uint(b), 0xfe);
+#endif
+  w = bf16_pair(a, b);
+  if (piece < 2) {
+    a -= __uint_as_float(w << 16);
+    b -= __uint_as_float(w & 0xffff0000u);
+  }
+}
 
 // A [32][DP] tile in three planes of 32 rows; a row's 16 spare bytes put 16
 // consecutive rows' 128-bit reads on distinct banks.
@@ -647,6 +683,24 @@ struct SplitTile {
         f[i][g] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (p && c + 4 * g < d) f[i][g] = *reinterpret_cast<const f32x4*>(p + c + 4 * g);
       }
+    }
+  }
+  // Piece n of 12 kPer of `store`: a third of a pair's split, the stores after a
+  // unit's last.
+  u32x4 w[3];
+  __device__ __forceinline__ void store_piece(int n, char* s, int tid) {
+    const int i = n / 12, e = n / 3 % 4, piece = n % 3;
+    float u = f[i][e >> 1][2 * (e & 1)], v = f[i][e >> 1][2 * (e & 1) + 1];
+    if (piece == 0) top = fmaxf(fmaxf(top, fabsf(u)), fabsf(v));
+    uint32_t part;
+    split_piece(piece, u, v, part, rem);
+    w[piece][e] = part;
+    f[i][e >> 1][2 * (e & 1)] = u;
+    f[i][e >> 1][2 * (e & 1) + 1] = v;
+    if (e == 3 && piece == 2) {
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+        *reinterpret_cast<u32x4*>(s + p * kPlane + row(i, tid) * kRow + 2 * col(i, tid)) = w[p];
     }
   }
   __device__ __forceinline__ void store(char* s, int tid) {
@@ -684,54 +738,100 @@ __device__ __forceinline__ void read_columns(const char* p, uint32_t& lo, uint32
 }
 
 // acc += tile . B over the head dim: the tile's 32 rows are the output's rows,
-// B's columns (b[c][part], lane = column) the output's.
-template <int DP>
-__device__ __forceinline__ f32x16 split_rows(const char* s, const u32x4 (&b)[DP / 16][3], int lr, int h) {
+// B's columns (b[c][part], lane = column) the output's.  A wave issues in order, so
+// the vector work that is to run beside the matrix ops stands between them:
+// `slot(i)` is called after matrix op i and its instructions stay there.  A step's
+// operands are read a step ahead.
+struct NoSlots {
+  __device__ __forceinline__ void operator()(int) const {}
+};
+
+template <int DP, typename Slot = NoSlots>
+__device__ __forceinline__ f32x16 split_rows(const char* s, const u32x4 (&b)[DP / 16][3], int lr, int h,
+                                             Slot slot = Slot()) {
+  constexpr bool kPinned = !std::is_same<Slot, NoSlots>::value;
   f32x16 acc = zero16();
   const char* p = s + lr * SplitTile<DP>::kRow + 16 * h;
+  constexpr int kAhead = kPinned ? 1 : 0;
+  u32x4 x[1 + kAhead][3];
+  auto read = [&](int c) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) x[c & kAhead][i] = *reinterpret_cast<const u32x4*>(p + i * SplitTile<DP>::kPlane + 32 * c);
+  };
+  if (kPinned) read(0);
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) {
-    u32x4 x[3];
+    if (c + kAhead < DP / 16) read(c + kAhead);
 #pragma unroll
-    for (int i = 0; i < 3; ++i) x[i] = *reinterpret_cast<const u32x4*>(p + i * SplitTile<DP>::kPlane + 32 * c);
-#pragma unroll
-    for (int i = 0; i < kSplitProducts; ++i) acc = mfma_bf16(x[kSplitA[i]], b[c][kSplitB[i]], acc);
+    for (int i = 0; i < kSplitProducts; ++i) {
+      acc = mfma_bf16(x[c & kAhead][kSplitA[i]], b[c][kSplitB[i]], acc);
+      if (kPinned) sched_fence();
+      slot(c * kSplitProducts + i);
+      if (kPinned) sched_fence();
+    }
   }
   return acc;
 }
 
+// acc[b] += tile^T . P over rows 16 K0 .. 16 K1 - 1 of the tile: column 32 b + lr of
+// it, its rows in the order of the accumulator registers that pp[k] (rows 16 k ..)
+// was made of.  `slot` as above.
+template <int DP, int K0, int K1, typename Slot = NoSlots>
+__device__ __forceinline__ void split_cols(const char* s, const u32x4 (&pp)[2][3], int lane, f32x16 (&acc)[DP / 32],
+                                           Slot slot = Slot()) {
+  using T = SplitTile<DP>;
+  constexpr bool kPinned = !std::is_same<Slot, NoSlots>::value;
+  constexpr int NB = DP / 32;
+  const int h = lane >> 5, j = lane & 15;
+  const char* p = s + (4 * h + (j >> 2)) * T::kRow + 2 * (16 * ((lane >> 4) & 1) + 4 * (j & 3));
+  constexpr int kAhead = kPinned ? 1 : 0;
+  u32x4 x[1 + kAhead][3];
+  auto read = [&](int g) {  // block g % NB of row half g / NB
+    const char* at = p + 16 * (g / NB) * T::kRow + 64 * (g % NB);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      uint32_t w[4];
+      read_columns(at + i * T::kPlane, w[0], w[1]);
+      read_columns(at + i * T::kPlane + 8 * T::kRow, w[2], w[3]);
+      x[g & kAhead][i] = u32x4{w[0], w[1], w[2], w[3]};
+    }
+  };
+  if (kPinned) read(K0 * NB);
+#pragma unroll
+  for (int g = K0 * NB; g < K1 * NB; ++g) {
+    if (g + kAhead < K1 * NB) read(g + kAhead);
+#pragma unroll
+    for (int i = 0; i < kSplitProducts; ++i) {
+      acc[g % NB] = mfma_bf16(x[g & kAhead][kSplitA[i]], pp[g / NB][kSplitB[i]], acc[g % NB]);
+      if (kPinned) sched_fence();
+      slot((g - K0 * NB) * kSplitProducts + i);
+      if (kPinned) sched_fence();
+    }
+  }
+}
+
 // The three parts of accumulator registers 8 k .. 8 k + 7, the right operand of
-// the products over the tile's rows.
-__device__ __forceinline__ void split_regs(const f32x16& s, int k, u32x4 (&pp)[3], uint32_t& rem) {
+// the products over rows 16 k .. of the tile.
+__device__ __forceinline__ void split_regs(const f32x16& s, int k, u32x4 (&pp)[2][3], uint32_t& rem) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     uint32_t w[3];
     bf16_split_pair(s[8 * k + 2 * e], s[8 * k + 2 * e + 1], w, rem);
 #pragma unroll
-    for (int p = 0; p < 3; ++p) pp[p][e] = w[p];
+    for (int p = 0; p < 3; ++p) pp[k][p][e] = w[p];
   }
 }
 
-// acc[b] += tile^T . (rows 16 k .. 16 k + 15 of P): column 32 b + lr of the tile,
-// its rows in the order of the accumulator registers that pp was made of.
-template <int DP>
-__device__ __forceinline__ void split_cols(const char* s, const u32x4 (&pp)[3], int k, int lane, f32x16 (&acc)[DP / 32]) {
-  using T = SplitTile<DP>;
-  const int h = lane >> 5, j = lane & 15;
-  const char* p = s + (16 * k + 4 * h + (j >> 2)) * T::kRow + 2 * (16 * ((lane >> 4) & 1) + 4 * (j & 3));
-#pragma unroll
-  for (int b = 0; b < DP / 32; ++b) {
-    u32x4 x[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      uint32_t w[4];
-      read_columns(p + i * T::kPlane + 64 * b, w[0], w[1]);
-      read_columns(p + i * T::kPlane + 64 * b + 8 * T::kRow, w[2], w[3]);
-      x[i] = u32x4{w[0], w[1], w[2], w[3]};
-    }
-#pragma unroll
-    for (int i = 0; i < kSplitProducts; ++i) acc[b] = mfma_bf16(x[kSplitA[i]], pp[kSplitB[i]], acc[b]);
-  }
+// Piece n of 24 of splitting registers s[0 .. 15] (a pair in three) into the right
+// operands pp of the products over the tile's rows.
+__device__ __forceinline__ void regs_piece(int n, f32x16& s, u32x4 (&pp)[2][3], uint32_t& rem) {
+  const int e = n / 3, piece = n % 3;
+  float u = s[2 * e], v = s[2 * e + 1];
+  uint32_t w;
+  split_piece(piece, u, v, w, rem);
+  s[2 * e] = u;
+  s[2 * e + 1] = v;
+  pp[e / 4][piece][e % 4] = w;
 }
 
 // A lane's row (its half's octets of each 16 columns) times f, in parts.
@@ -767,13 +867,13 @@ __device__ __forceinline__ float wave_top(float v) {
 
 // Forward.  The running maximum m of a row follows its scores only when they pass
 // it by 2^8 (the sums stay far from fp32's end), so O is rarely rescaled.
-template <int DP, int STAGES>
-__global__ void __launch_bounds__(kFaThreads, 2)
+template <int DP>
+__global__ void __launch_bounds__(kFaThreads, DP == 64 ? 2 : 1)
 cross_fwd_split_kernel(const CaArgs a) {
   using Tile = SplitTile<DP>;
   constexpr int NB = DP / 32;
-  __shared__ __attribute__((aligned(16))) char ks[STAGES][Tile::kBytes];
-  __shared__ __attribute__((aligned(16))) char vs[STAGES][Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) char ks[2][Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) char vs[2][Tile::kBytes];
   __shared__ uint32_t range[3];  // largest magnitude of K, of V (as bits), what their splits left over
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lr = lane & 31, h = lane >> 5;
@@ -800,8 +900,9 @@ cross_fwd_split_kernel(const CaArgs a) {
   for (int b = 0; b < NB; ++b) o[b] = zero16();
   float m = -INFINITY, l = 0.f;
 
-  // Online softmax of a tile of log2 scores: s becomes P, O is rescaled where m moves.
-  auto soft = [&](f32x16& s, int kv0) {
+  // A tile of log2 scores before its exponentials: what is masked, and m with what
+  // has been summed so far where m moves.
+  auto follow = [&](f32x16& s, int kv0) {
     if (kv0 + kTile > k1) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
@@ -822,6 +923,8 @@ cross_fwd_split_kernel(const CaArgs a) {
         for (int r = 0; r < 16; ++r) o[b][r] *= alpha;
       }
     }
+  };
+  auto exponentials = [&](f32x16& s) {
     const float mu = m == -INFINITY ? 0.f : m;
     float ps = 0.f;
 #pragma unroll
@@ -831,53 +934,78 @@ cross_fwd_split_kernel(const CaArgs a) {
     }
     l += half_swap_sum(ps);
   };
-  auto compute = [&](const char* kt, const char* vt, int kv0) {
-    f32x16 s = split_rows<DP>(kt, qp, lr, h);
-    soft(s, kv0);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      u32x4 pp[3];
-      split_regs(s, k, pp, p_rem);
-      split_cols<DP>(vt, pp, k, lane, o);
-    }
-  };
 
   const int ntiles = k1 > k0 ? (k1 - k0 + kTile - 1) / kTile : 0;
-  Tile kc, vc;
-  auto load = [&](int t) {
+  Tile kc[2], vc[2];
+  auto load_k = [&](Tile& x, int t) {
     const int row0 = k0 + t * kTile;
-    kc.load(a.d, tid, [&](int r) { return row0 + r < k1 ? K + (int64_t)(row0 + r) * a.k.st : nullptr; });
-    vc.load(a.d, tid, [&](int r) { return row0 + r < k1 ? V + (int64_t)(row0 + r) * a.v.st : nullptr; });
+    x.load(a.d, tid, [&](int r) { return row0 + r < k1 ? K + (int64_t)(row0 + r) * a.k.st : nullptr; });
   };
-  if (ntiles > 0) load(0);
-  if (STAGES == 2 && ntiles > 0) {
-    kc.store(ks[0], tid);
-    vc.store(vs[0], tid);
+  auto load_v = [&](Tile& x, int t) {
+    const int row0 = k0 + t * kTile;
+    x.load(a.d, tid, [&](int r) { return row0 + r < k1 ? V + (int64_t)(row0 + r) * a.v.st : nullptr; });
+  };
+  f32x16 s = zero16();
+  if (ntiles > 0) {
+    load_k(kc[0], 0);
+    load_v(vc[0], 0);
+    load_k(kc[1], 1);
+    kc[0].store(ks[0], tid);
+    vc[0].store(vs[0], tid);
+    load_k(kc[0], 2);
+    load_v(vc[0], 1);
+    kc[1].store(ks[1], tid);
   }
   lds_barrier();
-  for (int t = 0; t < ntiles; ++t) {
-    const bool has_next = t + 1 < ntiles;
-    if (STAGES == 1) {
-      kc.store(ks[0], tid);
-      vc.store(vs[0], tid);
-      lds_barrier();
-    }
-    if (has_next) load(t + 1);
-    if (work) compute(ks[STAGES == 2 ? t & 1 : 0], vs[STAGES == 2 ? t & 1 : 0], k0 + t * kTile);
-    if (STAGES == 2 && has_next) {
-      kc.store(ks[(t + 1) & 1], tid);
-      vc.store(vs[(t + 1) & 1], tid);
+  if (work && ntiles > 0) s = split_rows<DP>(ks[0], qp, lr, h);
+  lds_barrier();  // K tile 0's buffer is refilled in iteration 0
+  // Iteration t: K tile t + 1 and V tile t are in LDS; K t + 2 and V t + 1, loaded an
+  // iteration ago, are staged (kn, vn), K t + 3 and V t + 2 are sent for (kl, vl).
+  auto step = [&](int t, Tile& kn, Tile& vn, Tile& kl, Tile& vl) {
+    load_k(kl, t + 3);
+    load_v(vl, t + 2);
+    if (work) {
+      follow(s, k0 + t * kTile);
+      const float mu = m == -INFINITY ? 0.f : m;
+      float ps = 0.f;
+      u32x4 pp[2][3];
+      constexpr int kEach = DP / 64;  // matrix ops per piece
+      const f32x16 next = split_rows<DP>(ks[(t + 1) & 1], qp, lr, h, [&](int i) {
+        if (i % kEach != 0) return;
+        const int n = i / kEach, e = n / 3;
+        if (n % 3 == 0) {
+          s[2 * e] = fast_exp2(s[2 * e] - mu);
+          s[2 * e + 1] = fast_exp2(s[2 * e + 1] - mu);
+          ps += s[2 * e];
+          ps += s[2 * e + 1];
+        }
+        regs_piece(n, s, pp, p_rem);
+      });
+      l += half_swap_sum(ps);
+      split_cols<DP, 0, 2>(vs[t & 1], pp, lane, o, [&](int i) {
+        constexpr int kHalf = 12 * Tile::kPer;
+        if (i < kHalf) kn.store_piece(i, ks[t & 1], tid);
+        else vn.store_piece(i - kHalf, vs[(t + 1) & 1], tid);
+      });
+      s = next;
+    } else {
+      kn.store(ks[t & 1], tid);
+      vn.store(vs[(t + 1) & 1], tid);
     }
     lds_barrier();
+  };
+  for (int t = 0; t < ntiles; t += 2) {
+    step(t, kc[0], vc[0], kc[1], vc[1]);
+    if (t + 1 < ntiles) step(t + 1, kc[1], vc[1], kc[0], vc[0]);
   }
 
   // What the split does not cover: sums that might overflow, an element of q, K or
   // V that is not held exactly, and probabilities below 2^-110 where O is so
   // small that it feels them.  Such a wave's rows are redone with the fp32
   // instruction, straight from HBM.
-  atomicMax(&range[0], __float_as_uint(kc.top));  // >= 0: ordered as their bits
-  atomicMax(&range[1], __float_as_uint(vc.top));
-  atomicOr(&range[2], kc.rem | vc.rem);
+  atomicMax(&range[0], __float_as_uint(fmaxf(kc[0].top, kc[1].top)));  // >= 0: ordered as their bits
+  atomicMax(&range[1], __float_as_uint(fmaxf(vc[0].top, vc[1].top)));
+  atomicOr(&range[2], kc[0].rem | kc[1].rem | vc[0].rem | vc[1].rem);
   __syncthreads();
   const float v_top = __uint_as_float(range[1]), n = (float)(k1 - k0);
   bool redo = !q_exact || (range[2] & kSplitRemBits) != 0 ||
@@ -903,7 +1031,8 @@ cross_fwd_split_kernel(const CaArgs a) {
         const float qf = on && Q ? Q[c + h] * a.scale_log2 : 0.f;
         s = mfma32(kf, qf, s);
       }
-      soft(s, kv0);
+      follow(s, kv0);
+      exponentials(s);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const int col = b * 32 + lr;
@@ -929,8 +1058,9 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
   __shared__ uint32_t range[3];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lr = lane & 31, h = lane >> 5;
-  const int bh = blockIdx.x % a.BH, qb = blockIdx.x / a.BH;
-  const int len = ca_len(a, bh);
+  const int bh = blockIdx.x % a.BH, rest = blockIdx.x / a.BH;
+  const int part = rest % a.splits, qb = rest / a.splits;
+  const int k0 = part * a.chunk, k1 = min(ca_len(a, bh), k0 + a.chunk);
   const float* __restrict__ K = ca_head(a.k, a, bh);
   const float* __restrict__ V = ca_head(a.v, a, bh);
   const int qi = qb * kBlock + wave * kTile + lr;
@@ -954,7 +1084,7 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
   dsum = half_swap_sum(dsum);
   float l2 = row_ok ? a.lse[(int64_t)bh * a.R + qi] * kLog2e : INFINITY;
   if (l2 == -INFINITY) l2 = INFINITY;  // a row without keys has P = 0
-  if (row_ok && h == 0) a.D[(int64_t)bh * a.R + qi] = dsum;
+  if (row_ok && h == 0 && part == 0) a.D[(int64_t)bh * a.R + qi] = dsum;
 
   u32x4 qp[DP / 16][3], dop[DP / 16][3];
   float q_top = 0.f, do_top = 0.f, ds_top = 0.f;
@@ -973,15 +1103,15 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const float x = fast_exp2(s[r] - l2) * (dp[r] - dsum);
-      dp[r] = kv0 + acc_row(r, h) < len ? x : 0.f;
+      dp[r] = kv0 + acc_row(r, h) < k1 ? x : 0.f;
     }
   };
-  const int ntiles = (len + kTile - 1) / kTile;
+  const int ntiles = k1 > k0 ? (k1 - k0 + kTile - 1) / kTile : 0;
   Tile kc, vc;
   auto load = [&](int t) {
-    const int row0 = t * kTile;
-    kc.load(a.d, tid, [&](int r) { return row0 + r < len ? K + (int64_t)(row0 + r) * a.k.st : nullptr; });
-    vc.load(a.d, tid, [&](int r) { return row0 + r < len ? V + (int64_t)(row0 + r) * a.v.st : nullptr; });
+    const int row0 = k0 + t * kTile;
+    kc.load(a.d, tid, [&](int r) { return row0 + r < k1 ? K + (int64_t)(row0 + r) * a.k.st : nullptr; });
+    vc.load(a.d, tid, [&](int r) { return row0 + r < k1 ? V + (int64_t)(row0 + r) * a.v.st : nullptr; });
   };
   if (ntiles > 0) {
     load(0);
@@ -995,15 +1125,14 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
     if (work) {
       const f32x16 s = split_rows<DP>(ks[t & 1], qp, lr, h);
       f32x16 dp = split_rows<DP>(vs[t & 1], dop, lr, h);
-      dscore(s, dp, t * kTile);
+      dscore(s, dp, k0 + t * kTile);
 #pragma unroll
       for (int r = 0; r < 16; ++r) ds_top = fmaxf(ds_top, fabsf(dp[r]));
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        u32x4 pp[3];
-        split_regs(dp, k, pp, ds_rem);
-        split_cols<DP>(ks[t & 1], pp, k, lane, dq);
-      }
+      u32x4 pp[2][3];
+      split_regs(dp, 0, pp, ds_rem);
+      split_cols<DP, 0, 1>(ks[t & 1], pp, lane, dq);
+      split_regs(dp, 1, pp, ds_rem);
+      split_cols<DP, 1, 2>(ks[t & 1], pp, lane, dq);
     }
     if (has_next) {
       kc.store(ks[(t + 1) & 1], tid);
@@ -1017,12 +1146,12 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
   atomicMax(&range[1], __float_as_uint(vc.top));
   atomicOr(&range[2], kc.rem | vc.rem);
   __syncthreads();
-  const float k_top = __uint_as_float(range[0]), d = (float)a.d;
+  const float k_top = __uint_as_float(range[0]), d = (float)a.d, n = (float)(k1 - k0);
   ds_top = wave_top(ds_top);
   bool redo = !exact || (range[2] & kSplitRemBits) != 0 || split_overflows(q_top, k_top, d) ||
-              split_overflows(do_top, __uint_as_float(range[1]), d) || split_overflows(ds_top, k_top, (float)len);
+              split_overflows(do_top, __uint_as_float(range[1]), d) || split_overflows(ds_top, k_top, n);
   if (__any((ds_rem & kSplitRemBits) != 0)) {
-    const float floor = split_loss_floor(k_top, 0.f, (float)len);
+    const float floor = split_loss_floor(k_top, 0.f, n);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -1032,10 +1161,10 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) dq[b] = zero16();
     for (int t = 0; t < ntiles; ++t) {
-      const int kv0 = t * kTile;
+      const int kv0 = k0 + t * kTile;
       f32x16 s = zero16(), dp = zero16();
       for (int c = 0; c < a.d; c += 2) {
-        const bool in = c + h < a.d, key = in && kv0 + lr < len;
+        const bool in = c + h < a.d, key = in && kv0 + lr < k1;
         s = mfma32(key ? K[(int64_t)(kv0 + lr) * a.k.st + c + h] : 0.f, in && Q ? Q[c + h] * a.scale_log2 : 0.f, s);
         dp = mfma32(key ? V[(int64_t)(kv0 + lr) * a.v.st + c + h] : 0.f, in && dO ? dO[c + h] : 0.f, dp);
       }
@@ -1046,12 +1175,12 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
 #pragma unroll
         for (int st = 0; st < 16; ++st) {
           const int row = kv0 + acc_row(st, h);
-          dq[b] = mfma32(row < len && col < a.d ? K[(int64_t)row * a.k.st + col] : 0.f, dp[st], dq[b]);
+          dq[b] = mfma32(row < k1 && col < a.d ? K[(int64_t)row * a.k.st + col] : 0.f, dp[st], dq[b]);
         }
       }
     }
   }
-  if (row_ok) ca_store_scaled<DP, true>(a.dq.p + ca_row(a.dq, a, bh, qi), dq, a.scale, a.d, h);
+  if (row_ok) ca_store_dq<DP, true>(a, bh, part, qi, dq, h);
 }
 
 // dK and dV.
@@ -1066,7 +1195,8 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
   __shared__ uint32_t range[3];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lr = lane & 31, h = lane >> 5;
-  const int kb = blockIdx.x / a.BH, bh = blockIdx.x % a.BH;
+  const int bh = blockIdx.x % a.BH, rest = blockIdx.x / a.BH;
+  const int part = rest % a.kv_splits, kb = rest / a.kv_splits;
   const int len = ca_len(a, bh);
   const int kw = kb * kBlock + wave * kTile;
   const int kj = kw + lr;
@@ -1086,7 +1216,8 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
   f32x16 dk[NB], dv[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) dk[b] = dv[b] = zero16();
-  const int ntiles = kb * kBlock < len ? (a.R + kTile - 1) / kTile : 0;
+  const int t0 = part * a.kv_tiles;
+  const int t1 = kb * kBlock < len ? min((a.R + kTile - 1) / kTile, t0 + a.kv_tiles) : t0;
 
   // P (in s) and dS (in dp) of a tile; `stat(g, l4, d4)` gives the lse and D of rows 8 g + 4 h ..
   auto dscore = [&](f32x16& s, f32x16& dp, auto stat) {
@@ -1127,14 +1258,14 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
       ds[buf][tid] = dreg;
     }
   };
-  if (ntiles > 0) {
-    load(0);
+  if (t0 < t1) {
+    load(t0);
     store(0);
   }
   lds_barrier();
-  for (int t = 0; t < ntiles; ++t) {
-    const int cur = t & 1;
-    const bool has_next = t + 1 < ntiles;
+  for (int t = t0; t < t1; ++t) {
+    const int cur = (t - t0) & 1;
+    const bool has_next = t + 1 < t1;
     if (has_next) load(t + 1);
     if (work) {
       f32x16 s = split_rows<DP>(qs[cur], kp, lr, h);
@@ -1145,14 +1276,15 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
       });
 #pragma unroll
       for (int r = 0; r < 16; ++r) ds_top = fmaxf(ds_top, fabsf(dp[r]));
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        u32x4 pp[3];
-        split_regs(s, k, pp, p_rem);
-        split_cols<DP>(dos[cur], pp, k, lane, dv);
-        split_regs(dp, k, pp, ds_rem);
-        split_cols<DP>(qs[cur], pp, k, lane, dk);
-      }
+      u32x4 pp[2][3];
+      split_regs(s, 0, pp, p_rem);
+      split_cols<DP, 0, 1>(dos[cur], pp, lane, dv);
+      split_regs(dp, 0, pp, ds_rem);
+      split_cols<DP, 0, 1>(qs[cur], pp, lane, dk);
+      split_regs(s, 1, pp, p_rem);
+      split_cols<DP, 1, 2>(dos[cur], pp, lane, dv);
+      split_regs(dp, 1, pp, ds_rem);
+      split_cols<DP, 1, 2>(qs[cur], pp, lane, dk);
     }
     if (has_next) store(cur ^ 1);
     lds_barrier();
@@ -1173,10 +1305,10 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) redo = redo || fabsf(dv[b][r]) < fv || fabsf(dk[b][r]) < fk;
   }
-  if (work && ntiles > 0 && __any(redo)) {
+  if (work && t0 < t1 && __any(redo)) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) dk[b] = dv[b] = zero16();
-    for (int t = 0; t < ntiles; ++t) {
+    for (int t = t0; t < t1; ++t) {
       const int row0 = t * kTile;
       const bool mine = row0 + lr < a.R;
       const float* Q = mine ? a.q.p + ca_row(a.q, a, bh, row0 + lr) : nullptr;
@@ -1208,7 +1340,39 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
       }
     }
   }
-  if (kj < a.Tk) ca_store_key<DP, true>(a, bh, kj, key_ok, dk, dv, h);
+  if (kj < a.Tk) ca_store_key<DP, true>(a, bh, part, kj, key_ok, dk, dv, h);
+}
+
+// The parts of dQ (rows [0, n_q) of DP / 4 lanes), then of dK and dV, summed in order.
+template <int DP, bool VEC>
+__global__ void __launch_bounds__(256)
+cross_bwd_sum_kernel(const CaArgs a) {
+  constexpr int kLanes = DP / 4;
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  int64_t row = u / kLanes;
+  const int c = (int)(u % kLanes) * 4;
+  const int64_t nq = a.splits > 1 ? (int64_t)a.BH * a.R : 0, nk = a.kv_splits > 1 ? (int64_t)a.BH * a.Tk : 0;
+  const float* part = a.dq_part;
+  float* out;
+  int64_t n = nq;
+  int splits = a.splits;
+  if (row < nq) {
+    out = a.dq.p + ca_row(a.dq, a, (int)(row / a.R), (int)(row % a.R));
+  } else {
+    row -= nq;
+    n = nk;
+    splits = a.kv_splits;
+    if (row >= 2 * nk) return;
+    const bool v = row >= nk;
+    if (v) row -= nk;
+    part = v ? a.dv_part : a.dk_part;
+    const FaOut& x = v ? a.dv : a.dk;
+    out = ca_head(x, a, (int)(row / a.Tk)) + row % a.Tk * x.st;
+  }
+  if (c >= a.d) return;
+  f32x4 s = *reinterpret_cast<const f32x4*>(part + row * DP + c);
+  for (int p = 1; p < splits; ++p) s += *reinterpret_cast<const f32x4*>(part + (p * n + row) * DP + c);
+  store4<VEC>(out + c, s, a.d - c);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1218,19 +1382,56 @@ constexpr int kMaxSplits = 64;
 
 int pad_dim(int64_t d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
 
-// Key ranges a forward is split into, and their keys.  Enough workgroups to fill
-// the GPU (four to a CU for the few-row kernel, which lives on loads in flight,
-// two for the tiled one), ranges of at least 64 (128) keys.
-void ca_plan(int64_t bh, int64_t R, int64_t Tk, int* splits, int* chunk) {
-  const int64_t cus = device_cu_count();
-  const bool few = R <= kFewRows;
-  const int64_t grid = bh * (few ? 1 : ceil_div(R, kBlock));
-  const int64_t want = few ? 4 * cus : 2 * cus, least = few ? 64 : 128;
-  int64_t s = grid * 3 / 2 >= want ? 1 : ceil_div(want, grid);
-  s = std::max<int64_t>(1, std::min<int64_t>({s, Tk / least, (int64_t)kMaxSplits}));
-  const int64_t c = ceil_div(ceil_div(std::max<int64_t>(Tk, 1), s), kTile) * kTile;
-  *chunk = (int)c;
-  *splits = (int)std::max<int64_t>(1, ceil_div(Tk, c));
+// Ranges a pass's loop of `tiles` is split into, for grids that do not fill the
+// GPU's `slots` workgroups.  A tile takes about `us` microseconds and a workgroup
+// another two of its own, and parts cost a launch and their bytes twice; the fewest
+// microseconds win.  (Full grids gain nothing from whole rounds: 768 workgroups of
+// 512 slots as two parts each, three rounds of half the length, measured 579 us
+// against 565, for the matrix cores are at their power limit either way.)
+int ca_splits(int64_t grid, int64_t slots, int64_t tiles, int64_t least, double us, double part_bytes) {
+  int best = 1;
+  double cost = 0;
+  if (grid >= slots) return 1;
+  for (int s = 1; s <= kMaxSplits && (s == 1 || tiles / s >= least); ++s) {
+    const double t = std::max(1.0, (double)(grid * s) / slots) * ((double)ceil_div(tiles, s) * us + 2.0) +
+                     (s > 1 ? 4.0 + s * part_bytes / 2.0e6 : 0.0);
+    if (s == 1 || t < 0.97 * cost) {
+      best = s;
+      cost = t;
+    }
+  }
+  return best;
+}
+
+// Key ranges of a forward, and their keys.  The few-row kernel lives on loads in
+// flight and takes four workgroups to a CU, in ranges of at least 64 keys.
+void ca_plan(int64_t bh, int64_t R, int64_t Tk, int64_t d, int* splits, int* chunk) {
+  const int64_t cus = device_cu_count(), tiles = ceil_div(Tk, kTile);
+  int64_t s;
+  if (R <= kFewRows) {
+    s = bh * 3 / 2 >= 4 * cus ? 1 : ceil_div(4 * cus, bh);
+    s = std::max<int64_t>(1, std::min<int64_t>({s, Tk / 64, (int64_t)kMaxSplits}));
+  } else {
+    s = ca_splits(bh * ceil_div(R, kBlock), 2 * cus, tiles, 4, d > 64 ? 4.0 : 2.0, (double)bh * R * pad_dim(d) * 4);
+  }
+  const int64_t c = ceil_div(std::max<int64_t>(tiles, 1), s);
+  *chunk = (int)(c * kTile);
+  *splits = (int)std::max<int64_t>(1, ceil_div(tiles, c));
+}
+
+// Key ranges of dQ and ranges of query rows of dK and dV.
+void ca_bwd_plan(CaArgs& a) {
+  const int64_t cus = device_cu_count(), kt = ceil_div((int64_t)a.Tk, kTile), qt = ceil_div((int64_t)a.R, kTile);
+  const int64_t slots = (a.d > 64 ? 1 : 2) * cus, dp = pad_dim(a.d);
+  int64_t s = ca_splits(a.BH * ceil_div((int64_t)a.R, kBlock), slots, kt, 4, a.d > 64 ? 6.0 : 3.0,
+                        (double)a.BH * a.R * dp * 4);
+  int64_t c = ceil_div(std::max<int64_t>(kt, 1), s);
+  a.chunk = (int)(c * kTile);
+  a.splits = (int)std::max<int64_t>(1, ceil_div(kt, c));
+  s = ca_splits(a.BH * ceil_div((int64_t)a.Tk, kBlock), slots, qt, 4, a.d > 64 ? 10.0 : 5.0, (double)a.BH * a.Tk * dp * 8);
+  c = ceil_div(std::max<int64_t>(qt, 1), s);
+  a.kv_tiles = (int)c;
+  a.kv_splits = (int)std::max<int64_t>(1, ceil_div(qt, c));
 }
 
 // Whether the tiled passes run on the bf16 matrix cores.
@@ -1279,7 +1480,7 @@ int launch_fwd(const CaArgs& a, hipStream_t st) {
     bool split = false;
     if constexpr (VEC && DP >= 64) {
       split = ca_fwd_split(a);
-      if (split) cross_fwd_split_kernel<DP, DP == 64 ? 2 : 1><<<grid, dim3(kFaThreads), 0, st>>>(a);
+      if (split) cross_fwd_split_kernel<DP><<<grid, dim3(kFaThreads), 0, st>>>(a);
     }
     if (!split) cross_fwd_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
   }
@@ -1294,16 +1495,20 @@ template <int DP, bool VEC>
 int launch_bwd(const CaArgs& a, hipStream_t st) {
   const bool split = VEC && DP == 64 && ca_bwd_split(a);
   if (a.R > 0) {
-    const dim3 grid((unsigned)(ceil_div(a.R, kBlock) * a.BH));
+    const dim3 grid((unsigned)(ceil_div(a.R, kBlock) * a.BH * a.splits));
     if (split) cross_bwd_dq_split_kernel<<<grid, dim3(kFaThreads), 0, st>>>(a);
     else cross_bwd_dq_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
     const int rc = launch_status();
     if (rc != AAR_OK) return rc;
   }
   if (a.Tk == 0) return AAR_OK;
-  const dim3 grid((unsigned)(ceil_div(a.Tk, kBlock) * a.BH));
+  const dim3 grid((unsigned)(ceil_div(a.Tk, kBlock) * a.BH * a.kv_splits));
   if (split) cross_bwd_dkdv_split_kernel<<<grid, dim3(kFaThreads), 0, st>>>(a);
   else cross_bwd_dkdv_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
+  const int rc = launch_status();
+  const int64_t rows = (a.splits > 1 ? (int64_t)a.BH * a.R : 0) + (a.kv_splits > 1 ? 2 * (int64_t)a.BH * a.Tk : 0);
+  if (rc != AAR_OK || rows == 0) return rc;
+  cross_bwd_sum_kernel<DP, VEC><<<dim3((unsigned)ceil_div(rows * (DP / 4), (int64_t)256)), dim3(256), 0, st>>>(a);
   return launch_status();
 }
 
@@ -1330,6 +1535,18 @@ int ca_check(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t 
 
 size_t part_o_bytes(int64_t bh, int64_t R, int64_t d, int splits) {
   return (size_t)bh * splits * (size_t)R * pad_dim(d) * sizeof(float);
+}
+
+// Where the backward's workspace holds item i (D, dQ's parts, dK's, dV's); 4: its end.
+size_t bwd_bytes(const CaArgs& a, int i) {
+  const size_t dp = pad_dim(a.d), bh = a.BH;
+  const size_t size[4] = {(bh * a.R * sizeof(float) + 15) / 16 * 16,
+                          a.splits > 1 ? a.splits * bh * a.R * dp * sizeof(float) : 0,
+                          a.kv_splits > 1 ? a.kv_splits * bh * a.Tk * dp * sizeof(float) : 0,
+                          a.kv_splits > 1 ? a.kv_splits * bh * a.Tk * dp * sizeof(float) : 0};
+  size_t at = 0;
+  for (int k = 0; k < i; ++k) at += size[k];
+  return at;
 }
 
 CaArgs ca_args(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d, const int64_t* lens, float* lse,
@@ -1359,7 +1576,7 @@ extern "C" {
 size_t aar_cross_attn_fwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d) {
   if (ca_check(B, H, Hkv, Tq, Tk, d) != AAR_OK || B == 0 || H == 0 || Tq == 0 || Tk == 0) return 0;
   int splits, chunk;
-  ca_plan(B * Hkv, H / Hkv * Tq, Tk, &splits, &chunk);
+  ca_plan(B * Hkv, H / Hkv * Tq, Tk, d, &splits, &chunk);
   if (splits == 1) return 0;
   return part_o_bytes(B * Hkv, H / Hkv * Tq, d, splits) + (size_t)B * H * Tq * splits * sizeof(float);
 }
@@ -1376,7 +1593,7 @@ int aar_cross_attn_fwd_f32(const float* q, const float* k, const float* v, const
   a.k = ca_in(k, strides + 3);
   a.v = ca_in(v, strides + 6);
   a.o = ca_out(o, strides + 9);
-  ca_plan(a.BH, a.R, Tk, &a.splits, &a.chunk);
+  ca_plan(a.BH, a.R, Tk, d, &a.splits, &a.chunk);
   if (a.splits > 1) {
     const size_t need = aar_cross_attn_fwd_workspace_bytes(B, H, Hkv, Tq, Tk, d);
     if (!workspace || !aligned16(workspace) || workspace_bytes < need) return AAR_EWORKSPACE;
@@ -1386,10 +1603,12 @@ int aar_cross_attn_fwd_f32(const float* q, const float* k, const float* v, const
   return ca_dispatch<true>(a, ca_vec_ok(d, {q, k, v, o}, strides, 12), as_stream(stream));
 }
 
-// D of every query row
+// D of every query row, then the parts of dQ, dK and dV
 size_t aar_cross_attn_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d) {
-  if (ca_check(B, H, Hkv, Tq, Tk, d) != AAR_OK) return 0;
-  return (size_t)B * H * Tq * sizeof(float);
+  if (ca_check(B, H, Hkv, Tq, Tk, d) != AAR_OK || B == 0 || H == 0 || Tq == 0) return 0;
+  CaArgs a = ca_args(B, H, Hkv, Tq, Tk, d, nullptr, nullptr, 1.0f);
+  ca_bwd_plan(a);
+  return bwd_bytes(a, 4);
 }
 
 int aar_cross_attn_bwd_f32(const float* q, const float* k, const float* v, const int64_t* kv_lens, const float* o,
@@ -1403,10 +1622,16 @@ int aar_cross_attn_bwd_f32(const float* q, const float* k, const float* v, const
   if (Tq > 0 && (!q || !o || !lse || !dout || !dq)) return AAR_EINVAL;
   if (Tk > 0 && (!k || !v || !dk || !dv)) return AAR_EINVAL;
   if (Tq == 0 && Tk == 0) return AAR_OK;
-  if (Tq > 0 &&
-      (!workspace || workspace_bytes < aar_cross_attn_bwd_workspace_bytes(B, H, Hkv, Tq, Tk, d)))
-    return AAR_EWORKSPACE;
   CaArgs a = ca_args(B, H, Hkv, Tq, Tk, d, kv_lens, const_cast<float*>(lse), scale);
+  ca_bwd_plan(a);
+  if (Tq > 0) {
+    if (!workspace || !aligned16(workspace) || workspace_bytes < bwd_bytes(a, 4)) return AAR_EWORKSPACE;
+    char* ws = static_cast<char*>(workspace);
+    a.D = reinterpret_cast<float*>(ws);
+    a.dq_part = reinterpret_cast<float*>(ws + bwd_bytes(a, 1));
+    a.dk_part = reinterpret_cast<float*>(ws + bwd_bytes(a, 2));
+    a.dv_part = reinterpret_cast<float*>(ws + bwd_bytes(a, 3));
+  }
   a.q = ca_in(q, strides);
   a.k = ca_in(k, strides + 3);
   a.v = ca_in(v, strides + 6);
@@ -1415,8 +1640,6 @@ int aar_cross_attn_bwd_f32(const float* q, const float* k, const float* v, const
   a.dq = ca_out(dq, strides + 15);
   a.dk = ca_out(dk, strides + 18);
   a.dv = ca_out(dv, strides + 21);
-  a.D = static_cast<float*>(workspace);
-  a.splits = 1;
   return ca_dispatch<false>(a, ca_vec_ok(d, {q, k, v, o, dout, dq, dk, dv}, strides, 24), as_stream(stream));
 }
 

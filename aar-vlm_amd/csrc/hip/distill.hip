@@ -89,6 +89,13 @@ __device__ __forceinline__ void teacher_sum(const float* t, const int64_t* ids, 
   tm = mu;
 }
 
+// A row that is left out (no loss is -inf).
+__device__ __forceinline__ void leave_out(float* row_loss, float* stats, int64_t row) {
+  row_loss[row] = -INFINITY;
+  stats[2 * row] = 0.f;
+  stats[2 * row + 1] = INFINITY;
+}
+
 // One row per W waves; row_loss and stats.
 template <int W>
 __global__ void __launch_bounds__(W > 4 ? W * kWave : 256)
@@ -142,9 +149,7 @@ distill_row_kernel(const float* __restrict__ Z, const float* __restrict__ Tl, co
   if (row >= n || wr != 0) return;
   if (!on) {
     if (lane == 0) {
-      row_loss[row] = 0.f;
-      stats[2 * row] = 0.f;
-      stats[2 * row + 1] = INFINITY;
+      leave_out(row_loss, stats, row);
       if (bad && err) *err = 1;
     }
     return;
@@ -154,11 +159,7 @@ distill_row_kernel(const float* __restrict__ Z, const float* __restrict__ Tl, co
   float tm, ts;
   teacher_sum(t, ids, top, k, lane, tm, ts);
   if (ts == 0.f) {  // nothing above -inf: left out like a row without entries
-    if (lane == 0) {
-      row_loss[row] = 0.f;
-      stats[2 * row] = 0.f;
-      stats[2 * row + 1] = INFINITY;
-    }
+    if (lane == 0) leave_out(row_loss, stats, row);
     return;
   }
   const float ln_s = logf(a.s);
@@ -182,7 +183,7 @@ distill_row_kernel(const float* __restrict__ Z, const float* __restrict__ Tl, co
 // The mean of the counted rows' losses and their number: one workgroup, each
 // thread its rows in order (in double), then a fixed tree.
 constexpr int kMeanThreads = 1024;
-constexpr int kMeanChunk = 8;
+constexpr int kMeanChunk = 16;
 
 __global__ void __launch_bounds__(kMeanThreads)
 distill_mean_kernel(const float* __restrict__ row_loss, float* __restrict__ stats, float* __restrict__ loss, int64_t n) {
@@ -191,17 +192,17 @@ distill_mean_kernel(const float* __restrict__ row_loss, float* __restrict__ stat
   double s = 0.0;
   long long c = 0;
   for (int64_t base = 0; base < n; base += (int64_t)kMeanThreads * kMeanChunk) {
-    float l[kMeanChunk], e[kMeanChunk];
+    float l[kMeanChunk];
 #pragma unroll
     for (int u = 0; u < kMeanChunk; ++u) {
       const int64_t i = base + (int64_t)u * kMeanThreads + threadIdx.x;
-      l[u] = i < n ? row_loss[i] : 0.f;
-      e[u] = i < n ? stats[2 * i + 1] : INFINITY;
+      l[u] = i < n ? row_loss[i] : -INFINITY;
     }
 #pragma unroll
     for (int u = 0; u < kMeanChunk; ++u) {
+      if (l[u] == -INFINITY) continue;
       s += (double)l[u];
-      c += e[u] != INFINITY ? 1 : 0;
+      ++c;
     }
   }
 #pragma unroll
@@ -236,10 +237,11 @@ distill_bwd_kernel(const float* __restrict__ grad, const float* __restrict__ Z, 
   extern __shared__ int sh[];  // ids and p of the rows' entries
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wr = wave % W, rt = wr * kWave + lane;
-  const int64_t row = (int64_t)blockIdx.x * kRows + wave / W;
+  // the forward's last rows first: they may still be in the caches
+  const int64_t row = n - 1 - ((int64_t)blockIdx.x * kRows + wave / W);
   int* sid = sh + (wave / W) * 2 * top;
   float* sp = reinterpret_cast<float*>(sid + top);
-  const bool here = row < n;
+  const bool here = row >= 0;
   const float m = here ? stats[2 * row] : 0.f, s = here ? stats[2 * row + 1] : INFINITY;
   const bool on = s != INFINITY;
   const float* z = Z + row * V;
@@ -303,6 +305,168 @@ distill_bwd_kernel(const float* __restrict__ grad, const float* __restrict__ Z, 
   }
 }
 
+// Short rows (V <= 256, up to 64 entries): 16 lanes a row, four rows a wave, the
+// row in registers.  With a wave a row, most lanes of a character vocabulary's
+// rows are idle (16384 x 65: 12.9 + 12.2 us).
+constexpr int kShortVocab = 256, kShortTop = 64, kShortLanes = 16;
+constexpr int kShortRows = 256 / kShortLanes;  // of a workgroup
+
+__device__ __forceinline__ float sum16(float v) {
+  v += dpp_quad_xor1(v);
+  v += dpp_quad_xor2(v);
+  v += dpp_half_mirror(v);
+  v += dpp_row_mirror(v);
+  return v;
+}
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, dpp_quad_xor1(v));
+  v = fmaxf(v, dpp_quad_xor2(v));
+  v = fmaxf(v, dpp_half_mirror(v));
+  v = fmaxf(v, dpp_row_mirror(v));
+  return v;
+}
+
+// A row's teacher entries as its 16 lanes hold them: entry l + 16 i in slot i, its
+// weight e = 2^(k (t - max)) and their sum.
+struct ShortTeacher {
+  static constexpr int kN = kShortTop / kShortLanes;
+  int id[kN];
+  float t[kN], e[kN];  // t - max, and its exponential
+  float sum;
+  bool on, bad;
+  __device__ __forceinline__ void load(const float* Tl, const int64_t* Ti, bool here, int top, int V, float k, int l) {
+    bool any = false, out = false;
+    float tm = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int j = l + i * kShortLanes;
+      const int64_t v = here && j < top ? Ti[j] : -1;
+      t[i] = v >= 0 ? Tl[j] : -INFINITY;
+      any = any || v >= 0;
+      out = out || v < -1 || v >= V;
+      id[i] = v >= 0 && v < V ? (int)v : -1;
+      tm = fmaxf(tm, t[i]);
+    }
+    // across the row's 16 lanes
+    any = sum16(any ? 1.f : 0.f) > 0.f;
+    bad = sum16(out ? 1.f : 0.f) > 0.f;
+    tm = max16(tm);
+    const float mu = tm == -INFINITY ? 0.f : tm;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      t[i] -= mu;
+      e[i] = id[i] >= 0 ? fast_exp2(t[i] * k) : 0.f;
+      s += e[i];
+    }
+    sum = sum16(s);
+    on = any && !bad && sum != 0.f;
+  }
+};
+
+// A short row's logits: column l + 16 i in slot i (-inf past the row's end).
+template <int NV>
+__device__ __forceinline__ void short_row(const float* z, bool on, int V, int l, float (&x)[NV]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = l + i * kShortLanes;
+    x[i] = on && v < V ? z[v] : -INFINITY;
+  }
+}
+
+template <int NV>
+__global__ void __launch_bounds__(256)
+distill_short_row_kernel(const float* __restrict__ Z, const float* __restrict__ Tl, const int64_t* __restrict__ Ti,
+                         float* __restrict__ row_loss, float* __restrict__ stats, int64_t n, int V, int top, float k,
+                         float inv_tau, float tau2, int* __restrict__ err) {
+  const int l = threadIdx.x % kShortLanes;
+  const int64_t row = (int64_t)blockIdx.x * kShortRows + threadIdx.x / kShortLanes;
+  const bool here = row < n;
+  const float* z = Z + row * V;
+  ShortTeacher te;
+  te.load(Tl + row * top, Ti + row * top, here, top, V, k, l);
+  float x[NV];
+  short_row<NV>(z, te.on, V, l, x);
+  float m = x[0];
+#pragma unroll
+  for (int i = 1; i < NV; ++i) m = fmaxf(m, x[i]);
+  m = max16(m);
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (l + i * kShortLanes < V) s += fast_exp2((x[i] - m) * k);
+  s = sum16(s);
+  const float ln_s = logf(s);
+  float acc = 0.f;
+#pragma unroll
+  for (int i = 0; i < ShortTeacher::kN; ++i) {
+    if (te.id[i] < 0 || !te.on) continue;
+    const float lnq = (z[te.id[i]] - m) * inv_tau - ln_s;
+    if (!(te.e[i] == 0.f)) acc += te.e[i] * (te.t[i] * inv_tau - lnq);
+  }
+  acc = sum16(acc);
+  if (!here || l != 0) return;
+  if (te.bad && err) *err = 1;
+  if (!te.on) {
+    leave_out(row_loss, stats, row);
+  } else {
+    row_loss[row] = tau2 * (acc / te.sum - logf(te.sum));
+    stats[2 * row] = m;
+    stats[2 * row + 1] = s;
+  }
+}
+
+template <int NV>
+__global__ void __launch_bounds__(256)
+distill_short_bwd_kernel(const float* __restrict__ grad, const float* __restrict__ Z, const float* __restrict__ Tl,
+                         const int64_t* __restrict__ Ti, const float* __restrict__ stats, float* __restrict__ dZ,
+                         int64_t n, int V, int top, float k, float tau) {
+  __shared__ float ps[kShortRows][NV * kShortLanes];  // each column's p
+  __shared__ int sid[kShortRows][kShortTop];
+  __shared__ float sp[kShortRows][kShortTop];
+  const int l = threadIdx.x % kShortLanes, r = threadIdx.x / kShortLanes;
+  const int64_t row = (int64_t)blockIdx.x * kShortRows + r;
+  const bool here = row < n;
+  const float m = here ? stats[2 * row] : 0.f, s = here ? stats[2 * row + 1] : INFINITY;
+  const bool on = s != INFINITY;
+  ShortTeacher te;
+  te.load(Tl + row * top, Ti + row * top, here, top, V, k, l);
+  float x[NV];
+  short_row<NV>(Z + row * V, on, V, l, x);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) ps[r][l + i * kShortLanes] = 0.f;
+#pragma unroll
+  for (int i = 0; i < ShortTeacher::kN; ++i) {
+    sid[r][l + i * kShortLanes] = te.id[i];
+    sp[r][l + i * kShortLanes] = te.e[i] / te.sum;
+  }
+  __syncthreads();
+  if (on) {
+    for (int i = l; i < top; i += kShortLanes) {
+      const int id = sid[r][i];
+      if (id < 0) continue;
+      // the first entry of an id writes the sum over all of them
+      float p = 0.f;
+      bool first = true;
+      for (int j = 0; j < top; ++j) {
+        if (sid[r][j] != id) continue;
+        if (j < i) first = false;
+        p += sp[r][j];
+      }
+      if (first) ps[r][id] = p;
+    }
+  }
+  __syncthreads();
+  if (!here) return;
+  const float c = grad[0] * tau / stats[2 * n];
+  const float f = c / s;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = l + i * kShortLanes;
+    if (v < V) dZ[row * V + v] = on ? f * fast_exp2((x[i] - m) * k) - c * ps[r][v] : 0.f;
+  }
+}
+
 // Waves per row.  One wave holds a short row's loads in flight by itself; long
 // rows take a workgroup, the larger one where there are fewer of them than it
 // takes to fill the GPU with the smaller.
@@ -339,6 +503,24 @@ int launch_bwd(const float* grad, const float* z, const float* tl, const int64_t
   return launch_status();
 }
 
+bool short_rows(int64_t vocab, int64_t top) { return vocab <= kShortVocab && top <= kShortTop; }
+
+template <int NV>
+int launch_short(const float* z, const float* tl, const int64_t* ti, float* row_loss, float* stats, int64_t n, int V,
+                 int top, float tau, int* err, hipStream_t st) {
+  distill_short_row_kernel<NV><<<dim3((unsigned)ceil_div(n, kShortRows)), dim3(256), 0, st>>>(
+      z, tl, ti, row_loss, stats, n, V, top, kLog2e / tau, 1.0f / tau, tau * tau, err);
+  return launch_status();
+}
+
+template <int NV>
+int launch_short_bwd(const float* grad, const float* z, const float* tl, const int64_t* ti, const float* stats,
+                     float* dz, int64_t n, int V, int top, float tau, hipStream_t st) {
+  distill_short_bwd_kernel<NV><<<dim3((unsigned)ceil_div(n, kShortRows)), dim3(256), 0, st>>>(
+      grad, z, tl, ti, stats, dz, n, V, top, kLog2e / tau, tau);
+  return launch_status();
+}
+
 int distill_check(int64_t n, int64_t vocab, int64_t top, float tau) {
   if (n < 0 || vocab <= 0 || top <= 0 || !(tau > 0.f) || !(tau < INFINITY)) return AAR_EINVAL;
   if (top > kMaxTop || vocab > INT32_MAX - 4096 || n > (int64_t)UINT32_MAX / 1024) return AAR_EUNSUPPORTED;
@@ -367,6 +549,7 @@ int aar_distill_fwd_f32(const float* logits, const float* t_logits, const int64_
   if (n > 0) {
     const int w = waves_per_row(n, vocab);
     auto launch = w == 1 ? launch_rows<1> : (w == 4 ? launch_rows<4> : launch_rows<16>);
+    if (short_rows(vocab, top)) launch = vocab <= 80 ? launch_short<5> : launch_short<16>;
     rc = launch(logits, t_logits, t_ids, row_loss, stats, n, (int)vocab, (int)top, temperature, err, st);
     if (rc != AAR_OK) return rc;
   }
@@ -383,6 +566,7 @@ int aar_distill_bwd_f32(const float* grad, const float* logits, const float* t_l
   if (!grad || !logits || !t_logits || !t_ids || !stats || !dlogits) return AAR_EINVAL;
   const int w = waves_per_row(n, vocab);
   auto launch = w == 1 ? launch_bwd<1> : (w == 4 ? launch_bwd<4> : launch_bwd<16>);
+  if (short_rows(vocab, top)) launch = vocab <= 80 ? launch_short_bwd<5> : launch_short_bwd<16>;
   return launch(grad, logits, t_logits, t_ids, stats, dlogits, n, (int)vocab, (int)top, temperature,
                 as_stream(stream));
 }

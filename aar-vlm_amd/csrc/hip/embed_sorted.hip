@@ -42,9 +42,18 @@ embed_scaled_vec_kernel(const f32x4* __restrict__ w, const int64_t* __restrict__
   if (!ok && lane == 0 && err) *err = 1;
   const f32x4* src = w + (ok ? id : 0) * dim4;
   f32x4* dst = out + i * dim4;
-  for (int64_t k = lane; k < dim4; k += kWave) {
-    const f32x4 v = ok ? src[k] * scale : f32x4{0.f, 0.f, 0.f, 0.f};
-    __builtin_nontemporal_store(v, dst + k);
+  const float f = ok ? scale : 0.f;
+  constexpr int kU = 4;  // loads in flight
+  for (int64_t k = lane; k < dim4; k += kU * kWave) {
+    f32x4 v[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      v[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (ok && k + u * kWave < dim4) v[u] = src[k + u * kWave];
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+      if (k + u * kWave < dim4) __builtin_nontemporal_store(v[u] * f, dst + k + u * kWave);
   }
 }
 
@@ -61,10 +70,12 @@ embed_scaled_kernel(const float* __restrict__ w, const int64_t* __restrict__ ids
 }
 
 // Sorted tokens and run starts: start[v] for v <= vocab, token[] in runs of
-// equal ids, each in the tokens' order.
+// equal ids, each in the tokens' order, and sid[] their ids.  Bound by the latency
+// of the ids' loads, so a wave has 32 groups of 64 in flight, and those of up to
+// 32768 tokens stay in registers for the second reading.
 __global__ void __launch_bounds__(kSortThreads)
 embed_sort_kernel(const int64_t* __restrict__ ids, int n, int vocab, int slice, int* __restrict__ token,
-                  int* __restrict__ start) {
+                  int* __restrict__ sid, int* __restrict__ start) {
   __shared__ int cnt[kSortWaves * kMaxSlice];  // [wave][id]: counts, then where the wave's next token goes
   __shared__ int sums[kSortWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -77,8 +88,9 @@ embed_sort_kernel(const int64_t* __restrict__ ids, int n, int vocab, int slice, 
   const int t0 = min(n, wave * per), t1 = min(n, t0 + per);
   int* mine = cnt + wave * slice;
   int below = 0;
-  constexpr int kU = 4;
-  for (int b = t0; b < t1; b += kU * kWave) {
+  constexpr int kU = 32;
+  int r[kU];  // the groups' ids within the slice, -1 for the others
+  auto read = [&](int b) {
     int64_t id[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
@@ -87,9 +99,15 @@ embed_sort_kernel(const int64_t* __restrict__ ids, int n, int vocab, int slice, 
     }
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      if (id[u] >= 0 && id[u] < v0) ++below;
-      if (id[u] >= v0 && id[u] < v0 + nv) atomicAdd(&mine[(int)(id[u] - v0)], 1);
+      below += id[u] >= 0 && id[u] < v0 ? 1 : 0;
+      r[u] = id[u] >= v0 && id[u] < v0 + nv ? (int)(id[u] - v0) : -1;
     }
+  };
+  for (int b = t0; b < t1; b += kU * kWave) {
+    read(b);
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+      if (r[u] >= 0) atomicAdd(&mine[r[u]], 1);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) below += __shfl_xor(below, o, kWave);
@@ -128,26 +146,26 @@ embed_sort_kernel(const int64_t* __restrict__ ids, int n, int vocab, int slice, 
   // The tokens, group by group: the lanes that hold the same id take its next
   // places in lane order.
   for (int b = t0; b < t1; b += kU * kWave) {
-    int64_t id[kU];
+    if (per > kU * kWave) read(b);
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int i = b + u * kWave + lane;
-      id[u] = i < t1 ? ids[i] : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const bool in = id[u] >= v0 && id[u] < v0 + nv;
-      const int r = in ? (int)(id[u] - v0) : -1;
-      unsigned long long todo = __ballot(in);
+      unsigned long long todo = __ballot(r[u] >= 0);
+      if (todo == 0) continue;
+      const int at = r[u] >= 0 ? mine[r[u]] : 0;
+      int rank = 0, count = 0;  // among the group's lanes of the same id
       while (todo) {
-        const int rr = __builtin_amdgcn_readlane(r, __builtin_ctzll(todo));
-        const unsigned long long same = __ballot(r == rr);
-        const int first = __builtin_ctzll(same);
-        int at = 0;
-        if (lane == first) at = atomicAdd(&mine[rr], __builtin_popcountll(same));
-        at = __builtin_amdgcn_readlane(at, first);
-        if (r == rr) token[at + __builtin_popcountll(same & ((1ull << lane) - 1))] = b + u * kWave + lane;
+        const int rr = __builtin_amdgcn_readlane(r[u], __builtin_ctzll(todo));
+        const unsigned long long same = __ballot(r[u] == rr);
+        if (r[u] == rr) {
+          rank = __builtin_popcountll(same & ((1ull << lane) - 1));
+          count = __builtin_popcountll(same);
+        }
         todo &= ~same;
+      }
+      if (r[u] >= 0) {
+        token[at + rank] = b + u * kWave + lane;
+        sid[at + rank] = v0 + r[u];
+        if (rank == 0) mine[r[u]] = at + count;
       }
     }
   }
@@ -155,8 +173,8 @@ embed_sort_kernel(const int64_t* __restrict__ ids, int n, int vocab, int slice, 
 
 struct EmbedArgs {
   const float* g;
-  const int64_t* ids;
   const int* token;
+  const int* sid;
   const int* start;
   float* part;  // [chunks][2][dim]: the run that began before the chunk, the one that goes on after it
   float* dw;
@@ -222,7 +240,7 @@ embed_sum_kernel(const EmbedArgs a) {
   for (int b = p0; b < p1; b += kWave) {
     const int nb = min(kWave, p1 - b);
     const int tok = lane < nb ? a.token[b + lane] : 0;
-    const int id = lane < nb ? (int)a.ids[tok] : 0;
+    const int id = lane < nb ? a.sid[b + lane] : 0;
     for (int j = 0; j < nb; j += kRows) {
       V x[kRows];
 #pragma unroll
@@ -259,7 +277,7 @@ embed_join_kernel(const EmbedArgs a) {
   const int total = a.start[a.vocab];
   const int p0 = chunk * a.chunk, p1 = p0 + a.chunk;
   if (p1 >= total) return;  // the last chunk's runs end in it
-  const int v = (int)a.ids[a.token[p1 - 1]];
+  const int v = a.sid[p1 - 1];
   const int end = a.start[v + 1];
   if (a.start[v] < p0 || end <= p1) return;  // began before, or ends here
   const int last = (end - 1) / a.chunk;      // partial rows: chunk's second, then the first of chunk + 1 .. last
@@ -344,7 +362,7 @@ int aar_embedding_scaled_fwd_f32(const float* w, const int64_t* ids, float* out,
 size_t aar_embedding_sorted_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t dim) {
   if (n <= 0 || vocab <= 0 || dim <= 0 || !embed_shape_ok(n, vocab, dim)) return 0;
   const int64_t chunks = ceil_div(n, chunk_tokens(n));
-  return token_bytes(n) + start_bytes(vocab) + (size_t)chunks * 2 * (size_t)dim * sizeof(float);
+  return 2 * token_bytes(n) + start_bytes(vocab) + (size_t)chunks * 2 * (size_t)dim * sizeof(float);
 }
 
 int aar_embedding_sorted_bwd_f32(const float* g, const int64_t* ids, float* dw, int64_t n, int64_t vocab, int64_t dim,
@@ -360,13 +378,14 @@ int aar_embedding_sorted_bwd_f32(const float* g, const int64_t* ids, float* dw, 
   hipStream_t st = as_stream(stream);
   char* ws = static_cast<char*>(workspace);
   int* token = reinterpret_cast<int*>(ws);
-  int* start = reinterpret_cast<int*>(ws + token_bytes(n));
+  int* sid = reinterpret_cast<int*>(ws + token_bytes(n));
+  int* start = reinterpret_cast<int*>(ws + 2 * token_bytes(n));
   const int64_t slice = slice_ids(vocab), chunk = chunk_tokens(n);
-  EmbedArgs a{g, ids, token, start, reinterpret_cast<float*>(ws + token_bytes(n) + start_bytes(vocab)), dw, dim,
+  EmbedArgs a{g, token, sid, start, reinterpret_cast<float*>(ws + 2 * token_bytes(n) + start_bytes(vocab)), dw, dim,
               (int)n, (int)vocab, (int)chunk, (int)ceil_div(n, chunk), 0, scale};
   const bool vec = dim % 4 == 0 && aligned16(g) && aligned16(dw);
   embed_sort_kernel<<<dim3((unsigned)ceil_div(vocab, slice)), dim3(kSortThreads), 0, st>>>(ids, (int)n, (int)vocab,
-                                                                                          (int)slice, token, start);
+                                                                                          (int)slice, token, sid, start);
   const int rc = launch_status();
   if (rc != AAR_OK) return rc;
   return vec ? launch_sum<true>(a, st) : launch_sum<false>(a, st);

@@ -10,7 +10,8 @@
 // x and dy and writes dx (rstd is recomputed from x, which it needs anyway).
 // A head takes d/8 lanes with 4 + 4 elements each, the halves of its pairs, so
 // norm and rotation stay inside a lane but for one sum over the head's lanes; a
-// wave walks a row's heads and forms the row's angles once.  The angle in turns
+// wave walks a row's heads and forms the row's angles once, beside the first
+// heads' loads.  The angle in turns
 // is position * base^(-2c/r) / (2 pi) in fp64 (frequencies from the host, in
 // the kernel's arguments), whose fraction alone goes to fp32: positions of 10^6
 // and beyond lose nothing.  dw accumulates in registers over a persistent grid,
@@ -91,11 +92,81 @@ rope_vec_kernel(const RopeArgs a, const RopeFreq fr) {
     for (int e = 0; e < 4; ++e) turn[e] = fr.turn[c + e];
   }
   f32x4 dq1 = zero, dq2 = zero, dk1 = zero, dk2 = zero;
+  // One head of each lane's group: its output and, in the backward, its share of dw.
+  auto head = [&](int64_t row, int h, bool act, const f32x4& x1, const f32x4& x2, const f32x4& g1, const f32x4& g2,
+                  const f32x4& sn, const f32x4& cs) {
+    const bool is_q = h < a.hq;
+    const f32x4 w1 = is_q ? wq1 : wk1, w2 = is_q ? wq2 : wk2;
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ss += x1[e] * x1[e] + x2[e] * x2[e];
+    const float rstd = 1.0f / sqrtf(head_sum<LPH>(ss) * inv_d + a.eps);
+    f32x4 o1, o2;
+    if (!BWD) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float u1 = x1[e] * rstd * w1[e], u2 = x2[e] * rstd * w2[e];
+        o1[e] = u1 * cs[e] - u2 * sn[e];
+        o2[e] = u2 * cs[e] + u1 * sn[e];
+      }
+    } else {
+      f32x4 h1, h2, r1, r2;
+      float dot = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        r1[e] = g1[e] * cs[e] + g2[e] * sn[e];
+        r2[e] = g2[e] * cs[e] - g1[e] * sn[e];
+        h1[e] = x1[e] * rstd;
+        h2[e] = x2[e] * rstd;
+        dot += r1[e] * w1[e] * h1[e] + r2[e] * w2[e] * h2[e];
+      }
+      const float mean = head_sum<LPH>(dot) * inv_d;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o1[e] = rstd * (r1[e] * w1[e] - h1[e] * mean);
+        o2[e] = rstd * (r2[e] * w2[e] - h2[e] * mean);
+      }
+      if (act) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p1 = r1[e] * h1[e], p2 = r2[e] * h2[e];
+          dq1[e] += is_q ? p1 : 0.f;
+          dq2[e] += is_q ? p2 : 0.f;
+          dk1[e] += is_q ? 0.f : p1;
+          dk2[e] += is_q ? 0.f : p2;
+        }
+      }
+    }
+    if (act) {
+      float* yp = a.y + row * a.y_row + (int64_t)h * a.d + c;
+      __builtin_nontemporal_store(o1, reinterpret_cast<f32x4*>(yp));
+      __builtin_nontemporal_store(o2, reinterpret_cast<f32x4*>(yp + half));
+    }
+  };
   const int64_t units = a.rows * a.split;
   const int64_t step = (int64_t)gridDim.x * (kThreads / kWave);
   for (int64_t u = (int64_t)blockIdx.x * (kThreads / kWave) + wave; u < units; u += step) {
     const int64_t row = u / a.split;
     const int part = (int)(u - row * a.split);
+    // the first heads' loads run beside the angles
+    f32x4 x1, x2, g1, g2;
+    int h;
+    auto load = [&](int h0) {
+      h = h0 + lane / LPH;
+      x1 = x2 = g1 = g2 = zero;
+      if (on && h < a.heads) {
+        const float* xp = a.x + row * a.x_row + (int64_t)h * a.d + c;
+        x1 = *reinterpret_cast<const f32x4*>(xp);
+        x2 = *reinterpret_cast<const f32x4*>(xp + half);
+        if (BWD) {
+          const float* gp = a.gy + row * a.gy_row + (int64_t)h * a.d + c;
+          g1 = *reinterpret_cast<const f32x4*>(gp);
+          g2 = *reinterpret_cast<const f32x4*>(gp + half);
+        }
+      }
+    };
+    int h0 = part * kHeads;
+    load(h0);
     const double p = (double)a.pos[row % a.n_pos];
     f32x4 sn, cs;
 #pragma unroll
@@ -105,68 +176,11 @@ rope_vec_kernel(const RopeArgs a, const RopeFreq fr) {
       sn[e] = s1;
       cs[e] = c1;
     }
-    for (int h0 = part * kHeads; h0 < a.heads; h0 += a.split * kHeads) {
-      const int h = h0 + lane / LPH;
-      const bool act = on && h < a.heads;
-      const int64_t at = (int64_t)h * a.d + c;
-      f32x4 x1 = zero, x2 = zero, g1 = zero, g2 = zero;
-      if (act) {
-        const float* xp = a.x + row * a.x_row + at;
-        x1 = *reinterpret_cast<const f32x4*>(xp);
-        x2 = *reinterpret_cast<const f32x4*>(xp + half);
-        if (BWD) {
-          const float* gp = a.gy + row * a.gy_row + at;
-          g1 = *reinterpret_cast<const f32x4*>(gp);
-          g2 = *reinterpret_cast<const f32x4*>(gp + half);
-        }
-      }
-      const bool is_q = h < a.hq;
-      const f32x4 w1 = is_q ? wq1 : wk1, w2 = is_q ? wq2 : wk2;
-      float ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) ss += x1[e] * x1[e] + x2[e] * x2[e];
-      const float rstd = 1.0f / sqrtf(head_sum<LPH>(ss) * inv_d + a.eps);
-      f32x4 o1, o2;
-      if (!BWD) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float u1 = x1[e] * rstd * w1[e], u2 = x2[e] * rstd * w2[e];
-          o1[e] = u1 * cs[e] - u2 * sn[e];
-          o2[e] = u2 * cs[e] + u1 * sn[e];
-        }
-      } else {
-        f32x4 h1, h2, r1, r2;
-        float dot = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          r1[e] = g1[e] * cs[e] + g2[e] * sn[e];
-          r2[e] = g2[e] * cs[e] - g1[e] * sn[e];
-          h1[e] = x1[e] * rstd;
-          h2[e] = x2[e] * rstd;
-          dot += r1[e] * w1[e] * h1[e] + r2[e] * w2[e] * h2[e];
-        }
-        const float mean = head_sum<LPH>(dot) * inv_d;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          o1[e] = rstd * (r1[e] * w1[e] - h1[e] * mean);
-          o2[e] = rstd * (r2[e] * w2[e] - h2[e] * mean);
-        }
-        if (act) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float p1 = r1[e] * h1[e], p2 = r2[e] * h2[e];
-            dq1[e] += is_q ? p1 : 0.f;
-            dq2[e] += is_q ? p2 : 0.f;
-            dk1[e] += is_q ? 0.f : p1;
-            dk2[e] += is_q ? 0.f : p2;
-          }
-        }
-      }
-      if (act) {
-        float* yp = a.y + row * a.y_row + at;
-        *reinterpret_cast<f32x4*>(yp) = o1;
-        *reinterpret_cast<f32x4*>(yp + half) = o2;
-      }
+    for (;;) {
+      head(row, h, on && h < a.heads, x1, x2, g1, g2, sn, cs);
+      h0 += a.split * kHeads;
+      if (h0 >= a.heads) break;
+      load(h0);
     }
   }
   if (!BWD) return;
