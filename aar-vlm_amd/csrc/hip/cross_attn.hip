@@ -20,7 +20,6 @@
 
 #include <algorithm>
 #include <initializer_list>
-#include <type_traits>
 
 #include "bf16x3.hpp"
 #include "common.hpp"
@@ -140,11 +139,12 @@ __device__ __forceinline__ void ca_store_key(const CaArgs& a, int bh, int part, 
 // and V.  LPK lanes hold a key's row, four floats each, and walk the keys with
 // their own online softmax, U keys' loads in flight; the groups' and waves'
 // states meet once at the end.  The key range is split over enough workgroups to
-// fill the GPU, joined by cross_combine_kernel.
+// fill the GPU, joined by cross_combine_kernel.  32 x 6 heads' single rows over up to
+// 2048 keys, d 64 (151 MB): 29 us, 5.2 TB/s, and 4.7 us for the parts.
 template <int RQ, int LPK, bool VEC>
 __global__ void __launch_bounds__(256)
 cross_rows_kernel(const CaArgs a) {
-  constexpr int U = RQ >= 8 ? 2 : 4;
+  constexpr int U = 4;
   constexpr int kGroups = kWave / LPK;
   constexpr int kWaves = 4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -302,7 +302,10 @@ cross_combine_kernel(const CaArgs a) {
 // A workgroup takes 128 query rows (32 a wave, a lane its row) and its key range,
 // 32 keys at a time: S^T = K Q^T leaves a lane 16 keys of its row, whose online
 // softmax is in registers but for one exchange with lane ^ 32, and P feeds
-// O^T += V^T P^T from the registers it is left in.  K is staged a tile ahead of V.
+// O^T += V^T P^T from the registers it is left in.  This form and its gradients run
+// for rows of up to 32 floats and unaligned ones, bound by the fp32 matrix instruction:
+// 8 x 12 heads, 1024 x 4096, d 64 in 934 us, 110 TFLOP/s of the 153 that a large fp32
+// product reaches.
 template <int DP, bool VEC>
 __global__ void __launch_bounds__(kFaThreads)
 cross_fwd_kernel(const CaArgs a) {
@@ -631,101 +634,134 @@ cross_bwd_dkdv_kernel(const CaArgs a) {
   if (kj < a.Tk) ca_store_key<DP, VEC>(a, bh, part, kj, key_ok, dk, dv, h);
 }
 
-// ---------------------------------------------------- on the bf16 matrix cores
-// The same passes with every operand in three bf16 parts (bf16x3.hpp): six matrix
-// ops per 16 steps at 14 times the fp32 instruction's rate.  What a wave keeps in
-// registers for all tiles (q; q and dO; k and v) is split once; a tile is split on
-// its way into LDS, once a workgroup, as three row-major planes.  Products over
-// the head dim read rows of them; products over the tile's rows (V^T P^T, K^T
-// dS^T, dO^T P, Q^T dS) read columns through the transposing LDS read, so a tile
-// that serves both is split and stored once.  P and dS are split in the registers
-// the softmax leaves them in.
+// ---------------------------------------------------- on the fp16 matrix cores
+// The same passes with every operand in two fp16 parts: x 2^e = hi + lo, hi rounded
+// from x 2^e and lo from what that leaves, so that three matrix ops (lo hi, hi lo,
+// hi hi; 16 steps each at 16 times the fp32 instruction's rate) stand for one
+// fp32 product.  An operand is off by at most 2^-22 of itself or, where that is more,
+// 2^-38 of its row's largest element, lo lo is at most 2^-22 of a product and is left
+// out; sums are in fp32, with fewer roundings than the fp32 instruction's, which
+// leaves the results nearer to the exact ones.  8 x 12 heads, 1024 x 4096, d 64 (in
+// brackets with the fp32 instruction): forward 439 us (934), dQ 625 (1276), dK/dV 898
+// (1730), off by 0.76e-6 (1.2e-6) in O's norm, 1.0e-6 (1.3e-6) in dQ's, 0.80e-6
+// (0.88e-6) in dK's and dV's.  That is 235 TFLOP/s of the products they stand for,
+// 705 on the cores.  Three bf16 parts and six products hold all 24 bits, but took 590,
+// 806 and 1125 us.  Vector instructions (scales, exponentials, splits: 290 a wave and
+// tile in the forward beside 24 matrix ops) bound these: they take 84% of the cycles
+// while waves are there, the matrix ops 34%.
+//
+// e is a row's own, such that its largest element is in [2^13, 2^14).  Over the head
+// dim a row's factor is one of the output's row or column.  Over a tile's rows it
+// goes to the other operand, P or dS, which is scaled by the lane's own power of two
+// that follows the largest |P| 2^-e (|dS| 2^-e) so far: what is rounded there is at
+// most 2^-38 of the largest term of the lane's sum.
+//
+// What a wave keeps in registers for all tiles (q; q and dO; k and v) is split once; a
+// tile is split on its way into LDS, once a workgroup, as two row-major planes.
+// Products over the head dim read rows of them; products over the tile's rows (V^T
+// P^T, K^T dS^T, dO^T P, Q^T dS) read columns through the transposing LDS read, so a
+// tile that serves both is split and stored once.  P and dS are split in the
+// registers the softmax leaves them in.  Rows whose largest element is outside
+// [2^-63, 2^60) (infinities too) are not held so: the waves that meet one do their
+// rows again with the fp32 instruction, from HBM.
 
-// A third of a pair's split (bf16_split_pair in three pieces): a and b become what
-// is left over, w[piece] the part.
-__device__ __forceinline__ void split_piece(int piece, float& a, float& b, uint32_t& w, uint32_t& rem) {
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f32x16 mfma_f16(const u32x4& a, const u32x4& b, const f32x16& c) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  if (piece == 2) rem = __builtin_amdgcn_bitop3_b32(rem, __float_as_uint(a), __float_as_uint(b), 0xfe);
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                0);
+#else
+  return c;
 #endif
-  w = bf16_pair(a, b);
-  if (piece < 2) {
-    a -= __uint_as_float(w << 16);
-    b -= __uint_as_float(w & 0xffff0000u);
-  }
 }
 
-// A [32][DP] tile in three planes of 32 rows; a row's 16 spare bytes put 16
+// The products, smallest first.
+constexpr int kHalfProducts = 3;
+__device__ constexpr int kHalfA[kHalfProducts] = {1, 0, 0};
+__device__ constexpr int kHalfB[kHalfProducts] = {0, 1, 0};
+
+// The two parts of (a, b), a pair a word.
+__device__ __forceinline__ void half_split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const f32x2 v = {a, b};
+  const f16x2 x = __builtin_convertvector(v, f16x2);
+  const f32x2 rest = {a - (float)x[0], b - (float)x[1]};
+  hi = __builtin_bit_cast(uint32_t, x);
+  lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, f16x2));
+}
+
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // |e| <= 126
+
+// Exponent of the scale of a row whose largest magnitude is `top` (the largest scale
+// for zeros), and whether the parts do not hold it.
+__device__ __forceinline__ int half_exponent(float top, bool& bad) {
+  const uint32_t u = __float_as_uint(top), lo = (127 - 63) << 23, hi = (127 + 60) << 23;
+  bad = bad || (u != 0 && u - lo >= hi - lo);
+  return min(max(140 - (int)(u >> 23), -47), 60);
+}
+
+// A [32][DP] tile in two planes of 32 rows; a row's 16 spare bytes put 16
 // consecutive rows' 128-bit reads on distinct banks.
 template <int DP>
-struct SplitTile {
+struct HalfTile {
   static constexpr int kRow = 2 * DP + 16;  // bytes
   static constexpr int kPlane = kTile * kRow;
-  static constexpr int kBytes = 3 * kPlane;
+  static constexpr int kBytes = 2 * kPlane;
   static constexpr int kOcts = DP / 8;
   static constexpr int kPer = kTile * kOcts / kFaThreads;  // 8-column units a thread stages
-  static_assert(kPer * kFaThreads == kTile * kOcts, "whole units");
+  static_assert(kPer * kFaThreads == kTile * kOcts && kOcts <= 16, "whole units, a row in 16 lanes");
   f32x4 f[kPer][2];
-  float top = 0.f;   // largest magnitude of this thread's elements
-  uint32_t rem = 0;  // what the splits left over (bf16_split_pair)
+  int ex[kPer];  // exponents of the rows that `store` has scaled
 
   // Row of unit i of thread tid, and its first column.
   __device__ __forceinline__ static int row(int i, int tid) { return (tid + i * kFaThreads) / kOcts; }
-  __device__ __forceinline__ static int col(int i, int tid) { return 8 * (tid % kOcts); }
+  __device__ __forceinline__ static int col(int tid) { return 8 * (tid % kOcts); }
   // `at(r)` is the pointer to row r of the tile, null for a row that is not read.
   template <typename At>
   __device__ __forceinline__ void load(int d, int tid, At at) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const float* p = at(row(i, tid));
-      const int c = col(i, tid);
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         f[i][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (p && c + 4 * g < d) f[i][g] = *reinterpret_cast<const f32x4*>(p + c + 4 * g);
+        if (p && col(tid) + 4 * g < d) f[i][g] = *reinterpret_cast<const f32x4*>(p + col(tid) + 4 * g);
       }
     }
   }
-  // Piece n of 12 kPer of `store`: a third of a pair's split, the stores after a
-  // unit's last.
-  u32x4 w[3];
-  __device__ __forceinline__ void store_piece(int n, char* s, int tid) {
-    const int i = n / 12, e = n / 3 % 4, piece = n % 3;
-    float u = f[i][e >> 1][2 * (e & 1)], v = f[i][e >> 1][2 * (e & 1) + 1];
-    if (piece == 0) top = fmaxf(fmaxf(top, fabsf(u)), fabsf(v));
-    uint32_t part;
-    split_piece(piece, u, v, part, rem);
-    w[piece][e] = part;
-    f[i][e >> 1][2 * (e & 1)] = u;
-    f[i][e >> 1][2 * (e & 1) + 1] = v;
-    if (e == 3 && piece == 2) {
-#pragma unroll
-      for (int p = 0; p < 3; ++p)
-        *reinterpret_cast<u32x4*>(s + p * kPlane + row(i, tid) * kRow + 2 * col(i, tid)) = w[p];
-    }
-  }
-  __device__ __forceinline__ void store(char* s, int tid) {
+  __device__ __forceinline__ void store(char* s, int tid, bool& bad) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      u32x4 parts[3];
+      float top = 0.f;
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) top = fmaxf(fmaxf(top, fabsf(f[i][g][2 * e])), fabsf(f[i][g][2 * e + 1]));
+      top = fmaxf(top, dpp_quad_xor1(top));
+      top = fmaxf(top, dpp_quad_xor2(top));
+      top = fmaxf(top, dpp_half_mirror(top));
+      if (kOcts == 16) top = fmaxf(top, dpp_row_mirror(top));
+      ex[i] = half_exponent(top, bad);
+      const float m = pow2(ex[i]);
+      u32x4 hi, lo;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float x = f[i][e >> 1][2 * (e & 1)], y = f[i][e >> 1][2 * (e & 1) + 1];
-        uint32_t w[3];
-        top = fmaxf(fmaxf(top, fabsf(x)), fabsf(y));
-        bf16_split_pair(x, y, w, rem);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) parts[p][e] = w[p];
+        uint32_t x, y;
+        half_split_pair(f[i][e >> 1][2 * (e & 1)] * m, f[i][e >> 1][2 * (e & 1) + 1] * m, x, y);
+        hi[e] = x;
+        lo[e] = y;
       }
-#pragma unroll
-      for (int p = 0; p < 3; ++p)
-        *reinterpret_cast<u32x4*>(s + p * kPlane + row(i, tid) * kRow + 2 * col(i, tid)) = parts[p];
+      char* at = s + row(i, tid) * kRow + 2 * col(tid);
+      *reinterpret_cast<u32x4*>(at) = hi;
+      *reinterpret_cast<u32x4*>(at + kPlane) = lo;
     }
   }
 };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// ds_read_b64_tr_b16: 16 lanes read four rows of 16 bf16 each (lane j the four
+// ds_read_b64_tr_b16: 16 lanes read four rows of 16 halves each (lane j the four
 // from column 4 (j % 4) of row j / 4) and lane j receives column j of the rows.
 __device__ __forceinline__ void read_columns(const char* p, uint32_t& lo, uint32_t& hi) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -737,144 +773,131 @@ __device__ __forceinline__ void read_columns(const char* p, uint32_t& lo, uint32
 #endif
 }
 
-// acc += tile . B over the head dim: the tile's 32 rows are the output's rows,
-// B's columns (b[c][part], lane = column) the output's.  A wave issues in order, so
-// the vector work that is to run beside the matrix ops stands between them:
-// `slot(i)` is called after matrix op i and its instructions stay there.  A step's
-// operands are read a step ahead.
-struct NoSlots {
-  __device__ __forceinline__ void operator()(int) const {}
-};
-
-template <int DP, typename Slot = NoSlots>
-__device__ __forceinline__ f32x16 split_rows(const char* s, const u32x4 (&b)[DP / 16][3], int lr, int h,
-                                             Slot slot = Slot()) {
-  constexpr bool kPinned = !std::is_same<Slot, NoSlots>::value;
+// tile . B over the head dim: the tile's 32 rows are the output's rows, B's columns
+// (b[c][part], lane = column) the output's.
+template <int DP>
+__device__ __forceinline__ f32x16 half_rows(const char* s, const u32x4 (&b)[DP / 16][2], int lr, int h) {
   f32x16 acc = zero16();
-  const char* p = s + lr * SplitTile<DP>::kRow + 16 * h;
-  constexpr int kAhead = kPinned ? 1 : 0;
-  u32x4 x[1 + kAhead][3];
-  auto read = [&](int c) {
-#pragma unroll
-    for (int i = 0; i < 3; ++i) x[c & kAhead][i] = *reinterpret_cast<const u32x4*>(p + i * SplitTile<DP>::kPlane + 32 * c);
-  };
-  if (kPinned) read(0);
+  const char* p = s + lr * HalfTile<DP>::kRow + 16 * h;
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) {
-    if (c + kAhead < DP / 16) read(c + kAhead);
+    u32x4 x[2];
 #pragma unroll
-    for (int i = 0; i < kSplitProducts; ++i) {
-      acc = mfma_bf16(x[c & kAhead][kSplitA[i]], b[c][kSplitB[i]], acc);
-      if (kPinned) sched_fence();
-      slot(c * kSplitProducts + i);
-      if (kPinned) sched_fence();
-    }
+    for (int i = 0; i < 2; ++i) x[i] = *reinterpret_cast<const u32x4*>(p + i * HalfTile<DP>::kPlane + 32 * c);
+#pragma unroll
+    for (int i = 0; i < kHalfProducts; ++i) acc = mfma_f16(x[kHalfA[i]], b[c][kHalfB[i]], acc);
   }
   return acc;
 }
 
-// acc[b] += tile^T . P over rows 16 K0 .. 16 K1 - 1 of the tile: column 32 b + lr of
-// it, its rows in the order of the accumulator registers that pp[k] (rows 16 k ..)
-// was made of.  `slot` as above.
-template <int DP, int K0, int K1, typename Slot = NoSlots>
-__device__ __forceinline__ void split_cols(const char* s, const u32x4 (&pp)[2][3], int lane, f32x16 (&acc)[DP / 32],
-                                           Slot slot = Slot()) {
-  using T = SplitTile<DP>;
-  constexpr bool kPinned = !std::is_same<Slot, NoSlots>::value;
-  constexpr int NB = DP / 32;
+// acc[b] += tile^T . x over rows 16 k .. 16 k + 15 of the tile, x = accumulator
+// registers 8 k .. 8 k + 7: column 32 b + lr of the tile.
+template <int DP>
+__device__ __forceinline__ void half_cols(const char* s, const f32x16& x, int k, int lane, f32x16 (&acc)[DP / 32]) {
+  using T = HalfTile<DP>;
   const int h = lane >> 5, j = lane & 15;
-  const char* p = s + (4 * h + (j >> 2)) * T::kRow + 2 * (16 * ((lane >> 4) & 1) + 4 * (j & 3));
-  constexpr int kAhead = kPinned ? 1 : 0;
-  u32x4 x[1 + kAhead][3];
-  auto read = [&](int g) {  // block g % NB of row half g / NB
-    const char* at = p + 16 * (g / NB) * T::kRow + 64 * (g % NB);
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      uint32_t w[4];
-      read_columns(at + i * T::kPlane, w[0], w[1]);
-      read_columns(at + i * T::kPlane + 8 * T::kRow, w[2], w[3]);
-      x[g & kAhead][i] = u32x4{w[0], w[1], w[2], w[3]};
-    }
-  };
-  if (kPinned) read(K0 * NB);
-#pragma unroll
-  for (int g = K0 * NB; g < K1 * NB; ++g) {
-    if (g + kAhead < K1 * NB) read(g + kAhead);
-#pragma unroll
-    for (int i = 0; i < kSplitProducts; ++i) {
-      acc[g % NB] = mfma_bf16(x[g & kAhead][kSplitA[i]], pp[g / NB][kSplitB[i]], acc[g % NB]);
-      if (kPinned) sched_fence();
-      slot((g - K0 * NB) * kSplitProducts + i);
-      if (kPinned) sched_fence();
-    }
-  }
-}
-
-// The three parts of accumulator registers 8 k .. 8 k + 7, the right operand of
-// the products over rows 16 k .. of the tile.
-__device__ __forceinline__ void split_regs(const f32x16& s, int k, u32x4 (&pp)[2][3], uint32_t& rem) {
+  const char* p = s + (16 * k + 4 * h + (j >> 2)) * T::kRow + 2 * (16 * ((lane >> 4) & 1) + 4 * (j & 3));
+  u32x4 pp[2];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    uint32_t w[3];
-    bf16_split_pair(s[8 * k + 2 * e], s[8 * k + 2 * e + 1], w, rem);
+    uint32_t hi, lo;
+    half_split_pair(x[8 * k + 2 * e], x[8 * k + 2 * e + 1], hi, lo);
+    pp[0][e] = hi;
+    pp[1][e] = lo;
+  }
 #pragma unroll
-    for (int p = 0; p < 3; ++p) pp[k][p][e] = w[p];
+  for (int b = 0; b < DP / 32; ++b) {
+    u32x4 y[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t w[4];
+      read_columns(p + i * T::kPlane + 64 * b, w[0], w[1]);
+      read_columns(p + i * T::kPlane + 64 * b + 8 * T::kRow, w[2], w[3]);
+      y[i] = u32x4{w[0], w[1], w[2], w[3]};
+    }
+#pragma unroll
+    for (int i = 0; i < kHalfProducts; ++i) acc[b] = mfma_f16(y[kHalfA[i]], pp[kHalfB[i]], acc[b]);
   }
 }
 
-// Piece n of 24 of splitting registers s[0 .. 15] (a pair in three) into the right
-// operands pp of the products over the tile's rows.
-__device__ __forceinline__ void regs_piece(int n, f32x16& s, u32x4 (&pp)[2][3], uint32_t& rem) {
-  const int e = n / 3, piece = n % 3;
-  float u = s[2 * e], v = s[2 * e + 1];
-  uint32_t w;
-  split_piece(piece, u, v, w, rem);
-  s[2 * e] = u;
-  s[2 * e + 1] = v;
-  pp[e / 4][piece][e % 4] = w;
-}
-
-// A lane's row (its half's octets of each 16 columns) times f, in parts.
+// A lane's row (its half's octets of each 16 columns) times f, in parts; returns what
+// undoes the row's scale.
 template <int DP>
-__device__ __forceinline__ void split_row(const float* p, int d, float f, int h, u32x4 (&out)[DP / 16][3], float& top,
-                                          uint32_t& rem) {
+__device__ __forceinline__ float half_row(const float* p, int d, float f, int h, u32x4 (&out)[DP / 16][2], bool& bad) {
+  f32x4 x[DP / 16][2];
+  float top = 0.f;
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const int dd = 16 * c + 8 * h + 4 * g;
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
-      if (p && dd < d) x = *reinterpret_cast<const f32x4*>(p + dd);
+      x[c][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (p && dd < d) x[c][g] = *reinterpret_cast<const f32x4*>(p + dd) * f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float u = x[2 * e] * f, v = x[2 * e + 1] * f;
-        // rounded here: fused into the split's first subtraction, a product would
-        // leave bits that three parts do not hold
-        asm volatile("" : "+v"(u), "+v"(v));
-        uint32_t w[3];
-        top = fmaxf(fmaxf(top, fabsf(u)), fabsf(v));
-        bf16_split_pair(u, v, w, rem);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) out[c][i][2 * g + e] = w[i];
-      }
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[c][g][e]));
     }
   }
+  const int ex = half_exponent(half_swap_max(top), bad);
+  const float m = pow2(ex);
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t hi, lo;
+      half_split_pair(x[c][e >> 1][2 * (e & 1)] * m, x[c][e >> 1][2 * (e & 1) + 1] * m, hi, lo);
+      out[c][0][e] = hi;
+      out[c][1][e] = lo;
+    }
+  }
+  return pow2(-ex);
 }
 
-__device__ __forceinline__ float wave_top(float v) {
-  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_max(v))));
+// The power of two that a lane's P or dS, times 2^-e of the other operand's rows, is
+// scaled by.  x holds a tile's, scaled by it already, of magnitudes up to `top`: the
+// first tile sets it such that the largest is in [2^13, 2^14), a later one lowers it,
+// with the sums so far, when it passes 2^15.
+template <int NB>
+struct HalfScale {
+  int log = 0;
+  float most = -1.f, big = 0.f;  // `big`: the largest so far
+  __device__ __forceinline__ void follow(float top, f32x16& x, f32x16 (&acc)[NB], bool& bad) {
+    top = half_swap_max(top);
+    big = fmaxf(big, top);
+    if (!__any(top > most)) return;
+    const int to = top > most ? log + 140 - (int)(__float_as_uint(big) >> 23) : log;
+    bad = bad || top > pow2(120) || to < -100;  // more than fp32 would have left to scale
+    const int by = min(min(max(to, -100), 100) - log, 126);
+    const float f = ldexpf(1.f, by);
+    log += by;
+    big *= f;
+    most = 32768.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] *= f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[b][r] *= f;
+    }
+  }
+  __device__ __forceinline__ float undo() const { return pow2(-log); }
+};
+
+// Rows 8 g + 4 h .. of a tile's row values.
+__device__ __forceinline__ f32x4 row_values(const float* x, int g, int h) {
+  return *reinterpret_cast<const f32x4*>(x + 8 * g + 4 * h);
 }
 
-// Forward.  The running maximum m of a row follows its scores only when they pass
-// it by 2^8 (the sums stay far from fp32's end), so O is rarely rescaled.
+// Forward.  The running maximum m of a row follows its scores only when they pass it
+// by 2^4, so O is rarely rescaled; when it moves, the scale of P is found again.
 template <int DP>
-__global__ void __launch_bounds__(kFaThreads, DP == 64 ? 2 : 1)
+__global__ void __launch_bounds__(kFaThreads, DP == 64 ? 3 : 2)
 cross_fwd_split_kernel(const CaArgs a) {
-  using Tile = SplitTile<DP>;
+  using Tile = HalfTile<DP>;
   constexpr int NB = DP / 32;
   __shared__ __attribute__((aligned(16))) char ks[2][Tile::kBytes];
   __shared__ __attribute__((aligned(16))) char vs[2][Tile::kBytes];
-  __shared__ uint32_t range[3];  // largest magnitude of K, of V (as bits), what their splits left over
+  __shared__ __attribute__((aligned(16))) float kf[2][kTile], vf[2][kTile];  // 2^-e of the rows
+  __shared__ int not_held;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lr = lane & 31, h = lane >> 5;
   const int bh = blockIdx.x % a.BH;
@@ -887,137 +910,115 @@ cross_fwd_split_kernel(const CaArgs a) {
   const int qi = qb * kBlock + wave * kTile + lr;  // this lane's row
   const bool work = qb * kBlock + wave * kTile < a.R;
   const float* Q = qi < a.R ? a.q.p + ca_row(a.q, a, bh, qi) : nullptr;
-  if (tid < 3) range[tid] = 0u;
+  if (tid == 0) not_held = 0;
 
-  u32x4 qp[DP / 16][3];
-  float q_top = 0.f;
-  uint32_t q_rem = 0, p_rem = 0;
-  split_row<DP>(Q, a.d, a.scale_log2, h, qp, q_top, q_rem);
-  const bool q_exact = !__any((q_rem & kSplitRemBits) != 0);
-  q_top = wave_top(q_top);
+  u32x4 qp[DP / 16][2];
+  bool row_bad = false, bad = false;
+  const float qf = half_row<DP>(Q, a.d, a.scale_log2, h, qp, row_bad);
   f32x16 o[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) o[b] = zero16();
   float m = -INFINITY, l = 0.f;
+  HalfScale<NB> fit;
 
-  // A tile of log2 scores before its exponentials: what is masked, and m with what
-  // has been summed so far where m moves.
-  auto follow = [&](f32x16& s, int kv0) {
+  auto follow = [&](float mx, float slack) {
+    mx = half_swap_max(mx);
+    const bool move = mx > m + slack;
+    if (!__any(move)) return;
+    const float alpha = move ? fast_exp2(m - mx) : 1.f;
+    if (move) {
+      m = mx;
+      fit.most = -1.f;
+    }
+    l *= alpha;
+    fit.big *= alpha;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[b][r] *= alpha;
+    }
+  };
+  auto compute = [&](int buf, int kv0) {
+    f32x16 s = half_rows<DP>(ks[buf], qp, lr, h);
+    float mx = -INFINITY, ps = 0.f, top = 0.f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 k4 = row_values(kf[buf], g, h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[4 * g + e] *= k4[e];
+    }
     if (kv0 + kTile > k1) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         if (kv0 + acc_row(r, h) >= k1) s[r] = -INFINITY;
     }
-    float mx = s[0];
 #pragma unroll
-    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-    mx = half_swap_max(mx);
-    if (__any(mx > m + 8.f)) {
-      const float mn = mx > m + 8.f ? mx : m;
-      const float alpha = fast_exp2(m - (mn == -INFINITY ? 0.f : mn));
-      m = mn;
-      l *= alpha;
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    follow(mx * qf, 4.f);
+    const float mu = m == -INFINITY ? 0.f : m, f = pow2(fit.log);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 v4 = row_values(vf[buf], g, h);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[b][r] *= alpha;
+      for (int e = 0; e < 4; ++e) {
+        const float p = fast_exp2(s[4 * g + e] * qf - mu);
+        ps += p;
+        s[4 * g + e] = p * v4[e] * f;
+        top = fmaxf(top, s[4 * g + e]);
       }
     }
-  };
-  auto exponentials = [&](f32x16& s) {
-    const float mu = m == -INFINITY ? 0.f : m;
-    float ps = 0.f;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = fast_exp2(s[r] - mu);
-      ps += s[r];
-    }
     l += half_swap_sum(ps);
+    fit.follow(top, s, o, row_bad);
+    half_cols<DP>(vs[buf], s, 0, lane, o);
+    half_cols<DP>(vs[buf], s, 1, lane, o);
   };
 
   const int ntiles = k1 > k0 ? (k1 - k0 + kTile - 1) / kTile : 0;
   Tile kc[2], vc[2];
-  auto load_k = [&](Tile& x, int t) {
+  auto load = [&](int i, int t) {
     const int row0 = k0 + t * kTile;
-    x.load(a.d, tid, [&](int r) { return row0 + r < k1 ? K + (int64_t)(row0 + r) * a.k.st : nullptr; });
+    kc[i].load(a.d, tid, [&](int r) { return row0 + r < k1 ? K + (int64_t)(row0 + r) * a.k.st : nullptr; });
+    vc[i].load(a.d, tid, [&](int r) { return row0 + r < k1 ? V + (int64_t)(row0 + r) * a.v.st : nullptr; });
   };
-  auto load_v = [&](Tile& x, int t) {
-    const int row0 = k0 + t * kTile;
-    x.load(a.d, tid, [&](int r) { return row0 + r < k1 ? V + (int64_t)(row0 + r) * a.v.st : nullptr; });
+  auto store = [&](int i, int buf) {
+    kc[i].store(ks[buf], tid, bad);
+    vc[i].store(vs[buf], tid, bad);
+    if (Tile::col(tid) != 0) return;
+#pragma unroll
+    for (int n = 0; n < Tile::kPer; ++n) {
+      const int r = Tile::row(n, tid);
+      kf[buf][r] = pow2(-kc[i].ex[n]);
+      vf[buf][r] = pow2(-vc[i].ex[n]);
+    }
   };
-  f32x16 s = zero16();
   if (ntiles > 0) {
-    load_k(kc[0], 0);
-    load_v(vc[0], 0);
-    load_k(kc[1], 1);
-    kc[0].store(ks[0], tid);
-    vc[0].store(vs[0], tid);
-    load_k(kc[0], 2);
-    load_v(vc[0], 1);
-    kc[1].store(ks[1], tid);
+    load(0, 0);
+    load(1, 1);
+    store(0, 0);
+    load(0, 2);
   }
   lds_barrier();
-  if (work && ntiles > 0) s = split_rows<DP>(ks[0], qp, lr, h);
-  lds_barrier();  // K tile 0's buffer is refilled in iteration 0
-  // Iteration t: K tile t + 1 and V tile t are in LDS; K t + 2 and V t + 1, loaded an
-  // iteration ago, are staged (kn, vn), K t + 3 and V t + 2 are sent for (kl, vl).
-  auto step = [&](int t, Tile& kn, Tile& vn, Tile& kl, Tile& vl) {
-    load_k(kl, t + 3);
-    load_v(vl, t + 2);
-    if (work) {
-      follow(s, k0 + t * kTile);
-      const float mu = m == -INFINITY ? 0.f : m;
-      float ps = 0.f;
-      u32x4 pp[2][3];
-      constexpr int kEach = DP / 64;  // matrix ops per piece
-      const f32x16 next = split_rows<DP>(ks[(t + 1) & 1], qp, lr, h, [&](int i) {
-        if (i % kEach != 0) return;
-        const int n = i / kEach, e = n / 3;
-        if (n % 3 == 0) {
-          s[2 * e] = fast_exp2(s[2 * e] - mu);
-          s[2 * e + 1] = fast_exp2(s[2 * e + 1] - mu);
-          ps += s[2 * e];
-          ps += s[2 * e + 1];
-        }
-        regs_piece(n, s, pp, p_rem);
-      });
-      l += half_swap_sum(ps);
-      split_cols<DP, 0, 2>(vs[t & 1], pp, lane, o, [&](int i) {
-        constexpr int kHalf = 12 * Tile::kPer;
-        if (i < kHalf) kn.store_piece(i, ks[t & 1], tid);
-        else vn.store_piece(i - kHalf, vs[(t + 1) & 1], tid);
-      });
-      s = next;
-    } else {
-      kn.store(ks[t & 1], tid);
-      vn.store(vs[(t + 1) & 1], tid);
-    }
-    lds_barrier();
-  };
+  // Iteration t: tile t in LDS, t + 1 in registers, t + 2 on its way, t + 3 sent for.
   for (int t = 0; t < ntiles; t += 2) {
-    step(t, kc[0], vc[0], kc[1], vc[1]);
-    if (t + 1 < ntiles) step(t + 1, kc[1], vc[1], kc[0], vc[0]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (t + u >= ntiles) break;
+      if (work) compute(u, k0 + (t + u) * kTile);
+      store(1 - u, 1 - u);
+      load(1 - u, t + u + 3);
+      lds_barrier();
+    }
+  }
+  const float by = fit.undo();
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[b][r] *= by;
   }
 
-  // What the split does not cover: sums that might overflow, an element of q, K or
-  // V that is not held exactly, and probabilities below 2^-110 where O is so
-  // small that it feels them.  Such a wave's rows are redone with the fp32
-  // instruction, straight from HBM.
-  atomicMax(&range[0], __float_as_uint(fmaxf(kc[0].top, kc[1].top)));  // >= 0: ordered as their bits
-  atomicMax(&range[1], __float_as_uint(fmaxf(vc[0].top, vc[1].top)));
-  atomicOr(&range[2], kc[0].rem | kc[1].rem | vc[0].rem | vc[1].rem);
+  if (bad) not_held = 1;
   __syncthreads();
-  const float v_top = __uint_as_float(range[1]), n = (float)(k1 - k0);
-  bool redo = !q_exact || (range[2] & kSplitRemBits) != 0 ||
-              split_overflows(q_top, __uint_as_float(range[0]), (float)a.d) || split_overflows(256.f, v_top, n);
-  if (__any((p_rem & kSplitRemBits) != 0)) {
-    const float floor = split_loss_floor(v_top, 0.f, n);
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) redo = redo || fabsf(o[b][r]) < floor;
-  }
-  if (work && ntiles > 0 && __any(redo)) {
+  if (work && ntiles > 0 && __any(row_bad || not_held)) {
     m = -INFINITY;
     l = 0.f;
 #pragma unroll
@@ -1026,21 +1027,32 @@ cross_fwd_split_kernel(const CaArgs a) {
       const int kv0 = k0 + t * kTile;
       f32x16 s = zero16();
       for (int c = 0; c < a.d; c += 2) {
-        const bool on = c + h < a.d;
-        const float kf = on && kv0 + lr < k1 ? K[(int64_t)(kv0 + lr) * a.k.st + c + h] : 0.f;
-        const float qf = on && Q ? Q[c + h] * a.scale_log2 : 0.f;
-        s = mfma32(kf, qf, s);
+        const bool in = c + h < a.d;
+        s = mfma32(in && kv0 + lr < k1 ? K[(int64_t)(kv0 + lr) * a.k.st + c + h] : 0.f,
+                   in && Q ? Q[c + h] * a.scale_log2 : 0.f, s);
       }
-      follow(s, kv0);
-      exponentials(s);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        if (kv0 + acc_row(r, h) >= k1) s[r] = -INFINITY;
+        mx = fmaxf(mx, s[r]);
+      }
+      follow(mx, 0.f);
+      const float mu = m == -INFINITY ? 0.f : m;
+      float ps = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = fast_exp2(s[r] - mu);
+        ps += s[r];
+      }
+      l += half_swap_sum(ps);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const int col = b * 32 + lr;
 #pragma unroll
         for (int st = 0; st < 16; ++st) {
           const int row = kv0 + acc_row(st, h);
-          const float v = row < k1 && col < a.d ? V[(int64_t)row * a.v.st + col] : 0.f;
-          o[b] = mfma32(v, s[st], o[b]);
+          o[b] = mfma32(row < k1 && col < a.d ? V[(int64_t)row * a.v.st + col] : 0.f, s[st], o[b]);
         }
       }
     }
@@ -1049,13 +1061,15 @@ cross_fwd_split_kernel(const CaArgs a) {
 }
 
 // dQ (and D).
-__global__ void __launch_bounds__(kFaThreads, 2)
+template <int DP>
+__global__ void __launch_bounds__(kFaThreads, DP == 64 ? 3 : 1)
 cross_bwd_dq_split_kernel(const CaArgs a) {
-  constexpr int DP = 64, NB = 2;
-  using Tile = SplitTile<DP>;
+  constexpr int NB = DP / 32;
+  using Tile = HalfTile<DP>;
   __shared__ __attribute__((aligned(16))) char ks[2][Tile::kBytes];
   __shared__ __attribute__((aligned(16))) char vs[2][Tile::kBytes];
-  __shared__ uint32_t range[3];
+  __shared__ __attribute__((aligned(16))) float kf[2][kTile], vf[2][kTile];  // 2^-e of the rows
+  __shared__ int not_held;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lr = lane & 31, h = lane >> 5;
   const int bh = blockIdx.x % a.BH, rest = blockIdx.x / a.BH;
@@ -1067,7 +1081,7 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
   const bool row_ok = qi < a.R, work = qb * kBlock + wave * kTile < a.R;
   const float* Q = row_ok ? a.q.p + ca_row(a.q, a, bh, qi) : nullptr;
   const float* dO = row_ok ? a.dout.p + ca_row(a.dout, a, bh, qi) : nullptr;
-  if (tid < 3) range[tid] = 0u;
+  if (tid == 0) not_held = 0;
 
   float dsum = 0.f;
   if (row_ok) {
@@ -1086,26 +1100,15 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
   if (l2 == -INFINITY) l2 = INFINITY;  // a row without keys has P = 0
   if (row_ok && h == 0 && part == 0) a.D[(int64_t)bh * a.R + qi] = dsum;
 
-  u32x4 qp[DP / 16][3], dop[DP / 16][3];
-  float q_top = 0.f, do_top = 0.f, ds_top = 0.f;
-  uint32_t in_rem = 0, ds_rem = 0;
-  split_row<DP>(Q, a.d, a.scale_log2, h, qp, q_top, in_rem);
-  split_row<DP>(dO, a.d, 1.f, h, dop, do_top, in_rem);
-  const bool exact = !__any((in_rem & kSplitRemBits) != 0);
-  q_top = wave_top(q_top);
-  do_top = wave_top(do_top);
+  u32x4 qp[DP / 16][2], dop[DP / 16][2];
+  bool row_bad = false, bad = false;
+  const float qf = half_row<DP>(Q, a.d, a.scale_log2, h, qp, row_bad);
+  const float df = half_row<DP>(dO, a.d, 1.f, h, dop, row_bad);
   f32x16 dq[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) dq[b] = zero16();
+  HalfScale<NB> fit;
 
-  // dS of a tile from its log2 scores and dP.
-  auto dscore = [&](const f32x16& s, f32x16& dp, int kv0) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float x = fast_exp2(s[r] - l2) * (dp[r] - dsum);
-      dp[r] = kv0 + acc_row(r, h) < k1 ? x : 0.f;
-    }
-  };
   const int ntiles = k1 > k0 ? (k1 - k0 + kTile - 1) / kTile : 0;
   Tile kc, vc;
   auto load = [&](int t) {
@@ -1113,51 +1116,65 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
     kc.load(a.d, tid, [&](int r) { return row0 + r < k1 ? K + (int64_t)(row0 + r) * a.k.st : nullptr; });
     vc.load(a.d, tid, [&](int r) { return row0 + r < k1 ? V + (int64_t)(row0 + r) * a.v.st : nullptr; });
   };
+  auto store = [&](int buf) {
+    kc.store(ks[buf], tid, bad);
+    vc.store(vs[buf], tid, bad);
+    if (Tile::col(tid) != 0) return;
+#pragma unroll
+    for (int n = 0; n < Tile::kPer; ++n) {
+      const int r = Tile::row(n, tid);
+      kf[buf][r] = pow2(-kc.ex[n]);
+      vf[buf][r] = pow2(-vc.ex[n]);
+    }
+  };
   if (ntiles > 0) {
     load(0);
-    kc.store(ks[0], tid);
-    vc.store(vs[0], tid);
+    store(0);
   }
   lds_barrier();
   for (int t = 0; t < ntiles; ++t) {
+    const int buf = t & 1, kv0 = k0 + t * kTile;
     const bool has_next = t + 1 < ntiles;
     if (has_next) load(t + 1);
     if (work) {
-      const f32x16 s = split_rows<DP>(ks[t & 1], qp, lr, h);
-      f32x16 dp = split_rows<DP>(vs[t & 1], dop, lr, h);
-      dscore(s, dp, k0 + t * kTile);
+      const f32x16 s = half_rows<DP>(ks[buf], qp, lr, h);
+      f32x16 dp = half_rows<DP>(vs[buf], dop, lr, h);
+      float top = 0.f;
+      const float f = pow2(fit.log), dpf = df * f, dsf = dsum * f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) ds_top = fmaxf(ds_top, fabsf(dp[r]));
-      u32x4 pp[2][3];
-      split_regs(dp, 0, pp, ds_rem);
-      split_cols<DP, 0, 1>(ks[t & 1], pp, lane, dq);
-      split_regs(dp, 1, pp, ds_rem);
-      split_cols<DP, 1, 2>(ks[t & 1], pp, lane, dq);
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 k4 = row_values(kf[buf], g, h), v4 = row_values(vf[buf], g, h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          const float p = fast_exp2(s[r] * k4[e] * qf - l2);
+          dp[r] = p * (dp[r] * v4[e] * dpf - dsf) * k4[e];
+        }
+      }
+      if (kv0 + kTile > k1) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (kv0 + acc_row(r, h) >= k1) dp[r] = 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(dp[r]));
+      fit.follow(top, dp, dq, row_bad);
+      half_cols<DP>(ks[buf], dp, 0, lane, dq);
+      half_cols<DP>(ks[buf], dp, 1, lane, dq);
     }
-    if (has_next) {
-      kc.store(ks[(t + 1) & 1], tid);
-      vc.store(vs[(t + 1) & 1], tid);
-    }
+    if (has_next) store(buf ^ 1);
     lds_barrier();
   }
-
-  // As in the forward: a wave whose operands or sums the parts do not hold is redone.
-  atomicMax(&range[0], __float_as_uint(kc.top));
-  atomicMax(&range[1], __float_as_uint(vc.top));
-  atomicOr(&range[2], kc.rem | vc.rem);
-  __syncthreads();
-  const float k_top = __uint_as_float(range[0]), d = (float)a.d, n = (float)(k1 - k0);
-  ds_top = wave_top(ds_top);
-  bool redo = !exact || (range[2] & kSplitRemBits) != 0 || split_overflows(q_top, k_top, d) ||
-              split_overflows(do_top, __uint_as_float(range[1]), d) || split_overflows(ds_top, k_top, n);
-  if (__any((ds_rem & kSplitRemBits) != 0)) {
-    const float floor = split_loss_floor(k_top, 0.f, n);
+  const float by = fit.undo();
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+  for (int b = 0; b < NB; ++b) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) redo = redo || fabsf(dq[b][r]) < floor;
+    for (int r = 0; r < 16; ++r) dq[b][r] *= by;
   }
-  if (work && ntiles > 0 && __any(redo)) {
+
+  if (bad) not_held = 1;
+  __syncthreads();
+  if (work && ntiles > 0 && __any(row_bad || not_held)) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) dq[b] = zero16();
     for (int t = 0; t < ntiles; ++t) {
@@ -1168,7 +1185,11 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
         s = mfma32(key ? K[(int64_t)(kv0 + lr) * a.k.st + c + h] : 0.f, in && Q ? Q[c + h] * a.scale_log2 : 0.f, s);
         dp = mfma32(key ? V[(int64_t)(kv0 + lr) * a.v.st + c + h] : 0.f, in && dO ? dO[c + h] : 0.f, dp);
       }
-      dscore(s, dp, kv0);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = fast_exp2(s[r] - l2) * (dp[r] - dsum);
+        dp[r] = kv0 + acc_row(r, h) < k1 ? x : 0.f;
+      }
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const int col = b * 32 + lr;
@@ -1184,15 +1205,16 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
 }
 
 // dK and dV.
-__global__ void __launch_bounds__(kFaThreads, 2)
+template <int DP>
+__global__ void __launch_bounds__(kFaThreads, DP == 64 ? 2 : 1)
 cross_bwd_dkdv_split_kernel(const CaArgs a) {
-  constexpr int DP = 64, NB = 2;
-  using Tile = SplitTile<DP>;
+  constexpr int NB = DP / 32;
+  using Tile = HalfTile<DP>;
   __shared__ __attribute__((aligned(16))) char qs[2][Tile::kBytes];
   __shared__ __attribute__((aligned(16))) char dos[2][Tile::kBytes];
-  __shared__ __attribute__((aligned(16))) float ls[2][kTile];
-  __shared__ __attribute__((aligned(16))) float ds[2][kTile];
-  __shared__ uint32_t range[3];
+  // 2^-e of Q's rows, of dO's, of both; lse in log2 and D 2^-e of Q's
+  __shared__ __attribute__((aligned(16))) float qf[2][kTile], df[2][kTile], of[2][kTile], ls[2][kTile], ds[2][kTile];
+  __shared__ int not_held;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lr = lane & 31, h = lane >> 5;
   const int bh = blockIdx.x % a.BH, rest = blockIdx.x / a.BH;
@@ -1203,39 +1225,21 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
   const bool key_ok = kj < len, work = kw < len;
   const float* K = key_ok ? ca_head(a.k, a, bh) + (int64_t)kj * a.k.st : nullptr;
   const float* V = key_ok ? ca_head(a.v, a, bh) + (int64_t)kj * a.v.st : nullptr;
-  if (tid < 3) range[tid] = 0u;
+  if (tid == 0) not_held = 0;
 
-  u32x4 kp[DP / 16][3], vp[DP / 16][3];
-  float k_top = 0.f, v_top = 0.f, ds_top = 0.f;
-  uint32_t in_rem = 0, p_rem = 0, ds_rem = 0;
-  split_row<DP>(K, a.d, a.scale_log2, h, kp, k_top, in_rem);
-  split_row<DP>(V, a.d, 1.f, h, vp, v_top, in_rem);
-  const bool exact = !__any((in_rem & kSplitRemBits) != 0);
-  k_top = wave_top(k_top);
-  v_top = wave_top(v_top);
+  u32x4 kp[DP / 16][2], vp[DP / 16][2];
+  bool key_bad = false, bad = false;
+  const float kf = half_row<DP>(K, a.d, a.scale_log2, h, kp, key_bad);
+  const float vf = half_row<DP>(V, a.d, 1.f, h, vp, key_bad);
   f32x16 dk[NB], dv[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) dk[b] = dv[b] = zero16();
+  HalfScale<NB> fit_k, fit_v;
   const int t0 = part * a.kv_tiles;
   const int t1 = kb * kBlock < len ? min((a.R + kTile - 1) / kTile, t0 + a.kv_tiles) : t0;
 
-  // P (in s) and dS (in dp) of a tile; `stat(g, l4, d4)` gives the lse and D of rows 8 g + 4 h ..
-  auto dscore = [&](f32x16& s, f32x16& dp, auto stat) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      f32x4 l4, d4;
-      stat(g, l4, d4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 4 * g + e;
-        const float p = key_ok ? fast_exp2(s[r] - l4[e]) : 0.f;
-        s[r] = p;
-        dp[r] = key_ok ? p * (dp[r] - d4[e]) : 0.f;
-      }
-    }
-  };
   Tile qc, dc;
-  float lreg = 0.f, dreg = 0.f;
+  float lreg[Tile::kPer], dreg[Tile::kPer];
   auto lse_of = [&](int r) {
     const float x = r < a.R ? a.lse[(int64_t)bh * a.R + r] * kLog2e : INFINITY;
     return x == -INFINITY ? INFINITY : x;  // a row without keys, or past the end, has P = 0
@@ -1245,17 +1249,27 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
     const int row0 = t * kTile;
     qc.load(a.d, tid, [&](int r) { return row0 + r < a.R ? a.q.p + ca_row(a.q, a, bh, row0 + r) : nullptr; });
     dc.load(a.d, tid, [&](int r) { return row0 + r < a.R ? a.dout.p + ca_row(a.dout, a, bh, row0 + r) : nullptr; });
-    if (tid < kTile) {
-      lreg = lse_of(row0 + tid);
-      dreg = d_of(row0 + tid);
+#pragma unroll
+    for (int n = 0; n < Tile::kPer; ++n) {
+      lreg[n] = dreg[n] = 0.f;
+      if (Tile::col(tid) != 0) continue;
+      lreg[n] = lse_of(row0 + Tile::row(n, tid));
+      dreg[n] = d_of(row0 + Tile::row(n, tid));
     }
   };
   auto store = [&](int buf) {
-    qc.store(qs[buf], tid);
-    dc.store(dos[buf], tid);
-    if (tid < kTile) {
-      ls[buf][tid] = lreg;
-      ds[buf][tid] = dreg;
+    qc.store(qs[buf], tid, bad);
+    dc.store(dos[buf], tid, bad);
+    if (Tile::col(tid) != 0) return;
+#pragma unroll
+    for (int n = 0; n < Tile::kPer; ++n) {
+      const int r = Tile::row(n, tid);
+      const float q = pow2(-qc.ex[n]), o = pow2(-dc.ex[n]);
+      qf[buf][r] = q;
+      df[buf][r] = o;
+      of[buf][r] = q * o;
+      ls[buf][r] = lreg[n];
+      ds[buf][r] = dreg[n] * q;
     }
   };
   if (t0 < t1) {
@@ -1268,44 +1282,58 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
     const bool has_next = t + 1 < t1;
     if (has_next) load(t + 1);
     if (work) {
-      f32x16 s = split_rows<DP>(qs[cur], kp, lr, h);
-      f32x16 dp = split_rows<DP>(dos[cur], vp, lr, h);
-      dscore(s, dp, [&](int g, f32x4& l4, f32x4& d4) {
-        l4 = *reinterpret_cast<const f32x4*>(&ls[cur][8 * g + 4 * h]);
-        d4 = *reinterpret_cast<const f32x4*>(&ds[cur][8 * g + 4 * h]);
-      });
+      f32x16 s = half_rows<DP>(qs[cur], kp, lr, h);
+      sched_fence();
+      f32x16 x;
+      float top = 0.f;
+      const float vs = pow2(fit_v.log), ks = pow2(fit_k.log);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) ds_top = fmaxf(ds_top, fabsf(dp[r]));
-      u32x4 pp[2][3];
-      split_regs(s, 0, pp, p_rem);
-      split_cols<DP, 0, 1>(dos[cur], pp, lane, dv);
-      split_regs(dp, 0, pp, ds_rem);
-      split_cols<DP, 0, 1>(qs[cur], pp, lane, dk);
-      split_regs(s, 1, pp, p_rem);
-      split_cols<DP, 1, 2>(dos[cur], pp, lane, dv);
-      split_regs(dp, 1, pp, ds_rem);
-      split_cols<DP, 1, 2>(qs[cur], pp, lane, dk);
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 q4 = row_values(qf[cur], g, h), l4 = row_values(ls[cur], g, h), o4 = row_values(df[cur], g, h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          s[r] = key_ok ? fast_exp2(s[r] * q4[e] * kf - l4[e]) : 0.f;
+          x[r] = s[r] * o4[e] * vs;
+          top = fmaxf(top, x[r]);
+        }
+      }
+      fit_v.follow(top, x, dv, key_bad);
+      half_cols<DP>(dos[cur], x, 0, lane, dv);
+      half_cols<DP>(dos[cur], x, 1, lane, dv);
+      x = half_rows<DP>(dos[cur], vp, lr, h);
+      sched_fence();
+      top = 0.f;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 o4 = row_values(of[cur], g, h), d4 = row_values(ds[cur], g, h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          x[r] = s[r] * (x[r] * o4[e] * vf - d4[e]) * ks;
+          top = fmaxf(top, fabsf(x[r]));
+        }
+      }
+      fit_k.follow(top, x, dk, key_bad);
+      half_cols<DP>(qs[cur], x, 0, lane, dk);
+      half_cols<DP>(qs[cur], x, 1, lane, dk);
     }
     if (has_next) store(cur ^ 1);
     lds_barrier();
   }
-
-  atomicMax(&range[0], __float_as_uint(qc.top));
-  atomicMax(&range[1], __float_as_uint(dc.top));
-  atomicOr(&range[2], qc.rem | dc.rem);
-  __syncthreads();
-  const float q_top = __uint_as_float(range[0]), do_top = __uint_as_float(range[1]), d = (float)a.d, n = (float)a.R;
-  ds_top = wave_top(ds_top);
-  bool redo = !exact || (range[2] & kSplitRemBits) != 0 || split_overflows(k_top, q_top, d) ||
-              split_overflows(v_top, do_top, d) || split_overflows(1.f, do_top, n) || split_overflows(ds_top, q_top, n);
-  if (__any((p_rem & kSplitRemBits) != 0 || (ds_rem & kSplitRemBits) != 0)) {
-    const float fv = split_loss_floor(do_top, 0.f, n), fk = split_loss_floor(q_top, 0.f, n);
+  const float by_v = fit_v.undo(), by_k = fit_k.undo();
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+  for (int b = 0; b < NB; ++b) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) redo = redo || fabsf(dv[b][r]) < fv || fabsf(dk[b][r]) < fk;
+    for (int r = 0; r < 16; ++r) {
+      dv[b][r] *= by_v;
+      dk[b][r] *= by_k;
+    }
   }
-  if (work && t0 < t1 && __any(redo)) {
+
+  if (bad) not_held = 1;
+  __syncthreads();
+  if (work && t0 < t1 && __any(key_bad || not_held)) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) dk[b] = dv[b] = zero16();
     for (int t = t0; t < t1; ++t) {
@@ -1319,13 +1347,12 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
         s = mfma32(in && Q ? Q[c + h] : 0.f, in && K ? K[c + h] * a.scale_log2 : 0.f, s);
         dp = mfma32(in && dO ? dO[c + h] : 0.f, in && V ? V[c + h] : 0.f, dp);
       }
-      dscore(s, dp, [&](int g, f32x4& l4, f32x4& d4) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          l4[e] = lse_of(row0 + 8 * g + 4 * h + e);
-          d4[e] = d_of(row0 + 8 * g + 4 * h + e);
-        }
-      });
+      for (int r = 0; r < 16; ++r) {
+        const int i = row0 + acc_row(r, h);
+        s[r] = key_ok ? fast_exp2(s[r] - lse_of(i)) : 0.f;
+        dp[r] = key_ok ? s[r] * (dp[r] - d_of(i)) : 0.f;
+      }
 #pragma unroll
       for (int st = 0; st < 16; ++st) {
         const int r = row0 + acc_row(st, h);
@@ -1377,7 +1404,10 @@ cross_bwd_sum_kernel(const CaArgs a) {
 
 // ------------------------------------------------------------------ host side
 
-constexpr int kFewRows = 8;    // query rows a key/value head up to which cross_rows_kernel runs
+// Query rows a key/value head up to which cross_rows_kernel runs: 192 heads' 4 rows of
+// 577 keys in 18 us against the tiles' 24; 8 rows would take 23 against 24 (of 4096
+// keys 98 against 90).
+constexpr int kFewRows = 4;
 constexpr int kMaxSplits = 64;
 
 int pad_dim(int64_t d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
@@ -1434,9 +1464,12 @@ void ca_bwd_plan(CaArgs& a) {
   a.kv_splits = (int)std::max<int64_t>(1, ceil_div(qt, c));
 }
 
-// Whether the tiled passes run on the bf16 matrix cores.
-bool ca_fwd_split(const CaArgs& a) { return a.Tk > 64; }
-bool ca_bwd_split(const CaArgs& a) { return a.Tk > 64; }
+// Whether the tiled passes run on the fp16 matrix cores: where rows are 16-byte
+// aligned and longer than 32 floats.  Forward + backward of 384 heads' 256 x 300, d 64:
+// 212 us against 391 with the fp32 instruction, 256 x 7: 86 against 102; 16 x 7 alone
+// loses (27 against 24).  Up to 32 floats, padded to 64, they would do twice the work.
+template <int DP, bool VEC>
+constexpr bool kSplit = VEC && DP >= 64;
 
 bool ca_shape_ok(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk) {
   const int64_t most = int64_t(1) << 24;
@@ -1473,16 +1506,11 @@ int launch_fwd(const CaArgs& a, hipStream_t st) {
   if (a.R <= kFewRows) {
     if (a.R == 1) launch_few<1, VEC>(a, DP, st);
     else if (a.R == 2) launch_few<2, VEC>(a, DP, st);
-    else if (a.R <= 4) launch_few<4, VEC>(a, DP, st);
-    else launch_few<8, VEC>(a, DP, st);
+    else launch_few<4, VEC>(a, DP, st);
   } else {
     const dim3 grid((unsigned)(ceil_div(a.R, kBlock) * a.BH * a.splits));
-    bool split = false;
-    if constexpr (VEC && DP >= 64) {
-      split = ca_fwd_split(a);
-      if (split) cross_fwd_split_kernel<DP><<<grid, dim3(kFaThreads), 0, st>>>(a);
-    }
-    if (!split) cross_fwd_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
+    if constexpr (kSplit<DP, VEC>) cross_fwd_split_kernel<DP><<<grid, dim3(kFaThreads), 0, st>>>(a);
+    else cross_fwd_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
   }
   const int rc = launch_status();
   if (rc != AAR_OK || a.splits == 1) return rc;
@@ -1493,17 +1521,16 @@ int launch_fwd(const CaArgs& a, hipStream_t st) {
 
 template <int DP, bool VEC>
 int launch_bwd(const CaArgs& a, hipStream_t st) {
-  const bool split = VEC && DP == 64 && ca_bwd_split(a);
   if (a.R > 0) {
     const dim3 grid((unsigned)(ceil_div(a.R, kBlock) * a.BH * a.splits));
-    if (split) cross_bwd_dq_split_kernel<<<grid, dim3(kFaThreads), 0, st>>>(a);
+    if constexpr (kSplit<DP, VEC>) cross_bwd_dq_split_kernel<DP><<<grid, dim3(kFaThreads), 0, st>>>(a);
     else cross_bwd_dq_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
     const int rc = launch_status();
     if (rc != AAR_OK) return rc;
   }
   if (a.Tk == 0) return AAR_OK;
   const dim3 grid((unsigned)(ceil_div(a.Tk, kBlock) * a.BH * a.kv_splits));
-  if (split) cross_bwd_dkdv_split_kernel<<<grid, dim3(kFaThreads), 0, st>>>(a);
+  if constexpr (kSplit<DP, VEC>) cross_bwd_dkdv_split_kernel<DP><<<grid, dim3(kFaThreads), 0, st>>>(a);
   else cross_bwd_dkdv_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
   const int rc = launch_status();
   const int64_t rows = (a.splits > 1 ? (int64_t)a.BH * a.R : 0) + (a.kv_splits > 1 ? 2 * (int64_t)a.BH * a.Tk : 0);

@@ -156,6 +156,101 @@ def test_extreme_scores(L, Tq):
     assert (o == 0).all() and (lse == -math.inf).all()
 
 
+@pytest.mark.parametrize("d", [64, 128, 30])
+@pytest.mark.parametrize("Tq,Tk", [(1, 70), (40, 130), (290, 33)])
+def test_powers_of_two(L, d, Tq, Tk):
+    """Powers of two go through every product and sum unrounded, whatever form the
+    operands take inside: rows of dO of magnitudes 2^-40 to 2^40 give dQ's rows times
+    the same, V's gives O and dQ, K's against Q's nothing but the gradients'."""
+    q, do = rand(1, 2, 4, Tq, d), rand(2, 2, 4, Tq, d)
+    k, v = rand(3, 2, 2, Tk, d), rand(4, 2, 2, Tk, d)
+    lens = torch.tensor([Tk, Tk // 2], device="cuda")
+    o, lse, dq, dk, dv = run(L, q, k, v, lens, do)
+    f = torch.exp2(torch.randint(-40, 41, (2, 4, Tq, 1), generator=torch.Generator().manual_seed(5)).float()).cuda()
+    assert torch.equal(run(L, q, k, v, lens, do * f)[2], dq * f)
+    for e in (-40, 40):
+        g = run(L, q, k, v * 2.0 ** e, lens, do)
+        for a, b in zip(g, (o * 2.0 ** e, lse, dq * 2.0 ** e, dk * 2.0 ** e, dv)):
+            assert torch.equal(a, b)
+        g = run(L, q * 2.0 ** -e, k * 2.0 ** e, v, lens, do)
+        for a, b in zip(g, (o, lse, dq * 2.0 ** e, dk * 2.0 ** -e, dv)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("e", [-75, 62])
+@pytest.mark.parametrize("d", [64, 128])
+def test_very_small_and_very_large(L, d, e):
+    """Operands (all of one, or one row of it) whose magnitudes two fp16 parts do not hold."""
+    q, do = rand(1, 2, 2, 50, d), rand(2, 2, 2, 50, d)
+    k, v = rand(3, 2, 2, 100, d), rand(4, 2, 2, 100, d)
+    f, tol = 2.0 ** e, M.attn_tol(d, 100)
+    ref = M.cross_exact(q, k, v, None, do)
+    mass = M.cross_mass(q, k, v, None, do)
+    names = ("o", "lse", "dq", "dk", "dv")
+
+    def same(got, scales):
+        for name, g, r, s in zip(names, got, ref, scales):
+            M.near(g.double() / s, r, tol * (2 if name[0] == "d" else 1), name, mass.get(name))
+
+    same(run(L, q, k, v * f, None, do), (f, 1, f, f, 1))
+    same(run(L, q, k, v, None, do * f), (1, 1, f, f, f))
+    same(run(L, q / f, k * f, v, None, do), (1, 1, f, 1 / f, 1))
+    # one row alone
+    x = v.clone()
+    x[0, 1, 33] *= f
+    got, r = run(L, q, k, x, None, do), M.cross_exact(q, k, x, None, do)
+    w = M.cross_mass(q, k, x, None, do)
+    for name, a, b in zip(names, got, r):
+        M.near(a, b, tol * (2 if name[0] == "d" else 1), name, w.get(name))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_an_outlier_that_no_row_attends_to(L, d):
+    """A value 2^40 times the others' behind a score of -100, a value of zeros that takes most of
+    the weight, and values of 2^-30: the others keep their digits."""
+    q, do = rand(1, 1, 2, 70, d), rand(2, 1, 2, 70, d)
+    k, v = rand(3, 1, 2, 90, d), rand(4, 1, 2, 90, d)
+    q[..., 0] = 8.0
+    k[..., 0] = 0.0
+    k[:, :, 10, 0] = -100.0 / (8.0 * d ** -0.5)
+    v[:, :, 10] *= 2.0 ** 40
+    o, lse = run(L, q, k, v, None)
+    ro, rl = M.cross_exact(q, k, v)
+    M.near(o, ro, M.attn_tol(d, 90, 100.0), "o")
+    v[:, :, 10] *= 2.0 ** -40
+    k[:, :, 10, 0] = 12.0 / (8.0 * d ** -0.5)
+    v[:, :, 10] = 0.0
+    v[:, :, 40] *= 2.0 ** -30
+    got, ref, w = run(L, q, k, v, None, do), M.cross_exact(q, k, v, None, do), M.cross_mass(q, k, v, None, do)
+    for name, a, b in zip(("o", "lse", "dq", "dk", "dv"), got, ref):
+        M.near(a, b, M.attn_tol(d, 90, 16.0) * (2 if name[0] == "d" else 1), name, w.get(name))
+
+
+@pytest.mark.parametrize("d", [64, 128, 30])
+def test_infinities_and_nan(L, d):
+    """Where keys, values or gradients hold them, as fp32 arithmetic has it."""
+    q, do = rand(1, 2, 2, 40, d), rand(2, 2, 2, 40, d)
+    k, v = rand(3, 2, 2, 80, d), rand(4, 2, 2, 80, d)
+    tol = M.attn_tol(d, 80)
+    for bad in (math.inf, -math.inf, math.nan):
+        x = v.clone()
+        x[0, 1, 35, 3] = bad
+        o, lse = run(L, q, k, x, None)
+        ro, rl = M.cross_exact(q, k, x)
+        M.near(o, ro, tol, "o")
+        M.near(lse, rl, tol, "lse", M.cross_mass(q, k, v, None, do)["lse"])
+        g = do.clone()
+        g[1, 0, 7, 2] = bad
+        o, lse, dq, dk, dv = run(L, q, k, v, None, g)
+        clean = run(L, q, k, v, None, do)
+        # dP - D is inf - inf for the keys whose value has D's sign there, inf for the others
+        assert torch.isnan(dq[1, 0, 7]).all() and not torch.isfinite(dk[1, 0]).any()
+        assert not torch.isfinite(dv[1, 0, :, 2]).any()
+        other = torch.ones_like(dq, dtype=torch.bool)
+        other[1, 0] = False
+        assert torch.equal(dq[other], clean[2][other]) and torch.isfinite(dq[1, 0, 8:]).all()
+
+
 def test_gradients_against_differences(L):
     """d/dh of sum(do * O) along random directions, from forwards alone, in steps
     whose own error is of order h^2."""
