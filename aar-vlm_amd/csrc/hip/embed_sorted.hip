@@ -167,6 +167,8 @@ embed_sort_kernel(const int64_t* __restrict__ ids, int n, int vocab, int slice, 
         sid[at + rank] = v0 + r[u];
         if (rank == 0) mine[r[u]] = at + count;
       }
+      // The next group's lanes read what these wrote: LDS keeps a wave's order, and this the compiler's.
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
   }
 }
