@@ -305,11 +305,13 @@ distill_bwd_kernel(const float* __restrict__ grad, const float* __restrict__ Z, 
   }
 }
 
-// Short rows (V <= 256, up to 64 entries): 16 lanes a row, four rows a wave, the
+// Short rows (V <= 80, up to 16 entries): 16 lanes a row, four rows a wave, the
 // row in registers.  With a wave a row, most lanes of a character vocabulary's
-// rows are idle (16384 x 65: 12.9 + 12.2 us).
-constexpr int kShortVocab = 256, kShortTop = 64, kShortLanes = 16;
-constexpr int kShortRows = 256 / kShortLanes;  // of a workgroup
+// rows are idle: 16384 x 65 forward + backward 15.6 us against 30.9.  4096 x 256 with
+// 8 entries takes 14.8 us against 14.2 so, with 64 entries 28 against 18.
+constexpr int kShortVocab = 80, kShortTop = 16, kShortLanes = 16;
+constexpr int kShortRows = 256 / kShortLanes;       // of a workgroup
+constexpr int kShortCols = kShortVocab / kShortLanes;  // columns of a lane
 
 __device__ __forceinline__ float sum16(float v) {
   v += dpp_quad_xor1(v);
@@ -326,55 +328,37 @@ __device__ __forceinline__ float max16(float v) {
   return v;
 }
 
-// A row's teacher entries as its 16 lanes hold them: entry l + 16 i in slot i, its
-// weight e = 2^(k (t - max)) and their sum.
+// A row's teacher entries, one to each of its 16 lanes: its weight e = 2^(k (t - max))
+// and their sum.
 struct ShortTeacher {
-  static constexpr int kN = kShortTop / kShortLanes;
-  int id[kN];
-  float t[kN], e[kN];  // t - max, and its exponential
+  int id;
+  float t, e;  // t - max, and its exponential
   float sum;
   bool on, bad;
   __device__ __forceinline__ void load(const float* Tl, const int64_t* Ti, bool here, int top, int V, float k, int l) {
-    bool any = false, out = false;
-    float tm = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const int j = l + i * kShortLanes;
-      const int64_t v = here && j < top ? Ti[j] : -1;
-      t[i] = v >= 0 ? Tl[j] : -INFINITY;
-      any = any || v >= 0;
-      out = out || v < -1 || v >= V;
-      id[i] = v >= 0 && v < V ? (int)v : -1;
-      tm = fmaxf(tm, t[i]);
-    }
+    const int64_t v = here && l < top ? Ti[l] : -1;
+    t = v >= 0 ? Tl[l] : -INFINITY;
+    id = v >= 0 && v < V ? (int)v : -1;
     // across the row's 16 lanes
-    any = sum16(any ? 1.f : 0.f) > 0.f;
-    bad = sum16(out ? 1.f : 0.f) > 0.f;
-    tm = max16(tm);
-    const float mu = tm == -INFINITY ? 0.f : tm;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      t[i] -= mu;
-      e[i] = id[i] >= 0 ? fast_exp2(t[i] * k) : 0.f;
-      s += e[i];
-    }
-    sum = sum16(s);
+    const bool any = sum16(v >= 0 ? 1.f : 0.f) > 0.f;
+    bad = sum16(v < -1 || v >= V ? 1.f : 0.f) > 0.f;
+    const float tm = max16(t);
+    t -= tm == -INFINITY ? 0.f : tm;
+    e = id >= 0 ? fast_exp2(t * k) : 0.f;
+    sum = sum16(e);
     on = any && !bad && sum != 0.f;
   }
 };
 
 // A short row's logits: column l + 16 i in slot i (-inf past the row's end).
-template <int NV>
-__device__ __forceinline__ void short_row(const float* z, bool on, int V, int l, float (&x)[NV]) {
+__device__ __forceinline__ void short_row(const float* z, bool on, int V, int l, float (&x)[kShortCols]) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
+  for (int i = 0; i < kShortCols; ++i) {
     const int v = l + i * kShortLanes;
     x[i] = on && v < V ? z[v] : -INFINITY;
   }
 }
 
-template <int NV>
 __global__ void __launch_bounds__(256)
 distill_short_row_kernel(const float* __restrict__ Z, const float* __restrict__ Tl, const int64_t* __restrict__ Ti,
                          float* __restrict__ row_loss, float* __restrict__ stats, int64_t n, int V, int top, float k,
@@ -385,25 +369,20 @@ distill_short_row_kernel(const float* __restrict__ Z, const float* __restrict__ 
   const float* z = Z + row * V;
   ShortTeacher te;
   te.load(Tl + row * top, Ti + row * top, here, top, V, k, l);
-  float x[NV];
-  short_row<NV>(z, te.on, V, l, x);
+  float x[kShortCols];
+  short_row(z, te.on, V, l, x);
   float m = x[0];
 #pragma unroll
-  for (int i = 1; i < NV; ++i) m = fmaxf(m, x[i]);
+  for (int i = 1; i < kShortCols; ++i) m = fmaxf(m, x[i]);
   m = max16(m);
   float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < kShortCols; ++i)
     if (l + i * kShortLanes < V) s += fast_exp2((x[i] - m) * k);
   s = sum16(s);
   const float ln_s = logf(s);
   float acc = 0.f;
-#pragma unroll
-  for (int i = 0; i < ShortTeacher::kN; ++i) {
-    if (te.id[i] < 0 || !te.on) continue;
-    const float lnq = (z[te.id[i]] - m) * inv_tau - ln_s;
-    if (!(te.e[i] == 0.f)) acc += te.e[i] * (te.t[i] * inv_tau - lnq);
-  }
+  if (te.on && te.id >= 0 && !(te.e == 0.f)) acc = te.e * (te.t * inv_tau - ((z[te.id] - m) * inv_tau - ln_s));
   acc = sum16(acc);
   if (!here || l != 0) return;
   if (te.bad && err) *err = 1;
@@ -416,12 +395,11 @@ distill_short_row_kernel(const float* __restrict__ Z, const float* __restrict__ 
   }
 }
 
-template <int NV>
 __global__ void __launch_bounds__(256)
 distill_short_bwd_kernel(const float* __restrict__ grad, const float* __restrict__ Z, const float* __restrict__ Tl,
                          const int64_t* __restrict__ Ti, const float* __restrict__ stats, float* __restrict__ dZ,
                          int64_t n, int V, int top, float k, float tau) {
-  __shared__ float ps[kShortRows][NV * kShortLanes];  // each column's p
+  __shared__ float ps[kShortRows][kShortVocab];  // each column's p
   __shared__ int sid[kShortRows][kShortTop];
   __shared__ float sp[kShortRows][kShortTop];
   const int l = threadIdx.x % kShortLanes, r = threadIdx.x / kShortLanes;
@@ -431,48 +409,43 @@ distill_short_bwd_kernel(const float* __restrict__ grad, const float* __restrict
   const bool on = s != INFINITY;
   ShortTeacher te;
   te.load(Tl + row * top, Ti + row * top, here, top, V, k, l);
-  float x[NV];
-  short_row<NV>(Z + row * V, on, V, l, x);
+  float x[kShortCols];
+  short_row(Z + row * V, on, V, l, x);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) ps[r][l + i * kShortLanes] = 0.f;
-#pragma unroll
-  for (int i = 0; i < ShortTeacher::kN; ++i) {
-    sid[r][l + i * kShortLanes] = te.id[i];
-    sp[r][l + i * kShortLanes] = te.e[i] / te.sum;
-  }
+  for (int i = 0; i < kShortCols; ++i) ps[r][l + i * kShortLanes] = 0.f;
+  sid[r][l] = te.id;
+  sp[r][l] = te.e / te.sum;
   __syncthreads();
-  if (on) {
-    for (int i = l; i < top; i += kShortLanes) {
-      const int id = sid[r][i];
-      if (id < 0) continue;
-      // the first entry of an id writes the sum over all of them
-      float p = 0.f;
-      bool first = true;
-      for (int j = 0; j < top; ++j) {
-        if (sid[r][j] != id) continue;
-        if (j < i) first = false;
-        p += sp[r][j];
-      }
-      if (first) ps[r][id] = p;
+  if (on && te.id >= 0) {
+    // the first entry of an id writes the sum over all of them
+    float p = 0.f;
+    bool first = true;
+#pragma unroll
+    for (int j = 0; j < kShortTop; ++j) {
+      if (sid[r][j] != te.id) continue;
+      if (j < l) first = false;
+      p += sp[r][j];
     }
+    if (first) ps[r][te.id] = p;
   }
   __syncthreads();
   if (!here) return;
   const float c = grad[0] * tau / stats[2 * n];
   const float f = c / s;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
+  for (int i = 0; i < kShortCols; ++i) {
     const int v = l + i * kShortLanes;
     if (v < V) dZ[row * V + v] = on ? f * fast_exp2((x[i] - m) * k) - c * ps[r][v] : 0.f;
   }
 }
 
-// Waves per row.  One wave holds a short row's loads in flight by itself; long
-// rows take a workgroup, the larger one where there are fewer of them than it
-// takes to fill the GPU with the smaller.
+// Waves per row, forward + backward in us with 1, 4 and 16: 4096 x 2048 26.9, 30.6,
+// 72.8; 4096 x 4096 42.5, 40.5, 78.0; 64 x 50000 69.5, 30.6, 24.3; 500 x 50000 78.7,
+// 57.2, 58.1.  So one up to 2048 columns, then a workgroup of 4, of 16 where there are
+// no more rows than CUs.
 int waves_per_row(int64_t n, int64_t vocab) {
   if (vocab <= 2048) return 1;
-  return vocab >= 16384 && n < 2 * (int64_t)device_cu_count() ? 16 : 4;
+  return vocab >= 16384 && n <= (int64_t)device_cu_count() ? 16 : 4;
 }
 
 template <int W>
@@ -505,18 +478,16 @@ int launch_bwd(const float* grad, const float* z, const float* tl, const int64_t
 
 bool short_rows(int64_t vocab, int64_t top) { return vocab <= kShortVocab && top <= kShortTop; }
 
-template <int NV>
 int launch_short(const float* z, const float* tl, const int64_t* ti, float* row_loss, float* stats, int64_t n, int V,
                  int top, float tau, int* err, hipStream_t st) {
-  distill_short_row_kernel<NV><<<dim3((unsigned)ceil_div(n, kShortRows)), dim3(256), 0, st>>>(
+  distill_short_row_kernel<<<dim3((unsigned)ceil_div(n, kShortRows)), dim3(256), 0, st>>>(
       z, tl, ti, row_loss, stats, n, V, top, kLog2e / tau, 1.0f / tau, tau * tau, err);
   return launch_status();
 }
 
-template <int NV>
 int launch_short_bwd(const float* grad, const float* z, const float* tl, const int64_t* ti, const float* stats,
                      float* dz, int64_t n, int V, int top, float tau, hipStream_t st) {
-  distill_short_bwd_kernel<NV><<<dim3((unsigned)ceil_div(n, kShortRows)), dim3(256), 0, st>>>(
+  distill_short_bwd_kernel<<<dim3((unsigned)ceil_div(n, kShortRows)), dim3(256), 0, st>>>(
       grad, z, tl, ti, stats, dz, n, V, top, kLog2e / tau, tau);
   return launch_status();
 }
@@ -549,7 +520,7 @@ int aar_distill_fwd_f32(const float* logits, const float* t_logits, const int64_
   if (n > 0) {
     const int w = waves_per_row(n, vocab);
     auto launch = w == 1 ? launch_rows<1> : (w == 4 ? launch_rows<4> : launch_rows<16>);
-    if (short_rows(vocab, top)) launch = vocab <= 80 ? launch_short<5> : launch_short<16>;
+    if (short_rows(vocab, top)) launch = launch_short;
     rc = launch(logits, t_logits, t_ids, row_loss, stats, n, (int)vocab, (int)top, temperature, err, st);
     if (rc != AAR_OK) return rc;
   }
@@ -566,7 +537,7 @@ int aar_distill_bwd_f32(const float* grad, const float* logits, const float* t_l
   if (!grad || !logits || !t_logits || !t_ids || !stats || !dlogits) return AAR_EINVAL;
   const int w = waves_per_row(n, vocab);
   auto launch = w == 1 ? launch_bwd<1> : (w == 4 ? launch_bwd<4> : launch_bwd<16>);
-  if (short_rows(vocab, top)) launch = vocab <= 80 ? launch_short_bwd<5> : launch_short_bwd<16>;
+  if (short_rows(vocab, top)) launch = launch_short_bwd;
   return launch(grad, logits, t_logits, t_ids, stats, dlogits, n, (int)vocab, (int)top, temperature,
                 as_stream(stream));
 }

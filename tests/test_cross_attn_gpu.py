@@ -226,6 +226,31 @@ def test_an_outlier_that_no_row_attends_to(L, d):
         M.near(a, b, M.attn_tol(d, 90, 16.0) * (2 if name[0] == "d" else 1), name, w.get(name))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_small_columns_of_large_rows(L, d):
+    """Elements 2^-28 of their row's largest: in two fp16 parts under the row's scale they
+    are subnormal, held to 2^-38 of the largest; each product with them is off by
+    that times its weight, beside the roundings of the sums."""
+    q, do = rand(1, 1, 2, 50, d), rand(2, 1, 2, 50, d)
+    k, v = rand(3, 1, 2, 70, d), rand(4, 1, 2, 70, d)
+    small = 2.0 ** -28
+    v[..., 1:] *= small
+    o, lse = run(L, q, k, v, None)
+    ro, _ = M.cross_exact(q, k, v)
+    top = v.abs().max().item()
+    bound = 2.0 ** -38 * top + 4 * M.attn_tol(d, 70) * v[..., 1:].abs().max().item()
+    assert (o.double().cpu() - ro)[..., 1:].abs().max().item() <= bound
+    # K's small columns in dQ = scale dS K, with sum_j |dS_ij| <= 2 max|dO . v|
+    v = rand(4, 1, 2, 70, d)
+    k[..., 1:] *= small
+    q[..., 1:] *= 2.0
+    _, _, dq, _, _ = run(L, q, k, v, None, do)
+    rq = M.cross_exact(q, k, v, None, do)[2]
+    ds = 2 * (do @ v.transpose(2, 3)).abs().max().item() * d ** -0.5
+    bound = ds * (2.0 ** -38 * k.abs().max().item() + 8 * M.attn_tol(d, 70) * k[..., 1:].abs().max().item())
+    assert (dq.double().cpu() - rq)[..., 1:].abs().max().item() <= bound
+
+
 @pytest.mark.parametrize("d", [64, 128, 30])
 def test_infinities_and_nan(L, d):
     """Where keys, values or gradients hold them, as fp32 arithmetic has it."""

@@ -84,7 +84,9 @@ def check(L, z, t, ids, tau, grad=1.0, what=""):
 @pytest.mark.parametrize("tau", [1.0, 2.5])
 @pytest.mark.parametrize("n,V,K", [(1, 1, 1), (1, 2, 2), (5, 7, 3), (3, 65, 8), (1000, 65, 8), (77, 1000, 64),
                                    (9, 2047, 5), (10, 2049, 37), (6, 5003, 1), (515, 4096, 16), (3, 50001, 64),
-                                   (2, 16384, 1000), (600, 16387, 7), (2, 1024, 1024)])
+                                   (2, 16384, 1000), (600, 16387, 7), (2, 1024, 1024), (33, 16, 16), (33, 80, 16),
+                                   (33, 81, 16), (33, 80, 17), (18, 256, 64), (33, 2048, 9), (255, 16384, 3),
+                                   (257, 16384, 3)])
 def test_against_the_definition(L, n, V, K, tau):
     check(L, *make(n, V, K), tau, grad=0.7)
 

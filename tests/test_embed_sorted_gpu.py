@@ -63,7 +63,8 @@ def ids_of(kind, n, vocab, seed=1):
 @pytest.mark.parametrize("kind", ["uniform", "one", "sorted", "two", "zipf"])
 @pytest.mark.parametrize("n,vocab,dim", [
     (1, 1, 4), (1, 5000, 384), (2, 1, 1), (15, 16, 3), (16, 65, 64), (17, 65, 260), (1023, 65, 384), (1025, 257, 5),
-    (4096, 1000, 256), (16384, 65, 384), (16385, 50001, 68), (5000, 300001, 12), (40000, 7, 33), (70000, 1024, 8)])
+    (4096, 1000, 256), (16384, 65, 384), (16385, 50001, 68), (5000, 300001, 12), (40000, 7, 33), (70000, 1024, 8), (32768, 300, 20),
+    (32769, 300, 20), (65536, 65, 4), (65537, 33, 7)])
 def test_gradient(L, n, vocab, dim, kind):
     g = torch.randn(n, dim, generator=gen(2), device="cuda")
     check_grad(L, g, ids_of(kind, n, vocab), vocab)
