@@ -642,13 +642,13 @@ cross_bwd_dkdv_kernel(const CaArgs a) {
 // 2^-38 of its row's largest element, lo lo is at most 2^-22 of a product and is left
 // out; sums are in fp32, with fewer roundings than the fp32 instruction's, which
 // leaves the results nearer to the exact ones.  8 x 12 heads, 1024 x 4096, d 64 (in
-// brackets with the fp32 instruction): forward 439 us (934), dQ 625 (1276), dK/dV 898
+// brackets with the fp32 instruction): forward 418 us (934), dQ 605 (1276), dK/dV 857
 // (1730), off by 0.76e-6 (1.2e-6) in O's norm, 1.0e-6 (1.3e-6) in dQ's, 0.80e-6
-// (0.88e-6) in dK's and dV's.  That is 235 TFLOP/s of the products they stand for,
-// 705 on the cores.  Three bf16 parts and six products hold all 24 bits, but took 590,
-// 806 and 1125 us.  Vector instructions (scales, exponentials, splits: 290 a wave and
-// tile in the forward beside 24 matrix ops) bound these: they take 84% of the cycles
-// while waves are there, the matrix ops 34%.
+// (0.88e-6) in dK's and dV's.  That is 245 TFLOP/s of the products they stand for,
+// 735 on the cores.  Three bf16 parts and six products hold all 24 bits, but took 590,
+// 806 and 1125 us.  What bounds these is the power that vector and matrix units draw
+// together: the forward's 256 vector instructions a wave and tile (scales, exponentials,
+// splits) beside 24 matrix ops were 312, with 425 us, and the clock gave way.
 //
 // e is a row's own, such that its largest element is in [2^13, 2^14).  Over the head
 // dim a row's factor is one of the output's row or column.  Over a tile's rows it
@@ -682,23 +682,51 @@ constexpr int kHalfProducts = 3;
 __device__ constexpr int kHalfA[kHalfProducts] = {1, 0, 0};
 __device__ constexpr int kHalfB[kHalfProducts] = {0, 1, 0};
 
-// The two parts of (a, b), a pair a word.
-__device__ __forceinline__ void half_split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const f32x2 v = {a, b};
+// The two parts of (a, b) m, a pair a word; m is a power of two, so the fused
+// product and difference are exact.
+__device__ __forceinline__ void half_split_pair(float a, float b, float m, uint32_t& hi, uint32_t& lo) {
+  const f32x2 v = {a * m, b * m};
   const f16x2 x = __builtin_convertvector(v, f16x2);
-  const f32x2 rest = {a - (float)x[0], b - (float)x[1]};
+  const f32x2 rest = {fmaf(a, m, -(float)x[0]), fmaf(b, m, -(float)x[1])};
   hi = __builtin_bit_cast(uint32_t, x);
   lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, f16x2));
 }
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // |e| <= 126
 
-// Exponent of the scale of a row whose largest magnitude is `top` (the largest scale
-// for zeros), and whether the parts do not hold it.
-__device__ __forceinline__ int half_exponent(float top, bool& bad) {
-  const uint32_t u = __float_as_uint(top), lo = (127 - 63) << 23, hi = (127 + 60) << 23;
+// Exponent of the scale of a row whose largest magnitude has the bits u (the largest
+// scale for zeros), and whether the parts do not hold it.
+__device__ __forceinline__ int half_exponent(uint32_t u, bool& bad) {
+  const uint32_t lo = (127 - 63) << 23, hi = (127 + 60) << 23;
   bad = bad || (u != 0 && u - lo >= hi - lo);
   return min(max(140 - (int)(u >> 23), -47), 60);
+}
+
+// Largest of the 8 or 16 lanes of a tile's row (magnitudes, as their bits).
+template <int N>
+__device__ __forceinline__ uint32_t row_top(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false));
+  if (N == 16) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false));
+  return v;
+}
+
+// Rows as a buffer: reads at or past `bytes` from p give zeros.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+constexpr uint32_t kNowhere = 0x80000000u;  // an offset past every buffer's end
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const float* p, uint32_t bytes) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), 0, (int)bytes, 0x00027000);
+#endif
+}
+__device__ __forceinline__ f32x4 buffer_load4(__amdgpu_buffer_rsrc_t rows, uint32_t at) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, (int)at, 0, 0));
+#else
+  return f32x4{0.f, 0.f, 0.f, 0.f};
+#endif
 }
 
 // A [32][DP] tile in two planes of 32 rows; a row's 16 spare bytes put 16
@@ -717,17 +745,38 @@ struct HalfTile {
   // Row of unit i of thread tid, and its first column.
   __device__ __forceinline__ static int row(int i, int tid) { return (tid + i * kFaThreads) / kOcts; }
   __device__ __forceinline__ static int col(int tid) { return 8 * (tid % kOcts); }
-  // `at(r)` is the pointer to row r of the tile, null for a row that is not read.
-  template <typename At>
-  __device__ __forceinline__ void load(int d, int tid, At at) {
+  // Where this thread's units stand in rows of `st` floats, in bytes from row 0.
+  struct Place {
+    uint32_t at[kPer][2];
+    __device__ __forceinline__ Place(int64_t st, int d, int tid) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          at[i][g] = col(tid) + 4 * g < d ? (uint32_t)((row(i, tid) * st + col(tid) + 4 * g) * 4) : kNowhere;
+    }
+  };
+  // The 32 rows from p on, of which `rows` are read, others are zeros.
+  __device__ __forceinline__ void load(const float* p, int64_t st, int rows, int d, const Place& w) {
+    const int last = min(rows, kTile) - 1;  // no branch: loads in flight stay countable
+    const uint32_t bytes = (uint32_t)(last * (int)st + d) * 4u & ~(uint32_t)(last >> 31);
+    const __amdgpu_buffer_rsrc_t b = row_buffer(p, bytes);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) f[i][g] = buffer_load4(b, w.at[i][g]);
+  }
+  // Rows [row0, row0 + 32) of a list of `n` that is Tq rows of each of several heads.
+  __device__ __forceinline__ void load_heads(const float* p, int64_t sh, int64_t st, int Tq, int row0, int n, int d,
+                                             int tid) {
+    const __amdgpu_buffer_rsrc_t b = row_buffer(p, kNowhere - 1);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const float* p = at(row(i, tid));
+      const int r = row0 + row(i, tid), g = r / Tq, t = r - g * Tq;
+      const uint32_t at = (uint32_t)((g * sh + t * st + col(tid)) * 4);
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        f[i][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (p && col(tid) + 4 * g < d) f[i][g] = *reinterpret_cast<const f32x4*>(p + col(tid) + 4 * g);
-      }
+      for (int k = 0; k < 2; ++k)
+        f[i][k] = buffer_load4(b, r < n && col(tid) + 4 * k < d ? at + 16 * k : kNowhere);
     }
   }
   __device__ __forceinline__ void store(char* s, int tid, bool& bad) {
@@ -738,17 +787,13 @@ struct HalfTile {
       for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int e = 0; e < 2; ++e) top = fmaxf(fmaxf(top, fabsf(f[i][g][2 * e])), fabsf(f[i][g][2 * e + 1]));
-      top = fmaxf(top, dpp_quad_xor1(top));
-      top = fmaxf(top, dpp_quad_xor2(top));
-      top = fmaxf(top, dpp_half_mirror(top));
-      if (kOcts == 16) top = fmaxf(top, dpp_row_mirror(top));
-      ex[i] = half_exponent(top, bad);
+      ex[i] = half_exponent(row_top<kOcts>(__float_as_uint(top)), bad);
       const float m = pow2(ex[i]);
       u32x4 hi, lo;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         uint32_t x, y;
-        half_split_pair(f[i][e >> 1][2 * (e & 1)] * m, f[i][e >> 1][2 * (e & 1) + 1] * m, x, y);
+        half_split_pair(f[i][e >> 1][2 * (e & 1)], f[i][e >> 1][2 * (e & 1) + 1], m, x, y);
         hi[e] = x;
         lo[e] = y;
       }
@@ -791,9 +836,10 @@ __device__ __forceinline__ f32x16 half_rows(const char* s, const u32x4 (&b)[DP /
 }
 
 // acc[b] += tile^T . x over rows 16 k .. 16 k + 15 of the tile, x = accumulator
-// registers 8 k .. 8 k + 7: column 32 b + lr of the tile.
+// registers 8 k .. 8 k + 7 of x times f: column 32 b + lr of the tile.
 template <int DP>
-__device__ __forceinline__ void half_cols(const char* s, const f32x16& x, int k, int lane, f32x16 (&acc)[DP / 32]) {
+__device__ __forceinline__ void half_cols(const char* s, const f32x16& x, float f, int k, int lane,
+                                          f32x16 (&acc)[DP / 32]) {
   using T = HalfTile<DP>;
   const int h = lane >> 5, j = lane & 15;
   const char* p = s + (16 * k + 4 * h + (j >> 2)) * T::kRow + 2 * (16 * ((lane >> 4) & 1) + 4 * (j & 3));
@@ -801,7 +847,7 @@ __device__ __forceinline__ void half_cols(const char* s, const f32x16& x, int k,
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     uint32_t hi, lo;
-    half_split_pair(x[8 * k + 2 * e], x[8 * k + 2 * e + 1], hi, lo);
+    half_split_pair(x[8 * k + 2 * e], x[8 * k + 2 * e + 1], f, hi, lo);
     pp[0][e] = hi;
     pp[1][e] = lo;
   }
@@ -837,14 +883,14 @@ __device__ __forceinline__ float half_row(const float* p, int d, float f, int h,
       for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[c][g][e]));
     }
   }
-  const int ex = half_exponent(half_swap_max(top), bad);
+  const int ex = half_exponent(__float_as_uint(half_swap_max(top)), bad);
   const float m = pow2(ex);
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       uint32_t hi, lo;
-      half_split_pair(x[c][e >> 1][2 * (e & 1)] * m, x[c][e >> 1][2 * (e & 1) + 1] * m, hi, lo);
+      half_split_pair(x[c][e >> 1][2 * (e & 1)], x[c][e >> 1][2 * (e & 1) + 1], m, hi, lo);
       out[c][0][e] = hi;
       out[c][1][e] = lo;
     }
@@ -852,31 +898,31 @@ __device__ __forceinline__ float half_row(const float* p, int d, float f, int h,
   return pow2(-ex);
 }
 
-// The power of two that a lane's P or dS, times 2^-e of the other operand's rows, is
-// scaled by.  x holds a tile's, scaled by it already, of magnitudes up to `top`: the
-// first tile sets it such that the largest is in [2^13, 2^14), a later one lowers it,
-// with the sums so far, when it passes 2^15.
+// The power of two f = 2^log that a lane's P or dS, times 2^-e of the other operand's
+// rows, is scaled by, from the magnitudes up to `top` of a tile's: the first tile sets
+// it such that the largest is in [2^13, 2^14), a later one lowers it, with the sums so
+// far, when it passes 2^15.
 template <int NB>
 struct HalfScale {
   int log = 0;
-  float most = -1.f, big = 0.f;  // `big`: the largest so far
-  __device__ __forceinline__ void follow(float top, f32x16& x, f32x16 (&acc)[NB], bool& bad) {
+  float f = 1.f, most = -1.f, big = 0.f;  // `most`: what f holds; `big`: the largest so far
+  __device__ __forceinline__ void follow(float top, f32x16 (&acc)[NB], bool& bad) {
     top = half_swap_max(top);
     big = fmaxf(big, top);
     if (!__any(top > most)) return;
-    const int to = top > most ? log + 140 - (int)(__float_as_uint(big) >> 23) : log;
-    bad = bad || top > pow2(120) || to < -100;  // more than fp32 would have left to scale
-    const int by = min(min(max(to, -100), 100) - log, 126);
-    const float f = ldexpf(1.f, by);
-    log += by;
-    big *= f;
-    most = 32768.f;
+    if (top > most) {
+      const int to = 140 - (int)(__float_as_uint(big) >> 23);
+      bad = bad || to < -100;
+      const int by = min(min(max(to, -100), 100) - log, 126);
+      log += by;
+      f = pow2(log);
+      most = ldexpf(32768.f, -log);
+      const float g = ldexpf(1.f, by);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] *= f;
+      for (int b = 0; b < NB; ++b) {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[b][r] *= f;
+        for (int r = 0; r < 16; ++r) acc[b][r] *= g;
+      }
     }
   }
   __device__ __forceinline__ float undo() const { return pow2(-log); }
@@ -955,7 +1001,7 @@ cross_fwd_split_kernel(const CaArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
     follow(mx * qf, 4.f);
-    const float mu = m == -INFINITY ? 0.f : m, f = pow2(fit.log);
+    const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const f32x4 v4 = row_values(vf[buf], g, h);
@@ -963,22 +1009,23 @@ cross_fwd_split_kernel(const CaArgs a) {
       for (int e = 0; e < 4; ++e) {
         const float p = fast_exp2(s[4 * g + e] * qf - mu);
         ps += p;
-        s[4 * g + e] = p * v4[e] * f;
+        s[4 * g + e] = p * v4[e];
         top = fmaxf(top, s[4 * g + e]);
       }
     }
     l += half_swap_sum(ps);
-    fit.follow(top, s, o, row_bad);
-    half_cols<DP>(vs[buf], s, 0, lane, o);
-    half_cols<DP>(vs[buf], s, 1, lane, o);
+    fit.follow(top, o, row_bad);
+    half_cols<DP>(vs[buf], s, fit.f, 0, lane, o);
+    half_cols<DP>(vs[buf], s, fit.f, 1, lane, o);
   };
 
   const int ntiles = k1 > k0 ? (k1 - k0 + kTile - 1) / kTile : 0;
   Tile kc[2], vc[2];
+  const typename Tile::Place kat(a.k.st, a.d, tid), vat(a.v.st, a.d, tid);
   auto load = [&](int i, int t) {
     const int row0 = k0 + t * kTile;
-    kc[i].load(a.d, tid, [&](int r) { return row0 + r < k1 ? K + (int64_t)(row0 + r) * a.k.st : nullptr; });
-    vc[i].load(a.d, tid, [&](int r) { return row0 + r < k1 ? V + (int64_t)(row0 + r) * a.v.st : nullptr; });
+    kc[i].load(K + (int64_t)row0 * a.k.st, a.k.st, k1 - row0, a.d, kat);
+    vc[i].load(V + (int64_t)row0 * a.v.st, a.v.st, k1 - row0, a.d, vat);
   };
   auto store = [&](int i, int buf) {
     kc[i].store(ks[buf], tid, bad);
@@ -1111,10 +1158,11 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
 
   const int ntiles = k1 > k0 ? (k1 - k0 + kTile - 1) / kTile : 0;
   Tile kc, vc;
+  const typename Tile::Place kat(a.k.st, a.d, tid), vat(a.v.st, a.d, tid);
   auto load = [&](int t) {
     const int row0 = k0 + t * kTile;
-    kc.load(a.d, tid, [&](int r) { return row0 + r < k1 ? K + (int64_t)(row0 + r) * a.k.st : nullptr; });
-    vc.load(a.d, tid, [&](int r) { return row0 + r < k1 ? V + (int64_t)(row0 + r) * a.v.st : nullptr; });
+    kc.load(K + (int64_t)row0 * a.k.st, a.k.st, k1 - row0, a.d, kat);
+    vc.load(V + (int64_t)row0 * a.v.st, a.v.st, k1 - row0, a.d, vat);
   };
   auto store = [&](int buf) {
     kc.store(ks[buf], tid, bad);
@@ -1140,7 +1188,6 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
       const f32x16 s = half_rows<DP>(ks[buf], qp, lr, h);
       f32x16 dp = half_rows<DP>(vs[buf], dop, lr, h);
       float top = 0.f;
-      const float f = pow2(fit.log), dpf = df * f, dsf = dsum * f;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 k4 = row_values(kf[buf], g, h), v4 = row_values(vf[buf], g, h);
@@ -1148,7 +1195,7 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * g + e;
           const float p = fast_exp2(s[r] * k4[e] * qf - l2);
-          dp[r] = p * (dp[r] * v4[e] * dpf - dsf) * k4[e];
+          dp[r] = p * (dp[r] * v4[e] * df - dsum) * k4[e];
         }
       }
       if (kv0 + kTile > k1) {
@@ -1158,9 +1205,9 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(dp[r]));
-      fit.follow(top, dp, dq, row_bad);
-      half_cols<DP>(ks[buf], dp, 0, lane, dq);
-      half_cols<DP>(ks[buf], dp, 1, lane, dq);
+      fit.follow(top, dq, row_bad);
+      half_cols<DP>(ks[buf], dp, fit.f, 0, lane, dq);
+      half_cols<DP>(ks[buf], dp, fit.f, 1, lane, dq);
     }
     if (has_next) store(buf ^ 1);
     lds_barrier();
@@ -1239,6 +1286,9 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
   const int t1 = kb * kBlock < len ? min((a.R + kTile - 1) / kTile, t0 + a.kv_tiles) : t0;
 
   Tile qc, dc;
+  const float* Q = a.q.p + ca_row(a.q, a, bh, 0);
+  const float* dO = a.dout.p + ca_row(a.dout, a, bh, 0);
+  const typename Tile::Place qat(a.q.st, a.d, tid), oat(a.dout.st, a.d, tid);
   float lreg[Tile::kPer], dreg[Tile::kPer];
   auto lse_of = [&](int r) {
     const float x = r < a.R ? a.lse[(int64_t)bh * a.R + r] * kLog2e : INFINITY;
@@ -1247,8 +1297,13 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
   auto d_of = [&](int r) { return r < a.R ? a.D[(int64_t)bh * a.R + r] : 0.f; };
   auto load = [&](int t) {
     const int row0 = t * kTile;
-    qc.load(a.d, tid, [&](int r) { return row0 + r < a.R ? a.q.p + ca_row(a.q, a, bh, row0 + r) : nullptr; });
-    dc.load(a.d, tid, [&](int r) { return row0 + r < a.R ? a.dout.p + ca_row(a.dout, a, bh, row0 + r) : nullptr; });
+    if (a.G == 1) {
+      qc.load(Q + (int64_t)row0 * a.q.st, a.q.st, a.R - row0, a.d, qat);
+      dc.load(dO + (int64_t)row0 * a.dout.st, a.dout.st, a.R - row0, a.d, oat);
+    } else {
+      qc.load_heads(Q, a.q.sh, a.q.st, a.Tq, row0, a.R, a.d, tid);
+      dc.load_heads(dO, a.dout.sh, a.dout.st, a.Tq, row0, a.R, a.d, tid);
+    }
 #pragma unroll
     for (int n = 0; n < Tile::kPer; ++n) {
       lreg[n] = dreg[n] = 0.f;
@@ -1286,7 +1341,6 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
       sched_fence();
       f32x16 x;
       float top = 0.f;
-      const float vs = pow2(fit_v.log), ks = pow2(fit_k.log);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 q4 = row_values(qf[cur], g, h), l4 = row_values(ls[cur], g, h), o4 = row_values(df[cur], g, h);
@@ -1294,13 +1348,13 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * g + e;
           s[r] = key_ok ? fast_exp2(s[r] * q4[e] * kf - l4[e]) : 0.f;
-          x[r] = s[r] * o4[e] * vs;
+          x[r] = s[r] * o4[e];
           top = fmaxf(top, x[r]);
         }
       }
-      fit_v.follow(top, x, dv, key_bad);
-      half_cols<DP>(dos[cur], x, 0, lane, dv);
-      half_cols<DP>(dos[cur], x, 1, lane, dv);
+      fit_v.follow(top, dv, key_bad);
+      half_cols<DP>(dos[cur], x, fit_v.f, 0, lane, dv);
+      half_cols<DP>(dos[cur], x, fit_v.f, 1, lane, dv);
       x = half_rows<DP>(dos[cur], vp, lr, h);
       sched_fence();
       top = 0.f;
@@ -1310,13 +1364,13 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * g + e;
-          x[r] = s[r] * (x[r] * o4[e] * vf - d4[e]) * ks;
+          x[r] = s[r] * (x[r] * o4[e] * vf - d4[e]);
           top = fmaxf(top, fabsf(x[r]));
         }
       }
-      fit_k.follow(top, x, dk, key_bad);
-      half_cols<DP>(qs[cur], x, 0, lane, dk);
-      half_cols<DP>(qs[cur], x, 1, lane, dk);
+      fit_k.follow(top, dk, key_bad);
+      half_cols<DP>(qs[cur], x, fit_k.f, 0, lane, dk);
+      half_cols<DP>(qs[cur], x, fit_k.f, 1, lane, dk);
     }
     if (has_next) store(cur ^ 1);
     lds_barrier();
@@ -1481,6 +1535,15 @@ bool ca_shape_ok(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk) {
          B * H * Tq <= (int64_t)UINT32_MAX / 32;
 }
 
+// Whether the offsets of the fp16 passes' tiles fit in 31 bits of bytes, and no two
+// of their rows overlap: rows of K and V, and of Q and dO within a tile (one head a
+// key/value head) or within the heads that share a key.
+bool ca_rows_ok(const FaIn& x, int64_t d, int64_t heads, int64_t rows) {
+  const int64_t most = int64_t(1) << 28;
+  if (x.st < d || x.st > most / kTile || x.sh < 0) return false;
+  return heads == 1 || rows == 0 || (x.sh <= most / heads && x.st <= most / rows && heads * x.sh + rows * x.st <= most);
+}
+
 bool ca_vec_ok(int64_t d, std::initializer_list<const void*> ptrs, const int64_t* strides, int n) {
   if (d % 4 != 0) return false;
   for (const void* p : ptrs)
@@ -1627,7 +1690,8 @@ int aar_cross_attn_fwd_f32(const float* q, const float* k, const float* v, const
     a.part_o = static_cast<float*>(workspace);
     a.part_l = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_o_bytes(a.BH, a.R, d, a.splits));
   }
-  return ca_dispatch<true>(a, ca_vec_ok(d, {q, k, v, o}, strides, 12), as_stream(stream));
+  const bool near = a.R <= kFewRows || (ca_rows_ok(a.k, d, 1, Tk) && ca_rows_ok(a.v, d, 1, Tk));
+  return ca_dispatch<true>(a, near && ca_vec_ok(d, {q, k, v, o}, strides, 12), as_stream(stream));
 }
 
 // D of every query row, then the parts of dQ, dK and dV
@@ -1667,7 +1731,9 @@ int aar_cross_attn_bwd_f32(const float* q, const float* k, const float* v, const
   a.dq = ca_out(dq, strides + 15);
   a.dk = ca_out(dk, strides + 18);
   a.dv = ca_out(dv, strides + 21);
-  return ca_dispatch<false>(a, ca_vec_ok(d, {q, k, v, o, dout, dq, dk, dv}, strides, 24), as_stream(stream));
+  const bool near = ca_rows_ok(a.k, d, 1, Tk) && ca_rows_ok(a.v, d, 1, Tk) && ca_rows_ok(a.q, d, a.G, Tq) &&
+                    ca_rows_ok(a.dout, d, a.G, Tq);
+  return ca_dispatch<false>(a, near && ca_vec_ok(d, {q, k, v, o, dout, dq, dk, dv}, strides, 24), as_stream(stream));
 }
 
 }  // extern "C"

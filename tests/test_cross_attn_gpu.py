@@ -137,6 +137,45 @@ def test_strided_operands(L, Tq, d):
                 assert torch.equal(g, x), name
 
 
+@pytest.mark.parametrize("d", [64, 30])
+def test_broadcast_operands(L, d):
+    """Expanded keys, values and queries: strides of zero."""
+    q = rand(1, 1, 1, 40, d).expand(2, 4, 40, d)
+    k, v = rand(2, 2, 2, 1, d).expand(2, 2, 70, d), rand(3, 1, 1, 70, d).expand(2, 2, 70, d)
+    do = rand(4, 2, 4, 1, d).expand(2, 4, 40, d)
+    lens = torch.tensor([70, 33], device="cuda")
+    check(L, q, k, v, lens, do)
+    x = v.contiguous()
+    x[1, :, 33:] = math.inf
+    x[0, 0, 5, 3] = math.inf  # an infinite value, and expanded keys behind the length
+    o, lse = run(L, q, k, x, lens)
+    ro, _ = M.cross_exact(q, k, x, lens)
+    M.near(o, ro, M.attn_tol(d, 70), "o")
+
+
+@pytest.mark.parametrize("Tq", [1, 40])
+def test_far_rows(L, Tq):
+    """Rows and heads whose offsets pass 31 and 32 bits: a cache of 2^32 elements, heads of
+    a group 2^29 apart, rows 2^24 apart."""
+    H, Tk, d = 2, 70000, 64
+    rows = torch.empty(Tk * 65536, device="cuda").view(Tk, 65536)  # 2^32 elements and more
+    k, v = (torch.as_strided(rows, (1, 1, Tk, d), (0, 0, 65536, 1), at) for at in (0, 64))
+    k.copy_(rand(2, 1, 1, Tk, d))
+    v.copy_(rand(3, 1, 1, Tk, d))
+    q, do = rand(1, 1, H, Tq, d), rand(4, 1, H, Tq, d)
+    check(L, q, k, v, None, do)
+    del k, v
+    flat = rows.view(-1)
+    k, v = rand(2, 1, 1, 90, d), rand(3, 1, 1, 90, d)
+    for sh, st in ((2 ** 29, d), (d, 2 ** 24)):
+        qf = torch.as_strided(flat, (1, H, Tq, d), (0, sh, st, 1))
+        qf.copy_(q)
+        check(L, qf, k, v, None, do)
+    kf = torch.as_strided(flat, (1, 1, 90, d), (0, 0, 2 ** 24, 1))
+    kf.copy_(k)
+    check(L, q, kf, v, None, do)
+
+
 @pytest.mark.parametrize("Tq", [1, 50])
 def test_extreme_scores(L, Tq):
     """Scores of +-1000 (one key takes all), all keys equal, a negative scale, and
