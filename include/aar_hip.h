@@ -565,7 +565,9 @@ int aar_causal_mask_f32(const float* x, float* y, int64_t mats, int64_t T, float
  * aar_flash_fwd_strided_f32; 128-bit paths need 16-byte aligned pointers and d
  * and all strides multiples of 4.  d <= 128.  Where the query rows are too few to
  * fill the GPU the key range is split and joined through the workspace (0 bytes
- * otherwise; 16-byte aligned, AAR_EWORKSPACE). */
+ * otherwise; 16-byte aligned, AAR_EWORKSPACE).  Products of aligned rows of more
+ * than 32 floats, 2^23 apart at most, are formed from two fp16 parts of each
+ * operand: 22 bits of it, or 2^-38 of its row's largest element, with fp32 sums. */
 size_t aar_cross_attn_fwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d);
 int aar_cross_attn_fwd_f32(const float* q, const float* k, const float* v, const int64_t* kv_lens, float* o,
                            float* lse, int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d,
@@ -573,7 +575,10 @@ int aar_cross_attn_fwd_f32(const float* q, const float* k, const float* v, const
                            void* stream);
 /* dq, dk, dv (fully overwritten; keys hidden by kv_lens get zeros), summed over
  * the query heads that share a key/value head; no float atomics, the same bits
- * on every run.  24 strides: q, k, v, o, dout, dq, dk, dv. */
+ * on every run.  24 strides: q, k, v, o, dout, dq, dk, dv.  The gradients overlap
+ * neither the inputs nor each other.  The workspace holds dout . o of every query
+ * row, and parts of the sums where the passes do not fill the GPU; 16-byte aligned
+ * (AAR_EWORKSPACE; none without queries). */
 size_t aar_cross_attn_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d);
 int aar_cross_attn_bwd_f32(const float* q, const float* k, const float* v, const int64_t* kv_lens, const float* o,
                            const float* lse, const float* dout, float* dq, float* dk, float* dv, int64_t B,
@@ -630,7 +635,8 @@ int aar_qk_norm_rope_bwd_f32(const float* gy, int64_t gy_row, const float* x, in
 /* Distillation from a teacher's top logits: logits [n, vocab] (the student's),
  * t_logits and t_ids [n, top] (the teacher's best entries of each row and where
  * they stand).  An id of -1 marks an absent entry; a row without entries, or
- * with none above -inf, is left out (no loss, zero gradient, not counted).  With tau = temperature,
+ * with none above -inf, is left out (no loss, zero gradient, not counted).  With
+ * tau = temperature,
  *   p = softmax(t_logits / tau) over the row's entries, q = softmax(logits / tau)
  *   loss = tau^2 * mean over the counted rows of sum_k p_k (ln p_k - ln q[t_ids_k])
  * Entries may name the same id twice: their p add up.  An id below -1 or >= vocab
@@ -643,7 +649,8 @@ size_t aar_distill_workspace_bytes(int64_t n);
 int aar_distill_fwd_f32(const float* logits, const float* t_logits, const int64_t* t_ids, float* loss,
                         float* stats, int64_t n, int64_t vocab, int64_t top, float temperature, int* err,
                         void* workspace, size_t workspace_bytes, void* stream);
-/* dlogits [n, vocab] = grad[0] * tau / counted * (q - p), grad a device scalar. */
+/* dlogits [n, vocab] = grad[0] * tau / counted * (q - p), grad a device scalar;
+ * dlogits does not overlap logits. */
 int aar_distill_bwd_f32(const float* grad, const float* logits, const float* t_logits, const int64_t* t_ids,
                         const float* stats, float* dlogits, int64_t n, int64_t vocab, int64_t top,
                         float temperature, void* stream);
