@@ -144,7 +144,8 @@ class CrossEntropyLoss(Module):
 class DistillationLoss(Module):
     """temperature^2 * mean KL(teacher || student) over the teacher's top
     entries: teacher_logits and teacher_ids [..., K] for logits [..., V].  An id
-    of -1 marks an absent entry; rows without entries above -inf do not count."""
+    of -1 marks an absent entry; rows without entries above -inf do not count.
+    The teacher's logits are constants."""
 
     def __init__(self, temperature=1.0):
         super().__init__()

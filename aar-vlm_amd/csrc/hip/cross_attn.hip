@@ -59,6 +59,11 @@ __device__ __forceinline__ int64_t ca_row(const T& x, const CaArgs& a, int bh, i
   return (int64_t)(bh / a.Hkv) * x.sb + ((int64_t)(bh % a.Hkv) * a.G + g) * x.sh + (int64_t)t * x.st;
 }
 
+// The first head of key/value head bh's group in a query-shaped operand.
+__device__ __forceinline__ const float* ca_group(const FaIn& x, const CaArgs& a, int bh) {
+  return x.p + (int64_t)(bh / a.Hkv) * x.sb + (int64_t)(bh % a.Hkv) * a.G * x.sh;
+}
+
 template <typename T>
 __device__ __forceinline__ auto ca_head(const T& x, const CaArgs& a, int bh) {
   return x.p + (int64_t)(bh / a.Hkv) * x.sb + (int64_t)(bh % a.Hkv) * x.sh;
@@ -1286,8 +1291,8 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
   const int t1 = kb * kBlock < len ? min((a.R + kTile - 1) / kTile, t0 + a.kv_tiles) : t0;
 
   Tile qc, dc;
-  const float* Q = a.q.p + ca_row(a.q, a, bh, 0);
-  const float* dO = a.dout.p + ca_row(a.dout, a, bh, 0);
+  const float* Q = ca_group(a.q, a, bh);
+  const float* dO = ca_group(a.dout, a, bh);
   const typename Tile::Place qat(a.q.st, a.d, tid), oat(a.dout.st, a.d, tid);
   float lreg[Tile::kPer], dreg[Tile::kPer];
   auto lse_of = [&](int r) {
