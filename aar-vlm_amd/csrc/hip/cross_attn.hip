@@ -140,6 +140,17 @@ __device__ __forceinline__ void ca_store_key(const CaArgs& a, int bh, int part, 
 
 // -------------------------------------------------------------- few query rows
 
+// Sum over the LPK lanes that hold a key's row.
+template <int LPK>
+__device__ __forceinline__ float lanes_sum(float x) {
+  x += dpp_quad_xor1(x);
+  x += dpp_quad_xor2(x);
+  x += dpp_half_mirror(x);
+  if (LPK >= 16) x += dpp_row_mirror(x);
+  if (LPK >= 32) x += swizzle_xor16(x);
+  return x;
+}
+
 // Up to RQ query rows a key/value head (single tokens): bound by the bytes of K
 // and V.  LPK lanes hold a key's row, four floats each, and walk the keys with
 // their own online softmax, U keys' loads in flight; the groups' and waves'
@@ -187,12 +198,7 @@ cross_rows_kernel(const CaArgs a) {
       float s[U], mn = m[r];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        float x = kf[u][0] * q[r][0] + kf[u][1] * q[r][1] + kf[u][2] * q[r][2] + kf[u][3] * q[r][3];
-        x += dpp_quad_xor1(x);
-        x += dpp_quad_xor2(x);
-        x += dpp_half_mirror(x);
-        if (LPK >= 16) x += dpp_row_mirror(x);
-        if (LPK >= 32) x += swizzle_xor16(x);
+        const float x = lanes_sum<LPK>(kf[u][0] * q[r][0] + kf[u][1] * q[r][1] + kf[u][2] * q[r][2] + kf[u][3] * q[r][3]);
         s[u] = b + u * kGroups + sub < k1 ? x : -INFINITY;
         mn = fmaxf(mn, s[u]);
       }
@@ -264,6 +270,106 @@ cross_rows_kernel(const CaArgs a) {
     } else {
       if (cc < a.d) store4<VEC>(a.o.p + ca_row(a.o, a, bh, r) + cc, os, a.d - cc);
       if (cc == 0) a.lse[(int64_t)bh * a.R + r] = (mx + log2f(ls)) * kLn2;
+    }
+  }
+}
+
+// The gradients of up to RQ query rows a key/value head, bound by the bytes of K, V, dK
+// and dV like the forward by K's and V's: a key's row gives its scores and dP, hence its
+// dK and dV, and its share of dQ, in one pass.  dQ's sums meet as the forward's do.
+// 17 x 4 heads' single rows over 4340 keys, d 128 (604 MB): 100 us, 6.0 TB/s, and 7 us
+// for dQ's parts; the tiles' kernels, 31 of their 32 rows empty, take 420.
+template <int RQ, int LPK, bool VEC>
+__global__ void __launch_bounds__(256)
+cross_bwd_rows_kernel(const CaArgs a) {
+  constexpr int U = 4;
+  constexpr int kGroups = kWave / LPK;
+  constexpr int kWaves = 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int sub = lane / LPK, c = 4 * (lane % LPK);
+  const int bh = blockIdx.x % a.BH, part = blockIdx.x / a.BH;
+  const int len = ca_len(a, bh);
+  const int k0 = part * a.chunk, k1 = min(len, k0 + a.chunk), end = min(a.Tk, k0 + a.chunk);
+  const float* __restrict__ K = ca_head(a.k, a, bh);
+  const float* __restrict__ V = ca_head(a.v, a, bh);
+  float* __restrict__ dK = ca_head(a.dk, a, bh);
+  float* __restrict__ dV = ca_head(a.dv, a, bh);
+
+  f32x4 q[RQ], g[RQ], dq[RQ];
+  float l2[RQ], D[RQ];
+#pragma unroll
+  for (int r = 0; r < RQ; ++r) {
+    q[r] = g[r] = dq[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 o = q[r];
+    l2[r] = INFINITY;
+    if (r < a.R) {
+      if (c < a.d) {
+        q[r] = load4<VEC>(a.q.p + ca_row(a.q, a, bh, r) + c, a.d - c);
+        g[r] = load4<VEC>(a.dout.p + ca_row(a.dout, a, bh, r) + c, a.d - c);
+        o = load4<VEC>(a.o_in.p + ca_row(a.o_in, a, bh, r) + c, a.d - c);
+      }
+      l2[r] = a.lse[(int64_t)bh * a.R + r] * kLog2e;
+      if (l2[r] == -INFINITY) l2[r] = INFINITY;  // a row without keys has P = 0
+    }
+    D[r] = lanes_sum<LPK>(g[r][0] * o[0] + g[r][1] * o[1] + g[r][2] * o[2] + g[r][3] * o[3]);
+  }
+  for (int b = k0 + wave * U * kGroups; b < end; b += kWaves * U * kGroups) {
+    f32x4 kf[U], vf[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = b + u * kGroups + sub;
+      kf[u] = vf[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (key < k1 && c < a.d) {
+        kf[u] = load4<VEC>(K + (int64_t)key * a.k.st + c, a.d - c);
+        vf[u] = load4<VEC>(V + (int64_t)key * a.v.st + c, a.d - c);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = b + u * kGroups + sub;
+      f32x4 dk = {0.f, 0.f, 0.f, 0.f}, dv = dk;
+#pragma unroll
+      for (int r = 0; r < RQ; ++r) {
+        const float s = lanes_sum<LPK>(kf[u][0] * q[r][0] + kf[u][1] * q[r][1] + kf[u][2] * q[r][2] + kf[u][3] * q[r][3]);
+        const float dp = lanes_sum<LPK>(vf[u][0] * g[r][0] + vf[u][1] * g[r][1] + vf[u][2] * g[r][2] + vf[u][3] * g[r][3]);
+        if (r >= a.R || key >= k1) continue;
+        const float p = fast_exp2(s * a.scale_log2 - l2[r]), ds = p * (dp - D[r]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          dk[e] += ds * q[r][e];
+          dv[e] += p * g[r][e];
+          dq[r][e] += ds * kf[u][e];
+        }
+      }
+      if (key < end && c < a.d) {
+        store4<VEC>(dK + (int64_t)key * a.dk.st + c, dk * a.scale, a.d - c);
+        store4<VEC>(dV + (int64_t)key * a.dv.st + c, dv, a.d - c);
+      }
+    }
+  }
+
+  // The wave's groups, then the waves.
+  __shared__ f32x4 sdq[kWaves][RQ][LPK];
+#pragma unroll
+  for (int r = 0; r < RQ; ++r) {
+#pragma unroll
+    for (int o = LPK; o < kWave; o *= 2)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dq[r][e] += __shfl_xor(dq[r][e], o, kWave);
+    if (sub == 0) sdq[wave][r][lane] = dq[r];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < RQ * LPK; i += 256) {
+    const int r = i / LPK, cc = 4 * (i % LPK);
+    if (r >= a.R) continue;
+    f32x4 x = sdq[0][r][i % LPK];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) x += sdq[w][r][i % LPK];
+    x *= a.scale;
+    if (a.splits > 1) {
+      *reinterpret_cast<f32x4*>(a.dq_part + (((int64_t)part * a.BH + bh) * a.R + r) * (4 * LPK) + cc) = x;
+    } else if (cc < a.d) {
+      store4<VEC>(a.dq.p + ca_row(a.dq, a, bh, r) + cc, x, a.d - cc);
     }
   }
 }
@@ -1464,8 +1570,8 @@ cross_bwd_sum_kernel(const CaArgs a) {
 // ------------------------------------------------------------------ host side
 
 // Query rows a key/value head up to which cross_rows_kernel runs: 192 heads' 4 rows of
-// 577 keys in 18 us against the tiles' 24; 8 rows would take 23 against 24 (of 4096
-// keys 98 against 90).
+// 577 keys in 18 us against the tiles' 24, with gradients 45 against 80; 8 rows would
+// take 23 against 24 (of 4096 keys 98 against 90).
 constexpr int kFewRows = 4;
 constexpr int kMaxSplits = 64;
 
@@ -1492,14 +1598,19 @@ int ca_splits(int64_t grid, int64_t slots, int64_t tiles, int64_t least, double 
   return best;
 }
 
-// Key ranges of a forward, and their keys.  The few-row kernel lives on loads in
-// flight and takes four workgroups to a CU, in ranges of at least 64 keys.
+// Key ranges of the few-row kernels, which live on loads in flight: four workgroups to
+// a CU, in ranges of at least 64 keys.
+int64_t few_splits(int64_t bh, int64_t Tk) {
+  const int64_t cus = device_cu_count(), s = bh * 3 / 2 >= 4 * cus ? 1 : ceil_div(4 * cus, bh);
+  return std::max<int64_t>(1, std::min<int64_t>({s, Tk / 64, (int64_t)kMaxSplits}));
+}
+
+// Key ranges of a forward, and their keys.
 void ca_plan(int64_t bh, int64_t R, int64_t Tk, int64_t d, int* splits, int* chunk) {
   const int64_t cus = device_cu_count(), tiles = ceil_div(Tk, kTile);
   int64_t s;
   if (R <= kFewRows) {
-    s = bh * 3 / 2 >= 4 * cus ? 1 : ceil_div(4 * cus, bh);
-    s = std::max<int64_t>(1, std::min<int64_t>({s, Tk / 64, (int64_t)kMaxSplits}));
+    s = few_splits(bh, Tk);
   } else {
     s = ca_splits(bh * ceil_div(R, kBlock), 2 * cus, tiles, 4, d > 64 ? 4.0 : 2.0, (double)bh * R * pad_dim(d) * 4);
   }
@@ -1508,16 +1619,22 @@ void ca_plan(int64_t bh, int64_t R, int64_t Tk, int64_t d, int* splits, int* chu
   *splits = (int)std::max<int64_t>(1, ceil_div(tiles, c));
 }
 
+// Whether the gradients are cross_bwd_rows_kernel's.
+bool few_rows(const CaArgs& a) { return a.R > 0 && a.R <= kFewRows && a.Tk > 0; }
+
 // Key ranges of dQ and ranges of query rows of dK and dV.
 void ca_bwd_plan(CaArgs& a) {
   const int64_t cus = device_cu_count(), kt = ceil_div((int64_t)a.Tk, kTile), qt = ceil_div((int64_t)a.R, kTile);
   const int64_t slots = (a.d > 64 ? 1 : 2) * cus, dp = pad_dim(a.d);
-  int64_t s = ca_splits(a.BH * ceil_div((int64_t)a.R, kBlock), slots, kt, 4, a.d > 64 ? 6.0 : 3.0,
-                        (double)a.BH * a.R * dp * 4);
+  int64_t s = few_rows(a) ? few_splits(a.BH, a.Tk)
+                          : ca_splits(a.BH * ceil_div((int64_t)a.R, kBlock), slots, kt, 4, a.d > 64 ? 6.0 : 3.0,
+                                      (double)a.BH * a.R * dp * 4);
   int64_t c = ceil_div(std::max<int64_t>(kt, 1), s);
   a.chunk = (int)(c * kTile);
   a.splits = (int)std::max<int64_t>(1, ceil_div(kt, c));
-  s = ca_splits(a.BH * ceil_div((int64_t)a.Tk, kBlock), slots, qt, 4, a.d > 64 ? 10.0 : 5.0, (double)a.BH * a.Tk * dp * 8);
+  s = few_rows(a) ? 1
+                  : ca_splits(a.BH * ceil_div((int64_t)a.Tk, kBlock), slots, qt, 4, a.d > 64 ? 10.0 : 5.0,
+                              (double)a.BH * a.Tk * dp * 8);
   c = ceil_div(std::max<int64_t>(qt, 1), s);
   a.kv_tiles = (int)c;
   a.kv_splits = (int)std::max<int64_t>(1, ceil_div(qt, c));
@@ -1561,20 +1678,24 @@ bool ca_vec_ok(int64_t d, std::initializer_list<const void*> ptrs, const int64_t
 FaIn ca_in(const float* p, const int64_t* s) { return FaIn{p, s[0], s[1], s[2]}; }
 FaOut ca_out(float* p, const int64_t* s) { return FaOut{p, s[0], s[1], s[2]}; }
 
-template <int RQ, bool VEC>
-void launch_few(const CaArgs& a, int dp, hipStream_t st) {
+template <int DP, bool VEC, bool FWD>
+void launch_few(const CaArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)a.BH * a.splits)), block(256);
-  if (dp == 32) cross_rows_kernel<RQ, 8, VEC><<<grid, block, 0, st>>>(a);
-  else if (dp == 64) cross_rows_kernel<RQ, 16, VEC><<<grid, block, 0, st>>>(a);
-  else cross_rows_kernel<RQ, 32, VEC><<<grid, block, 0, st>>>(a);
+  if constexpr (FWD) {
+    if (a.R == 1) cross_rows_kernel<1, DP / 4, VEC><<<grid, block, 0, st>>>(a);
+    else if (a.R == 2) cross_rows_kernel<2, DP / 4, VEC><<<grid, block, 0, st>>>(a);
+    else cross_rows_kernel<4, DP / 4, VEC><<<grid, block, 0, st>>>(a);
+  } else {
+    if (a.R == 1) cross_bwd_rows_kernel<1, DP / 4, VEC><<<grid, block, 0, st>>>(a);
+    else if (a.R == 2) cross_bwd_rows_kernel<2, DP / 4, VEC><<<grid, block, 0, st>>>(a);
+    else cross_bwd_rows_kernel<4, DP / 4, VEC><<<grid, block, 0, st>>>(a);
+  }
 }
 
 template <int DP, bool VEC>
 int launch_fwd(const CaArgs& a, hipStream_t st) {
   if (a.R <= kFewRows) {
-    if (a.R == 1) launch_few<1, VEC>(a, DP, st);
-    else if (a.R == 2) launch_few<2, VEC>(a, DP, st);
-    else launch_few<4, VEC>(a, DP, st);
+    launch_few<DP, VEC, true>(a, st);
   } else {
     const dim3 grid((unsigned)(ceil_div(a.R, kBlock) * a.BH * a.splits));
     if constexpr (kSplit<DP, VEC>) cross_fwd_split_kernel<DP><<<grid, dim3(kFaThreads), 0, st>>>(a);
@@ -1589,18 +1710,23 @@ int launch_fwd(const CaArgs& a, hipStream_t st) {
 
 template <int DP, bool VEC>
 int launch_bwd(const CaArgs& a, hipStream_t st) {
-  if (a.R > 0) {
-    const dim3 grid((unsigned)(ceil_div(a.R, kBlock) * a.BH * a.splits));
-    if constexpr (kSplit<DP, VEC>) cross_bwd_dq_split_kernel<DP><<<grid, dim3(kFaThreads), 0, st>>>(a);
-    else cross_bwd_dq_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
-    const int rc = launch_status();
-    if (rc != AAR_OK) return rc;
+  int rc = AAR_OK;
+  if (few_rows(a)) {
+    launch_few<DP, VEC, false>(a, st);
+    rc = launch_status();
+  } else {
+    if (a.R > 0) {
+      const dim3 grid((unsigned)(ceil_div(a.R, kBlock) * a.BH * a.splits));
+      if constexpr (kSplit<DP, VEC>) cross_bwd_dq_split_kernel<DP><<<grid, dim3(kFaThreads), 0, st>>>(a);
+      else cross_bwd_dq_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
+      rc = launch_status();
+    }
+    if (rc != AAR_OK || a.Tk == 0) return rc;
+    const dim3 grid((unsigned)(ceil_div(a.Tk, kBlock) * a.BH * a.kv_splits));
+    if constexpr (kSplit<DP, VEC>) cross_bwd_dkdv_split_kernel<DP><<<grid, dim3(kFaThreads), 0, st>>>(a);
+    else cross_bwd_dkdv_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
+    rc = launch_status();
   }
-  if (a.Tk == 0) return AAR_OK;
-  const dim3 grid((unsigned)(ceil_div(a.Tk, kBlock) * a.BH * a.kv_splits));
-  if constexpr (kSplit<DP, VEC>) cross_bwd_dkdv_split_kernel<DP><<<grid, dim3(kFaThreads), 0, st>>>(a);
-  else cross_bwd_dkdv_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
-  const int rc = launch_status();
   const int64_t rows = (a.splits > 1 ? (int64_t)a.BH * a.R : 0) + (a.kv_splits > 1 ? 2 * (int64_t)a.BH * a.Tk : 0);
   if (rc != AAR_OK || rows == 0) return rc;
   cross_bwd_sum_kernel<DP, VEC><<<dim3((unsigned)ceil_div(rows * (DP / 4), (int64_t)256)), dim3(256), 0, st>>>(a);
@@ -1736,8 +1862,8 @@ int aar_cross_attn_bwd_f32(const float* q, const float* k, const float* v, const
   a.dq = ca_out(dq, strides + 15);
   a.dk = ca_out(dk, strides + 18);
   a.dv = ca_out(dv, strides + 21);
-  const bool near = ca_rows_ok(a.k, d, 1, Tk) && ca_rows_ok(a.v, d, 1, Tk) && ca_rows_ok(a.q, d, a.G, Tq) &&
-                    ca_rows_ok(a.dout, d, a.G, Tq);
+  const bool near = few_rows(a) || (ca_rows_ok(a.k, d, 1, Tk) && ca_rows_ok(a.v, d, 1, Tk) &&
+                                    ca_rows_ok(a.q, d, a.G, Tq) && ca_rows_ok(a.dout, d, a.G, Tq));
   return ca_dispatch<false>(a, near && ca_vec_ok(d, {q, k, v, o, dout, dq, dk, dv}, strides, 24), as_stream(stream));
 }
 

@@ -54,6 +54,7 @@ SHAPES = [
     (2, 2, 2, 32, 32, 64), (1, 3, 3, 33, 31, 96), (2, 4, 2, 100, 65, 64), (1, 2, 1, 129, 200, 36), (1, 1, 1, 300, 1, 64),
     (1, 2, 2, 257, 577, 64), (2, 8, 4, 65, 300, 128), (1, 3, 3, 50, 70, 1), (1, 2, 2, 40, 90, 3), (1, 2, 2, 64, 2049, 64),
     (4, 12, 12, 130, 260, 64), (1, 1, 1, 2000, 40, 64), (1, 1, 1, 1, 8192, 64), (16, 16, 16, 140, 140, 64),
+    (2, 2, 2, 3, 150, 30), (2, 4, 2, 2, 65, 64), (1, 1, 1, 4, 2100, 96), (3, 3, 3, 4, 1, 128), (2, 2, 2, 5, 500, 64),
 ]
 
 
@@ -66,6 +67,7 @@ def test_against_the_definition(L, shape):
 
 
 @pytest.mark.parametrize("shape", [(5, 2, 2, 1, 200, 64), (5, 4, 2, 3, 100, 128), (5, 2, 2, 40, 200, 64),
+                                   (5, 4, 2, 2, 100, 128), (5, 2, 2, 3, 700, 30),
                                    (5, 4, 1, 70, 333, 36), (5, 3, 3, 200, 130, 30), (5, 2, 2, 33, 900, 64)])
 def test_padded_contexts(L, shape):
     """Lengths none, one, a tile's border, some and all; what stands behind them is
