@@ -282,7 +282,7 @@ cross_rows_kernel(const CaArgs a) {
 template <int RQ, int LPK, bool VEC>
 __global__ void __launch_bounds__(256)
 cross_bwd_rows_kernel(const CaArgs a) {
-  constexpr int U = 4;
+  constexpr int U = RQ >= 8 ? 2 : 4;
   constexpr int kGroups = kWave / LPK;
   constexpr int kWaves = 4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -1570,9 +1570,10 @@ cross_bwd_sum_kernel(const CaArgs a) {
 // ------------------------------------------------------------------ host side
 
 // Query rows a key/value head up to which cross_rows_kernel runs: 192 heads' 4 rows of
-// 577 keys in 18 us against the tiles' 24, with gradients 45 against 80; 8 rows would
-// take 23 against 24 (of 4096 keys 98 against 90).
-constexpr int kFewRows = 4;
+// 577 keys in 18 us against the tiles' 24; 8 rows would take 23 against 24 (of 4096
+// keys 98 against 90).  And cross_bwd_rows_kernel, forward + backward: 4 rows of 577 keys
+// 45 us against 80, 8 rows 58 against 81 (of 4096 keys 281 against 466).
+constexpr int kFewRows = 4, kFewBwd = 8;
 constexpr int kMaxSplits = 64;
 
 int pad_dim(int64_t d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
@@ -1620,7 +1621,7 @@ void ca_plan(int64_t bh, int64_t R, int64_t Tk, int64_t d, int* splits, int* chu
 }
 
 // Whether the gradients are cross_bwd_rows_kernel's.
-bool few_rows(const CaArgs& a) { return a.R > 0 && a.R <= kFewRows && a.Tk > 0; }
+bool few_rows(const CaArgs& a) { return a.R > 0 && a.R <= kFewBwd && a.Tk > 0; }
 
 // Key ranges of dQ and ranges of query rows of dK and dV.
 void ca_bwd_plan(CaArgs& a) {
@@ -1688,7 +1689,8 @@ void launch_few(const CaArgs& a, hipStream_t st) {
   } else {
     if (a.R == 1) cross_bwd_rows_kernel<1, DP / 4, VEC><<<grid, block, 0, st>>>(a);
     else if (a.R == 2) cross_bwd_rows_kernel<2, DP / 4, VEC><<<grid, block, 0, st>>>(a);
-    else cross_bwd_rows_kernel<4, DP / 4, VEC><<<grid, block, 0, st>>>(a);
+    else if (a.R <= 4) cross_bwd_rows_kernel<4, DP / 4, VEC><<<grid, block, 0, st>>>(a);
+    else cross_bwd_rows_kernel<8, DP / 4, VEC><<<grid, block, 0, st>>>(a);
   }
 }
 
