@@ -824,7 +824,6 @@ __device__ __forceinline__ uint32_t row_top(uint32_t v) {
 }
 
 // Rows as a buffer: reads at or past `bytes` from p give zeros.
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kNowhere = 0x80000000u;  // an offset past every buffer's end
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const float* p, uint32_t bytes) {

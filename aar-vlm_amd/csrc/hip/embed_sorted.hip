@@ -17,8 +17,8 @@
 //            zero the rows that no token names.
 //  3 join    the workgroup of the chunk where a crossing run begins adds its
 //            partial rows, a quarter of them a wave, in a fixed order.
-// 32768 tokens of 50000 ids, 768 columns: lookup 29 us, sort 16, sum 50 (254 MB at 5.1
-// TB/s), join 7.  16384 tokens of 65 ids, 384 columns: 6, 12, 7 and 6, the launches'
+// 32768 tokens of 50000 ids, 768 columns: lookup 30 us, sort 16, sum 49 (254 MB at 5.2
+// TB/s), join 8.  16384 tokens of 65 ids, 384 columns: 6, 12, 7 and 6, the launches'
 // and the ids' latencies.
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -194,7 +194,8 @@ using EmbedVec = typename std::conditional<VEC, f32x4, float>::type;
 __device__ __forceinline__ float embed_zero(float*) { return 0.f; }
 __device__ __forceinline__ f32x4 embed_zero(f32x4*) { return f32x4{0.f, 0.f, 0.f, 0.f}; }
 
-constexpr int kZeroIds = 16;  // ids whose empty rows one wave zeroes
+// Ids whose empty rows one wave zeroes (89139 rows of 896: 59 us, with 16 ids 63, 64 65).
+constexpr int kZeroIds = 4;
 constexpr int kRows = 8;      // rows whose loads a wave has in flight
 
 template <bool VEC>
