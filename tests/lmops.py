@@ -113,7 +113,10 @@ def cross_exact(q, k, v, lens=None, do=None, scale=None):
 def attn_tol(d, n, smax=6.0):
     """What the roundings of an fp32 attention add up to, relative to its output:
     a score is a sum of d products, off by about sqrt(d) half steps of smax; the
-    row's sums have n terms; four standard deviations of the two."""
+    row's sums have n terms; four standard deviations of the two.  Where operands
+    stand in two fp16 parts, each off by 2^-22 = 4 U at most, and the product of the
+    second parts is left out, a product is off by 12 U at most and a score of d of them
+    by some 4 U of a score: less than a quarter of its own sums' share."""
     return 4 * U * (math.sqrt(d) * smax + math.sqrt(n) + 8)
 
 
