@@ -83,6 +83,7 @@ CASES = [
     (6, 6, 1, 2, 8, 8, 0), (21, 7, 4, 4, 30, 30, 0), (12, 12, 4, 2, 64, 32, 0), (12, 4, 3, 3, 64, 0, 0),
     (8, 8, 2, 2, 64, 64, 3), (5, 5, 1, 1, 2, 2, 0), (6, 6, 3, 2, 7, 4, 1), (40, 40, 4, 0, 64, 64, 0),
     (40, 40, 0, 4, 64, 64, 0), (3000, 1000, 5, 3, 64, 64, 0), (2, 2, 60, 12, 128, 128, 0), (4, 4, 2, 2, 255, 254, 0),
+    (5000, 1000, 4, 2, 30, 30, 0), (4500, 1500, 2, 1, 200, 100, 0), (4200, 4200, 3, 3, 100, 50, 2),
 ]
 
 
