@@ -414,10 +414,10 @@ cross_combine_kernel(const CaArgs a) {
 // 32 keys at a time: S^T = K Q^T leaves a lane 16 keys of its row, whose online
 // softmax is in registers but for one exchange with lane ^ 32, and P feeds
 // O^T += V^T P^T from the registers it is left in.  This form and its gradients run
-// for rows of up to 32 floats and unaligned ones, bound by the fp32 matrix instruction:
-// 8 x 12 heads, 1024 x 4096, d 64 in 934 us, 110 TFLOP/s of the 153 that a large fp32
-// product reaches.
-template <int DP, bool VEC>
+// for unaligned rows (and those further apart than a tile's reads below allow), bound by
+// the fp32 matrix instruction: 8 x 12 heads, 1024 x 4096, d 64, aligned, took 934 us,
+// 110 TFLOP/s of the 153 that a large fp32 product reaches.
+template <int DP>
 __global__ void __launch_bounds__(kFaThreads)
 cross_fwd_kernel(const CaArgs a) {
   constexpr int NC = DP / 8;
@@ -441,7 +441,7 @@ cross_fwd_kernel(const CaArgs a) {
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int dd = 8 * c + 4 * h;
-    qr[c] = qi < a.R ? load4<VEC>(Q + dd, a.d - dd) : f32x4{0.f, 0.f, 0.f, 0.f};
+    qr[c] = qi < a.R ? load4<false>(Q + dd, a.d - dd) : f32x4{0.f, 0.f, 0.f, 0.f};
   }
   f32x16 o[NB];
 #pragma unroll
@@ -450,7 +450,7 @@ cross_fwd_kernel(const CaArgs a) {
   const int ntiles = k1 > k0 ? (k1 - k0 + kTile - 1) / kTile : 0;
   const bool work = qb * kBlock + wave * kTile < a.R;
 
-  TileCopy<DP, VEC> kc, vc;
+  TileCopy<DP, false> kc, vc;
   if (ntiles > 0) {
     kc.load(K, a.k.st, k0, k1, a.d, tid);
     vc.load(V, a.v.st, k0, k1, a.d, tid);
@@ -515,7 +515,7 @@ cross_fwd_kernel(const CaArgs a) {
     }
     __syncthreads();
   }
-  if (qi < a.R) ca_store_row<DP, VEC>(a, bh, part, qi, h, o, m, l);
+  if (qi < a.R) ca_store_row<DP, false>(a, bh, part, qi, h, o, m, l);
 }
 
 // ------------------------------------------------------------------ backward
@@ -523,7 +523,7 @@ cross_fwd_kernel(const CaArgs a) {
 // dQ, and D of the rows for the dK/dV pass: a workgroup takes 128 query rows with
 // q and dO in registers and walks the keys: S^T, dP^T (lane = row), dS, dQ^T +=
 // K^T dS^T.
-template <int DP, bool VEC>
+template <int DP>
 __global__ void __launch_bounds__(kFaThreads)
 cross_bwd_dq_kernel(const CaArgs a) {
   constexpr int NC = DP / 8;
@@ -551,9 +551,9 @@ cross_bwd_dq_kernel(const CaArgs a) {
     for (int c = 0; c < NC; ++c) {
       const int dd = 8 * c + 4 * h;
       const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-      qr[c] = row_ok ? load4<VEC>(Q + dd, a.d - dd) : z;
-      dor[c] = row_ok ? load4<VEC>(dO + dd, a.d - dd) : z;
-      const f32x4 of = row_ok ? load4<VEC>(O + dd, a.d - dd) : z;
+      qr[c] = row_ok ? load4<false>(Q + dd, a.d - dd) : z;
+      dor[c] = row_ok ? load4<false>(dO + dd, a.d - dd) : z;
+      const f32x4 of = row_ok ? load4<false>(O + dd, a.d - dd) : z;
 #pragma unroll
       for (int e = 0; e < 4; ++e) dsum += dor[c][e] * of[e];
     }
@@ -569,7 +569,7 @@ cross_bwd_dq_kernel(const CaArgs a) {
   const int ntiles = k1 > k0 ? (k1 - k0 + kTile - 1) / kTile : 0;
   const bool work = qb * kBlock + wave * kTile < a.R;
 
-  TileCopy<DP, VEC> kc, vc;
+  TileCopy<DP, false> kc, vc;
   if (ntiles > 0) {
     kc.load(K, a.k.st, k0, k1, a.d, tid);
     vc.load(V, a.v.st, k0, k1, a.d, tid);
@@ -616,13 +616,13 @@ cross_bwd_dq_kernel(const CaArgs a) {
     }
     __syncthreads();
   }
-  if (row_ok) ca_store_dq<DP, VEC>(a, bh, part, qi, dq, h);
+  if (row_ok) ca_store_dq<DP, false>(a, bh, part, qi, dq, h);
 }
 
 // A [32][DP] tile of query rows (TileCopy over rows that may cross heads).
-template <int DP, bool VEC>
-struct CaRowTile : TileCopy<DP, VEC> {
-  using Base = TileCopy<DP, VEC>;
+template <int DP>
+struct CaRowTile : TileCopy<DP, false> {
+  using Base = TileCopy<DP, false>;
   __device__ __forceinline__ void load_rows(const FaIn& x, const CaArgs& a, int bh, int row0, int tid) {
 #pragma unroll
     for (int i = 0; i < Base::kPer; ++i) {
@@ -630,7 +630,7 @@ struct CaRowTile : TileCopy<DP, VEC> {
       const int r = row0 + u / (DP / 4);
       const int c = (u % (DP / 4)) * 4;
       f32x4 v = {0.f, 0.f, 0.f, 0.f};
-      if (u < Base::kUnits && r < a.R) v = load4<VEC>(x.p + ca_row(x, a, bh, r) + c, a.d - c);
+      if (u < Base::kUnits && r < a.R) v = load4<false>(x.p + ca_row(x, a, bh, r) + c, a.d - c);
       Base::reg[i] = v;
     }
   }
@@ -639,7 +639,7 @@ struct CaRowTile : TileCopy<DP, VEC> {
 // dK and dV: a workgroup takes 128 keys (32 a wave, a lane its key, k and v in
 // registers) and walks the query rows: S, dP (lane = key), P, dS, dV^T += dO^T P,
 // dK^T += Q^T dS.
-template <int DP, bool VEC>
+template <int DP>
 __global__ void __launch_bounds__(kFaThreads, DP <= 64 ? 2 : 1)
 cross_bwd_dkdv_kernel(const CaArgs a) {
   constexpr int NC = DP / 8;
@@ -664,8 +664,8 @@ cross_bwd_dkdv_kernel(const CaArgs a) {
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int dd = 8 * c + 4 * h;
-    kr[c] = key_ok ? load4<VEC>(K + (int64_t)kj * a.k.st + dd, a.d - dd) : f32x4{0.f, 0.f, 0.f, 0.f};
-    vr[c] = key_ok ? load4<VEC>(V + (int64_t)kj * a.v.st + dd, a.d - dd) : f32x4{0.f, 0.f, 0.f, 0.f};
+    kr[c] = key_ok ? load4<false>(K + (int64_t)kj * a.k.st + dd, a.d - dd) : f32x4{0.f, 0.f, 0.f, 0.f};
+    vr[c] = key_ok ? load4<false>(V + (int64_t)kj * a.v.st + dd, a.d - dd) : f32x4{0.f, 0.f, 0.f, 0.f};
   }
   f32x16 dk[NB], dv[NB];
 #pragma unroll
@@ -674,7 +674,7 @@ cross_bwd_dkdv_kernel(const CaArgs a) {
   const int t0 = part * a.kv_tiles;
   const int t1 = kb * kBlock < len ? min((a.R + kTile - 1) / kTile, t0 + a.kv_tiles) : t0;
 
-  CaRowTile<DP, VEC> qc, dc;
+  CaRowTile<DP> qc, dc;
   float lreg = 0.f, dreg = 0.f;
   auto load_tile = [&](int t) {
     qc.load_rows(a.q, a, bh, t * kTile, tid);
@@ -742,7 +742,7 @@ cross_bwd_dkdv_kernel(const CaArgs a) {
     if (has_next) store_tile(cur ^ 1);
     __syncthreads();
   }
-  if (kj < a.Tk) ca_store_key<DP, VEC>(a, bh, part, kj, key_ok, dk, dv, h);
+  if (kj < a.Tk) ca_store_key<DP, false>(a, bh, part, kj, key_ok, dk, dv, h);
 }
 
 // ---------------------------------------------------- on the fp16 matrix cores
@@ -1640,12 +1640,13 @@ void ca_bwd_plan(CaArgs& a) {
   a.kv_splits = (int)std::max<int64_t>(1, ceil_div(qt, c));
 }
 
-// Whether the tiled passes run on the fp16 matrix cores: where rows are 16-byte
-// aligned and longer than 32 floats.  Forward + backward of 384 heads' 256 x 300, d 64:
-// 212 us against 391 with the fp32 instruction, 256 x 7: 86 against 102; 16 x 7 alone
-// loses (27 against 24).  Up to 32 floats, padded to 64, they would do twice the work.
+// The head dim that the tiled passes are built for.  They run on the fp16 matrix cores
+// where rows are 16-byte aligned, with up to 64 floats padded to that.  Forward +
+// backward of 384 heads' 256 x 300, d 64: 212 us against 391 with the fp32 instruction,
+// 256 x 7: 86 against 102; 16 x 7 alone loses (27 against 24).  96 heads' 512 x 2048,
+// d 32: 409 us against 527.
 template <int DP, bool VEC>
-constexpr bool kSplit = VEC && DP >= 64;
+constexpr int kTileDim = VEC && DP < 64 ? 64 : DP;
 
 bool ca_shape_ok(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk) {
   const int64_t most = int64_t(1) << 24;
@@ -1695,42 +1696,50 @@ void launch_few(const CaArgs& a, hipStream_t st) {
 
 template <int DP, bool VEC>
 int launch_fwd(const CaArgs& a, hipStream_t st) {
-  if (a.R <= kFewRows) {
+  constexpr int TP = kTileDim<DP, VEC>;
+  const bool few = a.R <= kFewRows;
+  if (few) {
     launch_few<DP, VEC, true>(a, st);
   } else {
     const dim3 grid((unsigned)(ceil_div(a.R, kBlock) * a.BH * a.splits));
-    if constexpr (kSplit<DP, VEC>) cross_fwd_split_kernel<DP><<<grid, dim3(kFaThreads), 0, st>>>(a);
-    else cross_fwd_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
+    if constexpr (VEC) cross_fwd_split_kernel<TP><<<grid, dim3(kFaThreads), 0, st>>>(a);
+    else cross_fwd_kernel<TP><<<grid, dim3(kFaThreads), 0, st>>>(a);
   }
   const int rc = launch_status();
   if (rc != AAR_OK || a.splits == 1) return rc;
-  const int64_t lanes = (int64_t)a.BH * a.R * (DP / 4);
-  cross_combine_kernel<DP, VEC><<<dim3((unsigned)ceil_div(lanes, (int64_t)256)), dim3(256), 0, st>>>(a);
+  const int64_t rows = (int64_t)a.BH * a.R;
+  auto blocks = [&](int dim) { return dim3((unsigned)ceil_div(rows * (dim / 4), (int64_t)256)); };
+  if (few) cross_combine_kernel<DP, VEC><<<blocks(DP), dim3(256), 0, st>>>(a);
+  else cross_combine_kernel<TP, VEC><<<blocks(TP), dim3(256), 0, st>>>(a);
   return launch_status();
 }
 
 template <int DP, bool VEC>
 int launch_bwd(const CaArgs& a, hipStream_t st) {
+  constexpr int TP = kTileDim<DP, VEC>;
+  const bool few = few_rows(a);
   int rc = AAR_OK;
-  if (few_rows(a)) {
+  if (few) {
     launch_few<DP, VEC, false>(a, st);
     rc = launch_status();
   } else {
     if (a.R > 0) {
       const dim3 grid((unsigned)(ceil_div(a.R, kBlock) * a.BH * a.splits));
-      if constexpr (kSplit<DP, VEC>) cross_bwd_dq_split_kernel<DP><<<grid, dim3(kFaThreads), 0, st>>>(a);
-      else cross_bwd_dq_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
+      if constexpr (VEC) cross_bwd_dq_split_kernel<TP><<<grid, dim3(kFaThreads), 0, st>>>(a);
+      else cross_bwd_dq_kernel<TP><<<grid, dim3(kFaThreads), 0, st>>>(a);
       rc = launch_status();
     }
     if (rc != AAR_OK || a.Tk == 0) return rc;
     const dim3 grid((unsigned)(ceil_div(a.Tk, kBlock) * a.BH * a.kv_splits));
-    if constexpr (kSplit<DP, VEC>) cross_bwd_dkdv_split_kernel<DP><<<grid, dim3(kFaThreads), 0, st>>>(a);
-    else cross_bwd_dkdv_kernel<DP, VEC><<<grid, dim3(kFaThreads), 0, st>>>(a);
+    if constexpr (VEC) cross_bwd_dkdv_split_kernel<TP><<<grid, dim3(kFaThreads), 0, st>>>(a);
+    else cross_bwd_dkdv_kernel<TP><<<grid, dim3(kFaThreads), 0, st>>>(a);
     rc = launch_status();
   }
   const int64_t rows = (a.splits > 1 ? (int64_t)a.BH * a.R : 0) + (a.kv_splits > 1 ? 2 * (int64_t)a.BH * a.Tk : 0);
   if (rc != AAR_OK || rows == 0) return rc;
-  cross_bwd_sum_kernel<DP, VEC><<<dim3((unsigned)ceil_div(rows * (DP / 4), (int64_t)256)), dim3(256), 0, st>>>(a);
+  auto blocks = [&](int dim) { return dim3((unsigned)ceil_div(rows * (dim / 4), (int64_t)256)); };
+  if (few) cross_bwd_sum_kernel<DP, VEC><<<blocks(DP), dim3(256), 0, st>>>(a);
+  else cross_bwd_sum_kernel<TP, VEC><<<blocks(TP), dim3(256), 0, st>>>(a);
   return launch_status();
 }
 
@@ -1755,13 +1764,16 @@ int ca_check(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t 
   return AAR_OK;
 }
 
+// Floats of a part's row, at most.
+int part_dim(int64_t d) { return std::max(pad_dim(d), 64); }
+
 size_t part_o_bytes(int64_t bh, int64_t R, int64_t d, int splits) {
-  return (size_t)bh * splits * (size_t)R * pad_dim(d) * sizeof(float);
+  return (size_t)bh * splits * (size_t)R * part_dim(d) * sizeof(float);
 }
 
 // Where the backward's workspace holds item i (D, dQ's parts, dK's, dV's); 4: its end.
 size_t bwd_bytes(const CaArgs& a, int i) {
-  const size_t dp = pad_dim(a.d), bh = a.BH;
+  const size_t dp = part_dim(a.d), bh = a.BH;
   const size_t size[4] = {(bh * a.R * sizeof(float) + 15) / 16 * 16,
                           a.splits > 1 ? a.splits * bh * a.R * dp * sizeof(float) : 0,
                           a.kv_splits > 1 ? a.kv_splits * bh * a.Tk * dp * sizeof(float) : 0,

@@ -565,9 +565,10 @@ int aar_causal_mask_f32(const float* x, float* y, int64_t mats, int64_t T, float
  * aar_flash_fwd_strided_f32; 128-bit paths need 16-byte aligned pointers and d
  * and all strides multiples of 4.  d <= 128.  Where the query rows are too few to
  * fill the GPU the key range is split and joined through the workspace (0 bytes
- * otherwise; 16-byte aligned, AAR_EWORKSPACE).  Products of aligned rows of more
- * than 32 floats, 2^23 apart at most, are formed from two fp16 parts of each
- * operand: 22 bits of it, or 2^-38 of its row's largest element, with fp32 sums. */
+ * otherwise; 16-byte aligned, AAR_EWORKSPACE).  Products over aligned rows, 2^23
+ * floats apart at most, of more than 4 query rows a key/value head are formed from
+ * two fp16 parts of each operand: 22 bits of it, or 2^-38 of its row's largest
+ * element, with fp32 sums. */
 size_t aar_cross_attn_fwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d);
 int aar_cross_attn_fwd_f32(const float* q, const float* k, const float* v, const int64_t* kv_lens, float* o,
                            float* lse, int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d,

@@ -55,7 +55,8 @@ SHAPES = [
     (1, 2, 2, 257, 577, 64), (2, 8, 4, 65, 300, 128), (1, 3, 3, 50, 70, 1), (1, 2, 2, 40, 90, 3), (1, 2, 2, 64, 2049, 64),
     (4, 12, 12, 130, 260, 64), (1, 1, 1, 2000, 40, 64), (1, 1, 1, 1, 8192, 64), (16, 16, 16, 140, 140, 64),
     (2, 2, 2, 3, 150, 30), (2, 4, 2, 2, 65, 64), (1, 1, 1, 4, 2100, 96), (3, 3, 3, 4, 1, 128), (2, 2, 2, 5, 500, 64),
-    (1, 3, 3, 8, 1030, 128), (2, 6, 2, 3, 70, 30), (1, 1, 1, 9, 300, 32),
+    (1, 3, 3, 8, 1030, 128), (2, 6, 2, 3, 70, 30), (1, 1, 1, 9, 300, 32), (2, 4, 2, 70, 130, 32),
+    (1, 2, 2, 40, 90, 4), (1, 3, 3, 2000, 33, 16), (1, 1, 1, 40, 3000, 32),
 ]
 
 
