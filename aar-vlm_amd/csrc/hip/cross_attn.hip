@@ -1369,8 +1369,8 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
   using Tile = HalfTile<DP>;
   __shared__ __attribute__((aligned(16))) char qs[2][Tile::kBytes];
   __shared__ __attribute__((aligned(16))) char dos[2][Tile::kBytes];
-  // 2^-e of Q's rows, of dO's, of both; lse in log2 and D 2^-e of Q's
-  __shared__ __attribute__((aligned(16))) float qf[2][kTile], df[2][kTile], of[2][kTile], ls[2][kTile], ds[2][kTile];
+  // 2^-e of Q's rows and of dO's; lse in log2 and D
+  __shared__ __attribute__((aligned(16))) float qf[2][kTile], df[2][kTile], ls[2][kTile], ds[2][kTile];
   __shared__ int not_held;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lr = lane & 31, h = lane >> 5;
@@ -1429,12 +1429,10 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
 #pragma unroll
     for (int n = 0; n < Tile::kPer; ++n) {
       const int r = Tile::row(n, tid);
-      const float q = pow2(-qc.ex[n]), o = pow2(-dc.ex[n]);
-      qf[buf][r] = q;
-      df[buf][r] = o;
-      of[buf][r] = q * o;
+      qf[buf][r] = pow2(-qc.ex[n]);
+      df[buf][r] = pow2(-dc.ex[n]);
       ls[buf][r] = lreg[n];
-      ds[buf][r] = dreg[n] * q;
+      ds[buf][r] = dreg[n];
     }
   };
   if (t0 < t1) {
@@ -1470,11 +1468,12 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
       top = 0.f;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const f32x4 o4 = row_values(of[cur], g, h), d4 = row_values(ds[cur], g, h);
+        const f32x4 q4 = row_values(qf[cur], g, h), o4 = row_values(df[cur], g, h), d4 = row_values(ds[cur], g, h);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * g + e;
-          x[r] = s[r] * (x[r] * o4[e] * vf - d4[e]);
+          // P before Q's scale: dP - D is finite for all rows that are held, its product with that need not be
+          x[r] = s[r] * (x[r] * o4[e] * vf - d4[e]) * q4[e];
           top = fmaxf(top, fabsf(x[r]));
         }
       }
