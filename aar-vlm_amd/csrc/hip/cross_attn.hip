@@ -765,7 +765,7 @@ cross_bwd_dkdv_kernel(const CaArgs a) {
 // dim a row's factor is one of the output's row or column.  Over a tile's rows it
 // goes to the other operand, P or dS, which is scaled by the lane's own power of two
 // that follows the largest |P| 2^-e (|dS| 2^-e) so far: what is rounded there is at
-// most 2^-38 of the largest term of the lane's sum.
+// most 2^-38 of the largest term of the lane's sum, or 2^-150 where that is more.
 //
 // What a wave keeps in registers for all tiles (q; q and dO; k and v) is split once; a
 // tile is split on its way into LDS, once a workgroup, as two row-major planes.
@@ -773,7 +773,7 @@ cross_bwd_dkdv_kernel(const CaArgs a) {
 // P^T, K^T dS^T, dO^T P, Q^T dS) read columns through the transposing LDS read, so a
 // tile that serves both is split and stored once.  P and dS are split in the
 // registers the softmax leaves them in.  Rows whose largest element is outside
-// [2^-63, 2^60) (infinities too) are not held so: the waves that meet one do their
+// [2^-99, 2^60) (infinities too) are not held so: the waves that meet one do their
 // rows again with the fp32 instruction, from HBM.
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -805,13 +805,23 @@ __device__ __forceinline__ void half_split_pair(float a, float b, float m, uint3
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // |e| <= 126
 
-// Exponent of the scale of a row whose largest magnitude has the bits u (the largest
-// scale for zeros), and whether the parts do not hold it.
-__device__ __forceinline__ int half_exponent(uint32_t u, bool& bad) {
-  const uint32_t lo = (127 - 63) << 23, hi = (127 + 60) << 23;
+// A row's scale from the bits u of its largest magnitude: their exponent, of which the
+// factors below are made (the least for zeros), and whether the parts do not hold the
+// row: below 2^-99 the scale would pass 2^112, and what undoes it leave fp32's normal
+// range; sums of 128 products of 2^60 and 2^60 end at 2^127.
+__device__ __forceinline__ uint32_t half_exponent(uint32_t u, bool& bad) {
+  const uint32_t lo = (127 - 99) << 23, hi = (127 + 60) << 23;
   bad = bad || (u != 0 && u - lo >= hi - lo);
-  return min(max(140 - (int)(u >> 23), -47), 60);
+  return max(u, lo) & 0x7F800000u;
 }
+
+// The scale 2^e, and what undoes it: for a tile's row 2^(14 - e), which is 1 to 2 times
+// the row's largest magnitude, so that P or dS times it is as large as its largest term
+// and leaves fp32's range no sooner.  The 2^14 comes off with the factor of the lane's
+// own row in a score or dP, with HalfScale's in a sum.
+__device__ __forceinline__ float half_scale(uint32_t e) { return __uint_as_float((267u << 23) - e); }
+__device__ __forceinline__ float row_factor(uint32_t e) { return __uint_as_float(e + (1u << 23)); }
+__device__ __forceinline__ float lane_factor(uint32_t e) { return __uint_as_float(e - (27u << 23)); }
 
 // Largest of the 8 or 16 lanes of a tile's row (magnitudes, as their bits).
 template <int N>
@@ -850,7 +860,7 @@ struct HalfTile {
   static constexpr int kPer = kTile * kOcts / kFaThreads;  // 8-column units a thread stages
   static_assert(kPer * kFaThreads == kTile * kOcts && kOcts <= 16, "whole units, a row in 16 lanes");
   f32x4 f[kPer][2];
-  int ex[kPer];  // exponents of the rows that `store` has scaled
+  uint32_t ex[kPer];  // of the rows that `store` has scaled: half_exponent's
 
   // Row of unit i of thread tid, and its first column.
   __device__ __forceinline__ static int row(int i, int tid) { return (tid + i * kFaThreads) / kOcts; }
@@ -898,7 +908,7 @@ struct HalfTile {
 #pragma unroll
         for (int e = 0; e < 2; ++e) top = fmaxf(fmaxf(top, fabsf(f[i][g][2 * e])), fabsf(f[i][g][2 * e + 1]));
       ex[i] = half_exponent(row_top<kOcts>(__float_as_uint(top)), bad);
-      const float m = pow2(ex[i]);
+      const float m = half_scale(ex[i]);
       u32x4 hi, lo;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -976,8 +986,8 @@ __device__ __forceinline__ void half_cols(const char* s, const f32x16& x, float 
   }
 }
 
-// A lane's row (its half's octets of each 16 columns) times f, in parts; returns what
-// undoes the row's scale.
+// A lane's row (its half's octets of each 16 columns) times f, in parts; returns its
+// factor.
 template <int DP>
 __device__ __forceinline__ float half_row(const float* p, int d, float f, int h, u32x4 (&out)[DP / 16][2], bool& bad) {
   f32x4 x[DP / 16][2];
@@ -993,8 +1003,8 @@ __device__ __forceinline__ float half_row(const float* p, int d, float f, int h,
       for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[c][g][e]));
     }
   }
-  const int ex = half_exponent(__float_as_uint(half_swap_max(top)), bad);
-  const float m = pow2(ex);
+  const uint32_t ex = half_exponent(__float_as_uint(half_swap_max(top)), bad);
+  const float m = half_scale(ex);
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) {
 #pragma unroll
@@ -1005,13 +1015,14 @@ __device__ __forceinline__ float half_row(const float* p, int d, float f, int h,
       out[c][1][e] = lo;
     }
   }
-  return pow2(-ex);
+  return lane_factor(ex);
 }
 
-// The power of two f = 2^log that a lane's P or dS, times 2^-e of the other operand's
-// rows, is scaled by, from the magnitudes up to `top` of a tile's: the first tile sets
-// it such that the largest is in [2^13, 2^14), a later one lowers it, with the sums so
-// far, when it passes 2^15.
+// The power of two f = 2^log that a lane's P or dS, times the factors of the other
+// operand's rows, is scaled by, from the magnitudes up to `top` of a tile's: the first tile
+// sets it such that the largest is in [2^13, 2^14), a later one lowers it, with the sums
+// so far, when it passes 2^15.  Magnitudes below 2^-112 would need more than the largest
+// scale, 2^126; under that one what a part rounds is 2^-151, less than fp32 holds.
 template <int NB>
 struct HalfScale {
   int log = 0;
@@ -1022,8 +1033,8 @@ struct HalfScale {
     if (!__any(top > most)) return;
     if (top > most) {
       const int to = 140 - (int)(__float_as_uint(big) >> 23);
-      bad = bad || to < -100;
-      const int by = min(min(max(to, -100), 100) - log, 126);
+      bad = bad || to < -114;  // infinite
+      const int by = min(min(to, 126) - log, 126);
       log += by;
       f = pow2(log);
       most = ldexpf(32768.f, -log);
@@ -1035,7 +1046,15 @@ struct HalfScale {
       }
     }
   }
-  __device__ __forceinline__ float undo() const { return pow2(-log); }
+  // The sums themselves.
+  __device__ __forceinline__ void undo(f32x16 (&acc)[NB]) const {
+    const float by = pow2(-log);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[b][r] = acc[b][r] * 0x1p-14f * by;
+    }
+  }
 };
 
 // Rows 8 g + 4 h .. of a tile's row values.
@@ -1052,7 +1071,7 @@ cross_fwd_split_kernel(const CaArgs a) {
   constexpr int NB = DP / 32;
   __shared__ __attribute__((aligned(16))) char ks[2][Tile::kBytes];
   __shared__ __attribute__((aligned(16))) char vs[2][Tile::kBytes];
-  __shared__ __attribute__((aligned(16))) float kf[2][kTile], vf[2][kTile];  // 2^-e of the rows
+  __shared__ __attribute__((aligned(16))) float kf[2][kTile], vf[2][kTile];  // the rows' factors
   __shared__ int not_held;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lr = lane & 31, h = lane >> 5;
@@ -1144,8 +1163,8 @@ cross_fwd_split_kernel(const CaArgs a) {
 #pragma unroll
     for (int n = 0; n < Tile::kPer; ++n) {
       const int r = Tile::row(n, tid);
-      kf[buf][r] = pow2(-kc[i].ex[n]);
-      vf[buf][r] = pow2(-vc[i].ex[n]);
+      kf[buf][r] = row_factor(kc[i].ex[n]);
+      vf[buf][r] = row_factor(vc[i].ex[n]);
     }
   };
   if (ntiles > 0) {
@@ -1166,12 +1185,7 @@ cross_fwd_split_kernel(const CaArgs a) {
       lds_barrier();
     }
   }
-  const float by = fit.undo();
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[b][r] *= by;
-  }
+  fit.undo(o);
 
   if (bad) not_held = 1;
   __syncthreads();
@@ -1225,7 +1239,7 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
   using Tile = HalfTile<DP>;
   __shared__ __attribute__((aligned(16))) char ks[2][Tile::kBytes];
   __shared__ __attribute__((aligned(16))) char vs[2][Tile::kBytes];
-  __shared__ __attribute__((aligned(16))) float kf[2][kTile], vf[2][kTile];  // 2^-e of the rows
+  __shared__ __attribute__((aligned(16))) float kf[2][kTile], vf[2][kTile];  // the rows' factors
   __shared__ int not_held;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lr = lane & 31, h = lane >> 5;
@@ -1281,8 +1295,8 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
 #pragma unroll
     for (int n = 0; n < Tile::kPer; ++n) {
       const int r = Tile::row(n, tid);
-      kf[buf][r] = pow2(-kc.ex[n]);
-      vf[buf][r] = pow2(-vc.ex[n]);
+      kf[buf][r] = row_factor(kc.ex[n]);
+      vf[buf][r] = row_factor(vc.ex[n]);
     }
   };
   if (ntiles > 0) {
@@ -1322,12 +1336,7 @@ cross_bwd_dq_split_kernel(const CaArgs a) {
     if (has_next) store(buf ^ 1);
     lds_barrier();
   }
-  const float by = fit.undo();
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) dq[b][r] *= by;
-  }
+  fit.undo(dq);
 
   if (bad) not_held = 1;
   __syncthreads();
@@ -1369,7 +1378,7 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
   using Tile = HalfTile<DP>;
   __shared__ __attribute__((aligned(16))) char qs[2][Tile::kBytes];
   __shared__ __attribute__((aligned(16))) char dos[2][Tile::kBytes];
-  // 2^-e of Q's rows and of dO's; lse in log2 and D
+  // factors of Q's rows and of dO's; lse in log2 and D
   __shared__ __attribute__((aligned(16))) float qf[2][kTile], df[2][kTile], ls[2][kTile], ds[2][kTile];
   __shared__ int not_held;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -1429,8 +1438,8 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
 #pragma unroll
     for (int n = 0; n < Tile::kPer; ++n) {
       const int r = Tile::row(n, tid);
-      qf[buf][r] = pow2(-qc.ex[n]);
-      df[buf][r] = pow2(-dc.ex[n]);
+      qf[buf][r] = row_factor(qc.ex[n]);
+      df[buf][r] = row_factor(dc.ex[n]);
       ls[buf][r] = lreg[n];
       ds[buf][r] = dreg[n];
     }
@@ -1484,15 +1493,8 @@ cross_bwd_dkdv_split_kernel(const CaArgs a) {
     if (has_next) store(cur ^ 1);
     lds_barrier();
   }
-  const float by_v = fit_v.undo(), by_k = fit_k.undo();
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      dv[b][r] *= by_v;
-      dk[b][r] *= by_k;
-    }
-  }
+  fit_v.undo(dv);
+  fit_k.undo(dk);
 
   if (bad) not_held = 1;
   __syncthreads();

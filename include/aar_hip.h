@@ -568,7 +568,9 @@ int aar_causal_mask_f32(const float* x, float* y, int64_t mats, int64_t T, float
  * otherwise; 16-byte aligned, AAR_EWORKSPACE).  Products over aligned rows, 2^23
  * floats apart at most, of more than 4 query rows a key/value head are formed from
  * two fp16 parts of each operand: 22 bits of it, or 2^-38 of its row's largest
- * element, with fp32 sums. */
+ * element, with fp32 sums; so are P and dS, to 2^-38 of the largest term of their sum
+ * or 2^-150.  Rows whose largest element is not 0 and outside [2^-99, 2^60) take the
+ * fp32 instruction. */
 size_t aar_cross_attn_fwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d);
 int aar_cross_attn_fwd_f32(const float* q, const float* k, const float* v, const int64_t* kv_lens, float* o,
                            float* lse, int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t d,
