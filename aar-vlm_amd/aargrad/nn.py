@@ -248,6 +248,21 @@ def scaled_dot_product_attention(q, k, v, *, causal=False):
     return _core.matmul(_core.softmax(logits), v)
 
 
+_POSITIONS = {}  # (length, device): 0 .. length - 1, for lengths of powers of two
+
+
+def _positions_up_to(T, device):
+    """0 .. T-1 as the first entries of a tensor that all modules share: one for each
+    power of two from 1024 on, so what is kept is at most four times the longest, and none
+    is ever replaced (a captured graph may read it)."""
+    if T == 0:
+        return _core.from_numpy(np.arange(0, dtype=np.int64)).to(device)
+    key = (1 << max(10, (T - 1).bit_length()), device)
+    if key not in _POSITIONS:
+        _POSITIONS.setdefault(key, _core.from_numpy(np.arange(key[0], dtype=np.int64)).to(device))
+    return _core.slice(_POSITIONS[key], 0, 0, T)
+
+
 class MultiHeadAttention(Module):
     """Packed qkv projection, attention per head, output projection.
 
@@ -281,15 +296,11 @@ class MultiHeadAttention(Module):
             self.norm_eps = norm_eps
             self.q_norm = _new_parameter(np.ones(self.d_head))
             self.k_norm = _new_parameter(np.ones(self.d_head))
-            self._positions = {}
 
     def _positions_or_default(self, positions, x):
         if positions is not None or self.rotary_dim == 0:
             return positions
-        key = (x.shape[-2], x.device)
-        if key not in self._positions:
-            self._positions[key] = _core.from_numpy(np.arange(key[0], dtype=np.int64)).to(x.device)
-        return self._positions[key]
+        return _positions_up_to(x.shape[-2], x.device)
 
     def forward(self, x, positions=None):
         qkv = self.qkv_proj(x)
