@@ -184,7 +184,9 @@ struct EmbedArgs {
   float* part;  // [chunks][2][dim]: the run that began before the chunk, the one that goes on after it
   float* dw;
   int64_t dim;
-  int n, vocab, chunk, chunks, blocks;  // blocks: of 64 lanes' columns in a row
+  int n, vocab, chunk, chunks;
+  int block0, blocks;  // the launch's part of a row's blocks of 64 lanes' columns
+  int zero_waves;
   float scale;
 };
 
@@ -210,21 +212,22 @@ embed_sum_kernel(const EmbedArgs a) {
   if (unit >= (int64_t)a.chunks * a.blocks) {
     // rows without a token
     unit -= (int64_t)a.chunks * a.blocks;
-    const int64_t v0 = unit * kZeroIds;
-    if (v0 >= a.vocab) return;
-    const int v = (int)v0 + lane;
-    const bool empty = lane < kZeroIds && v < a.vocab && a.start[v] == a.start[v + 1];
-    unsigned long long todo = __ballot(empty);
-    while (todo) {
-      const int l = __builtin_ctzll(todo);
-      V* row = reinterpret_cast<V*>(a.dw + (v0 + l) * a.dim);
-      for (int64_t c = lane; c < dimv; c += kWave) __builtin_nontemporal_store(zero, row + c);
-      todo &= todo - 1;
+    if (unit >= a.zero_waves) return;
+    for (int64_t v0 = unit * kZeroIds; v0 < a.vocab; v0 += (int64_t)a.zero_waves * kZeroIds) {
+      const int v = (int)v0 + lane;
+      const bool empty = lane < kZeroIds && v < a.vocab && a.start[v] == a.start[v + 1];
+      unsigned long long todo = __ballot(empty);
+      while (todo) {
+        const int l = __builtin_ctzll(todo);
+        V* row = reinterpret_cast<V*>(a.dw + (v0 + l) * a.dim);
+        for (int64_t c = lane; c < dimv; c += kWave) __builtin_nontemporal_store(zero, row + c);
+        todo &= todo - 1;
+      }
     }
     return;
   }
   const int chunk = (int)(unit / a.blocks);
-  const int64_t col = (unit % a.blocks) * kWave + lane;
+  const int64_t col = (a.block0 + unit % a.blocks) * kWave + lane;
   const bool on = col < dimv;
   const int total = a.start[a.vocab];
   const int p0 = chunk * a.chunk, p1 = min(total, p0 + a.chunk);
@@ -279,7 +282,7 @@ embed_join_kernel(const EmbedArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int chunk = (int)(blockIdx.x / (unsigned)a.blocks);
   const int64_t dimv = a.dim / kE;
-  const int64_t col = (int64_t)(blockIdx.x % (unsigned)a.blocks) * kWave + lane;
+  const int64_t col = (a.block0 + (int64_t)(blockIdx.x % (unsigned)a.blocks)) * kWave + lane;
   const int total = a.start[a.vocab];
   const int p0 = chunk * a.chunk, p1 = p0 + a.chunk;
   if (p1 >= total) return;  // the last chunk's runs end in it
@@ -331,17 +334,28 @@ bool embed_shape_ok(int64_t n, int64_t vocab, int64_t dim) {
   return n <= INT32_MAX - 65536 && vocab <= INT32_MAX - 65536 && dim <= INT32_MAX;
 }
 
+// A launch's work items are counted in 32 bits, so tables of more than 2^26 ids are
+// zeroed by waves that take several fours of them, and rows of more columns than 2^24
+// waves (or the join's workgroups) cover go in several launches.
+constexpr int64_t kMaxWaves = (int64_t(1) << 24) - 1;
+
 template <bool VEC>
 int launch_sum(EmbedArgs a, hipStream_t st) {
-  a.blocks = (int)ceil_div(a.dim, (VEC ? 4 : 1) * kWave);
-  const int64_t units = (int64_t)a.chunks * a.blocks + ceil_div(a.vocab, kZeroIds);
-  if (ceil_div(units, 4) * 256 > (int64_t)UINT32_MAX || (int64_t)a.chunks * a.blocks * 256 > (int64_t)UINT32_MAX)
-    return AAR_EUNSUPPORTED;
-  embed_sum_kernel<VEC><<<dim3((unsigned)ceil_div(units, 4)), dim3(256), 0, st>>>(a);
-  const int rc = launch_status();
-  if (rc != AAR_OK || a.chunks < 2) return rc;
-  embed_join_kernel<VEC><<<dim3((unsigned)(a.chunks * a.blocks)), dim3(256), 0, st>>>(a);
-  return launch_status();
+  const int64_t blocks = ceil_div(a.dim, (VEC ? 4 : 1) * kWave), most = std::max<int64_t>(1, kMaxWaves / a.chunks);
+  for (int64_t b = 0; b < blocks; b += most) {
+    a.block0 = (int)b;
+    a.blocks = (int)std::min(most, blocks - b);
+    a.zero_waves = b == 0 ? (int)std::min<int64_t>(ceil_div(a.vocab, kZeroIds), kMaxWaves) : 0;
+    const int64_t sums = (int64_t)a.chunks * a.blocks;
+    embed_sum_kernel<VEC><<<dim3((unsigned)ceil_div(sums + a.zero_waves, 4)), dim3(256), 0, st>>>(a);
+    int rc = launch_status();
+    if (rc != AAR_OK) return rc;
+    if (a.chunks < 2) continue;
+    embed_join_kernel<VEC><<<dim3((unsigned)sums), dim3(256), 0, st>>>(a);
+    rc = launch_status();
+    if (rc != AAR_OK) return rc;
+  }
+  return AAR_OK;
 }
 
 }  // namespace
@@ -390,7 +404,7 @@ int aar_embedding_sorted_bwd_f32(const float* g, const int64_t* ids, float* dw, 
   int* start = reinterpret_cast<int*>(ws + 2 * token_bytes(n));
   const int64_t slice = slice_ids(vocab), chunk = chunk_tokens(n);
   EmbedArgs a{g, token, sid, start, reinterpret_cast<float*>(ws + 2 * token_bytes(n) + start_bytes(vocab)), dw, dim,
-              (int)n, (int)vocab, (int)chunk, (int)ceil_div(n, chunk), 0, scale};
+              (int)n, (int)vocab, (int)chunk, (int)ceil_div(n, chunk), 0, 0, 0, scale};
   const bool vec = dim % 4 == 0 && aligned16(g) && aligned16(dw);
   embed_sort_kernel<<<dim3((unsigned)ceil_div(vocab, slice)), dim3(kSortThreads), 0, st>>>(ids, (int)n, (int)vocab,
                                                                                           (int)slice, token, sid, start);

@@ -599,7 +599,8 @@ int aar_embedding_scaled_fwd_f32(const float* w, const int64_t* ids, float* out,
  * nothing).  The tokens are sorted by id and summed in their order, chunk by
  * chunk: no float atomics, the same bits on every run.  Any vocabulary (unlike
  * aar_embedding_bwd_f32, whose one-hot product is limited to n * vocab <= 2^30);
- * n and vocab below 2^31 (AAR_EUNSUPPORTED).  The workspace holds the sorted
+ * n and vocab at most 2^31 - 65537, dim below 2^31 (else AAR_EUNSUPPORTED, and a
+ * workspace of 0 bytes).  The workspace holds the sorted
  * tokens and the partial sums of rows that cross chunks; 16-byte aligned
  * (AAR_EWORKSPACE). */
 size_t aar_embedding_sorted_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t dim);

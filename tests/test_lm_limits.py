@@ -1,0 +1,25 @@
+"""CPU checks of the sizes that the encoder-reading decoder's entry points take and
+refuse: a size query and its call agree, before any launch."""
+from __future__ import annotations
+
+import pytest
+
+import lmops as M
+
+X = 4096  # a pointer that is never dereferenced: every call below returns before any device work
+
+
+@pytest.fixture(scope="module")
+def L():
+    return M.lib()
+
+
+def test_sorted_gradient_sizes(L):
+    most = 2 ** 31 - 65537
+    for n, vocab, dim, fine in ((4, 2 ** 28 + 77, 1, True), (4, most, 4, True), (4, most + 1, 4, False), (most, 65, 4, True),
+                                (most + 1, 65, 4, False), (16384, 5, 1048579, True), (32768, 5, 2 ** 31 - 1, True),
+                                (32768, 5, 2 ** 31, False)):
+        nb = L.aar_embedding_sorted_bwd_workspace_bytes(n, vocab, dim)
+        rc = L.aar_embedding_sorted_bwd_f32(X, X, X, n, vocab, dim, 1.0, None, 0, None)
+        assert (nb > 0, rc) == ((True, M.EWORKSPACE) if fine else (False, M.EUNSUPPORTED)), (n, vocab, dim)
+        assert not fine or nb >= 8 * n + 4 * vocab
