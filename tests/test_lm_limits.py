@@ -23,3 +23,13 @@ def test_sorted_gradient_sizes(L):
         rc = L.aar_embedding_sorted_bwd_f32(X, X, X, n, vocab, dim, 1.0, None, 0, None)
         assert (nb > 0, rc) == ((True, M.EWORKSPACE) if fine else (False, M.EUNSUPPORTED)), (n, vocab, dim)
         assert not fine or nb >= 8 * n + 4 * vocab
+
+
+def test_distillation_sizes(L):
+    for vocab, top, most in ((80, 16, 2 ** 28 - 16), (81, 16, 2 ** 26 - 4), (80, 17, 2 ** 26 - 4), (2048, 1, 2 ** 26 - 4),
+                             (2049, 1, 2 ** 24 - 1), (50000, 64, 2 ** 24 - 1)):
+        for n, fine in ((most, True), (most + 1, False)):
+            rc = L.aar_distill_fwd_f32(X, X, X, X, X, n, vocab, top, 1.0, None, None, 0, None)
+            assert rc == (M.EWORKSPACE if fine else M.EUNSUPPORTED), (vocab, top, n)
+            if not fine:
+                assert L.aar_distill_bwd_f32(X, X, X, X, X, X, n, vocab, top, 1.0, None) == M.EUNSUPPORTED

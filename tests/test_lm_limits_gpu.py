@@ -73,3 +73,37 @@ def test_gradient_of_rows_of_a_million_columns(L):
     assert int(torch.count_nonzero(dw[[0, 2, 4]])) == 0
     del g, ws, dw
     torch.cuda.empty_cache()
+
+
+def distill(L, z, t, ids, tau, grad=1.0):
+    n, V, K = z.shape[0], z.shape[1], ids.shape[1]
+    loss, stats = torch.full((1,), 7.0, device="cuda"), torch.empty(2 * n + 1, device="cuda")
+    dz, g = torch.full_like(z, 7.0), torch.tensor([grad], device="cuda")
+    nb = L.aar_distill_workspace_bytes(n)
+    ws = M.scratch(nb)
+    M.ok(L.aar_distill_fwd_f32(z.data_ptr(), t.data_ptr(), ids.data_ptr(), loss.data_ptr(), stats.data_ptr(), n, V, K, tau,
+                               None, ws.data_ptr(), nb, M.stream()))
+    M.ok(L.aar_distill_bwd_f32(g.data_ptr(), z.data_ptr(), t.data_ptr(), ids.data_ptr(), stats.data_ptr(), dz.data_ptr(), n,
+                               V, K, tau, M.stream()))
+    return loss, dz
+
+
+@pytest.mark.parametrize("V", [5, 96])
+def test_distillation_of_many_rows(L, V):
+    """16384 sequences of 256 tokens, and one row more: the loss is the mean over all of
+    them, a row's gradient that of the same row in a small batch, but for the mean."""
+    n, part = 16384 * 256 + 1, 1024
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    z = torch.randn(n, V, generator=gen, device="cuda")
+    t = torch.randn(n, 2, generator=gen, device="cuda")
+    ids = torch.randint(0, V, (n, 2), generator=gen, device="cuda")
+    loss, dz = distill(L, z, t, ids, 1.0, float(n))
+    for at in (0, 16384 * 255, n - part):
+        one, dpart = distill(L, z[at:at + part].clone(), t[at:at + part].clone(), ids[at:at + part].clone(), 1.0, float(part))
+        # grad / rows is 1 in both
+        assert torch.equal(dz[at:at + part], dpart)
+    p = torch.softmax(t.double(), -1)
+    logq = torch.log_softmax(z.double(), -1).gather(1, ids)
+    want = (torch.xlogy(p, p) - p * logq).sum(-1).mean().item()
+    # each row's loss is a difference of numbers of up to 16: 64 half steps, as for small batches
+    assert abs(loss.item() - want) <= 64 * M.U * 16
