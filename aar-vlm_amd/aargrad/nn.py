@@ -149,8 +149,8 @@ class DistillationLoss(Module):
 
     def __init__(self, temperature=1.0):
         super().__init__()
-        if not 0.0 < temperature < math.inf:
-            raise ValueError("DistillationLoss: temperature must be positive")
+        if not 2.0 ** -61 <= temperature <= 2.0 ** 61:  # the loss stays in fp32's range
+            raise ValueError("DistillationLoss: temperature must be positive, in [2^-61, 2^61]")
         self.temperature = temperature
 
     def forward(self, logits, teacher_logits, teacher_ids):

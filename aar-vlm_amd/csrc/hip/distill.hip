@@ -495,7 +495,8 @@ int launch_short_bwd(const float* grad, const float* z, const float* tl, const i
 // A launch's work items are counted in 32 bits: 2^28 - 16 short rows, 2^26 - 4 of a wave,
 // 2^24 - 1 of a workgroup (of 16 waves: no more than CUs).
 int distill_check(int64_t n, int64_t vocab, int64_t top, float tau) {
-  if (n < 0 || vocab <= 0 || top <= 0 || !(tau > 0.f) || !(tau < INFINITY)) return AAR_EINVAL;
+  // (tau^2 ln(vocab) and log2(e) / tau stay in fp32's range)
+  if (n < 0 || vocab <= 0 || top <= 0 || !(tau >= 0x1p-61f) || !(tau <= 0x1p61f)) return AAR_EINVAL;
   if (top > kMaxTop || vocab > INT32_MAX - 4096) return AAR_EUNSUPPORTED;
   const int64_t rows = short_rows(vocab, top) ? kShortRows : (waves_per_row(n, vocab) == 1 ? 4 : 1);  // of a workgroup
   return ceil_div(n, rows) * 256 > (int64_t)UINT32_MAX ? AAR_EUNSUPPORTED : AAR_OK;

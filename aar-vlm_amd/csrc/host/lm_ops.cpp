@@ -399,8 +399,8 @@ Tensor distill_loss(const Tensor& logits, const Tensor& teacher_logits, const Te
   const int64_t N = logits.shape[0], V = logits.shape[1], K = teacher_ids.shape[1];
   if (V == 0) throw std::invalid_argument("distill_loss: empty vocabulary");
   if (K < 1 || K > 1024) throw std::invalid_argument("distill_loss: K must be in [1, 1024]");
-  if (!(temperature > 0.0f) || !std::isfinite(temperature)) {
-    throw std::invalid_argument("distill_loss: temperature must be positive");
+  if (!(temperature >= 0x1p-61f) || !(temperature <= 0x1p61f)) {
+    throw std::invalid_argument("distill_loss: temperature must be positive, in [2^-61, 2^61]");
   }
   if (logits.device == Device::CPU) throw_cpu_compute(op);
   Tensor lc = as_contig(logits), tc = as_contig(teacher_logits), ic = as_contig(teacher_ids);

@@ -649,7 +649,7 @@ int aar_qk_norm_rope_bwd_f32(const float* gy, int64_t gy_row, const float* x, in
  * its sum of exp((z - max) / tau) (+inf for a row that is left out), then the
  * number of counted rows.  1 <= top <= 1024, vocab below 2^31 - 4096, and n at most
  * 2^28 - 16 where vocab <= 80 and top <= 16, 2^26 - 4 where vocab <= 2048, else
- * 2^24 - 1 (AAR_EUNSUPPORTED); temperature > 0. */
+ * 2^24 - 1 (AAR_EUNSUPPORTED); 2^-61 <= temperature <= 2^61 (AAR_EINVAL). */
 size_t aar_distill_workspace_bytes(int64_t n);
 int aar_distill_fwd_f32(const float* logits, const float* t_logits, const int64_t* t_ids, float* loss,
                         float* stats, int64_t n, int64_t vocab, int64_t top, float temperature, int* err,

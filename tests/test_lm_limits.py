@@ -2,6 +2,7 @@
 refuse: a size query and its call agree, before any launch."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 
 import lmops as M
@@ -33,3 +34,17 @@ def test_distillation_sizes(L):
             assert rc == (M.EWORKSPACE if fine else M.EUNSUPPORTED), (vocab, top, n)
             if not fine:
                 assert L.aar_distill_bwd_f32(X, X, X, X, X, X, n, vocab, top, 1.0, None) == M.EUNSUPPORTED
+
+
+def test_temperatures(L, ag):
+    """The loss is up to tau^2 ln V, which fp32 holds."""
+    up, down = 2.0 ** 61 * 1.001, 2.0 ** -61 * 0.999
+    for tau, rc in ((2.0 ** 61, M.EWORKSPACE), (2.0 ** -61, M.EWORKSPACE), (up, M.EINVAL), (down, M.EINVAL), (1e38, M.EINVAL)):
+        assert L.aar_distill_fwd_f32(X, X, X, X, X, 4, 8, 2, tau, None, None, 0, None) == rc, tau
+    for tau in (up, down, 1e30):
+        assert L.aar_distill_bwd_f32(X, X, X, X, X, X, 4, 8, 2, tau, None) == M.EINVAL
+        with pytest.raises(ValueError, match="temperature"):
+            ag.nn.DistillationLoss(tau)
+        with pytest.raises(ValueError, match="temperature"):
+            f = ag.from_numpy(np.zeros((4, 8), np.float32))
+            ag.distill_loss(f, f, ag.from_numpy(np.zeros((4, 8), np.int64)), tau)

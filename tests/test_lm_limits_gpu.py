@@ -107,3 +107,24 @@ def test_distillation_of_many_rows(L, V):
     want = (torch.xlogy(p, p) - p * logq).sum(-1).mean().item()
     # each row's loss is a difference of numbers of up to 16: 64 half steps, as for small batches
     assert abs(loss.item() - want) <= 64 * M.U * 16
+
+
+@pytest.mark.parametrize("tau", [2.0 ** -61, 2.0 ** -40, 2.0 ** 40, 2.0 ** 61])
+def test_distillation_at_extreme_temperatures(L, tau):
+    """The loss, up to tau^2 ln V, stays in fp32's range, so loss and gradient are finite, and infinite where the
+    student excludes what the teacher names."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for V, K in ((33, 5), (3001, 20)):
+        z = torch.randn(6, V, generator=gen, device="cuda")
+        t, ids = (torch.randn(6, V, generator=gen, device="cuda")).topk(K, -1)
+        loss, dz = distill(L, z, t.contiguous(), ids, tau)
+        p = torch.softmax(t.double() / tau, -1)
+        logq = torch.log_softmax(z.double() / tau, -1)
+        want = (tau * tau * (torch.xlogy(p, p) - p * logq.gather(1, ids)).sum(-1).mean()).item()
+        # a row's loss is a difference of numbers up to 12 / tau + ln V, each off by 64 half steps
+        assert abs(loss.item() - want) <= 64 * M.U * tau * tau * (12 / tau + 9)
+        dref = tau / 6 * torch.exp(logq).scatter_add(1, ids, -p)
+        # entries of q and p are at most 1; no two logits are so near that a small tau leaves their weights open
+        assert ((dz.double() - dref).abs() <= tau / 6 * 64 * M.U).all()
+        z[0, ids[0, 0]] = -float("inf")
+        assert distill(L, z, t.contiguous(), ids, tau)[0].item() == float("inf")
