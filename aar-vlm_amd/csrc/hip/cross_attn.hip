@@ -753,13 +753,14 @@ cross_bwd_dkdv_kernel(const CaArgs a) {
 // 2^-38 of its row's largest element, lo lo is at most 2^-22 of a product and is left
 // out; sums are in fp32, with fewer roundings than the fp32 instruction's, which
 // leaves the results nearer to the exact ones.  8 x 12 heads, 1024 x 4096, d 64 (in
-// brackets with the fp32 instruction): forward 418 us (934), dQ 605 (1276), dK/dV 857
+// brackets with the fp32 instruction): forward 392 us (934), dQ 575 (1276), dK/dV 820
 // (1730), off by 0.76e-6 (1.2e-6) in O's norm, 1.0e-6 (1.3e-6) in dQ's, 0.80e-6
-// (0.88e-6) in dK's and dV's.  That is 245 TFLOP/s of the products they stand for,
-// 735 on the cores.  Three bf16 parts and six products hold all 24 bits, but took 590,
-// 806 and 1125 us.  What bounds these is the power that vector and matrix units draw
-// together: the forward's 256 vector instructions a wave and tile (scales, exponentials,
-// splits) beside 24 matrix ops were 312, with 425 us, and the clock gave way.
+// (0.88e-6) in dK's and dV's.  That is 263 TFLOP/s of the forward's products, 789 on the
+// cores.  Three bf16 parts and six products hold all 24 bits, but took 590, 806 and 1125
+// us.  What bounds these is that a wave's matrix ops and its vector instructions (scales,
+// exponentials, splits) wait for each other: the forward's matrix units are busy for 40 %
+// of the cycles and its vector units for 64 %, dQ's for 39 and 45, dK/dV's for 37 and 49,
+// at 1.9 to 2.0 GHz.
 //
 // e is a row's own, such that its largest element is in [2^13, 2^14).  Over the head
 // dim a row's factor is one of the output's row or column.  Over a tile's rows it
@@ -774,7 +775,9 @@ cross_bwd_dkdv_kernel(const CaArgs a) {
 // tile that serves both is split and stored once.  P and dS are split in the
 // registers the softmax leaves them in.  Rows whose largest element is outside
 // [2^-99, 2^60) (infinities too) are not held so: the waves that meet one do their
-// rows again with the fp32 instruction, from HBM.
+// rows again with the fp32 instruction, from HBM, at a tenth of the speed.  8 x 12 heads,
+// 512 x 1024, forward + backward 293 us, with a row of dO of 2^-110 in every head 1773,
+// with an infinite value in every head 2826.
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -1581,9 +1584,12 @@ int pad_dim(int64_t d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
 // Ranges a pass's loop of `tiles` is split into, for grids that do not fill the
 // GPU's `slots` workgroups.  A tile takes about `us` microseconds and a workgroup
 // another two of its own, and parts cost a launch and their bytes twice; the fewest
-// microseconds win: 36 x 6 heads' 1865 rows over 31 keys, dK and dV, 183 us against
-// some 600 unsplit.  Full grids are not split: with six bf16 products, 768 workgroups
-// of 512 slots as two parts each took 579 us against 565.
+// microseconds win.  Forward + backward of 2 x 8 heads' 512 x 4096, d 64, 188 us, unsplit
+// 508; 36 x 6 heads' 1865 rows over 31 keys 346, 386; the forward of 4 x 16 heads on 4,
+// 301 x 1111, d 128, 64, 91.  Full grids are not split: 64 x 6 heads, 256 x 577, 331 us,
+// its 768 and 1920 workgroups as two parts each 489.  Two slots a CU, although the 64-wide
+// forward and dQ fit three: with three 2 x 8 heads' 512 x 4096 takes 51 us forward against
+// 48, 8 x 12 heads' 512 x 2048 and others the same.
 int ca_splits(int64_t grid, int64_t slots, int64_t tiles, int64_t least, double us, double part_bytes) {
   int best = 1;
   double cost = 0;

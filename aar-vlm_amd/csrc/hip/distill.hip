@@ -307,8 +307,10 @@ distill_bwd_kernel(const float* __restrict__ grad, const float* __restrict__ Z, 
 
 // Short rows (V <= 80, up to 16 entries): 16 lanes a row, four rows a wave, the
 // row in registers.  With a wave a row, most lanes of a character vocabulary's
-// rows are idle: 16384 x 65 forward + backward 15.6 us against 30.9.  4096 x 256 with
-// 8 entries takes 14.8 us against 14.2 so, with 64 entries 28 against 18.
+// rows are idle: 16384 x 65 forward + backward 14.5 us against 29.9, x 80 14.3 against
+// 28.1 (1000 rows the same either way).  With 8 columns a lane 16384 x 96 and x 128 would
+// take 14 against 28 too, 4096 x 256 with 8 entries 14.8 against 14.2, with 64 entries 28
+// against 18.
 constexpr int kShortVocab = 80, kShortTop = 16, kShortLanes = 16;
 constexpr int kShortRows = 256 / kShortLanes;       // of a workgroup
 constexpr int kShortCols = kShortVocab / kShortLanes;  // columns of a lane

@@ -12,12 +12,13 @@
 // norm and rotation stay inside a lane but for one sum over the head's lanes; a
 // wave walks a row's heads and forms the row's angles once, beside the first
 // heads' loads.  The angle in turns is position * base^(-2c/r) / (2 pi) in fp64
-// (frequencies from the host, in the kernel's arguments), whose fraction alone goes
-// to fp32: positions of 10^6 and beyond lose nothing.  dw accumulates in registers
-// over a persistent grid, one partial row per workgroup, joined in a fixed order: no
-// atomics.  32768 rows of 40 heads, d 128: forward 255 us, 5.3 TB/s, backward 390 us,
-// 5.2 TB/s; 16384 rows of 12 heads, d 64: 17.5 us (100 MB, from the caches in part)
-// and 26.8 us, of which 4 us join dw.
+// (frequencies from the host, in the kernel's arguments), whose fraction alone, in
+// [-1/2, 1/2], goes to fp32: an angle is off by up to 2 pi 2^-26 = 1e-7, at a position of
+// 10^6 as at the first, which is of the order of the turned values' own roundings.  dw
+// accumulates in registers over a persistent grid, one partial row per workgroup, joined
+// in a fixed order: no atomics.  32768 rows of 40 heads, d 128: forward 257 us, 5.2 TB/s, backward 378 us,
+// 5.3 TB/s; 16384 rows of 12 heads, d 64: 17.8 us (100 MB, from the caches in part)
+// and 28.9 us, and 4.2 us to join dw.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -213,8 +214,8 @@ rope_vec_kernel(const RopeArgs a, const RopeFreq fr) {
 // Any even rotary width, any d up to 64 kN, any alignment: lane l of a wave has a head's
 // elements l, l + 64, ...; the partner of a pair is read again.  As above a wave walks
 // a row's heads and forms the row's angles once, beside the first head's loads.
-// 16384 rows of 12 heads, d 30, forward + backward 98 us, with the angles formed for
-// every head and four slots a lane whatever d 200.
+// 16384 rows of 12 heads, d 30, forward + backward 100 us (32, 64 and 4 to join dw; 94 MB),
+// with the angles formed for every head and four slots a lane whatever d 200.
 template <int kN, bool BWD>
 __global__ void __launch_bounds__(kThreads)
 rope_any_kernel(const RopeArgs a, const RopeFreq fr) {

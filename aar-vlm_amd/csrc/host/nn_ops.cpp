@@ -183,7 +183,10 @@ class SumAllFunction : public Function {
 };
 
 // dW of a lookup: the one-hot product, or by sorted tokens where that product
-// is refused (n * vocab above 2^30).
+// is refused (n * vocab above 2^30).  2^30 is no crossover: below it the product stays
+// because its sums' order is what callers have had.  It is the faster one only for small
+// batches (512 tokens of 1000 ids, 256 columns: 15 us, sorted 17; 16384 of 65, 384 columns:
+// 22, 21; of 1000: 104, 21; of 50000: 3473, 32), so large vocabularies take embedding_scaled.
 Tensor table_grad(const Tensor& gc, const Tensor& ids, int64_t V) {
   const int64_t D = gc.shape.back();
   const int64_t n = n_of(ids);

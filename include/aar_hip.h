@@ -563,8 +563,10 @@ int aar_causal_mask_f32(const float* x, float* y, int64_t mats, int64_t T, float
  * a row without keys has O = 0 and lse = -inf.  `strides` lists (sb, sh, st) in
  * elements of q, k, v, o (12 values; head dim contiguous), as in
  * aar_flash_fwd_strided_f32; 128-bit paths need 16-byte aligned pointers and d
- * and all strides multiples of 4.  d <= 128.  Where the query rows are too few to
- * fill the GPU the key range is split and joined through the workspace (0 bytes
+ * and all strides multiples of 4.  d <= 128 (AAR_EINVAL).  B, H, Tq, Tk, B * Hkv and
+ * (H / Hkv) * Tq at most 2^24, B * H * Tq below 2^27, and over all B * Hkv key/value
+ * heads fewer than 2^24 blocks of 128 query rows, and of 128 keys (AAR_EUNSUPPORTED).
+ * Where the query rows are too few to fill the GPU the key range is split and joined through the workspace (0 bytes
  * otherwise; 16-byte aligned, AAR_EWORKSPACE).  Products over aligned rows, 2^23
  * floats apart at most, of more than 4 query rows a key/value head are formed from
  * two fp16 parts of each operand: 22 bits of it, or 2^-38 of its row's largest
@@ -591,7 +593,7 @@ int aar_cross_attn_bwd_f32(const float* q, const float* k, const float* v, const
 /* out[i][:] = scale * w[ids[i]][:] (w [vocab, dim], ids int64 [n]): an
  * embedding lookup whose rows are scaled, as where the table is shared with the
  * vocabulary head.  An id outside [0, vocab) yields a zero row and sets
- * *err = 1 (err may be NULL). */
+ * *err = 1 (err may be NULL).  n at most 2^26 - 4 (AAR_EUNSUPPORTED). */
 int aar_embedding_scaled_fwd_f32(const float* w, const int64_t* ids, float* out, int64_t n, int64_t vocab,
                                  int64_t dim, float scale, int* err, void* stream);
 /* dw[v][:] = scale * sum of g[i][:] over the i with ids[i] == v (dw [vocab, dim]
@@ -617,8 +619,9 @@ int aar_embedding_sorted_bwd_f32(const float* g, const int64_t* ids, float* dw, 
  *   y[c]         = u[c]                               c >= r
  * position of row i = positions[i % n_positions] (int64, on the device; rows a
  * multiple of n_positions: one list for a batch of equally long sequences, or
- * one position a row).  The angle is formed in 64 bits, so far positions lose
- * nothing.  2 <= d <= 256; r even, 0 <= r <= d (0: norms only, positions may be
+ * one position a row).  The angle is formed in 64 bits and its fraction of a turn
+ * rounded to 32, so it is off by 1e-7 at most, far positions' as well.  2 <= d <= 256
+ * (past it AAR_EUNSUPPORTED, as q_heads + k_heads above 2^20 or rows above 2^40); r even, 0 <= r <= d (0: norms only, positions may be
  * NULL); base > 0; eps >= 0; x_row and y_row of at least (q_heads + k_heads) * d
  * where rows > 1.  y may be x (y_row == x_row). */
 int aar_qk_norm_rope_fwd_f32(const float* x, int64_t x_row, const float* wq, const float* wk,
