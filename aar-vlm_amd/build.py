@@ -49,6 +49,8 @@ LIB_NAME = "libaar_hip.so"
 HIP_FILE_FLAGS = {
     "flash_attn": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "cross_attn": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "window_attn": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "kv_attn": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "gemm_small": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

@@ -663,6 +663,103 @@ int aar_distill_bwd_f32(const float* grad, const float* logits, const float* t_l
                         const float* stats, float* dlogits, int64_t n, int64_t vocab, int64_t top,
                         float temperature, void* stream);
 
+/* ------------- attention over part of a text, and a cache of its keys and values ----
+ * No counterparts in the reference, whose attention reads the whole text and whose
+ * generation has no cache. */
+
+/* Causal self attention with a sliding window and sinks: queries [B, H, T, d], keys
+ * and values [B, Hkv, T, d], H a multiple of Hkv, query head h with key/value head
+ * h / (H / Hkv); query i sees the keys j <= i with i - j < window or j < sinks (the
+ * first tokens stay visible).  window >= 1, sinks >= 0 (AAR_EINVAL); a window of T
+ * or more is causal attention.
+ *   O = softmax(scale * Q K^T) V over the keys seen,  lse = m + ln(l) ([B, H, T]).
+ * `strides` lists (sb, sh, st) in elements of q, k, v, o (12 values; head dim
+ * contiguous), as in aar_flash_fwd_strided_f32.  1 <= d <= 128 (AAR_EINVAL); row
+ * strides st of q, k, v (and dout) from d to 2^23 (AAR_EUNSUPPORTED; of fewer than two
+ * rows any).  16-byte aligned pointers, d and strides multiples of 4 read 128 bits at
+ * once, others 32.  T at most 2^24, B, H at most 2^20, and fewer than 2^24 blocks of 128
+ * rows over all heads (AAR_EUNSUPPORTED).
+ * Products are formed from two fp16 parts of each operand, as in
+ * aar_cross_attn_fwd_f32 with its bounds; rows whose largest element is not 0 and
+ * outside [2^-99, 2^60) take the fp32 instruction. */
+size_t aar_window_attn_fwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t d, int64_t window,
+                                           int64_t sinks);
+int aar_window_attn_fwd_f32(const float* q, const float* k, const float* v, float* o, float* lse, int64_t B, int64_t H,
+                            int64_t Hkv, int64_t T, int64_t d, const int64_t* strides, int64_t window, int64_t sinks,
+                            float scale, void* workspace, size_t workspace_bytes, void* stream);
+/* dq, dk, dv (fully overwritten), summed over the query heads that share a
+ * key/value head; no float atomics, the same bits on every run.  24 strides: q, k, v, o,
+ * dout, dq, dk, dv.  The gradients overlap neither the inputs nor each other.  The
+ * workspace holds dout . o of every query row, and parts of sums; 16-byte aligned
+ * (AAR_EWORKSPACE). */
+size_t aar_window_attn_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t d, int64_t window,
+                                           int64_t sinks);
+int aar_window_attn_bwd_f32(const float* q, const float* k, const float* v, const float* o, const float* lse,
+                            const float* dout, float* dq, float* dk, float* dv, int64_t B, int64_t H, int64_t Hkv,
+                            int64_t T, int64_t d, const int64_t* strides, int64_t window, int64_t sinks, float scale,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* A key/value cache of one layer, in pages of `page` tokens (32, 64 or 128) held in
+ * 8 bits: x = number * scale, numbers -127 .. 127, one fp32 scale for each page, head,
+ * and keys or values: the largest |x| of the rows the page holds / 127.  The caller owns
+ * the memory, and the table that says which pages a sequence's tokens stand in: token j
+ * of sequence b in page table[b][j / page].  Full pages never change, so sequences may
+ * share them.
+ * A page's bytes hold number + 128; with dp = d rounded up to 16, key c of token j at
+ * j * dp + c, and value c, behind the keys' page * dp bytes, at
+ *   (j / 32) * 32 * dp + 32 * c + 4 * r(j / 4 % 8) + j % 4,  r: three bits reversed.
+ * The struct is read during the call.  Sequences x kv_heads up to 2^22, kv_heads up to
+ * 2^16, table_width * page up to 2^30 (AAR_EUNSUPPORTED), d from 1 to 128 (AAR_EINVAL). */
+typedef struct aar_kv_cache {
+  uint8_t* pages;       /* [n_pages][kv_heads][2][page * dp], 16-byte aligned (AAR_EINVAL) */
+  float* scales;        /* [n_pages][kv_heads][2] */
+  float* open;          /* [sequences][kv_heads][2][page][d]: rows of each sequence's last
+                           page while it is not full (read and written by append alone) */
+  const int64_t* table; /* [sequences][table_width], on the device */
+  int64_t sequences, table_width, n_pages, kv_heads, page, d;
+} aar_kv_cache;
+
+/* Bytes of one page (0 for sizes out of range). */
+size_t aar_kv_cache_page_bytes(int64_t kv_heads, int64_t page, int64_t d);
+
+/* In all three calls `lens` (int64 [sequences], on the device) is the number of tokens
+ * of each sequence with the call's new ones, so that the layers of a model share one
+ * array.  The new tokens are the last new_lens[b] of them (int64 on the device; NULL: T);
+ * rows t >= new_lens[b] are not read.  A sequence whose numbers do not fit (lens[b]
+ * outside [0, table_width * page], new_lens[b] outside [0, min(T, lens[b])]) sets *err = 1
+ * (err may be NULL) and is left out; so does a page that is looked up and whose id is
+ * outside [0, n_pages), and that page.  Pages that the call has no use for are not
+ * looked up.
+ *
+ * aar_kv_cache_append_f32: the new tokens' rows k and v, [sequences, kv_heads, T, d] with
+ * strides (sb, sh, st) of each (6 values, head dim contiguous), into their pages, and
+ * into `open` those of a last page that is not full.  A page's numbers are
+ * rounded once, to nearest (ties to even), from fp32 rows whatever calls these came in;
+ * places of tokens to come hold 0.  A page, head and keys or values that hold an infinity
+ * or NaN read as NaN.  The tokens before the new ones have to be the ones that
+ * earlier calls appended.  Pages that new tokens go to are in no other sequence. */
+int aar_kv_cache_append_f32(const aar_kv_cache* cache, const float* k, const float* v, const int64_t* strides,
+                            const int64_t* lens, const int64_t* new_lens, int64_t T, int* err, void* stream);
+/* Tokens from[b] .. from[b] + T - 1 (NULL: from 0) as fp32 rows; those that the sequence
+ * does not hold, and those of a page without an id, are zeros. */
+int aar_kv_cache_read_f32(const aar_kv_cache* cache, const int64_t* from, const int64_t* lens, float* k, float* v,
+                          const int64_t* strides, int64_t T, int* err, void* stream);
+/* Attention of the new tokens, which the cache already holds: q and o [sequences, H, T,
+ * d] (strides of q, then o), H a multiple of kv_heads; the query at position i sees the
+ * tokens j <= i with i - j < window or j < sinks (window >= 1; 2^30 or more: all).
+ *   O = softmax(scale * Q K^T) V with the keys and values that the numbers stand for;
+ * rows t >= new_lens[b] and rows that see nothing are zeros.  Pages without an id are
+ * hidden.  Values up to 2^90 in magnitude; queries of any.  The products' fp16 parts hold
+ * 22 bits of q, or 2^-38 of its row's largest element, and of P.  Where there are too few
+ * rows to fill the GPU the tokens are split and joined through the workspace (0 bytes
+ * otherwise; 16-byte aligned, AAR_EWORKSPACE).  H and T up to 2^24, and sequences *
+ * kv_heads * (H / kv_heads * T / 16) below 2^22 (AAR_EUNSUPPORTED). */
+size_t aar_kv_cache_attn_workspace_bytes(const aar_kv_cache* cache, int64_t H, int64_t T, int64_t window,
+                                         int64_t sinks);
+int aar_kv_cache_attn_f32(const aar_kv_cache* cache, const float* q, float* o, const int64_t* strides,
+                          const int64_t* lens, const int64_t* new_lens, int64_t H, int64_t T, int64_t window,
+                          int64_t sinks, float scale, void* workspace, size_t workspace_bytes, int* err, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
