@@ -57,6 +57,8 @@ from ._core import (  # noqa: E402
     qk_norm_rope,
     embedding_scaled,
     distill_loss,
+    window_attention,
+    KVCache,
     cuda_synchronize,
 )
 
@@ -103,6 +105,8 @@ __all__ = [
     "qk_norm_rope",
     "embedding_scaled",
     "distill_loss",
+    "window_attention",
+    "KVCache",
     "cuda_synchronize",
     "nn",
     "optim",

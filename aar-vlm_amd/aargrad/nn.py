@@ -275,13 +275,24 @@ class MultiHeadAttention(Module):
     With ``qk_norm`` every query and key head is RMS-normed (weights ``q_norm``
     and ``k_norm``) and the first ``rotary_dim`` columns of each (None: all, 0:
     none) are rotated by the position, in one pass before the attention;
-    positions are 0 .. T-1 unless ``forward`` is given others ([T] or [B, T])."""
+    positions are 0 .. T-1 unless ``forward`` is given others ([T] or [B, T]).
+
+    With a ``window`` (and ``causal``) a token sees the window's last tokens, itself
+    among them, and the text's first ``sinks``.
+
+    ``decode`` runs new tokens against a KVCache that holds those before them."""
 
     def __init__(self, d_model, n_heads, *, causal=False, bias=True, rng=None, qk_norm=False, rotary_dim=None,
-                 rope_base=10000.0, norm_eps=1e-6):
+                 rope_base=10000.0, norm_eps=1e-6, window=None, sinks=0):
         super().__init__()
         if d_model % n_heads != 0:
             raise ValueError("d_model must be divisible by n_heads")
+        if window is not None and not causal:
+            raise ValueError("MultiHeadAttention: a window needs causal attention")
+        if (window is not None and window < 1) or sinks < 0 or (window is None and sinks != 0):
+            raise ValueError("MultiHeadAttention: window must be at least 1, and sinks belong to one")
+        self.window = window
+        self.sinks = sinks
         self.d_model = d_model
         self.n_heads = n_heads
         self.d_head = d_model // n_heads
@@ -303,6 +314,8 @@ class MultiHeadAttention(Module):
         return _positions_up_to(x.shape[-2], x.device)
 
     def forward(self, x, positions=None):
+        if self.window is not None and self.qk_norm:
+            return self.forward_views(x, positions)
         qkv = self.qkv_proj(x)
         if self.qk_norm:
             heads = _core._flash_attention_qkv_rope(
@@ -310,9 +323,26 @@ class MultiHeadAttention(Module):
                 self.causal, self.rotary_dim, self.rope_base, self.norm_eps)
         elif positions is not None:
             raise ValueError("MultiHeadAttention: positions need qk_norm")
+        elif self.window is not None:
+            heads = _core._window_attention_qkv(qkv, self.n_heads, self.n_heads, self.window, self.sinks)
         else:
             heads = _core._flash_attention_qkv(qkv, self.n_heads, self.causal)
         return self.out_proj(heads)
+
+    def decode(self, x, cache, layer):
+        """The new tokens x [sequences, T, d_model] of ``cache.extend`` (T the largest
+        count) through layer ``layer`` of the cache: their keys and values go in, their
+        queries see what is held.  Positions are the cache's.  Rows past a sequence's
+        count are its bias alone; no gradient passes through the cache."""
+        if not self.causal or cache.window != (self.window or 0) or cache.sinks != self.sinks:
+            raise ValueError("MultiHeadAttention.decode: needs causal attention and the cache's window and sinks")
+        B, T, _ = x.shape
+        q, k, v = self._split_heads(self.qkv_proj(x))
+        if self.qk_norm:
+            q, k = self._rotate_heads(q, k, cache.positions() if self.rotary_dim else None)
+        cache.append(layer, k, v)
+        merged = _core.transpose(cache.attend(layer, q), 1, 2)  # [B, T, H, d]
+        return self.out_proj(_core.reshape(merged, [B, T, self.d_model]))
 
     def _split_heads(self, packed):
         """[B, T, 3*D] -> three [B, H, T, d] views (q, k, v)."""
@@ -342,7 +372,11 @@ class MultiHeadAttention(Module):
             q, k = self._rotate_heads(q, k, self._positions_or_default(positions, x))
         elif positions is not None:
             raise ValueError("MultiHeadAttention: positions need qk_norm")
-        merged = _core.transpose(_core.flash_attention(q, k, v, self.causal), 1, 2)  # [B, T, H, d]
+        if self.window is not None:
+            heads = _core.window_attention(q, k, v, self.window, self.sinks)
+        else:
+            heads = _core.flash_attention(q, k, v, self.causal)
+        merged = _core.transpose(heads, 1, 2)  # [B, T, H, d]
         return self.out_proj(_core.reshape(merged, [B, T, self.d_model]))
 
 

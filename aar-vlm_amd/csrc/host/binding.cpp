@@ -12,6 +12,7 @@
 #include <sstream>
 
 #include "aar_hip.h"
+#include "kv_cache.hpp"
 #include "ops.hpp"
 #include "tensor.hpp"
 
@@ -174,7 +175,42 @@ PYBIND11_MODULE(_core, m) {
         "temperature^2 * mean KL of softmax(teacher / temperature), over each row's K entries, from "
         "softmax(logits / temperature); an id of -1 marks an absent entry, a row without entries above -inf does not count.");
 
+  // Attention over part of a text, and a cache of its keys and values.
+  m.def("window_attention", &window_attention, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("window"),
+        py::arg("sinks") = 0, gil_release(),
+        "Causal softmax(q k^T / sqrt(d)) v of q [B, H, T, d] over k, v [B, Hkv, T, d] (H a multiple of Hkv), query i "
+        "with the keys j <= i that have i - j < window or j < sinks.");
+  py::class_<KVCache, std::shared_ptr<KVCache>>(
+      m, "KVCache",
+      "Keys and values of a decoder's layers in pages of 8-bit numbers, a scale for each page and head. A step is "
+      "extend(counts), then append(layer, k, v) and attend(layer, q) for every layer; see nn.MultiHeadAttention.decode.")
+      .def(py::init<int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t>(), py::arg("layers"),
+           py::arg("sequences"), py::arg("kv_heads"), py::arg("d_head"), py::arg("max_tokens"), py::arg("page") = 64,
+           py::arg("pages") = 0, py::arg("window") = 0, py::arg("sinks") = 0, gil_release())
+      .def("extend", &KVCache::extend, py::arg("counts"), gil_release(),
+           "counts[b] new tokens of sequence b: takes pages for them and gives back those that the window has left.")
+      .def("append", &KVCache::append, py::arg("layer"), py::arg("k"), py::arg("v"), gil_release(),
+           "The new tokens' keys and values, [sequences, kv_heads, max(counts), d]; no gradient passes.")
+      .def("attend", &KVCache::attend, py::arg("layer"), py::arg("q"), gil_release(),
+           "Attention of the new tokens' queries [sequences, H, max(counts), d] (a view of rows of all heads); rows from "
+           "counts[b] on are zeros.")
+      .def("positions", &KVCache::positions, gil_release(), "Positions of the new tokens, Int64 [sequences, max(counts)].")
+      .def("read", &KVCache::read, py::arg("layer"), py::arg("first"), py::arg("n"), gil_release(),
+           "Tokens first .. first + n - 1 as (keys, values) [sequences, kv_heads, n, d], zeros where there is none.")
+      .def("fork", &KVCache::fork, py::arg("src"), py::arg("dst"), gil_release(),
+           "Sequence dst continues from what src holds; full pages are shared.")
+      .def("free", &KVCache::free, py::arg("sequence"), gil_release(), "Empties a sequence.")
+      .def_property_readonly("lengths", &KVCache::lengths)
+      .def_property_readonly("free_pages", &KVCache::free_pages)
+      .def_property_readonly("layers", &KVCache::layers)
+      .def_property_readonly("window", &KVCache::window)
+      .def_property_readonly("sinks", &KVCache::sinks)
+      .def_property_readonly("nbytes", &KVCache::nbytes);
+
   // Extensions of this build (not in the reference API).
+  m.def("_window_attention_qkv", &window_attention_qkv, py::arg("qkv"), py::arg("n_heads"), py::arg("n_kv_heads"),
+        py::arg("window"), py::arg("sinks") = 0, gil_release(),
+        "window_attention over a packed projection [..., T, (n_heads + 2 * n_kv_heads) * d] -> [..., T, n_heads * d].");
   m.def("_cross_attention_packed", &cross_attention_packed, py::arg("q"), py::arg("kv"), py::arg("n_heads"),
         py::arg("n_kv_heads"), py::arg("kv_lens") = std::shared_ptr<Tensor>(), gil_release(),
         "cross_attention over projections read in place: q [B, Tq, H*d], kv [B, Tk, 2*Hkv*d] -> [B, Tq, H*d].");

@@ -212,11 +212,13 @@ void check_device_errors() {
   if (!words) return;
   int host[kErrSlots] = {};
   check_status(aar_memcpy(host, words, sizeof(host), 2, current_stream()), "device error word");
-  if (host[kErrEmbeddingId] || host[kErrCrossEntropyTarget] || host[kErrTokenWindow] || host[kErrDistillId]) {
+  if (host[kErrEmbeddingId] || host[kErrCrossEntropyTarget] || host[kErrTokenWindow] || host[kErrDistillId] ||
+      host[kErrCachePage]) {
     check_status(aar_memset_zero(words, sizeof(host), current_stream()), "device error word");
     if (host[kErrEmbeddingId]) throw std::out_of_range("embedding: id out of range [0, vocab_size)");
     if (host[kErrCrossEntropyTarget]) throw std::out_of_range("cross_entropy: target out of range [0, V)");
     if (host[kErrDistillId]) throw std::out_of_range("distill_loss: teacher id out of range [-1, V)");
+    if (host[kErrCachePage]) throw std::out_of_range("KVCache: page or length out of range");
     throw std::out_of_range("token_windows: window start out of range");
   }
 }

@@ -113,6 +113,13 @@ Tensor embedding_sorted_grad(const Tensor& g, const Tensor& ids, int64_t vocab, 
 // Distillation of logits [N, V] from a teacher's top entries [N, K] (id -1: absent).
 Tensor distill_loss(const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_ids, float temperature);
 
+// Attention over part of a text (no counterpart in the reference; kv_ops.cpp): causal
+// attention of q [B, H, T, d] over k, v [B, Hkv, T, d], H a multiple of Hkv; query i sees
+// the keys j <= i with i - j < window or j < sinks.
+Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks);
+// The same over a packed projection [..., T, (H + 2 Hkv) d] -> [..., T, H d].
+Tensor window_attention_qkv(const Tensor& qkv, int64_t n_heads, int64_t n_kv_heads, int64_t window, int64_t sinks);
+
 // Token-window batch (x, y) of shape [starts, seq_len] gathered on the device
 // from an int64 token stream (python/shakespeare/scripts/data.py:38-53).
 std::tuple<Tensor, Tensor> token_windows(const Tensor& tokens, const Tensor& starts, int64_t seq_len);

@@ -144,10 +144,10 @@ void* current_stream();
 void copy_bytes(void* dst, Device dst_device, const void* src, Device src_device, size_t nbytes);
 
 // Deferred device-side errors.  Kernels that cannot throw (an embedding id,
-// a cross-entropy target, a distillation id or a token window out of range) set a word here; the host raises
+// a cross-entropy target, a distillation id, a token window or a cache's page out of range) set a word here; the host raises
 // std::out_of_range at its next synchronisation point (a device-to-host copy
 // or cuda_synchronize), the way the reference raises on its CPU path.
-enum DeviceErrorSlot { kErrEmbeddingId = 0, kErrCrossEntropyTarget = 1, kErrTokenWindow = 2, kErrDistillId = 3, kErrSlots = 4 };
+enum DeviceErrorSlot { kErrEmbeddingId = 0, kErrCrossEntropyTarget = 1, kErrTokenWindow = 2, kErrDistillId = 3, kErrCachePage = 4, kErrSlots = 5 };
 int* device_error_word(DeviceErrorSlot slot);
 void check_device_errors();
 void zero_bytes(void* p, Device device, size_t nbytes);
