@@ -44,7 +44,9 @@ struct KvAttn {
 };
 
 constexpr int kKeys = 32;  // of a tile
-constexpr int kWaves = 4;
+constexpr int kRows = 16;  // of a workgroup
+// Waves that a SIMD holds: what their registers allow.
+constexpr int kv_resident(int dt) { return dt <= 64 ? 4 : 2; }
 
 // D = A B + C for 16 x 16 over 32: lane (r = lane % 16, g = lane / 16) holds A[r][8g ..
 // 8g+7] and B[8g .. 8g+7][r], and C[4g .. 4g+3][r].
@@ -71,11 +73,13 @@ __device__ __forceinline__ u32x4 halves_of(uint32_t x, uint32_t y) {
   return u32x4{halves_of<0>(x), halves_of<2>(x), halves_of<0>(y), halves_of<2>(y)};
 }
 
-// (a, b) in two fp16 parts, a pair a word.
-__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
+// (a, b) in two fp16 parts, a pair a word.  one: 1, unknown to the compiler, so that a
+// difference is one mixed multiply-add and not a conversion and a subtraction.
+__device__ __forceinline__ void split_pair(float a, float b, float one, uint32_t& hi, uint32_t& lo) {
   const f16x2 x = __builtin_convertvector(f32x2{a, b}, f16x2);
   hi = __builtin_bit_cast(uint32_t, x);
-  lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a - (float)x[0], b - (float)x[1]}, f16x2));
+  const f32x2 rest = {fmaf(a, one, -(float)x[0]), fmaf(b, one, -(float)x[1])};
+  lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, f16x2));
 }
 
 // Over the four lanes that hold a query row.
@@ -95,300 +99,321 @@ struct Tiles {
   __device__ __forceinline__ int at(int i) const { return i < sinks ? i : near + i - sinks; }
 };
 
+// Bytes on the device: a pointer put together from a lane's words has to say so, or its
+// loads are flat ones, which wait for LDS too.
+typedef const __attribute__((address_space(1))) uint8_t* DeviceBytes;
+
 // What a wave reads of a tile: rows of keys 16 bytes a lane, columns of values 8.
 template <int DT>
 struct Tile {
   static constexpr int NK = (DT + 63) / 64, NB = DT / 16;
   u32x4 k[2][NK];
   u32x2 v[NB];
-  __device__ __forceinline__ void load(const uint8_t* keys, const uint8_t* values, int dp, int lane) {
+  __device__ __forceinline__ void load_keys(DeviceBytes keys, int dp, int lane) {
     const int r = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
       for (int c = 0; c < NK; ++c) {
         k[n][c] = u32x4{0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
-        if (64 * c + 16 * g < dp) k[n][c] = *reinterpret_cast<const u32x4*>(keys + (16 * n + r) * dp + 64 * c + 16 * g);
+        if (64 * c + 16 * g < dp) k[n][c] = *(const __attribute__((address_space(1))) u32x4*)(keys + (16 * n + r) * dp + 64 * c + 16 * g);
       }
     }
-    const int at = 8 * ((g & 1) << 1 | g >> 1);
+  }
+  __device__ __forceinline__ void load_values(DeviceBytes values, int dp, int lane) {
+    const int r = lane & 15, g = lane >> 4, at = 8 * ((g & 1) << 1 | g >> 1);
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-      if (16 * b < dp) v[b] = *reinterpret_cast<const u32x2*>(values + (16 * b + r) * 32 + at);
+    for (int b = 0; b < NB; ++b) {
+      v[b] = u32x2{0x80808080u, 0x80808080u};
+      if (16 * b < dp) v[b] = *(const __attribute__((address_space(1))) u32x2*)(values + (16 * b + r) * 32 + at);
+    }
   }
 };
 
-// A workgroup takes 16 NC query rows of a key/value head (the rows of the G query
-// heads that share it, one list) and a range of their tiles; its waves take every
-// fourth tile, each with an online softmax of its own, and meet at the end.
-template <int DT, int NC, bool VEC>
-__global__ void __launch_bounds__(kWaves * kWave)
+// A workgroup takes 16 query rows of a key/value head (the rows of the G query
+// heads that share it, one list) and a range of their tiles; its W waves take every
+// W-th tile, each with an online softmax of its own, and meet at the end.
+template <int DT, int W, bool VEC>
+__global__ void __launch_bounds__(W * kWave, kv_resident(DT))
 kv_attn_kernel(const KvPages c, const KvAttn a) {
   constexpr int NK = Tile<DT>::NK, NB = Tile<DT>::NB, NP = 2 * NK;  // NP: 32-column steps of a score
-  __shared__ f32x4 so[kWaves / 2][NC][NB][kWave];
-  __shared__ float sm[kWaves / 2][NC][kWave], sl[kWaves / 2][NC][kWave];
+  __shared__ f32x4 so[W][NB][kWave];
+  __shared__ float sm[W][kWave], sl[W][kWave];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 15, g = lane >> 4;
   const int BH = c.B * c.Hkv, bh = blockIdx.x % BH, b = bh / c.Hkv, hk = bh % c.Hkv;
-  const int rest = blockIdx.x / BH, part = rest % a.splits, block = rest / a.splits;
+  const int part = blockIdx.x / BH % a.splits, block = blockIdx.x / BH / a.splits;
+  const int row0 = block * kRows, row1 = min(a.R, row0 + kRows) - 1;
+  const int row = row0 + r, head = row / a.T, t = row - head * a.T;  // the lane's
+
+  // the row of q, on its way before the numbers that say whether it counts
+  f32x4 x[NP][2];
+  const float* q = a.q.p + (int64_t)b * a.q.sb + ((int64_t)hk * a.G + head) * a.q.sh + (int64_t)t * a.q.st;
+#pragma unroll
+  for (int s = 0; s < NP; ++s) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int col = 64 * (s >> 1) + 16 * g + 8 * (s & 1) + 4 * p;
+      x[s][p] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (row < a.R && col < c.d) x[s][p] = load4<VEC>(q + col, c.d - col);
+    }
+  }
   const KvSpan span = kv_span(c, a.lens, a.new_lens, a.T, b);
   if (!span.ok && a.err) *a.err = 1;
-  const int n = span.len - span.first, row0 = block * 16 * NC, row1 = min(a.R, row0 + 16 * NC) - 1;
 
   // the tokens that the block's rows belong to
+  const int n = span.len - span.first;
   int t0 = 0, t1 = a.T - 1;
   if (row0 / a.T == row1 / a.T) {
     t0 = row0 % a.T;
     t1 = row1 % a.T;
   }
   t1 = min(t1, n - 1);
+  const int pos = row < a.R && t < n ? span.first + t : -1;  // -1: a row that is none
   const Tiles tiles(a, span.first, t0, t1);
   const int i0 = (int)((int64_t)tiles.count * part / a.splits), i1 = (int)((int64_t)tiles.count * (part + 1) / a.splits);
 
-  // q in parts, and each row's position (-1: a row that is none) and factor
-  u32x4 qp[NC][NP][2];
-  int pos[NC], ex[NC];
-#pragma unroll
-  for (int w = 0; w < NC; ++w) {
-    const int row = row0 + 16 * w + r, head = row / a.T, t = row - head * a.T;
-    const bool real = row < a.R && t < n;
-    pos[w] = real ? span.first + t : -1;
-    const float* q = a.q.p + (int64_t)b * a.q.sb + ((int64_t)hk * a.G + head) * a.q.sh + (int64_t)t * a.q.st;
-    f32x4 x[NP][2];
-    float top = 0.f;
-#pragma unroll
-    for (int s = 0; s < NP; ++s) {
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int col = 64 * (s >> 1) + 16 * g + 8 * (s & 1) + 4 * p;
-        x[s][p] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (real && col < c.d) x[s][p] = load4<VEC>(q + col, c.d - col);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[s][p][e]));
-      }
-    }
-    top = row_max(top);
-    ex[w] = top > 0.f ? 14 - ilogbf(top) - 1 : 0;
-#pragma unroll
-    for (int s = 0; s < NP; ++s) {
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        uint32_t hi, lo;
-        split_pair(ldexpf(x[s][p >> 1][2 * (p & 1)], ex[w]), ldexpf(x[s][p >> 1][2 * (p & 1) + 1], ex[w]), hi, lo);
-        qp[w][s][0][p] = hi;
-        qp[w][s][1][p] = lo;
-      }
-    }
-  }
-
-  f32x4 o[NC][NB];
-  float m[NC], l[NC];
-#pragma unroll
-  for (int w = 0; w < NC; ++w) {
-    m[w] = -INFINITY;
-    l[w] = 0.f;
-#pragma unroll
-    for (int d = 0; d < NB; ++d) o[w][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-
-  auto compute = [&](const Tile<DT>& x, int key0, float sk, float sv) {
-    f32x4 s[NC][2];
-#pragma unroll
-    for (int w = 0; w < NC; ++w) s[w][0] = s[w][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int p = 0; p < NP; ++p) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const u32x4 k = halves_of(x.k[h][p >> 1][2 * (p & 1)], x.k[h][p >> 1][2 * (p & 1) + 1]);
-#pragma unroll
-        for (int w = 0; w < NC; ++w) {
-          s[w][h] = mfma16(k, qp[w][p][1], s[w][h]);
-          s[w][h] = mfma16(k, qp[w][p][0], s[w][h]);
-        }
-      }
-    }
-    u32x4 pp[NC][2];
-    float weight[NC];  // of the values: 0 where the row sees none of the tile
-    const bool all = key0 + kKeys - 1 <= span.first + t0 && (key0 > span.first + t1 - a.window || key0 + kKeys <= a.sinks);
-#pragma unroll
-    for (int w = 0; w < NC; ++w) {
-      const float f = ldexpf(sk * a.scale_log2, -ex[w]);
-      float mx = -INFINITY;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = s[w][h][e] * f;
-          if (!all) {
-            const int key = key0 + 16 * h + 4 * g + e;
-            const bool sees = key <= pos[w] && (key > pos[w] - a.window || key < a.sinks);
-            v = sees ? v : -INFINITY;
-          }
-          s[w][h][e] = v;
-          mx = fmaxf(mx, v);
-        }
-      }
-      // a scale that is not finite reaches the rows that see it alone
-      weight[w] = all || row_max(mx) != -INFINITY ? sv : 0.f;
-      if (__any(mx > m[w] + 4.f)) {  // the maximum follows only where P would pass 2^4
-        mx = fmaxf(row_max(mx), m[w]);
-        const float alpha = mx > m[w] ? exp2f(m[w] - mx) : 1.f;
-        m[w] = mx;
-        l[w] *= alpha;
-#pragma unroll
-        for (int d = 0; d < NB; ++d) o[w][d] *= alpha;
-      }
-      const float mu = m[w] == -INFINITY ? -11.f : m[w] - 11.f;
-      float sum = 0.f;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[w][h][e] = fast_exp2(s[w][h][e] - mu);
-          sum += s[w][h][e];
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t hi, lo;
-          split_pair(s[w][h][2 * e], s[w][h][2 * e + 1], hi, lo);
-          pp[w][0][2 * h + e] = hi;
-          pp[w][1][2 * h + e] = lo;
-        }
-      }
-      l[w] += sum;
-    }
-#pragma unroll
-    for (int d = 0; d < NB; ++d) {
-      if (16 * d >= c.dp) continue;
-      const u32x4 v = halves_of(x.v[d][0], x.v[d][1]);
-#pragma unroll
-      for (int w = 0; w < NC; ++w) {
-        f32x4 t = mfma16(v, pp[w][1], f32x4{0.f, 0.f, 0.f, 0.f});
-        t = mfma16(v, pp[w][0], t);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[w][d][e] = fmaf(weight[w], t[e], o[w][d][e]);
-      }
-    }
-  };
-
   // 64 of the wave's tiles at a time: a lane looks one up
-  for (int base = i0 + wave; base < i1; base += kWaves * kWave) {
-    const int mine = base + kWaves * lane;
-    int key = 0;
+  int key = 0;
+  float sk = 0.f, sv = 0.f;
+  const uint8_t* at = nullptr;
+  uint64_t rest = 0;  // the lanes of the tiles to come
+  auto keys_at = [&](int i) {
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)(uintptr_t)at, i);
+    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)((uintptr_t)at >> 32), i);
+    return (DeviceBytes)((uint64_t)hi << 32 | lo);
+  };
+  Tile<DT> tile;
+  int i = -1;  // the present tile's lane
+  auto look_up = [&](int base) {
+    const int mine = base + W * lane;
     int64_t id = -1;
-    float sk = 0.f, sv = 0.f;
     if (mine < i1) {
       key = tiles.at(mine) * kKeys;
       id = c.id(b, key >> c.shift);
       if (id < 0 && a.err) *a.err = 1;
-      if (id >= 0) {
-        const float* s = c.scale(id, hk);
-        sk = s[0];
-        sv = s[1];
-      }
     }
-    const uint8_t* at = id < 0 ? nullptr : c.head(id, hk, 0) + (key & (c.page() - 1)) * c.dp;
-    const uint64_t live = __ballot(id >= 0);
-    const int count = min(kWave, (i1 - base + kWaves - 1) / kWaves);
-    Tile<DT> x[2];
-    auto fetch = [&](int i, Tile<DT>& t) {
-      if (i >= count || !(live >> i & 1)) return;
-      const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)(uintptr_t)at, i);
-      const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)((uintptr_t)at >> 32), i);
-      const uint8_t* p = reinterpret_cast<const uint8_t*>((uint64_t)hi << 32 | lo);
-      t.load(p, p + c.half(), c.dp, lane);
-    };
-    auto step = [&](int i, const Tile<DT>& t) {
-      if (i >= count || !(live >> i & 1)) return;
-      compute(t, __builtin_amdgcn_readlane(key, i), __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sk), i)),
-              __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sv), i)));
-    };
-    fetch(0, x[0]);
-    for (int i = 0; i < count; i += 2) {
-      fetch(i + 1, x[1]);
-      step(i, x[0]);
-      fetch(i + 2, x[0]);
-      step(i + 1, x[1]);
+    if (id >= 0) {
+      at = c.head(id, hk, 0) + (key & (c.page() - 1)) * c.dp;
+      const float* s = c.scale(id, hk);
+      sk = s[0];
+      sv = s[1];
+    }
+    rest = __ballot(id >= 0);
+    i = rest != 0 ? __ffsll((unsigned long long)rest) - 1 : -1;
+    if (i < 0) return;
+    tile.load_keys(keys_at(i), c.dp, lane);
+    tile.load_values(keys_at(i) + c.half(), c.dp, lane);
+  };
+  look_up(i0 + wave);
+
+  // q in parts, its row's factor 2^-ex
+  u32x4 qp[NP][2];
+  float top = 0.f;
+#pragma unroll
+  for (int s = 0; s < NP; ++s) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[s][p][e]));
+    }
+  }
+  top = row_max(top);
+  const int ex = top > 0.f ? 13 - ilogbf(top) : 0;
+  const float sign = copysignf(1.f, a.scale_log2);
+  float one = 1.f;
+  asm("" : "+v"(one));
+#pragma unroll
+  for (int s = 0; s < NP; ++s) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      uint32_t hi, lo;
+      split_pair(ldexpf(x[s][p >> 1][2 * (p & 1)] * sign, ex), ldexpf(x[s][p >> 1][2 * (p & 1) + 1] * sign, ex), one, hi,
+                 lo);
+      qp[s][0][p] = hi;
+      qp[s][1][p] = lo;
     }
   }
 
-  // the waves' sums meet, half of them at a time
+  f32x4 o[NB];
 #pragma unroll
-  for (int w = 0; w < NC; ++w) l[w] = row_sum(l[w]);
+  for (int d = 0; d < NB; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+
+  // `next_keys` and `next_values` send for the next tile's as soon as this one's are used
+  auto compute = [&](int key0, float sk, float sv, auto next_keys, auto next_values) {
+    f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-  for (int half = kWaves / 2; half > 0; half /= 2) {
-    if (wave >= half && wave < 2 * half) {
+    for (int p = 0; p < NP; ++p) {
+      u32x4 k[2];
 #pragma unroll
-      for (int w = 0; w < NC; ++w) {
-        sm[wave - half][w][lane] = m[w];
-        sl[wave - half][w][lane] = l[w];
+      for (int h = 0; h < 2; ++h) k[h] = halves_of(tile.k[h][p >> 1][2 * (p & 1)], tile.k[h][p >> 1][2 * (p & 1) + 1]);
 #pragma unroll
-        for (int d = 0; d < NB; ++d) so[wave - half][w][d][lane] = o[w][d];
+      for (int part = 1; part >= 0; --part) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[h] = mfma16(k[h], qp[p][part], s[h]);
       }
     }
-    __syncthreads();
-    if (wave < half) {
+    next_keys();
+
+    // positive, so that the largest product is the largest score
+    const float f = fmaxf(ldexpf(sk * fabsf(a.scale_log2), -ex), 0x1p-126f);
+    const bool all = key0 + kKeys - 1 <= span.first + t0 && (key0 > span.first + t1 - a.window || key0 + kKeys <= a.sinks);
+    float mx = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < NC; ++w) {
-        const float other = sm[wave][w][lane], mx = fmaxf(m[w], other), mu = mx == -INFINITY ? 0.f : mx;
-        const float f = exp2f(m[w] - mu), h = exp2f(other - mu);
-        m[w] = mx;
-        l[w] = l[w] * f + sl[wave][w][lane] * h;
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int d = 0; d < NB; ++d) {
-          const f32x4 x = so[wave][w][d][lane];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[w][d][e] = o[w][d][e] * f + x[e] * h;
+      for (int e = 0; e < 4; ++e) {
+        if (!all) {
+          const int key = key0 + 16 * h + 4 * g + e;
+          const bool sees = key <= pos && (key > pos - a.window || key < a.sinks);
+          s[h][e] = sees ? s[h][e] : -INFINITY;
         }
+        mx = fmaxf(mx, s[h][e]);
       }
     }
-    __syncthreads();
-  }
-  if (wave != 0) return;
+    mx *= f;
+    // a scale that is not finite reaches the rows that see it alone
+    const float weight = all || row_max(mx) != -INFINITY ? sv : 0.f;
+    if (__any(mx > m + 4.f)) {  // the maximum follows only where P would pass 2^4
+      mx = fmaxf(row_max(mx), m);
+      const float alpha = mx > m ? exp2f(m - mx) : 1.f;
+      m = mx;
+      l *= alpha;
 #pragma unroll
-  for (int w = 0; w < NC; ++w) {
-    const int in = 16 * w + r, row = row0 + in, head = row / a.T, t = row - head * a.T;
-    if (row >= a.R) continue;
-    const bool none = pos[w] < 0 || l[w] == 0.f;  // a row that sees nothing, or is none
-    const float inv = 1.0f / l[w];
-    const int64_t at = (((int64_t)block * BH + bh) * a.splits + part) * (16 * NC) + in;
-    float* orow = a.splits > 1 ? a.part_o + at * DT
-                               : a.o.p + (int64_t)b * a.o.sb + ((int64_t)hk * a.G + head) * a.o.sh + (int64_t)t * a.o.st;
-#pragma unroll
-    for (int d = 0; d < NB; ++d) {
-      const int col = 16 * d + 4 * g;
-      f32x4 v;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = none ? 0.f : o[w][d][e] * inv;
-      if (a.splits > 1) *reinterpret_cast<f32x4*>(orow + col) = v;
-      else if (col < c.d) store4<VEC>(orow + col, v, c.d - col);
+      for (int d = 0; d < NB; ++d) o[d] *= alpha;
     }
-    if (a.splits > 1 && g == 0) a.part_l[at] = none ? -INFINITY : m[w] + log2f(l[w]);
+    const float mu = m == -INFINITY ? 11.f : 11.f - m;
+    u32x4 pp[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[h][e] = fast_exp2(fmaf(s[h][e], f, mu));
+        sum += s[h][e];
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        uint32_t hi, lo;
+        split_pair(s[h][2 * e], s[h][2 * e + 1], one, hi, lo);
+        pp[0][2 * h + e] = hi;
+        pp[1][2 * h + e] = lo;
+      }
+    }
+    l += sum;
+#pragma unroll
+    for (int d = 0; d < NB; d += 2) {
+      if (16 * d >= c.dp) continue;
+      u32x4 v[2];
+      f32x4 y[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) v[n] = halves_of(tile.v[d + n][0], tile.v[d + n][1]);
+      // a matrix op waits for the one whose sum it continues: two sums take turns
+#pragma unroll
+      for (int n = 0; n < 2; ++n) y[n] = mfma16(v[n], pp[1], f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+      for (int n = 0; n < 2; ++n) y[n] = mfma16(v[n], pp[0], y[n]);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d + n][e] = fmaf(weight, y[n][e], o[d + n][e]);
+      }
+    }
+    next_values();
+  };
+
+  for (int base = i0 + wave; base < i1;) {
+    while (i >= 0) {
+      rest &= rest - 1;
+      const int next = rest != 0 ? __ffsll((unsigned long long)rest) - 1 : -1;
+      const DeviceBytes p = keys_at(next < 0 ? i : next);
+      compute(__builtin_amdgcn_readlane(key, i), __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sk), i)),
+              __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sv), i)),
+              [&] { tile.load_keys(p, c.dp, lane); }, [&] { tile.load_values(p + c.half(), c.dp, lane); });
+      i = next;
+    }
+    base += W * kWave;
+    if (base < i1) look_up(base);
   }
+
+  // the waves' sums meet: a thread takes every W-th block of columns of its lane's row
+  sm[wave][lane] = m;
+  sl[wave][lane] = row_sum(l);
+#pragma unroll
+  for (int d = 0; d < NB; ++d) so[wave][d][lane] = o[d];
+  __syncthreads();
+  if (row >= a.R) return;
+  float f[W], mx = sm[0][lane], sum = 0.f;
+#pragma unroll
+  for (int v = 1; v < W; ++v) mx = fmaxf(mx, sm[v][lane]);
+  const float mu = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+  for (int v = 0; v < W; ++v) {
+    f[v] = exp2f(sm[v][lane] - mu);
+    sum += sl[v][lane] * f[v];
+  }
+  const bool none = pos < 0 || sum == 0.f;  // a row that sees nothing, or is none
+  const float inv = 1.0f / sum;
+  const int64_t prow = (((int64_t)block * BH + bh) * a.splits + part) * kRows + r;
+  float* orow = a.splits > 1 ? a.part_o + prow * DT
+                             : a.o.p + (int64_t)b * a.o.sb + ((int64_t)hk * a.G + head) * a.o.sh + (int64_t)t * a.o.st;
+  for (int d = wave; d < NB; d += W) {
+    const int col = 16 * d + 4 * g;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < W; ++v) {
+      const f32x4 z = so[v][d][lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += z[e] * f[v];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = none ? 0.f : y[e] * inv;
+    if (a.splits > 1) *reinterpret_cast<f32x4*>(orow + col) = y;
+    else if (col < c.d) store4<VEC>(orow + col, y, c.d - col);
+  }
+  if (a.splits > 1 && wave == 0 && g == 0) a.part_l[prow] = none ? -INFINITY : mx + log2f(sum);
 }
 
 // The parts of every query row, as cross attention's: with L_p = m_p + log2(l_p),
 //   O = sum_p 2^(L_p - M) O_p / sum_p 2^(L_p - M),  M the largest L_p.
-template <int DT, int NC, bool VEC>
+template <int DT, bool VEC>
 __global__ void __launch_bounds__(256)
 kv_attn_join_kernel(const KvPages c, const KvAttn a) {
-  constexpr int kLanes = DT / 4, kRows = 16 * NC;
+  constexpr int kLanes = DT / 4;
   const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x, item = u / kLanes;
   const int BH = c.B * c.Hkv, bh = (int)(item / a.R), row = (int)(item % a.R), col = (int)(u % kLanes) * 4;
   if (bh >= BH) return;
   const int64_t at = ((int64_t)(row / kRows) * BH + bh) * a.splits * kRows + row % kRows;
-  float mx = -INFINITY;
-  for (int p = 0; p < a.splits; ++p) mx = fmaxf(mx, a.part_l[at + p * kRows]);
-  const float mu = mx == -INFINITY ? 0.f : mx;
-  float w = 0.f;
+  // eight parts' loads in flight
+  constexpr int U = 8;
+  float mx = -INFINITY, w = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int p = 0; p < a.splits; ++p) {
-    const float f = exp2f(a.part_l[at + p * kRows] - mu);
-    const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + (at + p * kRows) * DT + col);
-    w += f;
+  for (int p0 = 0; p0 < a.splits; p0 += U) {
+    float l[U];
+    f32x4 x[U];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += f * x[e];
+    for (int i = 0; i < U; ++i) {
+      const int p = min(p0 + i, a.splits - 1);
+      l[i] = a.part_l[at + (int64_t)p * kRows];
+      x[i] = *reinterpret_cast<const f32x4*>(a.part_o + (at + (int64_t)p * kRows) * DT + col);
+    }
+    float top = mx;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (p0 + i >= a.splits) l[i] = -INFINITY;
+      top = fmaxf(top, l[i]);
+    }
+    const float mu = top == -INFINITY ? 0.f : top, f = exp2f(mx - mu);
+    w *= f;
+    o *= f;
+    mx = top;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const float h = exp2f(l[i] - mu);
+      w += h;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += h * x[i][e];
+    }
   }
   const float inv = w == 0.f ? 0.f : 1.0f / w;
 #pragma unroll
@@ -403,24 +428,26 @@ kv_attn_join_kernel(const KvPages c, const KvAttn a) {
 
 int kv_tile_dim(int64_t d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
 
-// 16-row groups of a workgroup: as many as its rows fill.
-int kv_groups(int64_t R, int64_t d) { return R <= 16 ? 1 : (R <= 32 || d > 64 ? 2 : 4); }
-
 struct KvPlan {
-  int groups, splits;
+  int splits, waves;
   int64_t blocks;
 };
 
 KvPlan kv_plan(const aar_kv_cache& c, int64_t H, int64_t T, int64_t window, int64_t sinks) {
   const int64_t R = H / c.kv_heads * T, cus = device_cu_count();
   KvPlan p;
-  p.groups = kv_groups(R, c.d);
-  p.blocks = ceil_div(R, 16 * p.groups);
+  p.blocks = ceil_div(R, kRows);
   const int64_t grid = p.blocks * c.sequences * c.kv_heads;
   const int64_t most = std::min(c.table_width * c.page, std::min(window, kKvMost) + std::min(sinks, kKvMost) + T);
   const int64_t tiles = ceil_div(most, kKeys);
-  const int64_t s = grid >= 2 * cus ? 1 : std::min(ceil_div(4 * cus, grid), tiles / (2 * kWaves));
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
+  const int resident = kv_resident(kv_tile_dim(c.d));
+  p.waves = 4;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({resident * cus / grid, tiles / (2 * p.waves), 64}));
+  // a workgroup that fills a CU, and no join
+  if (p.splits > 1 && grid <= cus && tiles <= (4 * grid >= 3 * cus ? 32 : 8) * resident) {
+    p.waves = 4 * resident;
+    p.splits = 1;
+  }
   return p;
 }
 
@@ -431,39 +458,34 @@ int kv_attn_check(const aar_kv_cache* c, int64_t H, int64_t T, int64_t window, i
   if (T > (1 << 24) || H > (1 << 24) || H / c->kv_heads * T > (1 << 24)) return AAR_EUNSUPPORTED;
   // a dispatch holds its work items in 32 bits
   const int64_t blocks = ceil_div(H / c->kv_heads * T, 16) * c->sequences * c->kv_heads;
-  if (blocks > (int64_t)UINT32_MAX / (64 * kWaves * kWave)) return AAR_EUNSUPPORTED;
+  if (blocks > (int64_t)UINT32_MAX / (16 * 4 * kWave)) return AAR_EUNSUPPORTED;
   return AAR_OK;
 }
 
 size_t kv_part_rows(const aar_kv_cache& c, const KvPlan& p) {
-  return (size_t)p.blocks * c.sequences * c.kv_heads * p.splits * 16 * p.groups;
-}
-
-template <int DT, int NC, bool VEC>
-int launch_attn(const KvPages& c, const KvAttn& a, hipStream_t st) {
-  const int64_t BH = (int64_t)c.B * c.Hkv;
-  kv_attn_kernel<DT, NC, VEC><<<dim3((unsigned)(BH * a.blocks * a.splits)), dim3(kWaves * kWave), 0, st>>>(c, a);
-  const int rc = launch_status();
-  if (rc != AAR_OK || a.splits == 1) return rc;
-  const int64_t units = BH * a.R * (DT / 4);
-  kv_attn_join_kernel<DT, NC, VEC><<<dim3((unsigned)ceil_div(units, 256)), dim3(256), 0, st>>>(c, a);
-  return launch_status();
+  return (size_t)p.blocks * c.sequences * c.kv_heads * p.splits * kRows;
 }
 
 template <int DT, bool VEC>
-int kv_attn_groups(const KvPages& c, const KvAttn& a, int groups, hipStream_t st) {
-  if (groups == 1) return launch_attn<DT, 1, VEC>(c, a, st);
-  if (groups == 2) return launch_attn<DT, 2, VEC>(c, a, st);
-  if constexpr (DT <= 64) return launch_attn<DT, 4, VEC>(c, a, st);
-  return AAR_EUNSUPPORTED;
+int launch_attn(const KvPages& c, const KvAttn& a, int waves, hipStream_t st) {
+  constexpr int kMost = 4 * kv_resident(DT);
+  const int64_t BH = (int64_t)c.B * c.Hkv;
+  const dim3 grid((unsigned)(BH * a.blocks * a.splits)), block(waves * kWave);
+  if (waves == kMost) kv_attn_kernel<DT, kMost, VEC><<<grid, block, 0, st>>>(c, a);
+  else kv_attn_kernel<DT, 4, VEC><<<grid, block, 0, st>>>(c, a);
+  const int rc = launch_status();
+  if (rc != AAR_OK || a.splits == 1) return rc;
+  const int64_t units = BH * a.R * (DT / 4);
+  kv_attn_join_kernel<DT, VEC><<<dim3((unsigned)ceil_div(units, 256)), dim3(256), 0, st>>>(c, a);
+  return launch_status();
 }
 
 template <bool VEC>
-int kv_attn_dims(const KvPages& c, const KvAttn& a, int groups, hipStream_t st) {
+int kv_attn_dims(const KvPages& c, const KvAttn& a, int waves, hipStream_t st) {
   const int dt = kv_tile_dim(c.d);
-  if (dt == 32) return kv_attn_groups<32, VEC>(c, a, groups, st);
-  if (dt == 64) return kv_attn_groups<64, VEC>(c, a, groups, st);
-  return kv_attn_groups<128, VEC>(c, a, groups, st);
+  if (dt == 32) return launch_attn<32, VEC>(c, a, waves, st);
+  if (dt == 64) return launch_attn<64, VEC>(c, a, waves, st);
+  return launch_attn<128, VEC>(c, a, waves, st);
 }
 
 }  // namespace
@@ -516,7 +538,8 @@ int aar_kv_cache_attn_f32(const aar_kv_cache* cache, const float* q, float* o, c
   }
   bool vec = c.d % 4 == 0 && aligned16(q) && aligned16(o);
   for (int i = 0; i < 6; ++i) vec = vec && strides[i] % 4 == 0;
-  return vec ? kv_attn_dims<true>(c, a, p.groups, as_stream(stream)) : kv_attn_dims<false>(c, a, p.groups, as_stream(stream));
+  return vec ? kv_attn_dims<true>(c, a, p.waves, as_stream(stream))
+             : kv_attn_dims<false>(c, a, p.waves, as_stream(stream));
 }
 
 }  // extern "C"
