@@ -45,8 +45,11 @@ struct KvAttn {
 
 constexpr int kKeys = 32;  // of a tile
 constexpr int kRows = 16;  // of a workgroup
-// Waves that a SIMD holds: what their registers allow.
-constexpr int kv_resident(int dt) { return dt <= 64 ? 4 : 2; }
+// Waves that a SIMD holds, by their registers: of workgroups of 4 waves, and of one that
+// fills a CU.  Four of the small ones a SIMD, which would fit for dt = 64 but for two
+// registers, take 36.0 us where three take 34.7 (32 x 12 heads' single rows, 4096 tokens).
+constexpr int kv_resident(int dt) { return dt <= 64 ? 3 : 2; }
+constexpr int kv_wide(int dt) { return dt <= 64 ? 4 : 2; }
 
 // D = A B + C for 16 x 16 over 32: lane (r = lane % 16, g = lane / 16) holds A[r][8g ..
 // 8g+7] and B[8g .. 8g+7][r], and C[4g .. 4g+3][r].
@@ -134,7 +137,7 @@ struct Tile {
 // heads that share it, one list) and a range of their tiles; its W waves take every
 // W-th tile, each with an online softmax of its own, and meet at the end.
 template <int DT, int W, bool VEC>
-__global__ void __launch_bounds__(W * kWave, kv_resident(DT))
+__global__ void __launch_bounds__(W * kWave, W == 4 ? kv_resident(DT) : kv_wide(DT))
 kv_attn_kernel(const KvPages c, const KvAttn a) {
   constexpr int NK = Tile<DT>::NK, NB = Tile<DT>::NB, NP = 2 * NK;  // NP: 32-column steps of a score
   __shared__ f32x4 so[W][NB][kWave];
@@ -440,12 +443,12 @@ KvPlan kv_plan(const aar_kv_cache& c, int64_t H, int64_t T, int64_t window, int6
   const int64_t grid = p.blocks * c.sequences * c.kv_heads;
   const int64_t most = std::min(c.table_width * c.page, std::min(window, kKvMost) + std::min(sinks, kKvMost) + T);
   const int64_t tiles = ceil_div(most, kKeys);
-  const int resident = kv_resident(kv_tile_dim(c.d));
+  const int dt = kv_tile_dim(c.d), wide = 4 * kv_wide(dt);
   p.waves = 4;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({resident * cus / grid, tiles / (2 * p.waves), 64}));
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({kv_resident(dt) * cus / grid, tiles / (2 * p.waves), 64}));
   // a workgroup that fills a CU, and no join
-  if (p.splits > 1 && grid <= cus && tiles <= (4 * grid >= 3 * cus ? 32 : 8) * resident) {
-    p.waves = 4 * resident;
+  if (p.splits > 1 && grid <= cus && tiles <= (4 * grid >= 3 * cus ? 8 : 2) * wide) {
+    p.waves = wide;
     p.splits = 1;
   }
   return p;
@@ -468,7 +471,7 @@ size_t kv_part_rows(const aar_kv_cache& c, const KvPlan& p) {
 
 template <int DT, bool VEC>
 int launch_attn(const KvPages& c, const KvAttn& a, int waves, hipStream_t st) {
-  constexpr int kMost = 4 * kv_resident(DT);
+  constexpr int kMost = 4 * kv_wide(DT);
   const int64_t BH = (int64_t)c.B * c.Hkv;
   const dim3 grid((unsigned)(BH * a.blocks * a.splits)), block(waves * kWave);
   if (waves == kMost) kv_attn_kernel<DT, kMost, VEC><<<grid, block, 0, st>>>(c, a);

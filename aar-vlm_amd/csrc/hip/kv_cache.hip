@@ -46,14 +46,31 @@ __device__ __forceinline__ uint32_t* value_word(uint8_t* half, const Unit& w, in
   return reinterpret_cast<uint32_t*>(half + (w.j >> 5) * 32 * dp + (w.c + e) * 32 + value_quad(w.q));
 }
 
-// x / s to the nearest whole number, ties to even, from inv, nearly 1 / s: the
-// remainder of x after q steps is exact, and more than half a step of it (or just
-// that, q odd) is one step further.
-__device__ __forceinline__ int kv_round(float x, float s, float inv) {
+// x / s to the nearest whole number, ties to even, plus 128, from inv, nearly 1 / s: the
+// remainder of x after q steps is exact, and more than half a step of it (or just that,
+// q odd) is one step further.
+__device__ __forceinline__ uint32_t kv_byte(float x, float s, float inv) {
   float q = rintf(x * inv);
   const float r = fmaf(-q, s, x), over = fabsf(r) - 0.5f * s;
   if (over > 0.f || (over == 0.f && ((int)q & 1))) q += copysignf(1.f, r);
-  return (int)fminf(fmaxf(q, -127.f), 127.f);
+  return (uint32_t)((int)fminf(fmaxf(q, -127.f), 127.f) + 128);
+}
+
+// The same for all but about one in 50 000: 2^23 and a half of it take the fraction off,
+// and the low byte is the number + 128; near enough to a border to be wrong sets `near`.
+// For steps above 2^-100, whose largest quotient rounds to 127.
+__device__ __forceinline__ uint32_t kv_byte_fast(float x, float s, float inv, bool& near) {
+  const float y = fmaf(x, inv, 12582912.f + 128.f), q = y - (12582912.f + 128.f);
+  near = near || fabsf(fmaf(-q, s, x)) >= 0.5f * s;
+  return __float_as_uint(y);
+}
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), hi = __builtin_amdgcn_perm(d, c, 0x04000c0cu);
+  return lo | hi;
+#else
+  return a;
+#endif
 }
 
 // Largest of the workgroup's values.
@@ -96,18 +113,25 @@ kv_append_kernel(const KvPages c, const KvRows a) {
     const int base = p << c.shift, lo = max(s, base) - base, hi = min(e - base, page);
     const int64_t id = c.id(b, p);
     f32x4 v[UNITS][4];
+    // no branches: all of a thread's loads in flight
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) {
+      const Unit w(min((int)(threadIdx.x + i * blockDim.x), units - 1), c.dp);
+      const int col = min(w.c, (c.d - 1) & ~3);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int j = min(w.j + t, hi - 1);
+        const float* row = j < lo ? open + (int64_t)j * c.d : rows + (int64_t)(base + j - s) * x.st;
+        v[i][t] = load4<VEC>(row + col, c.d - col);
+      }
+    }
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < UNITS; ++i) {
-      const int u = threadIdx.x + i * blockDim.x;
-      const Unit w(u, c.dp);
+      const Unit w(threadIdx.x + i * blockDim.x, c.dp);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int j = w.j + t;
-        v[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (u >= units || j >= hi || w.c >= c.d) continue;
-        if (j < lo) v[i][t] = load4<VEC>(open + (int64_t)j * c.d + w.c, c.d - w.c);
-        else v[i][t] = load4<VEC>(rows + (int64_t)(base + j - s) * x.st + w.c, c.d - w.c);
+        if (w.j + t >= hi || w.c >= c.d) v[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < 4; ++n) top = max(top, __float_as_uint(fabsf(v[i][t][n])));
       }
@@ -115,7 +139,8 @@ kv_append_kernel(const KvPages c, const KvRows a) {
     top = group_max(top, smax);  // as bits: a NaN is the largest
     const float scale = __uint_as_float(top) / 127.0f;
     // of steps below 2^-100 the inverse may be infinite: both sides times 2^64
-    const float f = scale < 0x1p-100f ? 0x1p64f : 1.f, step = scale * f, inv = 1.0f / step;
+    const bool tiny = scale < 0x1p-100f;
+    const float f = tiny ? 0x1p64f : 1.f, step = scale * f, inv = 1.0f / step;
     const bool flat = !(scale > 0.f && scale < INFINITY);  // all 0, or not finite: numbers of 0
     if (id < 0 && a.err) *a.err = 1;
     if (id >= 0 && threadIdx.x == 0) c.scale(id, h)[kv] = scale;
@@ -126,20 +151,24 @@ kv_append_kernel(const KvPages c, const KvRows a) {
       if (u >= units) continue;
       const Unit w(u, c.dp);
       if (id >= 0) {
-        uint32_t n[4] = {0, 0, 0, 0};  // a word for each token (keys) or column (values)
+        uint32_t n[4][4];
+        bool near = tiny || flat;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t byte = flat ? 128u : (uint32_t)(kv_round(v[i][t][k] * f, step, inv) + 128);
-            if (kv) n[k] |= byte << (8 * t);
-            else n[t] |= byte << (8 * k);
+          for (int k = 0; k < 4; ++k) n[t][k] = kv_byte_fast(v[i][t][k], step, inv, near);
+        }
+        if (near) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) n[t][k] = flat ? 128u : kv_byte(v[i][t][k] * f, step, inv);
           }
         }
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          if (kv) *value_word(half, w, t, c.dp) = n[t];
-          else *reinterpret_cast<uint32_t*>(half + (w.j + t) * c.dp + w.c) = n[t];
+          if (kv) *value_word(half, w, t, c.dp) = low_bytes(n[0][t], n[1][t], n[2][t], n[3][t]);
+          else *reinterpret_cast<uint32_t*>(half + (w.j + t) * c.dp + w.c) = low_bytes(n[t][0], n[t][1], n[t][2], n[t][3]);
         }
       }
       if (p != p1 || !left || w.c >= c.d) continue;
