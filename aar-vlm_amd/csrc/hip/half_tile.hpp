@@ -168,8 +168,6 @@ struct HalfTile {
         f[i][k] = buffer_load4(b, r < n && col(tid) + 4 * k < d ? at + 16 * k : kNowhere);
     }
   }
-  // MASKED: rows with a NaN are `bad` too, where not all of the output's rows may have it.
-  template <bool MASKED = false>
   __device__ __forceinline__ void store(char* s, int tid, bool& bad) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -177,10 +175,7 @@ struct HalfTile {
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float x = fabsf(f[i][g][2 * e]), y = fabsf(f[i][g][2 * e + 1]);
-          top = MASKED ? nan_max(nan_max(top, x), y) : fmaxf(fmaxf(top, x), y);
-        }
+        for (int e = 0; e < 2; ++e) top = fmaxf(fmaxf(top, fabsf(f[i][g][2 * e])), fabsf(f[i][g][2 * e + 1]));
       ex[i] = half_exponent(row_top<kOcts>(__float_as_uint(top)), bad);
       const float m = half_scale(ex[i]);
       u32x4 hi, lo;
@@ -229,9 +224,18 @@ __device__ __forceinline__ f32x16 half_rows(const char* s, const u32x4 (&b)[DP /
   return acc;
 }
 
+// The two parts of (a, b), a pair a word.  one: 1, unknown to the compiler, so that a
+// difference is one mixed multiply-add and not a conversion and a subtraction.
+__device__ __forceinline__ void half_split_plain(float a, float b, float one, uint32_t& hi, uint32_t& lo) {
+  const f16x2 x = __builtin_convertvector(f32x2{a, b}, f16x2);
+  const f32x2 rest = {fmaf(a, one, -(float)x[0]), fmaf(b, one, -(float)x[1])};
+  hi = __builtin_bit_cast(uint32_t, x);
+  lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, f16x2));
+}
+
 // acc[b] += tile^T . x over rows 16 k .. 16 k + 15 of the tile, x = accumulator
-// registers 8 k .. 8 k + 7 of x times f: column 32 b + lr of the tile.
-template <int DP>
+// registers 8 k .. 8 k + 7 of x times f (PLAIN: of x, f = 1): column 32 b + lr of the tile.
+template <int DP, bool PLAIN = false>
 __device__ __forceinline__ void half_cols(const char* s, const f32x16& x, float f, int k, int lane,
                                           f32x16 (&acc)[DP / 32]) {
   using T = HalfTile<DP>;
@@ -241,7 +245,8 @@ __device__ __forceinline__ void half_cols(const char* s, const f32x16& x, float 
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     uint32_t hi, lo;
-    half_split_pair(x[8 * k + 2 * e], x[8 * k + 2 * e + 1], f, hi, lo);
+    if (PLAIN) half_split_plain(x[8 * k + 2 * e], x[8 * k + 2 * e + 1], f, hi, lo);
+    else half_split_pair(x[8 * k + 2 * e], x[8 * k + 2 * e + 1], f, hi, lo);
     pp[0][e] = hi;
     pp[1][e] = lo;
   }

@@ -10,8 +10,8 @@
 //
 // A block of 128 queries visits the tiles of 32 keys that any of its rows sees: the
 // sinks' and the window's.  A block of 128 keys visits the queries up to W - 1 behind
-// its last key, of all heads that share it; a block that holds sinks visits all later
-// ones, in parts of a common length that are summed at the end.
+// its last key, of all heads that share it; the later ones that see its sinks are visited
+// for the sinks' tiles alone, in parts that are summed at the end.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -29,12 +29,14 @@ namespace {
 struct WaArgs {
   FaIn q, k, v, o_in, dout;
   FaOut o, dq, dk, dv;
-  float* lse;      // [B * H][T]
-  float* D;        // [B * H][T], backward
-  float *dk_part, *dv_part;  // [B * Hkv][items][128][DP] partial sums
+  float* lse;                // [B * H][T]
+  char *kv_img, *qd_img;     // [B * Hkv][tiles] pairs of K's and V's planes, [B * H][tiles] of Q's and dO's
+  uint32_t *kv_top, *qd_top;  // the same of their exponents (wa_top)
+  float *l2, *D;             // [B * H][32 * tiles] lse in log2 (+inf past T) and dO . O of every query row
+  float *dk_part, *dv_part;  // [B * Hkv][sink_tiles][far_parts][32][DP] sums of the sinks' far queries
   int T, d, H, G, Hkv, BH, BHkv;  // BH = B * H query heads, BHkv = B * Hkv
-  int W, S;
-  int chunk, sink_blocks, sink_parts, parts;  // dK/dV: tiles of a part, blocks that hold sinks, their parts, others'
+  int W, S, tiles;                // tiles of 32 rows
+  int sink_tiles, far_parts, far_chunk;  // dK/dV: key tiles that hold sinks, parts of their far queries (0: none), tiles of one
   float scale, scale_log2;
 };
 
@@ -85,47 +87,178 @@ __device__ __forceinline__ void wa_store(float* row, const f32x16 (&x)[DP / 32],
   }
 }
 
-// Forward.  The running maximum of a row follows its scores only when they pass it by
-// 2^4, so O is rarely rescaled; when it moves, the scale of P is found again.
+// A tile's exponent as its planes are scaled by: half_exponent's of its largest element,
+// the lowest bit set where the planes do not hold it (elements that are not finite or
+// out of range, or rows whose largest elements are more than 2^12 apart: a row could
+// lose bits to one that a query does not see).
+__device__ __forceinline__ uint32_t top_bits(uint32_t t) { return t & ~1u; }
+// log2 of row_factor: 2^14 over the scale.
+__device__ __forceinline__ int top_log(uint32_t t) { return (int)(t >> 23) - 126; }
+
+// Scale of a tile's planes from the bits of its rows' largest elements: `hi` the most of
+// them, `lo` the least of those that are not 0.  Sets the lowest bit where these do not
+// hold the tile.
+__device__ __forceinline__ uint32_t tile_top(uint32_t hi, uint32_t lo) {
+  bool bad = false;
+  const uint32_t ex = half_exponent(hi, bad);
+  return ex | (bad || (hi != 0 && (lo >> 23) + 12 < (hi >> 23)) ? 1u : 0u);
+}
+
+// The planes of a tile's 32 rows of K or V, once for all the blocks that read them, as the
+// matrix passes have them in LDS: these then move by DMA alone, and their factors are a
+// tile's.  Bound by the bytes.
+template <int DP, bool VEC>
+__global__ void __launch_bounds__(kFaThreads)
+window_split_kernel(const WaArgs a) {
+  using Tile = HalfTile<DP>;
+  __shared__ uint32_t most[4], least[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int second = blockIdx.x & 1, at = blockIdx.x >> 1, bhk = at / a.tiles, row0 = at % a.tiles * kTile;
+  const FaIn& x = second ? a.v : a.k;
+  Tile t;
+  t.template load<VEC>(wa_kv_head(x, a, bhk) + (int64_t)row0 * x.st, x.st, a.T - row0, a.d,
+                       typename Tile::Place(x.st, a.d, tid));
+
+  // the largest element of the tile and the least of its rows' (as bits, NaN the largest)
+  uint32_t hi = 0, lo = 0xffffffffu;
+#pragma unroll
+  for (int i = 0; i < Tile::kPer; ++i) {
+    float top = 0.f;
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = nan_max(top, fabsf(t.f[i][g][e]));
+    const uint32_t row = row_top<Tile::kOcts>(__float_as_uint(top) & 0x7fffffffu);
+    hi = max(hi, row);
+    if (row != 0) lo = min(lo, row);
+  }
+#pragma unroll
+  for (int o = 32; o >= 8; o /= 2) {
+    hi = max(hi, (uint32_t)__shfl_xor((int)hi, o, kWave));
+    lo = min(lo, (uint32_t)__shfl_xor((int)lo, o, kWave));
+  }
+  if (lane == 0) {
+    most[wave] = hi;
+    least[wave] = lo;
+  }
+  __syncthreads();
+  const uint32_t top = tile_top(max(max(most[0], most[1]), max(most[2], most[3])),
+                                min(min(least[0], least[1]), min(least[2], least[3])));
+  if (tid == 0) a.kv_top[blockIdx.x] = top;
+
+  char* img = a.kv_img + (int64_t)blockIdx.x * Tile::kBytes;
+  const float m = half_scale(top_bits(top));
+#pragma unroll
+  for (int i = 0; i < Tile::kPer; ++i) {
+    u32x4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t y, z;
+      half_split_pair(t.f[i][e >> 1][2 * (e & 1)], t.f[i][e >> 1][2 * (e & 1) + 1], m, y, z);
+      h[e] = y;
+      l[e] = z;
+    }
+    char* to = img + Tile::row(i, tid) * Tile::kRow + 2 * Tile::col(tid);
+    *reinterpret_cast<u32x4*>(to) = h;
+    *reinterpret_cast<u32x4*>(to + Tile::kPlane) = l;
+  }
+}
+
+// A wave's 32 rows (a lane its half's octets of each 16 columns; zeros without p) in parts
+// of a tile's scale: into registers, and as planes to `img`.  Returns the tile's exponent.
+template <int DP, bool VEC>
+__device__ __forceinline__ uint32_t split_rows(const float* p, int d, int lr, int h, u32x4 (&out)[DP / 16][2], char* img) {
+  f32x4 x[DP / 16][2];
+  float top = 0.f;
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int dd = 16 * c + 8 * h + 4 * g;
+      x[c][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (p && dd < d) x[c][g] = load4<VEC>(p + dd, d - dd);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = nan_max(top, fabsf(x[c][g][e]));
+    }
+  }
+  uint32_t row = __float_as_uint(top) & 0x7fffffffu;
+  row = max(row, (uint32_t)__shfl_xor((int)row, 32, kWave));
+  uint32_t hi = row, lo = row != 0 ? row : 0xffffffffu;
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) {
+    hi = max(hi, (uint32_t)__shfl_xor((int)hi, o, kWave));
+    lo = min(lo, (uint32_t)__shfl_xor((int)lo, o, kWave));
+  }
+  const uint32_t t = tile_top(hi, lo);
+  const float m = half_scale(top_bits(t));
+  char* to = img + lr * HalfTile<DP>::kRow + 16 * h;
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t y, z;
+      half_split_pair(x[c][e >> 1][2 * (e & 1)], x[c][e >> 1][2 * (e & 1) + 1], m, y, z);
+      out[c][0][e] = y;
+      out[c][1][e] = z;
+    }
+    *reinterpret_cast<u32x4*>(to + 32 * c) = out[c][0];
+    *reinterpret_cast<u32x4*>(to + 32 * c + HalfTile<DP>::kPlane) = out[c][1];
+  }
+  return t;
+}
+
+// A pair of planes from HBM into LDS: 1024 bytes a wave and DMA.
+template <int DP, int WAVES = 4>
+__device__ __forceinline__ void stage_pair(const char* src, char* lds, int wave, int lane) {
+  constexpr int n = 2 * HalfTile<DP>::kBytes / 1024;
+  static_assert(n * 1024 == 2 * HalfTile<DP>::kBytes, "whole DMAs");
+#pragma unroll
+  for (int k = 0; k < (n + WAVES - 1) / WAVES; ++k) {
+    const int i = wave + WAVES * k;
+    if (i < n) dma16_untracked_s(lane * 16 + i * 1024, src, (lds_void_t*)(lds + i * 1024));
+  }
+}
+
+// Forward.  P is formed as 2^(s + v - R + 11), with v the exponent of the tile's values and
+// R, the row's, such that it stays below 2^15: the largest s + v so far, followed only when
+// it is passed by 2^4, so O is rarely rescaled.  So O is sum P V 2^(25 - R), and l is kept
+// as l 2^(-R - 29).
 template <int DP, bool VEC>
 __global__ void __launch_bounds__(kFaThreads, DP == 64 ? 3 : 2)
 window_fwd_kernel(const WaArgs a) {
   using Tile = HalfTile<DP>;
   constexpr int NB = DP / 32;
-  __shared__ __attribute__((aligned(16))) char ks[2][Tile::kBytes];
-  __shared__ __attribute__((aligned(16))) char vs[2][Tile::kBytes];
-  __shared__ __attribute__((aligned(16))) float kf[2][kTile], vf[2][kTile];  // the rows' factors
-  __shared__ int not_held;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ __attribute__((aligned(16))) char kv[2][2 * Tile::kBytes];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
-  const int bh = blockIdx.x % a.BH, qb = blockIdx.x / a.BH;
-  const float* __restrict__ K = wa_kv_head(a.k, a, wa_kv(a, bh));
-  const float* __restrict__ V = wa_kv_head(a.v, a, wa_kv(a, bh));
+  const int bh = blockIdx.x % a.BH, qb = blockIdx.x / a.BH, bhk = wa_kv(a, bh);
   const int q0 = qb * kBlock, w0 = q0 + wave * kTile, qi = w0 + lr;  // this lane's row
   const float* Q = qi < a.T ? wa_head(a.q, a, bh) + (int64_t)qi * a.q.st : nullptr;
   const WaTiles tiles(a, q0, min(q0 + kBlock, a.T) - 1);
-  if (tid == 0) not_held = 0;
+  const char* img = a.kv_img + (int64_t)bhk * a.tiles * 2 * Tile::kBytes;
+  const uint32_t* tops = a.kv_top + (int64_t)bhk * a.tiles * 2;
+  auto stage = [&](int t, int buf) {
+    stage_pair<DP>(img + (int64_t)(tiles.key(t) / kTile) * 2 * Tile::kBytes, kv[buf], wave, lane);
+  };
+  stage(0, 0);
 
   u32x4 qp[DP / 16][2];
-  bool row_bad = false, bad = false;
+  bool row_bad = false;
+  uint32_t held = 0;  // the lowest bit: a tile that is not
   const float qf = half_row<DP, VEC>(Q, a.d, a.scale_log2, h, qp, row_bad);
   f32x16 o[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) o[b] = zero16();
-  float m = -INFINITY, l = 0.f;
-  HalfScale<NB> fit;
+  float R = -INFINITY, l = 0.f, one = 1.f;
+  asm("" : "+v"(one));
 
   auto follow = [&](float mx, float slack) {
+    if (!__any(mx > R + slack)) return;
     mx = half_swap_max(mx);
-    const bool move = mx > m + slack;
-    if (!__any(move)) return;
-    const float alpha = move ? fast_exp2(m - mx) : 1.f;
-    if (move) {
-      m = mx;
-      fit.most = -1.f;
-    }
+    const bool move = mx > R + slack;
+    const float alpha = move ? fast_exp2(R - mx) : 1.f;
+    if (move) R = mx;
     l *= alpha;
-    fit.big *= alpha;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -138,78 +271,39 @@ window_fwd_kernel(const WaArgs a) {
     for (int r = 0; r < 16; ++r)
       if (!wa_sees(a, qi, kv0 + acc_row(r, h))) s[r] = -INFINITY;
   };
-  auto compute = [&](int buf, int kv0) {
-    f32x16 s = half_rows<DP>(ks[buf], qp, lr, h);
-    float mx = -INFINITY, ps = 0.f, top = 0.f;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32x4 k4 = row_values(kf[buf], g, h);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[4 * g + e] *= k4[e];
-    }
+
+  for (int t = 0; t < tiles.count; ++t) {
+    const int buf = t & 1, kv0 = tiles.key(t);
+    wait_vm_lgkm0<0>();  // this wave's share of tile t is in LDS, and its reads of t - 1 are done
+    ring_barrier();
+    if (t + 1 < tiles.count) stage(t + 1, buf ^ 1);
+    if (w0 >= a.T || !wa_any(a, w0, kv0)) continue;
+    const uint32_t kt = tops[kv0 / kTile * 2], vt = tops[kv0 / kTile * 2 + 1];
+    held |= kt | vt;
+    f32x16 s = half_rows<DP>(kv[buf], qp, lr, h);
     hide(s, kv0);
+    const float cs = qf * row_factor(top_bits(kt)), vl = (float)top_log(vt);
+    float mx = -INFINITY, ps = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
-    follow(mx * qf, 4.f);
-    const float mu = m == -INFINITY ? 0.f : m;
+    follow(fmaf(mx, cs, vl), 4.f);
+    const float by = R == -INFINITY ? 0.f : vl - R + 11.f;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32x4 v4 = row_values(vf[buf], g, h);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p = fast_exp2(s[4 * g + e] * qf - mu);
-        ps += p;
-        s[4 * g + e] = p * v4[e];
-        top = fmaxf(top, s[4 * g + e]);
-      }
+    for (int r = 0; r < 16; ++r) {
+      s[r] = fast_exp2(fmaf(s[r], cs, by));
+      ps += s[r];
     }
-    l += half_swap_sum(ps);
-    fit.follow(top, o, row_bad);
-    half_cols<DP>(vs[buf], s, fit.f, 0, lane, o);
-    half_cols<DP>(vs[buf], s, fit.f, 1, lane, o);
-  };
-
-  Tile kc[2], vc[2];
-  const typename Tile::Place kat(a.k.st, a.d, tid), vat(a.v.st, a.d, tid);
-  auto load = [&](int i, int t) {
-    const int row0 = tiles.key(min(t, tiles.count - 1));
-    kc[i].template load<VEC>(K + (int64_t)row0 * a.k.st, a.k.st, a.T - row0, a.d, kat);
-    vc[i].template load<VEC>(V + (int64_t)row0 * a.v.st, a.v.st, a.T - row0, a.d, vat);
-  };
-  auto store = [&](int i, int buf) {
-    kc[i].template store<true>(ks[buf], tid, bad);
-    vc[i].template store<true>(vs[buf], tid, bad);
-    if (Tile::col(tid) != 0) return;
-#pragma unroll
-    for (int n = 0; n < Tile::kPer; ++n) {
-      const int r = Tile::row(n, tid);
-      kf[buf][r] = row_factor(kc[i].ex[n]);
-      vf[buf][r] = row_factor(vc[i].ex[n]);
-    }
-  };
-  load(0, 0);
-  load(1, 1);
-  store(0, 0);
-  load(0, 2);
-  lds_barrier();
-  // Iteration t: tile t in LDS, t + 1 in registers, t + 2 on its way, t + 3 sent for.
-  for (int t = 0; t < tiles.count; t += 2) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (t + u >= tiles.count) break;
-      const int kv0 = tiles.key(t + u);
-      if (w0 < a.T && wa_any(a, w0, kv0)) compute(u, kv0);
-      store(1 - u, 1 - u);
-      load(1 - u, t + u + 3);
-      lds_barrier();
-    }
+    l = fmaf(ps, pow2(-top_log(vt) - 40), l);
+    half_cols<DP, true>(kv[buf] + Tile::kBytes, s, one, 0, lane, o);
+    half_cols<DP, true>(kv[buf] + Tile::kBytes, s, one, 1, lane, o);
   }
-  fit.undo(o);
+  l = half_swap_sum(l);
+  float f = 0x1p-54f / l, lse = log2f(l) + R + 29.f;
 
-  if (bad) not_held = 1;
-  __syncthreads();
-  if (w0 < a.T && __any(row_bad || not_held)) {
-    m = -INFINITY;
+  if (w0 < a.T && __any(row_bad || (held & 1))) {
+    const float* __restrict__ K = wa_kv_head(a.k, a, bhk);
+    const float* __restrict__ V = wa_kv_head(a.v, a, bhk);
+    R = -INFINITY;
     l = 0.f;
 #pragma unroll
     for (int b = 0; b < NB; ++b) o[b] = zero16();
@@ -223,12 +317,11 @@ window_fwd_kernel(const WaArgs a) {
                    in && Q ? Q[c + h] * a.scale_log2 : 0.f, s);
       }
       hide(s, kv0);
-      float mx = -INFINITY;
+      float mx = -INFINITY, ps = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
       follow(mx, 0.f);
-      const float mu = m == -INFINITY ? 0.f : m;
-      float ps = 0.f;
+      const float mu = R == -INFINITY ? 0.f : R;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[r] = fast_exp2(s[r] - mu);
@@ -246,54 +339,68 @@ window_fwd_kernel(const WaArgs a) {
       }
       add_not_finite(V, a.v.st, kv0, a.T, a.d, s, [&](int j) { return wa_sees(a, qi, j); }, o);
     }
+    f = 1.0f / l;
+    lse = log2f(l) + R;
   }
   if (qi >= a.T) return;
-  wa_store<DP, VEC>(wa_head(a.o, a, bh) + (int64_t)qi * a.o.st, o, 1.0f / l, a.d, h);
-  if (h == 0) a.lse[(int64_t)bh * a.T + qi] = (m + log2f(l)) * kLn2;
+  wa_store<DP, VEC>(wa_head(a.o, a, bh) + (int64_t)qi * a.o.st, o, f, a.d, h);
+  if (h == 0) a.lse[(int64_t)bh * a.T + qi] = lse * kLn2;
 }
 
-// dQ (and D).
+// dQ, and what dK's and dV's pass reads of a query row: the planes of Q and dO, D and lse.
 template <int DP, bool VEC>
-__global__ void __launch_bounds__(kFaThreads, DP == 64 ? 3 : 1)
+__global__ void __launch_bounds__(kFaThreads, DP == 64 ? 2 : 1)
 window_bwd_dq_kernel(const WaArgs a) {
   constexpr int NB = DP / 32;
   using Tile = HalfTile<DP>;
-  __shared__ __attribute__((aligned(16))) char ks[2][Tile::kBytes];
-  __shared__ __attribute__((aligned(16))) char vs[2][Tile::kBytes];
-  __shared__ __attribute__((aligned(16))) float kf[2][kTile], vf[2][kTile];  // the rows' factors
-  __shared__ int not_held;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ __attribute__((aligned(16))) char kv[2][2 * Tile::kBytes];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
-  const int bh = blockIdx.x % a.BH, qb = blockIdx.x / a.BH;
-  const float* __restrict__ K = wa_kv_head(a.k, a, wa_kv(a, bh));
-  const float* __restrict__ V = wa_kv_head(a.v, a, wa_kv(a, bh));
+  const int bh = blockIdx.x % a.BH, qb = blockIdx.x / a.BH, bhk = wa_kv(a, bh);
   const int q0 = qb * kBlock, w0 = q0 + wave * kTile, qi = w0 + lr;
   const bool row_ok = qi < a.T;
   const float* Q = row_ok ? wa_head(a.q, a, bh) + (int64_t)qi * a.q.st : nullptr;
   const float* dO = row_ok ? wa_head(a.dout, a, bh) + (int64_t)qi * a.dout.st : nullptr;
   const WaTiles tiles(a, q0, min(q0 + kBlock, a.T) - 1);
-  if (tid == 0) not_held = 0;
+  const char* img = a.kv_img + (int64_t)bhk * a.tiles * 2 * Tile::kBytes;
+  const uint32_t* tops = a.kv_top + (int64_t)bhk * a.tiles * 2;
+  auto stage = [&](int t, int buf) {
+    stage_pair<DP>(img + (int64_t)(tiles.key(t) / kTile) * 2 * Tile::kBytes, kv[buf], wave, lane);
+  };
+  stage(0, 0);
 
-  float dsum = 0.f;
-  if (row_ok) {
-    const float* O = wa_head(a.o_in, a, bh) + (int64_t)qi * a.o_in.st;
-#pragma unroll
-    for (int c = 0; c < DP / 8; ++c) {
-      const int dd = 8 * c + 4 * h;
-      if (dd < a.d) {
-        const f32x4 x = load4<VEC>(dO + dd, a.d - dd), y = load4<VEC>(O + dd, a.d - dd);
-        dsum += x[0] * y[0] + x[1] * y[1] + x[2] * y[2] + x[3] * y[3];
-      }
-    }
-  }
-  dsum = half_swap_sum(dsum);
-  const float l2 = row_ok ? a.lse[(int64_t)bh * a.T + qi] * kLog2e : INFINITY;
-  if (row_ok && h == 0) a.D[(int64_t)bh * a.T + qi] = dsum;
-
+  float l2 = INFINITY, dsum = 0.f;
   u32x4 qp[DP / 16][2], dop[DP / 16][2];
-  bool row_bad = false, bad = false;
-  const float qf = half_row<DP, VEC>(Q, a.d, a.scale_log2, h, qp, row_bad);
-  const float df = half_row<DP, VEC>(dO, a.d, 1.f, h, dop, row_bad);
+  bool row_bad = false;
+  uint32_t held = 0;
+  float qf = 0.f, df = 0.f;
+  if (w0 < a.T) {
+    if (row_ok) {
+      const float* O = wa_head(a.o_in, a, bh) + (int64_t)qi * a.o_in.st;
+#pragma unroll
+      for (int c = 0; c < DP / 8; ++c) {
+        const int dd = 8 * c + 4 * h;
+        if (dd < a.d) {
+          const f32x4 x = load4<VEC>(dO + dd, a.d - dd), y = load4<VEC>(O + dd, a.d - dd);
+          dsum += x[0] * y[0] + x[1] * y[1] + x[2] * y[2] + x[3] * y[3];
+        }
+      }
+      l2 = a.lse[(int64_t)bh * a.T + qi] * kLog2e;
+    }
+    dsum = half_swap_sum(dsum);
+    const int64_t tile = (int64_t)bh * a.tiles + w0 / kTile;
+    if (h == 0) {
+      a.D[tile * kTile + lr] = dsum;
+      a.l2[tile * kTile + lr] = l2;
+    }
+    char* to = a.qd_img + tile * 2 * Tile::kBytes;
+    const uint32_t qt = split_rows<DP, VEC>(Q, a.d, lr, h, qp, to);
+    const uint32_t ot = split_rows<DP, VEC>(dO, a.d, lr, h, dop, to + Tile::kBytes);
+    if (lane < 2) a.qd_top[2 * tile + lane] = lane ? ot : qt;
+    held = qt | ot;
+    qf = lane_factor(top_bits(qt)) * a.scale_log2;
+    df = lane_factor(top_bits(ot));
+  }
   f32x16 dq[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) dq[b] = zero16();
@@ -305,60 +412,33 @@ window_bwd_dq_kernel(const WaArgs a) {
     for (int r = 0; r < 16; ++r)
       if (!wa_sees(a, qi, kv0 + acc_row(r, h))) x[r] = 0.f;
   };
-  Tile kc, vc;
-  const typename Tile::Place kat(a.k.st, a.d, tid), vat(a.v.st, a.d, tid);
-  auto load = [&](int t) {
-    const int row0 = tiles.key(t);
-    kc.template load<VEC>(K + (int64_t)row0 * a.k.st, a.k.st, a.T - row0, a.d, kat);
-    vc.template load<VEC>(V + (int64_t)row0 * a.v.st, a.v.st, a.T - row0, a.d, vat);
-  };
-  auto store = [&](int buf) {
-    kc.template store<true>(ks[buf], tid, bad);
-    vc.template store<true>(vs[buf], tid, bad);
-    if (Tile::col(tid) != 0) return;
-#pragma unroll
-    for (int n = 0; n < Tile::kPer; ++n) {
-      const int r = Tile::row(n, tid);
-      kf[buf][r] = row_factor(kc.ex[n]);
-      vf[buf][r] = row_factor(vc.ex[n]);
-    }
-  };
-  load(0);
-  store(0);
-  lds_barrier();
   for (int t = 0; t < tiles.count; ++t) {
     const int buf = t & 1, kv0 = tiles.key(t);
-    const bool has_next = t + 1 < tiles.count;
-    if (has_next) load(t + 1);
-    if (w0 < a.T && wa_any(a, w0, kv0)) {
-      const f32x16 s = half_rows<DP>(ks[buf], qp, lr, h);
-      f32x16 dp = half_rows<DP>(vs[buf], dop, lr, h);
-      float top = 0.f;
+    wait_vm_lgkm0<0>();
+    ring_barrier();
+    if (t + 1 < tiles.count) stage(t + 1, buf ^ 1);
+    if (w0 >= a.T || !wa_any(a, w0, kv0)) continue;
+    const uint32_t kt = tops[kv0 / kTile * 2], vt = tops[kv0 / kTile * 2 + 1];
+    held |= kt | vt;
+    const f32x16 s = half_rows<DP>(kv[buf], qp, lr, h);
+    f32x16 dp = half_rows<DP>(kv[buf] + Tile::kBytes, dop, lr, h);
+    const float kfac = row_factor(top_bits(kt)), cs = qf * kfac, cd = df * row_factor(top_bits(vt));
+    float top = 0.f;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 k4 = row_values(kf[buf], g, h), v4 = row_values(vf[buf], g, h);
+    for (int r = 0; r < 16; ++r) dp[r] = fast_exp2(fmaf(s[r], cs, -l2)) * fmaf(dp[r], cd, -dsum);
+    hide(dp, kv0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * g + e;
-          const float p = fast_exp2(s[r] * k4[e] * qf - l2);
-          dp[r] = p * (dp[r] * v4[e] * df - dsum) * k4[e];
-        }
-      }
-      hide(dp, kv0);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(dp[r]));
-      fit.follow(top, dq, row_bad);
-      half_cols<DP>(ks[buf], dp, fit.f, 0, lane, dq);
-      half_cols<DP>(ks[buf], dp, fit.f, 1, lane, dq);
-    }
-    if (has_next) store(buf ^ 1);
-    lds_barrier();
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(dp[r]));
+    fit.follow(top * kfac, dq, row_bad);
+    const float f = fminf(fit.f * kfac, 0x1p126f);
+    half_cols<DP>(kv[buf], dp, f, 0, lane, dq);
+    half_cols<DP>(kv[buf], dp, f, 1, lane, dq);
   }
   fit.undo(dq);
 
-  if (bad) not_held = 1;
-  __syncthreads();
-  if (w0 < a.T && __any(row_bad || not_held)) {
+  if (w0 < a.T && __any(row_bad || (held & 1))) {
+    const float* __restrict__ K = wa_kv_head(a.k, a, bhk);
+    const float* __restrict__ V = wa_kv_head(a.v, a, bhk);
 #pragma unroll
     for (int b = 0; b < NB; ++b) dq[b] = zero16();
     for (int t = 0; t < tiles.count; ++t) {
@@ -378,8 +458,8 @@ window_bwd_dq_kernel(const WaArgs a) {
         const int col = b * 32 + lr;
 #pragma unroll
         for (int st = 0; st < 16; ++st) {
-          const int row = kv0 + acc_row(st, h);
-          dq[b] = mfma32(row < a.T && col < a.d ? finite(K[(int64_t)row * a.k.st + col]) : 0.f, dp[st], dq[b]);
+          const int key = kv0 + acc_row(st, h);
+          dq[b] = mfma32(key < a.T && col < a.d ? finite(K[(int64_t)key * a.k.st + col]) : 0.f, dp[st], dq[b]);
         }
       }
       add_not_finite(K, a.k.st, kv0, a.T, a.d, dp, [&](int j) { return wa_sees(a, qi, j); }, dq);
@@ -388,56 +468,74 @@ window_bwd_dq_kernel(const WaArgs a) {
   if (row_ok) wa_store<DP, VEC>(wa_head(a.dq, a, bh) + (int64_t)qi * a.dq.st, dq, a.scale, a.d, h);
 }
 
-// A part of a key block's list of query tiles: `heads` lists of `count` tiles from the
-// block's first key on.
-struct WaPart {
-  int kb, part, parts, first, count, begin, end;
-  int64_t slot;  // of its partial sums
-  // Item i of a key/value head: the parts of the blocks that hold sinks, then the others'.
-  __device__ __forceinline__ WaPart(const WaArgs& a, int bhk, int item) {
-    const int sinks = a.sink_blocks * a.sink_parts, blocks = (a.T + kBlock - 1) / kBlock;
-    const bool sink = item < sinks;
-    const int i = sink ? item : item - sinks;
-    parts = sink ? a.sink_parts : a.parts;
-    kb = (sink ? 0 : a.sink_blocks) + i / parts;
-    part = i % parts;
-    first = kb * (kBlock / kTile);
-    // the last query that sees a key of the block
-    const int64_t most = (int64_t)kb * kBlock + kBlock - 1 + a.W - 1;
-    const int last = sink || most >= a.T ? a.T - 1 : (int)most;
-    count = last / kTile + 1 - first;
-    begin = min(part * a.chunk, a.G * count);
-    end = min(begin + a.chunk, a.G * count);
-    slot = (int64_t)bhk * (sinks + (int64_t)(blocks - a.sink_blocks) * a.parts) + item;
+// The list of query tiles of 32 WAVES keys from k0 on: `count` tiles from `first` on of
+// each of the G heads that share them, items [begin, end) of it.  Four waves: a key block
+// with the queries up to the last that its window reaches (all later ones if it holds
+// sinks and these have no parts of their own).  One: 32 keys that hold sinks with a part of
+// the far queries, those behind their block's window.
+template <int WAVES>
+struct WaList {
+  int k0, part, first, count, begin, end;
+  __device__ __forceinline__ WaList(const WaArgs& a, int item) {
+    const int tile = WAVES == 4 ? 4 * item : item / a.far_parts;
+    part = WAVES == 4 ? 0 : item % a.far_parts;
+    k0 = tile * kTile;
+    // the last query that the window of a key of the block reaches
+    const int64_t most = (int64_t)k0 / kBlock * kBlock + kBlock - 1 + a.W - 1;
+    int last = most >= a.T ? a.T - 1 : (int)most;
+    if (WAVES == 4) {
+      if (k0 < a.S && a.far_parts == 0) last = a.T - 1;
+      first = tile;
+      count = last / kTile + 1 - first;
+      begin = 0;
+      end = a.G * count;
+    } else {
+      first = last / kTile + 1;
+      count = a.tiles - first;
+      begin = min(part * a.far_chunk, a.G * count);
+      end = min(begin + a.far_chunk, a.G * count);
+    }
   }
 };
 
-// dK and dV: a workgroup takes 128 keys, 32 a wave, a lane its key, and a part of the
-// query tiles that see them.
-template <int DP, bool VEC>
-__global__ void __launch_bounds__(kFaThreads, DP == 64 ? 2 : 1)
+// dK and dV: a wave takes 32 keys, a lane its key, and walks its workgroup's list.
+template <int DP, bool VEC, int WAVES>
+__global__ void __launch_bounds__(WAVES * kWave, DP == 64 ? 2 : 1)
 window_bwd_dkdv_kernel(const WaArgs a) {
   constexpr int NB = DP / 32;
   using Tile = HalfTile<DP>;
-  __shared__ __attribute__((aligned(16))) char qs[2][Tile::kBytes];
-  __shared__ __attribute__((aligned(16))) char dos[2][Tile::kBytes];
-  // factors of Q's rows and of dO's; lse in log2 and D
-  __shared__ __attribute__((aligned(16))) float qf[2][kTile], df[2][kTile], ls[2][kTile], ds[2][kTile];
-  __shared__ int not_held;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ __attribute__((aligned(16))) char qd[2][2 * Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) float stats[2][2 * kTile];  // lse in log2, D
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
-  const int bhk = blockIdx.x % a.BHkv;
-  const WaPart part(a, bhk, blockIdx.x / a.BHkv);
-  const int kw = part.kb * kBlock + wave * kTile;  // the wave's first key
+  const int bhk = blockIdx.x % a.BHkv, item = blockIdx.x / a.BHkv;
+  const WaList<WAVES> part(a, item);
+  const int kw = part.k0 + wave * kTile;  // the wave's first key
   const int kj = kw + lr;
   const bool key_ok = kj < a.T;
   const float* K = key_ok ? wa_kv_head(a.k, a, bhk) + (int64_t)kj * a.k.st : nullptr;
   const float* V = key_ok ? wa_kv_head(a.v, a, bhk) + (int64_t)kj * a.v.st : nullptr;
   const int head0 = bhk / a.Hkv * a.H + bhk % a.Hkv * a.G;  // the first query head
-  if (tid == 0) not_held = 0;
+  // where item t of the list stands among all heads' tiles
+  struct Place {
+    int head, tile;
+  };
+  auto place_of = [&](int t) { return Place{head0 + t / part.count, part.first + t % part.count}; };
+  auto next_of = [&](Place p) {
+    return p.tile + 1 < part.first + part.count ? Place{p.head, p.tile + 1} : Place{p.head + 1, part.first};
+  };
+  auto stage = [&](Place p, int buf) {
+    // the same in all lanes, which the compiler does not see through the loop
+    const int64_t at = (int64_t)__builtin_amdgcn_readfirstlane(p.head) * a.tiles + __builtin_amdgcn_readfirstlane(p.tile);
+    stage_pair<DP, WAVES>(a.qd_img + at * 2 * Tile::kBytes, qd[buf], wave, lane);
+    if (wave == WAVES - 1) dma4_untracked((lane < kTile ? a.l2 : a.D) + at * kTile + lr, (lds_void_t*)stats[buf]);
+  };
+  Place here = part.begin < part.end ? place_of(part.begin) : Place{head0, part.first};
+  if (part.begin < part.end) stage(here, 0);
 
   u32x4 kp[DP / 16][2], vp[DP / 16][2];
-  bool key_bad = false, bad = false;
+  bool key_bad = false;
+  uint32_t held = 0;
   const float kf = half_row<DP, VEC>(K, a.d, a.scale_log2, h, kp, key_bad);
   const float vf = half_row<DP, VEC>(V, a.d, 1.f, h, vp, key_bad);
   f32x16 dk[NB], dv[NB];
@@ -445,36 +543,6 @@ window_bwd_dkdv_kernel(const WaArgs a) {
   for (int b = 0; b < NB; ++b) dk[b] = dv[b] = zero16();
   HalfScale<NB> fit_k, fit_v;
 
-  Tile qc, dc;
-  const typename Tile::Place qat(a.q.st, a.d, tid), oat(a.dout.st, a.d, tid);
-  float lreg[Tile::kPer], dreg[Tile::kPer];
-  auto row_of = [&](int t) { return (part.first + t % part.count) * kTile; };
-  auto load = [&](int t) {
-    const int bh = head0 + t / part.count, row0 = row_of(t);
-    qc.template load<VEC>(wa_head(a.q, a, bh) + (int64_t)row0 * a.q.st, a.q.st, a.T - row0, a.d, qat);
-    dc.template load<VEC>(wa_head(a.dout, a, bh) + (int64_t)row0 * a.dout.st, a.dout.st, a.T - row0, a.d, oat);
-#pragma unroll
-    for (int n = 0; n < Tile::kPer; ++n) {
-      lreg[n] = dreg[n] = 0.f;
-      const int r = row0 + Tile::row(n, tid);
-      if (Tile::col(tid) != 0) continue;
-      lreg[n] = r < a.T ? a.lse[(int64_t)bh * a.T + r] * kLog2e : INFINITY;
-      dreg[n] = r < a.T ? a.D[(int64_t)bh * a.T + r] : 0.f;
-    }
-  };
-  auto store = [&](int buf) {
-    qc.template store<true>(qs[buf], tid, bad);
-    dc.template store<true>(dos[buf], tid, bad);
-    if (Tile::col(tid) != 0) return;
-#pragma unroll
-    for (int n = 0; n < Tile::kPer; ++n) {
-      const int r = Tile::row(n, tid);
-      qf[buf][r] = row_factor(qc.ex[n]);
-      df[buf][r] = row_factor(dc.ex[n]);
-      ls[buf][r] = lreg[n];
-      ds[buf][r] = dreg[n];
-    }
-  };
   // P or dS of the queries from i0 on that do not see the lane's key
   auto hide = [&](f32x16& p, int i0) {
     if (wa_all(a, i0, kw)) return;
@@ -482,79 +550,64 @@ window_bwd_dkdv_kernel(const WaArgs a) {
     for (int r = 0; r < 16; ++r)
       if (!wa_sees(a, i0 + acc_row(r, h), kj)) p[r] = 0.f;
   };
-  if (part.begin < part.end) {
-    load(part.begin);
-    store(0);
-  }
-  lds_barrier();
   for (int t = part.begin; t < part.end; ++t) {
-    const int cur = (t - part.begin) & 1, i0 = row_of(t);
-    const bool has_next = t + 1 < part.end;
-    if (has_next) load(t + 1);
-    if (kw < a.T && wa_any(a, i0, kw)) {
-      f32x16 s = half_rows<DP>(qs[cur], kp, lr, h);
-      sched_fence();
-      f32x16 x;
-      float top = 0.f;
+    const int cur = (t - part.begin) & 1, i0 = here.tile * kTile;
+    const int64_t at = (int64_t)here.head * a.tiles + here.tile;
+    here = next_of(here);
+    wait_vm_lgkm0<0>();
+    ring_barrier();
+    if (t + 1 < part.end) stage(here, cur ^ 1);
+    if (kw >= a.T || !wa_any(a, i0, kw)) continue;
+    const uint32_t qt = a.qd_top[2 * at], ot = a.qd_top[2 * at + 1];
+    held |= qt | ot;
+    const char* dos = qd[cur] + Tile::kBytes;
+    const float qfac = row_factor(top_bits(qt)), ofac = row_factor(top_bits(ot)), cs = kf * qfac, cd = vf * ofac;
+    f32x16 s = half_rows<DP>(qd[cur], kp, lr, h);
+    sched_fence();
+    float top = 0.f;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 q4 = row_values(qf[cur], g, h), l4 = row_values(ls[cur], g, h);
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 l4 = row_values(stats[cur], g, h);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * g + e;
-          s[r] = key_ok ? fast_exp2(s[r] * q4[e] * kf - l4[e]) : 0.f;
-        }
-      }
-      hide(s, i0);
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 o4 = row_values(df[cur], g, h);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * g + e;
-          x[r] = s[r] * o4[e];
-          top = fmaxf(top, x[r]);
-        }
-      }
-      fit_v.follow(top, dv, key_bad);
-      half_cols<DP>(dos[cur], x, fit_v.f, 0, lane, dv);
-      half_cols<DP>(dos[cur], x, fit_v.f, 1, lane, dv);
-      x = half_rows<DP>(dos[cur], vp, lr, h);
-      sched_fence();
-      top = 0.f;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 q4 = row_values(qf[cur], g, h), o4 = row_values(df[cur], g, h), d4 = row_values(ds[cur], g, h);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * g + e;
-          // P before Q's scale: dP - D is finite for all rows that are held, its product with that need not be
-          x[r] = s[r] * (x[r] * o4[e] * vf - d4[e]) * q4[e];
-        }
-      }
-      hide(x, i0);  // where D is not finite
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(x[r]));
-      fit_k.follow(top, dk, key_bad);
-      half_cols<DP>(qs[cur], x, fit_k.f, 0, lane, dk);
-      half_cols<DP>(qs[cur], x, fit_k.f, 1, lane, dk);
+      for (int e = 0; e < 4; ++e) s[4 * g + e] = fast_exp2(fmaf(s[4 * g + e], cs, -l4[e]));
     }
-    if (has_next) store(cur ^ 1);
-    lds_barrier();
+    hide(s, i0);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+    fit_v.follow(top * ofac, dv, key_bad);
+    float f = fminf(fit_v.f * ofac, 0x1p126f);
+    half_cols<DP>(dos, s, f, 0, lane, dv);
+    half_cols<DP>(dos, s, f, 1, lane, dv);
+    f32x16 x = half_rows<DP>(dos, vp, lr, h);
+    sched_fence();
+    top = 0.f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 d4 = row_values(stats[cur] + kTile, g, h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * g + e] = s[4 * g + e] * fmaf(x[4 * g + e], cd, -d4[e]);
+    }
+    hide(x, i0);  // where D is not finite
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(x[r]));
+    fit_k.follow(top * qfac, dk, key_bad);
+    f = fminf(fit_k.f * qfac, 0x1p126f);
+    half_cols<DP>(qd[cur], x, f, 0, lane, dk);
+    half_cols<DP>(qd[cur], x, f, 1, lane, dk);
   }
   fit_v.undo(dv);
   fit_k.undo(dk);
 
-  if (bad) not_held = 1;
-  __syncthreads();
-  if (kw < a.T && part.begin < part.end && __any(key_bad || not_held)) {
+  if (kw < a.T && part.begin < part.end && __any(key_bad || (held & 1))) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) dk[b] = dv[b] = zero16();
     for (int t = part.begin; t < part.end; ++t) {
-      const int i0 = row_of(t), bh = head0 + t / part.count;
+      const Place p = place_of(t);
+      const int i0 = p.tile * kTile, bh = p.head;
       if (!wa_any(a, i0, kw)) continue;
       const float* Qh = wa_head(a.q, a, bh);
       const float* dOh = wa_head(a.dout, a, bh);
+      const int64_t stat = (int64_t)bh * a.tiles * kTile;
       const bool mine = i0 + lr < a.T;
       f32x16 s = zero16(), dp = zero16();
       for (int c = 0; c < a.d; c += 2) {
@@ -566,9 +619,8 @@ window_bwd_dkdv_kernel(const WaArgs a) {
       for (int r = 0; r < 16; ++r) {
         const int i = i0 + acc_row(r, h);
         const bool sees = key_ok && i < a.T && wa_sees(a, i, kj);
-        const int64_t at = (int64_t)bh * a.T + (i < a.T ? i : 0);
-        s[r] = sees ? fast_exp2(s[r] - a.lse[at] * kLog2e) : 0.f;
-        dp[r] = sees ? s[r] * (dp[r] - a.D[at]) : 0.f;
+        s[r] = sees ? fast_exp2(s[r] - a.l2[stat + i]) : 0.f;
+        dp[r] = sees ? s[r] * (dp[r] - a.D[stat + i]) : 0.f;
       }
 #pragma unroll
       for (int st = 0; st < 16; ++st) {
@@ -587,37 +639,36 @@ window_bwd_dkdv_kernel(const WaArgs a) {
     }
   }
   if (!key_ok) return;
-  if (part.parts > 1) {
-    const int64_t at = (part.slot * kBlock + wave * kTile + lr) * DP;
-    wa_store<DP, true>(a.dk_part + at, dk, a.scale, DP, h);
-    wa_store<DP, true>(a.dv_part + at, dv, 1.0f, DP, h);
-  } else {
+  if (WAVES == 4) {
     wa_store<DP, VEC>(wa_kv_head(a.dk, a, bhk) + (int64_t)kj * a.dk.st, dk, a.scale, a.d, h);
     wa_store<DP, VEC>(wa_kv_head(a.dv, a, bhk) + (int64_t)kj * a.dv.st, dv, 1.0f, a.d, h);
+  } else {
+    const int64_t at = (((int64_t)bhk * a.sink_tiles * a.far_parts + item) * kTile + lr) * DP;
+    wa_store<DP, true>(a.dk_part + at, dk, a.scale, DP, h);
+    wa_store<DP, true>(a.dv_part + at, dv, 1.0f, DP, h);
   }
 }
 
-// The parts of dK and dV of the first `rows` keys of every head, summed in order.
+// The sinks' dK and dV: their far queries' parts, in order, on top of the near ones' sums.
 template <int DP, bool VEC>
 __global__ void __launch_bounds__(256)
-window_bwd_sum_kernel(const WaArgs a, int first, int rows) {
+window_bwd_sum_kernel(const WaArgs a) {
   constexpr int kLanes = DP / 4;
   const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x, item = u / kLanes;
-  const int c = (int)(u % kLanes) * 4, bhk = (int)(item / rows), key = first + (int)(item % rows);
+  const int c = (int)(u % kLanes) * 4, bhk = (int)(item / a.S), key = (int)(item % a.S);
   if (bhk >= a.BHkv || c >= a.d) return;
-  const int kb = key / kBlock;
-  const bool sink = kb < a.sink_blocks;
-  const WaPart part(a, bhk, sink ? kb * a.sink_parts : a.sink_blocks * a.sink_parts + (kb - a.sink_blocks) * a.parts);
-  const int parts = (a.G * part.count + a.chunk - 1) / a.chunk;
-  const int64_t at = (part.slot * kBlock + key % kBlock) * DP + c;
-  f32x4 dk = *reinterpret_cast<const f32x4*>(a.dk_part + at), dv = *reinterpret_cast<const f32x4*>(a.dv_part + at);
+  const int64_t at =
+      (((int64_t)bhk * a.sink_tiles + key / kTile) * a.far_parts * kTile + key % kTile) * DP + c;
+  float* ok = wa_kv_head(a.dk, a, bhk) + (int64_t)key * a.dk.st + c;
+  float* ov = wa_kv_head(a.dv, a, bhk) + (int64_t)key * a.dv.st + c;
+  f32x4 dk = load4<VEC>(ok, a.d - c), dv = load4<VEC>(ov, a.d - c);
 #pragma unroll 4
-  for (int p = 1; p < parts; ++p) {
-    dk += *reinterpret_cast<const f32x4*>(a.dk_part + at + (int64_t)p * kBlock * DP);
-    dv += *reinterpret_cast<const f32x4*>(a.dv_part + at + (int64_t)p * kBlock * DP);
+  for (int p = 0; p < a.far_parts; ++p) {
+    dk += *reinterpret_cast<const f32x4*>(a.dk_part + at + (int64_t)p * kTile * DP);
+    dv += *reinterpret_cast<const f32x4*>(a.dv_part + at + (int64_t)p * kTile * DP);
   }
-  store4<VEC>(wa_kv_head(a.dk, a, bhk) + (int64_t)key * a.dk.st + c, dk, a.d - c);
-  store4<VEC>(wa_kv_head(a.dv, a, bhk) + (int64_t)key * a.dv.st + c, dv, a.d - c);
+  store4<VEC>(ok, dk, a.d - c);
+  store4<VEC>(ov, dv, a.d - c);
 }
 
 // ------------------------------------------------------------------ host side
@@ -628,8 +679,8 @@ int wa_check(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t d, int64_t wi
   if (B < 0 || H < 0 || Hkv < 0 || T < 0 || d <= 0 || d > 128 || window < 1 || sinks < 0) return AAR_EINVAL;
   if ((H == 0) != (Hkv == 0) || (H > 0 && H % Hkv != 0)) return AAR_EINVAL;
   if (B > (1 << 20) || H > (1 << 20) || T > (1 << 24)) return AAR_EUNSUPPORTED;
-  // a dispatch holds its work items in 32 bits
-  if (B * H * ceil_div(T, kBlock) >= (1 << 24) || B * H * T > (int64_t)UINT32_MAX / 32) return AAR_EUNSUPPORTED;
+  // a dispatch holds its work items in 32 bits: two tiles of 256 threads for 32 keys
+  if (B * H * ceil_div(T, kBlock) >= (1 << 20) || B * H * T > (int64_t)UINT32_MAX / 64) return AAR_EUNSUPPORTED;
   return AAR_OK;
 }
 
@@ -644,32 +695,52 @@ WaArgs wa_args(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t d, int64_t 
   a.BHkv = (int)(B * Hkv);
   a.W = (int)std::min(window, T);
   a.S = (int)std::min(sinks, T);
+  a.tiles = (int)ceil_div(T, kTile);
   a.scale = scale;
   a.scale_log2 = scale * kLog2e;
   return a;
 }
 
-// Parts of dK's and dV's query tiles.
+// Parts of the sinks' far queries: where the block that holds the first sinks would have
+// a list more than twice as long as the others', for up to 64 tiles of sinks.
 void wa_bwd_plan(WaArgs& a) {
-  const int blocks = (int)ceil_div(a.T, kBlock), all = (int)ceil_div(a.T, kTile);
-  const int near = (int)std::min<int64_t>(all, ceil_div(kBlock + (int64_t)a.W - 1, kTile) + 1);
-  a.sink_blocks = (int)std::min<int64_t>(ceil_div(a.S, kBlock), blocks);
-  // at most 64 parts of the sinks' blocks in all, each as long as another block's list at least
-  a.chunk = std::max(a.G * near, (int)ceil_div((int64_t)a.G * all, std::max(1, 64 / std::max(1, a.sink_blocks))));
-  a.parts = 1;
-  a.sink_parts = (int)ceil_div((int64_t)a.G * all, a.chunk);
+  const int64_t near = std::min<int64_t>(a.T - 1, kBlock - 1 + (int64_t)a.W - 1) / kTile + 1, far = a.tiles - near;
+  a.sink_tiles = (int)ceil_div(a.S, kTile);
+  a.far_parts = a.far_chunk = 0;
+  if (a.sink_tiles == 0 || a.sink_tiles > 64 || far <= near) return;
+  // two waves a SIMD
+  const int64_t waves = 8 * device_cu_count(), all = (int64_t)a.BHkv * a.sink_tiles * a.G * far;
+  a.far_chunk = (int)std::max<int64_t>(8, ceil_div(all, waves));
+  a.far_parts = (int)ceil_div(a.G * far, (int64_t)a.far_chunk);
 }
 
-int64_t wa_items(const WaArgs& a) {
-  return (int64_t)a.sink_blocks * a.sink_parts + (ceil_div(a.T, kBlock) - a.sink_blocks) * a.parts;
+// Where the workspace holds item i: K's and V's planes and exponents, then for the
+// backward Q's and dO's, l2, D, and the parts of dK and dV; `most`: its end.
+size_t wa_bytes(const WaArgs& a, int i) {
+  const size_t pair = 2 * (wa_dim(a.d) == 64 ? HalfTile<64>::kBytes : HalfTile<128>::kBytes);
+  const size_t kv = (size_t)a.BHkv * a.tiles, q = (size_t)a.BH * a.tiles;
+  const size_t part = (size_t)a.BHkv * a.sink_tiles * a.far_parts * kTile * wa_dim(a.d) * sizeof(float);
+  const size_t size[8] = {kv * pair, kv * 8, q * pair, q * 8, q * kTile * sizeof(float), q * kTile * sizeof(float), part, part};
+  size_t at = 0;
+  for (int k = 0; k < i; ++k) at += (size[k] + 15) / 16 * 16;
+  return at;
 }
-bool wa_split(const WaArgs& a) { return a.parts > 1 || (a.sink_blocks > 0 && a.sink_parts > 1); }
+constexpr int kWaFwd = 2, kWaBwd = 8;
 
-// D, then the parts of dK and of dV.
-size_t wa_part_bytes(const WaArgs& a) {
-  return wa_split(a) ? (size_t)a.BHkv * wa_items(a) * kBlock * wa_dim(a.d) * sizeof(float) : 0;
+bool wa_workspace(WaArgs& a, void* workspace, size_t bytes, int items) {
+  if (!workspace || !aligned16(workspace) || bytes < wa_bytes(a, items)) return false;
+  char* ws = static_cast<char*>(workspace);
+  a.kv_img = ws;
+  a.kv_top = reinterpret_cast<uint32_t*>(ws + wa_bytes(a, 1));
+  if (items == kWaFwd) return true;
+  a.qd_img = ws + wa_bytes(a, 2);
+  a.qd_top = reinterpret_cast<uint32_t*>(ws + wa_bytes(a, 3));
+  a.l2 = reinterpret_cast<float*>(ws + wa_bytes(a, 4));
+  a.D = reinterpret_cast<float*>(ws + wa_bytes(a, 5));
+  a.dk_part = reinterpret_cast<float*>(ws + wa_bytes(a, 6));
+  a.dv_part = reinterpret_cast<float*>(ws + wa_bytes(a, 7));
+  return true;
 }
-size_t wa_d_bytes(const WaArgs& a) { return ((size_t)a.BH * a.T * sizeof(float) + 15) / 16 * 16; }
 
 // Row strides whose tiles' offsets fit, and whose rows do not overlap.
 bool wa_rows_ok(const int64_t* strides, std::initializer_list<int> operands, int64_t T, int64_t d) {
@@ -694,22 +765,31 @@ FaOut wa_out(float* p, const int64_t* s) { return FaOut{p, s[0], s[1], s[2]}; }
 
 template <int DP, bool VEC>
 int launch_fwd(const WaArgs& a, hipStream_t st) {
+  window_split_kernel<DP, VEC><<<dim3((unsigned)(2 * a.BHkv * (int64_t)a.tiles)), dim3(kFaThreads), 0, st>>>(a);
+  const int rc = launch_status();
+  if (rc != AAR_OK) return rc;
   window_fwd_kernel<DP, VEC><<<dim3((unsigned)(ceil_div(a.T, kBlock) * a.BH)), dim3(kFaThreads), 0, st>>>(a);
   return launch_status();
 }
 
 template <int DP, bool VEC>
 int launch_bwd(const WaArgs& a, hipStream_t st) {
-  window_bwd_dq_kernel<DP, VEC><<<dim3((unsigned)(ceil_div(a.T, kBlock) * a.BH)), dim3(kFaThreads), 0, st>>>(a);
+  const int64_t blocks = ceil_div(a.T, kBlock);
+  window_split_kernel<DP, VEC><<<dim3((unsigned)(2 * a.BHkv * (int64_t)a.tiles)), dim3(kFaThreads), 0, st>>>(a);
   int rc = launch_status();
   if (rc != AAR_OK) return rc;
-  window_bwd_dkdv_kernel<DP, VEC><<<dim3((unsigned)(wa_items(a) * a.BHkv)), dim3(kFaThreads), 0, st>>>(a);
+  window_bwd_dq_kernel<DP, VEC><<<dim3((unsigned)(blocks * a.BH)), dim3(kFaThreads), 0, st>>>(a);
   rc = launch_status();
-  if (rc != AAR_OK || !wa_split(a)) return rc;
-  const int first = a.sink_blocks > 0 && a.sink_parts > 1 ? 0 : a.sink_blocks * kBlock;
-  const int last = a.parts > 1 ? a.T : std::min(a.T, a.sink_blocks * kBlock), rows = last - first;
-  const int64_t units = (int64_t)a.BHkv * rows * (DP / 4);
-  window_bwd_sum_kernel<DP, VEC><<<dim3((unsigned)ceil_div(units, 256)), dim3(256), 0, st>>>(a, first, rows);
+  if (rc != AAR_OK) return rc;
+  window_bwd_dkdv_kernel<DP, VEC, 4><<<dim3((unsigned)(blocks * a.BHkv)), dim3(kFaThreads), 0, st>>>(a);
+  rc = launch_status();
+  if (rc != AAR_OK || a.far_parts == 0) return rc;
+  const int64_t far = (int64_t)a.BHkv * a.sink_tiles * a.far_parts;
+  window_bwd_dkdv_kernel<DP, VEC, 1><<<dim3((unsigned)far), dim3(kWave), 0, st>>>(a);
+  rc = launch_status();
+  if (rc != AAR_OK) return rc;
+  const int64_t units = (int64_t)a.BHkv * a.S * (DP / 4);
+  window_bwd_sum_kernel<DP, VEC><<<dim3((unsigned)ceil_div(units, 256)), dim3(256), 0, st>>>(a);
   return launch_status();
 }
 
@@ -722,20 +802,20 @@ extern "C" {
 
 size_t aar_window_attn_fwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t d, int64_t window,
                                            int64_t sinks) {
-  (void)B, (void)H, (void)Hkv, (void)T, (void)d, (void)window, (void)sinks;
-  return 0;
+  if (wa_check(B, H, Hkv, T, d, window, sinks) != AAR_OK || B == 0 || H == 0 || T == 0) return 0;
+  return wa_bytes(wa_args(B, H, Hkv, T, d, window, sinks, 1.0f), kWaFwd);
 }
 
 int aar_window_attn_fwd_f32(const float* q, const float* k, const float* v, float* o, float* lse, int64_t B, int64_t H,
                             int64_t Hkv, int64_t T, int64_t d, const int64_t* strides, int64_t window, int64_t sinks,
                             float scale, void* workspace, size_t workspace_bytes, void* stream) {
-  (void)workspace, (void)workspace_bytes;
   const int rc = wa_check(B, H, Hkv, T, d, window, sinks);
   if (rc != AAR_OK) return rc;
   if (B == 0 || H == 0 || T == 0) return AAR_OK;
   if (!q || !k || !v || !o || !lse || !strides) return AAR_EINVAL;
   if (!wa_rows_ok(strides, {0, 1, 2}, T, d)) return AAR_EUNSUPPORTED;
   WaArgs a = wa_args(B, H, Hkv, T, d, window, sinks, scale);
+  if (!wa_workspace(a, workspace, workspace_bytes, kWaFwd)) return AAR_EWORKSPACE;
   a.lse = lse;
   a.q = wa_in(q, strides, T, d);
   a.k = wa_in(k, strides + 3, T, d);
@@ -752,7 +832,7 @@ size_t aar_window_attn_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, in
   if (wa_check(B, H, Hkv, T, d, window, sinks) != AAR_OK || B == 0 || H == 0 || T == 0) return 0;
   WaArgs a = wa_args(B, H, Hkv, T, d, window, sinks, 1.0f);
   wa_bwd_plan(a);
-  return wa_d_bytes(a) + 2 * wa_part_bytes(a);
+  return wa_bytes(a, kWaBwd);
 }
 
 int aar_window_attn_bwd_f32(const float* q, const float* k, const float* v, const float* o, const float* lse,
@@ -763,19 +843,15 @@ int aar_window_attn_bwd_f32(const float* q, const float* k, const float* v, cons
   if (rc != AAR_OK) return rc;
   if (B == 0 || H == 0 || T == 0) return AAR_OK;
   if (!q || !k || !v || !o || !lse || !dout || !dq || !dk || !dv || !strides) return AAR_EINVAL;
-  if (!wa_rows_ok(strides, {0, 1, 2, 4}, T, d)) return AAR_EUNSUPPORTED;
+  if (!wa_rows_ok(strides, {0, 1, 2, 3, 4}, T, d)) return AAR_EUNSUPPORTED;
   WaArgs a = wa_args(B, H, Hkv, T, d, window, sinks, scale);
   wa_bwd_plan(a);
-  if (!workspace || !aligned16(workspace) || workspace_bytes < wa_d_bytes(a) + 2 * wa_part_bytes(a)) return AAR_EWORKSPACE;
-  char* ws = static_cast<char*>(workspace);
-  a.D = reinterpret_cast<float*>(ws);
-  a.dk_part = reinterpret_cast<float*>(ws + wa_d_bytes(a));
-  a.dv_part = reinterpret_cast<float*>(ws + wa_d_bytes(a) + wa_part_bytes(a));
+  if (!wa_workspace(a, workspace, workspace_bytes, kWaBwd)) return AAR_EWORKSPACE;
   a.lse = const_cast<float*>(lse);
   a.q = wa_in(q, strides, T, d);
   a.k = wa_in(k, strides + 3, T, d);
   a.v = wa_in(v, strides + 6, T, d);
-  a.o_in = FaIn{o, strides[9], strides[10], strides[11]};
+  a.o_in = wa_in(o, strides + 9, T, d);
   a.dout = wa_in(dout, strides + 12, T, d);
   a.dq = wa_out(dq, strides + 15);
   a.dk = wa_out(dk, strides + 18);

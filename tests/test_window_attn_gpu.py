@@ -76,7 +76,9 @@ def test_a_window_of_everything_is_causal_attention(L):
     # and one token's window its own value
     o, lse, dq, dk, dv = K.window_run(L, q, k, v, do, 1, 0)
     M.near(o, v, 2 * M.U + 2.0 ** -22, "o")
-    M.near(dv, do, 2 * M.U + 2.0 ** -22, "dv")
+    # P = 2^(s - lse) there: lse, its product with log2(e) and the difference's operands are
+    # each rounded, half a step of at most |lse| log2(e) <= 1.5 |lse|, and 2^x moves by less than x
+    M.near(dv, do, 2 * M.U + 2.0 ** -22 + 3 * M.U * 1.5 * lse.abs().max().item(), "dv")
 
 
 @pytest.mark.parametrize("d", [64, 128, 36])
