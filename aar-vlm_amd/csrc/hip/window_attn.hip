@@ -207,28 +207,46 @@ __device__ __forceinline__ uint32_t split_rows(const float* p, int d, int lr, in
   return t;
 }
 
-// A pair of planes from HBM into LDS: 1024 bytes a wave and DMA.
-template <int DP, int WAVES = 4>
+// A pair of planes from HBM into LDS: 1024 bytes a wave and DMA, as many DMAs for every
+// wave (the last ones of some move the same bytes again).
+template <int DP, int WAVES>
+constexpr int kStageDmas = (2 * HalfTile<DP>::kBytes / 1024 + WAVES - 1) / WAVES;
+template <int DP, int WAVES>
 __device__ __forceinline__ void stage_pair(const char* src, char* lds, int wave, int lane) {
   constexpr int n = 2 * HalfTile<DP>::kBytes / 1024;
   static_assert(n * 1024 == 2 * HalfTile<DP>::kBytes, "whole DMAs");
 #pragma unroll
-  for (int k = 0; k < (n + WAVES - 1) / WAVES; ++k) {
-    const int i = wave + WAVES * k;
-    if (i < n) dma16_untracked_s(lane * 16 + i * 1024, src, (lds_void_t*)(lds + i * 1024));
+  for (int k = 0; k < kStageDmas<DP, WAVES>; ++k) {
+    const int i = min(wave + WAVES * k, n - 1);
+    dma16_untracked_s(lane * 16 + i * 1024, src, (lds_void_t*)(lds + i * 1024));
   }
+}
+
+// Stages of the rings that tiles arrive in: two where the grid fills the GPU, and where a
+// CU has one workgroup at most as many as its LDS holds, so that the first tiles of a
+// short list are all on their way at once.
+constexpr int wa_deep(int dp) { return dp == 64 ? 7 : 4; }
+
+// Until the next tile of a ring has arrived, with `behind` tiles of `dmas` DMAs a wave sent
+// for after it (of fewer than `most`, until all have): and every wave is done with the
+// tile before.
+template <int MOST, int DMAS>
+__device__ __forceinline__ void ring_next(int behind) {
+  if (MOST > 0 && behind >= MOST) wait_vm_lgkm0<MOST * DMAS>();
+  else wait_vm_lgkm0<0>();
+  ring_barrier();
 }
 
 // Forward.  P is formed as 2^(s + v - R + 11), with v the exponent of the tile's values and
 // R, the row's, such that it stays below 2^15: the largest s + v so far, followed only when
 // it is passed by 2^4, so O is rarely rescaled.  So O is sum P V 2^(25 - R), and l is kept
 // as l 2^(-R - 29).
-template <int DP, bool VEC>
-__global__ void __launch_bounds__(kFaThreads, DP == 64 ? 3 : 2)
+template <int DP, bool VEC, int STAGES>
+__global__ void __launch_bounds__(kFaThreads, STAGES > 2 ? 1 : (DP == 64 ? 3 : 2))
 window_fwd_kernel(const WaArgs a) {
   using Tile = HalfTile<DP>;
   constexpr int NB = DP / 32;
-  __shared__ __attribute__((aligned(16))) char kv[2][2 * Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) char kv[STAGES][2 * Tile::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
   const int bh = blockIdx.x % a.BH, qb = blockIdx.x / a.BH, bhk = wa_kv(a, bh);
@@ -238,9 +256,11 @@ window_fwd_kernel(const WaArgs a) {
   const char* img = a.kv_img + (int64_t)bhk * a.tiles * 2 * Tile::kBytes;
   const uint32_t* tops = a.kv_top + (int64_t)bhk * a.tiles * 2;
   auto stage = [&](int t, int buf) {
-    stage_pair<DP>(img + (int64_t)(tiles.key(t) / kTile) * 2 * Tile::kBytes, kv[buf], wave, lane);
+    stage_pair<DP, 4>(img + (int64_t)(tiles.key(t) / kTile) * 2 * Tile::kBytes, kv[buf], wave, lane);
   };
-  stage(0, 0);
+#pragma unroll
+  for (int t = 0; t < STAGES - 1; ++t)
+    if (t < tiles.count) stage(t, t);
 
   u32x4 qp[DP / 16][2];
   bool row_bad = false;
@@ -272,11 +292,12 @@ window_fwd_kernel(const WaArgs a) {
       if (!wa_sees(a, qi, kv0 + acc_row(r, h))) s[r] = -INFINITY;
   };
 
-  for (int t = 0; t < tiles.count; ++t) {
-    const int buf = t & 1, kv0 = tiles.key(t);
-    wait_vm_lgkm0<0>();  // this wave's share of tile t is in LDS, and its reads of t - 1 are done
-    ring_barrier();
-    if (t + 1 < tiles.count) stage(t + 1, buf ^ 1);
+  for (int t = 0, buf = -1, to = STAGES - 2; t < tiles.count; ++t) {
+    const int kv0 = tiles.key(t);
+    buf = buf + 1 < STAGES ? buf + 1 : 0;
+    to = to + 1 < STAGES ? to + 1 : 0;
+    ring_next<STAGES - 2, kStageDmas<DP, 4>>(tiles.count - 1 - t);
+    if (t + STAGES - 1 < tiles.count) stage(t + STAGES - 1, to);
     if (w0 >= a.T || !wa_any(a, w0, kv0)) continue;
     const uint32_t kt = tops[kv0 / kTile * 2], vt = tops[kv0 / kTile * 2 + 1];
     held |= kt | vt;
@@ -348,12 +369,12 @@ window_fwd_kernel(const WaArgs a) {
 }
 
 // dQ, and what dK's and dV's pass reads of a query row: the planes of Q and dO, D and lse.
-template <int DP, bool VEC>
-__global__ void __launch_bounds__(kFaThreads, DP == 64 ? 2 : 1)
+template <int DP, bool VEC, int STAGES>
+__global__ void __launch_bounds__(kFaThreads, STAGES == 2 && DP == 64 ? 2 : 1)
 window_bwd_dq_kernel(const WaArgs a) {
   constexpr int NB = DP / 32;
   using Tile = HalfTile<DP>;
-  __shared__ __attribute__((aligned(16))) char kv[2][2 * Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) char kv[STAGES][2 * Tile::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
   const int bh = blockIdx.x % a.BH, qb = blockIdx.x / a.BH, bhk = wa_kv(a, bh);
@@ -365,9 +386,11 @@ window_bwd_dq_kernel(const WaArgs a) {
   const char* img = a.kv_img + (int64_t)bhk * a.tiles * 2 * Tile::kBytes;
   const uint32_t* tops = a.kv_top + (int64_t)bhk * a.tiles * 2;
   auto stage = [&](int t, int buf) {
-    stage_pair<DP>(img + (int64_t)(tiles.key(t) / kTile) * 2 * Tile::kBytes, kv[buf], wave, lane);
+    stage_pair<DP, 4>(img + (int64_t)(tiles.key(t) / kTile) * 2 * Tile::kBytes, kv[buf], wave, lane);
   };
-  stage(0, 0);
+#pragma unroll
+  for (int t = 0; t < STAGES - 1; ++t)
+    if (t < tiles.count) stage(t, t);
 
   float l2 = INFINITY, dsum = 0.f;
   u32x4 qp[DP / 16][2], dop[DP / 16][2];
@@ -412,11 +435,12 @@ window_bwd_dq_kernel(const WaArgs a) {
     for (int r = 0; r < 16; ++r)
       if (!wa_sees(a, qi, kv0 + acc_row(r, h))) x[r] = 0.f;
   };
-  for (int t = 0; t < tiles.count; ++t) {
-    const int buf = t & 1, kv0 = tiles.key(t);
-    wait_vm_lgkm0<0>();
-    ring_barrier();
-    if (t + 1 < tiles.count) stage(t + 1, buf ^ 1);
+  for (int t = 0, buf = -1, to = STAGES - 2; t < tiles.count; ++t) {
+    const int kv0 = tiles.key(t);
+    buf = buf + 1 < STAGES ? buf + 1 : 0;
+    to = to + 1 < STAGES ? to + 1 : 0;
+    ring_next<STAGES - 2, kStageDmas<DP, 4>>(tiles.count - 1 - t);
+    if (t + STAGES - 1 < tiles.count) stage(t + STAGES - 1, to);
     if (w0 >= a.T || !wa_any(a, w0, kv0)) continue;
     const uint32_t kt = tops[kv0 / kTile * 2], vt = tops[kv0 / kTile * 2 + 1];
     held |= kt | vt;
@@ -499,13 +523,13 @@ struct WaList {
 };
 
 // dK and dV: a wave takes 32 keys, a lane its key, and walks its workgroup's list.
-template <int DP, bool VEC, int WAVES>
-__global__ void __launch_bounds__(WAVES * kWave, DP == 64 ? 2 : 1)
+template <int DP, bool VEC, int WAVES, int STAGES>
+__global__ void __launch_bounds__(WAVES * kWave, STAGES == 2 && DP == 64 ? 2 : 1)
 window_bwd_dkdv_kernel(const WaArgs a) {
   constexpr int NB = DP / 32;
   using Tile = HalfTile<DP>;
-  __shared__ __attribute__((aligned(16))) char qd[2][2 * Tile::kBytes];
-  __shared__ __attribute__((aligned(16))) float stats[2][2 * kTile];  // lse in log2, D
+  __shared__ __attribute__((aligned(16))) char qd[STAGES][2 * Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) float stats[STAGES][2 * kTile];  // lse in log2, D
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
   const int bhk = blockIdx.x % a.BHkv, item = blockIdx.x / a.BHkv;
@@ -528,10 +552,15 @@ window_bwd_dkdv_kernel(const WaArgs a) {
     // the same in all lanes, which the compiler does not see through the loop
     const int64_t at = (int64_t)__builtin_amdgcn_readfirstlane(p.head) * a.tiles + __builtin_amdgcn_readfirstlane(p.tile);
     stage_pair<DP, WAVES>(a.qd_img + at * 2 * Tile::kBytes, qd[buf], wave, lane);
-    if (wave == WAVES - 1) dma4_untracked((lane < kTile ? a.l2 : a.D) + at * kTile + lr, (lds_void_t*)stats[buf]);
+    dma4_untracked((lane < kTile ? a.l2 : a.D) + at * kTile + lr, (lds_void_t*)stats[buf]);
   };
-  Place here = part.begin < part.end ? place_of(part.begin) : Place{head0, part.first};
-  if (part.begin < part.end) stage(here, 0);
+  Place here = part.begin < part.end ? place_of(part.begin) : Place{head0, part.first}, ahead = here;
+#pragma unroll
+  for (int n = 0; n < STAGES - 1; ++n) {
+    if (part.begin + n >= part.end) break;
+    stage(ahead, n);
+    ahead = next_of(ahead);
+  }
 
   u32x4 kp[DP / 16][2], vp[DP / 16][2];
   bool key_bad = false;
@@ -550,13 +579,17 @@ window_bwd_dkdv_kernel(const WaArgs a) {
     for (int r = 0; r < 16; ++r)
       if (!wa_sees(a, i0 + acc_row(r, h), kj)) p[r] = 0.f;
   };
-  for (int t = part.begin; t < part.end; ++t) {
-    const int cur = (t - part.begin) & 1, i0 = here.tile * kTile;
+  for (int t = part.begin, cur = -1, to = STAGES - 2; t < part.end; ++t) {
+    const int i0 = here.tile * kTile;
     const int64_t at = (int64_t)here.head * a.tiles + here.tile;
     here = next_of(here);
-    wait_vm_lgkm0<0>();
-    ring_barrier();
-    if (t + 1 < part.end) stage(here, cur ^ 1);
+    cur = cur + 1 < STAGES ? cur + 1 : 0;
+    to = to + 1 < STAGES ? to + 1 : 0;
+    ring_next<STAGES - 2, kStageDmas<DP, WAVES> + 1>(part.end - 1 - t);
+    if (t + STAGES - 1 < part.end) {
+      stage(ahead, to);
+      ahead = next_of(ahead);
+    }
     if (kw >= a.T || !wa_any(a, i0, kw)) continue;
     const uint32_t qt = a.qd_top[2 * at], ot = a.qd_top[2 * at + 1];
     held |= qt | ot;
@@ -649,23 +682,35 @@ window_bwd_dkdv_kernel(const WaArgs a) {
   }
 }
 
-// The sinks' dK and dV: their far queries' parts, in order, on top of the near ones' sums.
+// The sinks' dK and dV: their far queries' parts, in an order of their own, on top of the
+// near ones' sums.  A workgroup takes a key, 256 / (DP / 4) groups of its threads parts in
+// turn.
 template <int DP, bool VEC>
 __global__ void __launch_bounds__(256)
 window_bwd_sum_kernel(const WaArgs a) {
-  constexpr int kLanes = DP / 4;
-  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x, item = u / kLanes;
-  const int c = (int)(u % kLanes) * 4, bhk = (int)(item / a.S), key = (int)(item % a.S);
-  if (bhk >= a.BHkv || c >= a.d) return;
-  const int64_t at =
-      (((int64_t)bhk * a.sink_tiles + key / kTile) * a.far_parts * kTile + key % kTile) * DP + c;
-  float* ok = wa_kv_head(a.dk, a, bhk) + (int64_t)key * a.dk.st + c;
-  float* ov = wa_kv_head(a.dv, a, bhk) + (int64_t)key * a.dv.st + c;
-  f32x4 dk = load4<VEC>(ok, a.d - c), dv = load4<VEC>(ov, a.d - c);
+  constexpr int kLanes = DP / 4, kGroups = 256 / kLanes;
+  __shared__ f32x4 sk[kGroups][kLanes], sv[kGroups][kLanes];
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, c = 4 * lane;
+  const int bhk = blockIdx.x / a.S, key = blockIdx.x % a.S;
+  const int64_t at = (((int64_t)bhk * a.sink_tiles + key / kTile) * a.far_parts * kTile + key % kTile) * DP + c;
+  f32x4 dk = {0.f, 0.f, 0.f, 0.f}, dv = dk;
 #pragma unroll 4
-  for (int p = 0; p < a.far_parts; ++p) {
+  for (int p = group; p < a.far_parts; p += kGroups) {
     dk += *reinterpret_cast<const f32x4*>(a.dk_part + at + (int64_t)p * kTile * DP);
     dv += *reinterpret_cast<const f32x4*>(a.dv_part + at + (int64_t)p * kTile * DP);
+  }
+  sk[group][lane] = dk;
+  sv[group][lane] = dv;
+  __syncthreads();
+  if (group != 0 || c >= a.d) return;
+  float* ok = wa_kv_head(a.dk, a, bhk) + (int64_t)key * a.dk.st + c;
+  float* ov = wa_kv_head(a.dv, a, bhk) + (int64_t)key * a.dv.st + c;
+  dk = load4<VEC>(ok, a.d - c);
+  dv = load4<VEC>(ov, a.d - c);
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    dk += sk[g][lane];
+    dv += sv[g][lane];
   }
   store4<VEC>(ok, dk, a.d - c);
   store4<VEC>(ov, dv, a.d - c);
@@ -708,8 +753,8 @@ void wa_bwd_plan(WaArgs& a) {
   a.sink_tiles = (int)ceil_div(a.S, kTile);
   a.far_parts = a.far_chunk = 0;
   if (a.sink_tiles == 0 || a.sink_tiles > 64 || far <= near) return;
-  // two waves a SIMD
-  const int64_t waves = 8 * device_cu_count(), all = (int64_t)a.BHkv * a.sink_tiles * a.G * far;
+  // a wave a SIMD
+  const int64_t waves = 4 * device_cu_count(), all = (int64_t)a.BHkv * a.sink_tiles * a.G * far;
   a.far_chunk = (int)std::max<int64_t>(8, ceil_div(all, waves));
   a.far_parts = (int)ceil_div(a.G * far, (int64_t)a.far_chunk);
 }
@@ -764,32 +809,40 @@ FaIn wa_in(const float* p, const int64_t* s, int64_t T, int64_t d) { return FaIn
 FaOut wa_out(float* p, const int64_t* s) { return FaOut{p, s[0], s[1], s[2]}; }
 
 template <int DP, bool VEC>
-int launch_fwd(const WaArgs& a, hipStream_t st) {
+int launch_split(const WaArgs& a, hipStream_t st) {
   window_split_kernel<DP, VEC><<<dim3((unsigned)(2 * a.BHkv * (int64_t)a.tiles)), dim3(kFaThreads), 0, st>>>(a);
-  const int rc = launch_status();
+  return launch_status();
+}
+
+template <int DP, bool VEC>
+int launch_fwd(const WaArgs& a, hipStream_t st) {
+  const int rc = launch_split<DP, VEC>(a, st);
   if (rc != AAR_OK) return rc;
-  window_fwd_kernel<DP, VEC><<<dim3((unsigned)(ceil_div(a.T, kBlock) * a.BH)), dim3(kFaThreads), 0, st>>>(a);
+  const dim3 grid((unsigned)(ceil_div(a.T, kBlock) * a.BH)), block(kFaThreads);
+  if ((int)grid.x <= device_cu_count()) window_fwd_kernel<DP, VEC, wa_deep(DP)><<<grid, block, 0, st>>>(a);
+  else window_fwd_kernel<DP, VEC, 2><<<grid, block, 0, st>>>(a);
   return launch_status();
 }
 
 template <int DP, bool VEC>
 int launch_bwd(const WaArgs& a, hipStream_t st) {
-  const int64_t blocks = ceil_div(a.T, kBlock);
-  window_split_kernel<DP, VEC><<<dim3((unsigned)(2 * a.BHkv * (int64_t)a.tiles)), dim3(kFaThreads), 0, st>>>(a);
-  int rc = launch_status();
+  int rc = launch_split<DP, VEC>(a, st);
   if (rc != AAR_OK) return rc;
-  window_bwd_dq_kernel<DP, VEC><<<dim3((unsigned)(blocks * a.BH)), dim3(kFaThreads), 0, st>>>(a);
+  const int64_t blocks = ceil_div(a.T, kBlock);
+  const dim3 rows((unsigned)(blocks * a.BH)), keys((unsigned)(blocks * a.BHkv)), block(kFaThreads);
+  if ((int)rows.x <= device_cu_count()) window_bwd_dq_kernel<DP, VEC, wa_deep(DP)><<<rows, block, 0, st>>>(a);
+  else window_bwd_dq_kernel<DP, VEC, 2><<<rows, block, 0, st>>>(a);
   rc = launch_status();
   if (rc != AAR_OK) return rc;
-  window_bwd_dkdv_kernel<DP, VEC, 4><<<dim3((unsigned)(blocks * a.BHkv)), dim3(kFaThreads), 0, st>>>(a);
+  if ((int)keys.x <= device_cu_count()) window_bwd_dkdv_kernel<DP, VEC, 4, wa_deep(DP)><<<keys, block, 0, st>>>(a);
+  else window_bwd_dkdv_kernel<DP, VEC, 4, 2><<<keys, block, 0, st>>>(a);
   rc = launch_status();
   if (rc != AAR_OK || a.far_parts == 0) return rc;
   const int64_t far = (int64_t)a.BHkv * a.sink_tiles * a.far_parts;
-  window_bwd_dkdv_kernel<DP, VEC, 1><<<dim3((unsigned)far), dim3(kWave), 0, st>>>(a);
+  window_bwd_dkdv_kernel<DP, VEC, 1, 2><<<dim3((unsigned)far), dim3(kWave), 0, st>>>(a);
   rc = launch_status();
   if (rc != AAR_OK) return rc;
-  const int64_t units = (int64_t)a.BHkv * a.S * (DP / 4);
-  window_bwd_sum_kernel<DP, VEC><<<dim3((unsigned)ceil_div(units, 256)), dim3(256), 0, st>>>(a);
+  window_bwd_sum_kernel<DP, VEC><<<dim3((unsigned)((int64_t)a.BHkv * a.S)), dim3(256), 0, st>>>(a);
   return launch_status();
 }
 
