@@ -31,7 +31,6 @@ struct WaArgs {
   FaOut o, dq, dk, dv;
   float* lse;                // [B * H][T]
   char *kv_img, *qd_img;     // [B * Hkv][tiles] pairs of K's and V's planes, [B * H][tiles] of Q's and dO's
-  uint32_t *kv_top, *qd_top;  // the same of their exponents (wa_top)
   float *l2, *D;             // [B * H][32 * tiles] lse in log2 (+inf past T) and dO . O of every query row
   float *dk_part, *dv_part;  // [B * Hkv][sink_tiles][far_parts][32][DP] sums of the sinks' far queries
   int T, d, H, G, Hkv, BH, BHkv;  // BH = B * H query heads, BHkv = B * Hkv
@@ -87,13 +86,19 @@ __device__ __forceinline__ void wa_store(float* row, const f32x16 (&x)[DP / 32],
   }
 }
 
-// A tile's exponent as its planes are scaled by: half_exponent's of its largest element,
+// A tile's exponent, by which its planes are scaled: half_exponent's of its largest element,
 // the lowest bit set where the planes do not hold it (elements that are not finite or
 // out of range, or rows whose largest elements are more than 2^12 apart: a row could
 // lose bits to one that a query does not see).
 __device__ __forceinline__ uint32_t top_bits(uint32_t t) { return t & ~1u; }
 // log2 of row_factor: 2^14 over the scale.
 __device__ __forceinline__ int top_log(uint32_t t) { return (int)(t >> 23) - 126; }
+// It travels with the planes, in the spare bytes of their first row: a load of its own
+// would wait for the DMAs sent before it.
+template <int DP>
+__device__ __forceinline__ uint32_t top_of(const char* planes) {
+  return __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t*>(planes + 2 * DP));
+}
 
 // Scale of a tile's planes from the bits of its rows' largest elements: `hi` the most of
 // them, `lo` the least of those that are not 0.  Sets the lowest bit where these do not
@@ -144,9 +149,8 @@ window_split_kernel(const WaArgs a) {
   __syncthreads();
   const uint32_t top = tile_top(max(max(most[0], most[1]), max(most[2], most[3])),
                                 min(min(least[0], least[1]), min(least[2], least[3])));
-  if (tid == 0) a.kv_top[blockIdx.x] = top;
-
   char* img = a.kv_img + (int64_t)blockIdx.x * Tile::kBytes;
+  if (tid == 0) *reinterpret_cast<uint32_t*>(img + 2 * DP) = top;
   const float m = half_scale(top_bits(top));
 #pragma unroll
   for (int i = 0; i < Tile::kPer; ++i) {
@@ -191,6 +195,7 @@ __device__ __forceinline__ uint32_t split_rows(const float* p, int d, int lr, in
   }
   const uint32_t t = tile_top(hi, lo);
   const float m = half_scale(top_bits(t));
+  if (lr == 0 && h == 0) *reinterpret_cast<uint32_t*>(img + 2 * DP) = t;
   char* to = img + lr * HalfTile<DP>::kRow + 16 * h;
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) {
@@ -254,7 +259,6 @@ window_fwd_kernel(const WaArgs a) {
   const float* Q = qi < a.T ? wa_head(a.q, a, bh) + (int64_t)qi * a.q.st : nullptr;
   const WaTiles tiles(a, q0, min(q0 + kBlock, a.T) - 1);
   const char* img = a.kv_img + (int64_t)bhk * a.tiles * 2 * Tile::kBytes;
-  const uint32_t* tops = a.kv_top + (int64_t)bhk * a.tiles * 2;
   auto stage = [&](int t, int buf) {
     stage_pair<DP, 4>(img + (int64_t)(tiles.key(t) / kTile) * 2 * Tile::kBytes, kv[buf], wave, lane);
   };
@@ -299,7 +303,7 @@ window_fwd_kernel(const WaArgs a) {
     ring_next<STAGES - 2, kStageDmas<DP, 4>>(tiles.count - 1 - t);
     if (t + STAGES - 1 < tiles.count) stage(t + STAGES - 1, to);
     if (w0 >= a.T || !wa_any(a, w0, kv0)) continue;
-    const uint32_t kt = tops[kv0 / kTile * 2], vt = tops[kv0 / kTile * 2 + 1];
+    const uint32_t kt = top_of<DP>(kv[buf]), vt = top_of<DP>(kv[buf] + Tile::kBytes);
     held |= kt | vt;
     f32x16 s = half_rows<DP>(kv[buf], qp, lr, h);
     hide(s, kv0);
@@ -384,7 +388,6 @@ window_bwd_dq_kernel(const WaArgs a) {
   const float* dO = row_ok ? wa_head(a.dout, a, bh) + (int64_t)qi * a.dout.st : nullptr;
   const WaTiles tiles(a, q0, min(q0 + kBlock, a.T) - 1);
   const char* img = a.kv_img + (int64_t)bhk * a.tiles * 2 * Tile::kBytes;
-  const uint32_t* tops = a.kv_top + (int64_t)bhk * a.tiles * 2;
   auto stage = [&](int t, int buf) {
     stage_pair<DP, 4>(img + (int64_t)(tiles.key(t) / kTile) * 2 * Tile::kBytes, kv[buf], wave, lane);
   };
@@ -419,7 +422,6 @@ window_bwd_dq_kernel(const WaArgs a) {
     char* to = a.qd_img + tile * 2 * Tile::kBytes;
     const uint32_t qt = split_rows<DP, VEC>(Q, a.d, lr, h, qp, to);
     const uint32_t ot = split_rows<DP, VEC>(dO, a.d, lr, h, dop, to + Tile::kBytes);
-    if (lane < 2) a.qd_top[2 * tile + lane] = lane ? ot : qt;
     held = qt | ot;
     qf = lane_factor(top_bits(qt)) * a.scale_log2;
     df = lane_factor(top_bits(ot));
@@ -442,7 +444,7 @@ window_bwd_dq_kernel(const WaArgs a) {
     ring_next<STAGES - 2, kStageDmas<DP, 4>>(tiles.count - 1 - t);
     if (t + STAGES - 1 < tiles.count) stage(t + STAGES - 1, to);
     if (w0 >= a.T || !wa_any(a, w0, kv0)) continue;
-    const uint32_t kt = tops[kv0 / kTile * 2], vt = tops[kv0 / kTile * 2 + 1];
+    const uint32_t kt = top_of<DP>(kv[buf]), vt = top_of<DP>(kv[buf] + Tile::kBytes);
     held |= kt | vt;
     const f32x16 s = half_rows<DP>(kv[buf], qp, lr, h);
     f32x16 dp = half_rows<DP>(kv[buf] + Tile::kBytes, dop, lr, h);
@@ -581,7 +583,6 @@ window_bwd_dkdv_kernel(const WaArgs a) {
   };
   for (int t = part.begin, cur = -1, to = STAGES - 2; t < part.end; ++t) {
     const int i0 = here.tile * kTile;
-    const int64_t at = (int64_t)here.head * a.tiles + here.tile;
     here = next_of(here);
     cur = cur + 1 < STAGES ? cur + 1 : 0;
     to = to + 1 < STAGES ? to + 1 : 0;
@@ -591,7 +592,7 @@ window_bwd_dkdv_kernel(const WaArgs a) {
       ahead = next_of(ahead);
     }
     if (kw >= a.T || !wa_any(a, i0, kw)) continue;
-    const uint32_t qt = a.qd_top[2 * at], ot = a.qd_top[2 * at + 1];
+    const uint32_t qt = top_of<DP>(qd[cur]), ot = top_of<DP>(qd[cur] + Tile::kBytes);
     held |= qt | ot;
     const char* dos = qd[cur] + Tile::kBytes;
     const float qfac = row_factor(top_bits(qt)), ofac = row_factor(top_bits(ot)), cs = kf * qfac, cd = vf * ofac;
@@ -759,31 +760,29 @@ void wa_bwd_plan(WaArgs& a) {
   a.far_parts = (int)ceil_div(a.G * far, (int64_t)a.far_chunk);
 }
 
-// Where the workspace holds item i: K's and V's planes and exponents, then for the
-// backward Q's and dO's, l2, D, and the parts of dK and dV; `most`: its end.
+// Where the workspace holds item i: K's and V's planes, then for the backward Q's and
+// dO's, l2, D, and the parts of dK and dV.
 size_t wa_bytes(const WaArgs& a, int i) {
   const size_t pair = 2 * (wa_dim(a.d) == 64 ? HalfTile<64>::kBytes : HalfTile<128>::kBytes);
   const size_t kv = (size_t)a.BHkv * a.tiles, q = (size_t)a.BH * a.tiles;
   const size_t part = (size_t)a.BHkv * a.sink_tiles * a.far_parts * kTile * wa_dim(a.d) * sizeof(float);
-  const size_t size[8] = {kv * pair, kv * 8, q * pair, q * 8, q * kTile * sizeof(float), q * kTile * sizeof(float), part, part};
+  const size_t size[6] = {kv * pair, q * pair, q * kTile * sizeof(float), q * kTile * sizeof(float), part, part};
   size_t at = 0;
   for (int k = 0; k < i; ++k) at += (size[k] + 15) / 16 * 16;
   return at;
 }
-constexpr int kWaFwd = 2, kWaBwd = 8;
+constexpr int kWaFwd = 1, kWaBwd = 6;  // items of a forward and of a backward
 
 bool wa_workspace(WaArgs& a, void* workspace, size_t bytes, int items) {
   if (!workspace || !aligned16(workspace) || bytes < wa_bytes(a, items)) return false;
   char* ws = static_cast<char*>(workspace);
   a.kv_img = ws;
-  a.kv_top = reinterpret_cast<uint32_t*>(ws + wa_bytes(a, 1));
   if (items == kWaFwd) return true;
-  a.qd_img = ws + wa_bytes(a, 2);
-  a.qd_top = reinterpret_cast<uint32_t*>(ws + wa_bytes(a, 3));
-  a.l2 = reinterpret_cast<float*>(ws + wa_bytes(a, 4));
-  a.D = reinterpret_cast<float*>(ws + wa_bytes(a, 5));
-  a.dk_part = reinterpret_cast<float*>(ws + wa_bytes(a, 6));
-  a.dv_part = reinterpret_cast<float*>(ws + wa_bytes(a, 7));
+  a.qd_img = ws + wa_bytes(a, 1);
+  a.l2 = reinterpret_cast<float*>(ws + wa_bytes(a, 2));
+  a.D = reinterpret_cast<float*>(ws + wa_bytes(a, 3));
+  a.dk_part = reinterpret_cast<float*>(ws + wa_bytes(a, 4));
+  a.dv_part = reinterpret_cast<float*>(ws + wa_bytes(a, 5));
   return true;
 }
 
