@@ -265,19 +265,15 @@ __device__ __forceinline__ void half_cols(const char* s, const f32x16& x, float 
   }
 }
 
-// A lane's row (its half's octets of each 16 columns) times f, in parts; returns its
+// A lane's row (its half's octets of each 16 columns), or times f from p, in parts; returns its
 // factor.
-template <int DP, bool VEC = true>
-__device__ __forceinline__ float half_row(const float* p, int d, float f, int h, u32x4 (&out)[DP / 16][2], bool& bad) {
-  f32x4 x[DP / 16][2];
+template <int DP>
+__device__ __forceinline__ float half_row(const f32x4 (&x)[DP / 16][2], u32x4 (&out)[DP / 16][2], bool& bad) {
   float top = 0.f;
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-      const int dd = 16 * c + 8 * h + 4 * g;
-      x[c][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (p && dd < d) x[c][g] = load4<VEC>(p + dd, d - dd) * f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[c][g][e]));
     }
@@ -295,6 +291,20 @@ __device__ __forceinline__ float half_row(const float* p, int d, float f, int h,
     }
   }
   return lane_factor(ex);
+}
+template <int DP, bool VEC = true>
+__device__ __forceinline__ float half_row(const float* p, int d, float f, int h, u32x4 (&out)[DP / 16][2], bool& bad) {
+  f32x4 x[DP / 16][2];
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int dd = 16 * c + 8 * h + 4 * g;
+      x[c][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (p && dd < d) x[c][g] = load4<VEC>(p + dd, d - dd) * f;
+    }
+  }
+  return half_row<DP>(x, out, bad);
 }
 
 // The power of two f = 2^log that a lane's P or dS, times the factors of the other

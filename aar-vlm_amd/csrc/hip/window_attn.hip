@@ -35,6 +35,7 @@ struct WaArgs {
   float *dk_part, *dv_part;  // [B * Hkv][sink_tiles][far_parts][32][DP] sums of the sinks' far queries
   int T, d, H, G, Hkv, BH, BHkv;  // BH = B * H query heads, BHkv = B * Hkv
   int W, S, tiles;                // tiles of 32 rows
+  bool whole;                     // a head's tiles fit in LDS
   int sink_tiles, far_parts, far_chunk;  // dK/dV: key tiles that hold sinks, parts of their far queries (0: none), tiles of one
   float scale, scale_log2;
 };
@@ -168,19 +169,58 @@ window_split_kernel(const WaArgs a) {
   }
 }
 
-// A wave's 32 rows (a lane its half's octets of each 16 columns; zeros without p) in parts
-// of a tile's scale: into registers, and as planes to `img`.  Returns the tile's exponent.
+// A wave's 32 rows, a lane its row's octets of its half of each 16 columns (zeros past the
+// text).  Its loads are all sent at once: a branch around each makes every one wait for
+// the one before (8 of them 6 us).
 template <int DP, bool VEC>
-__device__ __forceinline__ uint32_t split_rows(const float* p, int d, int lr, int h, u32x4 (&out)[DP / 16][2], char* img) {
+struct LaneRow {
   f32x4 x[DP / 16][2];
+  // p: row `row0` of the head; rows from T on are not read
+  __device__ __forceinline__ LaneRow(const float* p, int64_t st, int row0, int T, int d, int lr, int h) {
+    const __amdgpu_buffer_rsrc_t b = row_buffer(p, kNowhere - 1);
+    const uint32_t at = (uint32_t)lr * (uint32_t)st * 4u;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int dd = 16 * c + 8 * h + 4 * g;
+        const uint32_t off = row0 + lr < T && dd < d ? at + 4u * dd : kNowhere;
+        x[c][g] = VEC ? buffer_load4(b, off) : buffer_load1x4(b, off, d - dd);
+      }
+    }
+  }
+  __device__ __forceinline__ float half(float f, u32x4 (&out)[DP / 16][2], bool& bad) {  // half_row's, of f times the row
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) x[c][g] *= f;
+    }
+    return half_row<DP>(x, out, bad);
+  }
+  __device__ __forceinline__ float dot(const LaneRow& y) const {  // of the lane's octets
+    float s = 0.f;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = fmaf(x[c][g][e], y.x[c][g][e], s);
+      }
+    }
+    return s;
+  }
+};
+
+// A wave's 32 rows in parts of a tile's scale: into registers, and as planes to `img` (HBM
+// or LDS; null: not).  Returns the tile's exponent.
+template <int DP, bool VEC>
+__device__ __forceinline__ uint32_t split_rows(const LaneRow<DP, VEC>& rows, int lr, int h, u32x4 (&out)[DP / 16][2], char* img) {
+  const auto& x = rows.x;
   float top = 0.f;
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-      const int dd = 16 * c + 8 * h + 4 * g;
-      x[c][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (p && dd < d) x[c][g] = load4<VEC>(p + dd, d - dd);
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = nan_max(top, fabsf(x[c][g][e]));
     }
@@ -195,7 +235,7 @@ __device__ __forceinline__ uint32_t split_rows(const float* p, int d, int lr, in
   }
   const uint32_t t = tile_top(hi, lo);
   const float m = half_scale(top_bits(t));
-  if (lr == 0 && h == 0) *reinterpret_cast<uint32_t*>(img + 2 * DP) = t;
+  if (img && lr == 0 && h == 0) *reinterpret_cast<uint32_t*>(img + 2 * DP) = t;
   char* to = img + lr * HalfTile<DP>::kRow + 16 * h;
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) {
@@ -206,6 +246,7 @@ __device__ __forceinline__ uint32_t split_rows(const float* p, int d, int lr, in
       out[c][0][e] = y;
       out[c][1][e] = z;
     }
+    if (!img) continue;
     *reinterpret_cast<u32x4*>(to + 32 * c) = out[c][0];
     *reinterpret_cast<u32x4*>(to + 32 * c + HalfTile<DP>::kPlane) = out[c][1];
   }
@@ -227,7 +268,13 @@ __device__ __forceinline__ void stage_pair(const char* src, char* lds, int wave,
   }
 }
 
-// Stages of the rings that tiles arrive in: two where the grid fills the GPU, and where a
+// Texts of up to TILES tiles are kept in LDS whole: a workgroup takes a head, a wave splits
+// a tile of K and of V (of Q and of dO) straight into LDS, and then its own 32 rows need
+// no barrier, no planes in HBM and no other workgroup's.  TILES = 0: longer texts.
+constexpr int wa_whole(int dp) { return dp == 64 ? 8 : 4; }
+constexpr int wa_threads(int tiles) { return tiles ? tiles * kWave : kFaThreads; }
+
+// Stages of the rings that longer texts' tiles arrive in: two where the grid fills the GPU, and where a
 // CU has one workgroup at most as many as its LDS holds, so that the first tiles of a
 // short list are all on their way at once.
 constexpr int wa_deep(int dp) { return dp == 64 ? 7 : 4; }
@@ -246,30 +293,40 @@ __device__ __forceinline__ void ring_next(int behind) {
 // R, the row's, such that it stays below 2^15: the largest s + v so far, followed only when
 // it is passed by 2^4, so O is rarely rescaled.  So O is sum P V 2^(25 - R), and l is kept
 // as l 2^(-R - 29).
-template <int DP, bool VEC, int STAGES>
-__global__ void __launch_bounds__(kFaThreads, STAGES > 2 ? 1 : (DP == 64 ? 3 : 2))
+template <int DP, bool VEC, int STAGES, int TILES>
+__global__ void __launch_bounds__(wa_threads(TILES), TILES ? (DP == 64 ? 2 : 1) : (STAGES > 2 ? 1 : (DP == 64 ? 3 : 2)))
 window_fwd_kernel(const WaArgs a) {
   using Tile = HalfTile<DP>;
   constexpr int NB = DP / 32;
-  __shared__ __attribute__((aligned(16))) char kv[STAGES][2 * Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) char kv[TILES ? TILES : STAGES][2 * Tile::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
   const int bh = blockIdx.x % a.BH, qb = blockIdx.x / a.BH, bhk = wa_kv(a, bh);
   const int q0 = qb * kBlock, w0 = q0 + wave * kTile, qi = w0 + lr;  // this lane's row
-  const float* Q = qi < a.T ? wa_head(a.q, a, bh) + (int64_t)qi * a.q.st : nullptr;
-  const WaTiles tiles(a, q0, min(q0 + kBlock, a.T) - 1);
+  const int wr = min(w0, a.T - 1);  // a row that is there
+  auto rows_of = [&](const FaIn& x, const float* head) {
+    return LaneRow<DP, VEC>(head + (int64_t)wr * x.st, x.st, w0, a.T, a.d, lr, h);
+  };
+  const WaTiles tiles(a, TILES ? w0 : q0, min(TILES ? w0 + kTile : q0 + kBlock, a.T) - 1);
   const char* img = a.kv_img + (int64_t)bhk * a.tiles * 2 * Tile::kBytes;
   auto stage = [&](int t, int buf) {
     stage_pair<DP, 4>(img + (int64_t)(tiles.key(t) / kTile) * 2 * Tile::kBytes, kv[buf], wave, lane);
   };
 #pragma unroll
   for (int t = 0; t < STAGES - 1; ++t)
-    if (t < tiles.count) stage(t, t);
+    if (!TILES && t < tiles.count) stage(t, t);
 
+  LaneRow<DP, VEC> row = rows_of(a.q, wa_head(a.q, a, bh));
   u32x4 qp[DP / 16][2];
+  if (TILES) {
+    const LaneRow<DP, VEC> k = rows_of(a.k, wa_kv_head(a.k, a, bhk)), v = rows_of(a.v, wa_kv_head(a.v, a, bhk));
+    split_rows<DP, VEC>(k, lr, h, qp, kv[wave]);
+    split_rows<DP, VEC>(v, lr, h, qp, kv[wave] + Tile::kBytes);
+  }
   bool row_bad = false;
   uint32_t held = 0;  // the lowest bit: a tile that is not
-  const float qf = half_row<DP, VEC>(Q, a.d, a.scale_log2, h, qp, row_bad);
+  const float qf = row.half(a.scale_log2, qp, row_bad);
+  if (TILES) __syncthreads();
   f32x16 o[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) o[b] = zero16();
@@ -298,10 +355,14 @@ window_fwd_kernel(const WaArgs a) {
 
   for (int t = 0, buf = -1, to = STAGES - 2; t < tiles.count; ++t) {
     const int kv0 = tiles.key(t);
-    buf = buf + 1 < STAGES ? buf + 1 : 0;
-    to = to + 1 < STAGES ? to + 1 : 0;
-    ring_next<STAGES - 2, kStageDmas<DP, 4>>(tiles.count - 1 - t);
-    if (t + STAGES - 1 < tiles.count) stage(t + STAGES - 1, to);
+    if (TILES) {
+      buf = kv0 / kTile;
+    } else {
+      buf = buf + 1 < STAGES ? buf + 1 : 0;
+      to = to + 1 < STAGES ? to + 1 : 0;
+      ring_next<STAGES - 2, kStageDmas<DP, 4>>(tiles.count - 1 - t);
+      if (t + STAGES - 1 < tiles.count) stage(t + STAGES - 1, to);
+    }
     if (w0 >= a.T || !wa_any(a, w0, kv0)) continue;
     const uint32_t kt = top_of<DP>(kv[buf]), vt = top_of<DP>(kv[buf] + Tile::kBytes);
     held |= kt | vt;
@@ -328,6 +389,7 @@ window_fwd_kernel(const WaArgs a) {
   if (w0 < a.T && __any(row_bad || (held & 1))) {
     const float* __restrict__ K = wa_kv_head(a.k, a, bhk);
     const float* __restrict__ V = wa_kv_head(a.v, a, bhk);
+    const float* Q = qi < a.T ? wa_head(a.q, a, bh) + (int64_t)qi * a.q.st : nullptr;
     R = -INFINITY;
     l = 0.f;
 #pragma unroll
@@ -373,59 +435,57 @@ window_fwd_kernel(const WaArgs a) {
 }
 
 // dQ, and what dK's and dV's pass reads of a query row: the planes of Q and dO, D and lse.
-template <int DP, bool VEC, int STAGES>
-__global__ void __launch_bounds__(kFaThreads, STAGES == 2 && DP == 64 ? 2 : 1)
+template <int DP, bool VEC, int STAGES, int TILES>
+__global__ void __launch_bounds__(wa_threads(TILES), (TILES || STAGES == 2) && DP == 64 ? 2 : 1)
 window_bwd_dq_kernel(const WaArgs a) {
   constexpr int NB = DP / 32;
   using Tile = HalfTile<DP>;
-  __shared__ __attribute__((aligned(16))) char kv[STAGES][2 * Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) char kv[TILES ? TILES : STAGES][2 * Tile::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
   const int bh = blockIdx.x % a.BH, qb = blockIdx.x / a.BH, bhk = wa_kv(a, bh);
   const int q0 = qb * kBlock, w0 = q0 + wave * kTile, qi = w0 + lr;
   const bool row_ok = qi < a.T;
-  const float* Q = row_ok ? wa_head(a.q, a, bh) + (int64_t)qi * a.q.st : nullptr;
-  const float* dO = row_ok ? wa_head(a.dout, a, bh) + (int64_t)qi * a.dout.st : nullptr;
-  const WaTiles tiles(a, q0, min(q0 + kBlock, a.T) - 1);
+  const int wr = min(w0, a.T - 1);  // a row that is there
+  auto rows_of = [&](const FaIn& x, const float* head) {
+    return LaneRow<DP, VEC>(head + (int64_t)wr * x.st, x.st, w0, a.T, a.d, lr, h);
+  };
+  const WaTiles tiles(a, TILES ? w0 : q0, min(TILES ? w0 + kTile : q0 + kBlock, a.T) - 1);
   const char* img = a.kv_img + (int64_t)bhk * a.tiles * 2 * Tile::kBytes;
   auto stage = [&](int t, int buf) {
     stage_pair<DP, 4>(img + (int64_t)(tiles.key(t) / kTile) * 2 * Tile::kBytes, kv[buf], wave, lane);
   };
 #pragma unroll
   for (int t = 0; t < STAGES - 1; ++t)
-    if (t < tiles.count) stage(t, t);
+    if (!TILES && t < tiles.count) stage(t, t);
 
-  float l2 = INFINITY, dsum = 0.f;
+  const LaneRow<DP, VEC> q = rows_of(a.q, wa_head(a.q, a, bh)), dO = rows_of(a.dout, wa_head(a.dout, a, bh));
+  const LaneRow<DP, VEC> O = rows_of(a.o_in, wa_head(a.o_in, a, bh));
+  const float lse = a.lse[(int64_t)bh * a.T + min(qi, a.T - 1)];
   u32x4 qp[DP / 16][2], dop[DP / 16][2];
+  if (TILES) {
+    const LaneRow<DP, VEC> k = rows_of(a.k, wa_kv_head(a.k, a, bhk)), v = rows_of(a.v, wa_kv_head(a.v, a, bhk));
+    split_rows<DP, VEC>(k, lr, h, qp, kv[wave]);
+    split_rows<DP, VEC>(v, lr, h, qp, kv[wave] + Tile::kBytes);
+  }
+  const float l2 = row_ok ? lse * kLog2e : INFINITY, dsum = half_swap_sum(dO.dot(O));
   bool row_bad = false;
   uint32_t held = 0;
   float qf = 0.f, df = 0.f;
   if (w0 < a.T) {
-    if (row_ok) {
-      const float* O = wa_head(a.o_in, a, bh) + (int64_t)qi * a.o_in.st;
-#pragma unroll
-      for (int c = 0; c < DP / 8; ++c) {
-        const int dd = 8 * c + 4 * h;
-        if (dd < a.d) {
-          const f32x4 x = load4<VEC>(dO + dd, a.d - dd), y = load4<VEC>(O + dd, a.d - dd);
-          dsum += x[0] * y[0] + x[1] * y[1] + x[2] * y[2] + x[3] * y[3];
-        }
-      }
-      l2 = a.lse[(int64_t)bh * a.T + qi] * kLog2e;
-    }
-    dsum = half_swap_sum(dsum);
     const int64_t tile = (int64_t)bh * a.tiles + w0 / kTile;
     if (h == 0) {
       a.D[tile * kTile + lr] = dsum;
       a.l2[tile * kTile + lr] = l2;
     }
     char* to = a.qd_img + tile * 2 * Tile::kBytes;
-    const uint32_t qt = split_rows<DP, VEC>(Q, a.d, lr, h, qp, to);
-    const uint32_t ot = split_rows<DP, VEC>(dO, a.d, lr, h, dop, to + Tile::kBytes);
+    const uint32_t qt = split_rows<DP, VEC>(q, lr, h, qp, TILES ? nullptr : to);
+    const uint32_t ot = split_rows<DP, VEC>(dO, lr, h, dop, TILES ? nullptr : to + Tile::kBytes);
     held = qt | ot;
     qf = lane_factor(top_bits(qt)) * a.scale_log2;
     df = lane_factor(top_bits(ot));
   }
+  if (TILES) __syncthreads();
   f32x16 dq[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) dq[b] = zero16();
@@ -439,10 +499,14 @@ window_bwd_dq_kernel(const WaArgs a) {
   };
   for (int t = 0, buf = -1, to = STAGES - 2; t < tiles.count; ++t) {
     const int kv0 = tiles.key(t);
-    buf = buf + 1 < STAGES ? buf + 1 : 0;
-    to = to + 1 < STAGES ? to + 1 : 0;
-    ring_next<STAGES - 2, kStageDmas<DP, 4>>(tiles.count - 1 - t);
-    if (t + STAGES - 1 < tiles.count) stage(t + STAGES - 1, to);
+    if (TILES) {
+      buf = kv0 / kTile;
+    } else {
+      buf = buf + 1 < STAGES ? buf + 1 : 0;
+      to = to + 1 < STAGES ? to + 1 : 0;
+      ring_next<STAGES - 2, kStageDmas<DP, 4>>(tiles.count - 1 - t);
+      if (t + STAGES - 1 < tiles.count) stage(t + STAGES - 1, to);
+    }
     if (w0 >= a.T || !wa_any(a, w0, kv0)) continue;
     const uint32_t kt = top_of<DP>(kv[buf]), vt = top_of<DP>(kv[buf] + Tile::kBytes);
     held |= kt | vt;
@@ -465,6 +529,8 @@ window_bwd_dq_kernel(const WaArgs a) {
   if (w0 < a.T && __any(row_bad || (held & 1))) {
     const float* __restrict__ K = wa_kv_head(a.k, a, bhk);
     const float* __restrict__ V = wa_kv_head(a.v, a, bhk);
+    const float* Q = row_ok ? wa_head(a.q, a, bh) + (int64_t)qi * a.q.st : nullptr;
+    const float* dO = row_ok ? wa_head(a.dout, a, bh) + (int64_t)qi * a.dout.st : nullptr;
 #pragma unroll
     for (int b = 0; b < NB; ++b) dq[b] = zero16();
     for (int t = 0; t < tiles.count; ++t) {
@@ -502,8 +568,9 @@ window_bwd_dq_kernel(const WaArgs a) {
 template <int WAVES>
 struct WaList {
   int k0, part, first, count, begin, end;
-  __device__ __forceinline__ WaList(const WaArgs& a, int item) {
-    const int tile = WAVES == 4 ? 4 * item : item / a.far_parts;
+  // wave: of a workgroup that takes a whole head, a list for each
+  __device__ __forceinline__ WaList(const WaArgs& a, int item, int wave) {
+    const int tile = WAVES == 4 ? 4 * item + wave : item / a.far_parts;
     part = WAVES == 4 ? 0 : item % a.far_parts;
     k0 = tile * kTile;
     // the last query that the window of a key of the block reaches
@@ -525,22 +592,24 @@ struct WaList {
 };
 
 // dK and dV: a wave takes 32 keys, a lane its key, and walks its workgroup's list.
-template <int DP, bool VEC, int WAVES, int STAGES>
-__global__ void __launch_bounds__(WAVES * kWave, STAGES == 2 && DP == 64 ? 2 : 1)
+template <int DP, bool VEC, int WAVES, int STAGES, int TILES>
+__global__ void __launch_bounds__(TILES ? wa_threads(TILES) : WAVES * kWave, (TILES || STAGES == 2) && DP == 64 ? 2 : 1)
 window_bwd_dkdv_kernel(const WaArgs a) {
   constexpr int NB = DP / 32;
   using Tile = HalfTile<DP>;
-  __shared__ __attribute__((aligned(16))) char qd[STAGES][2 * Tile::kBytes];
-  __shared__ __attribute__((aligned(16))) float stats[STAGES][2 * kTile];  // lse in log2, D
+  __shared__ __attribute__((aligned(16))) char qd[TILES ? TILES : STAGES][2 * Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) float stats[TILES ? TILES : STAGES][2 * kTile];  // lse in log2, D
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
   const int bhk = blockIdx.x % a.BHkv, item = blockIdx.x / a.BHkv;
-  const WaList<WAVES> part(a, item);
-  const int kw = part.k0 + wave * kTile;  // the wave's first key
+  const WaList<WAVES> part(a, item, TILES ? wave : 0);
+  const int kw = TILES ? wave * kTile : part.k0 + wave * kTile;  // the wave's first key
   const int kj = kw + lr;
   const bool key_ok = kj < a.T;
-  const float* K = key_ok ? wa_kv_head(a.k, a, bhk) + (int64_t)kj * a.k.st : nullptr;
-  const float* V = key_ok ? wa_kv_head(a.v, a, bhk) + (int64_t)kj * a.v.st : nullptr;
+  const int wr = min(kw, a.T - 1);  // a row that is there
+  auto rows_of = [&](const FaIn& x, const float* head) {
+    return LaneRow<DP, VEC>(head + (int64_t)wr * x.st, x.st, kw, a.T, a.d, lr, h);
+  };
   const int head0 = bhk / a.Hkv * a.H + bhk % a.Hkv * a.G;  // the first query head
   // where item t of the list stands among all heads' tiles
   struct Place {
@@ -559,7 +628,7 @@ window_bwd_dkdv_kernel(const WaArgs a) {
   Place here = part.begin < part.end ? place_of(part.begin) : Place{head0, part.first}, ahead = here;
 #pragma unroll
   for (int n = 0; n < STAGES - 1; ++n) {
-    if (part.begin + n >= part.end) break;
+    if (TILES || part.begin + n >= part.end) break;
     stage(ahead, n);
     ahead = next_of(ahead);
   }
@@ -567,8 +636,12 @@ window_bwd_dkdv_kernel(const WaArgs a) {
   u32x4 kp[DP / 16][2], vp[DP / 16][2];
   bool key_bad = false;
   uint32_t held = 0;
-  const float kf = half_row<DP, VEC>(K, a.d, a.scale_log2, h, kp, key_bad);
-  const float vf = half_row<DP, VEC>(V, a.d, 1.f, h, vp, key_bad);
+  float kf, vf;
+  {
+    LaneRow<DP, VEC> k = rows_of(a.k, wa_kv_head(a.k, a, bhk)), v = rows_of(a.v, wa_kv_head(a.v, a, bhk));
+    kf = k.half(a.scale_log2, kp, key_bad);
+    vf = v.half(1.f, vp, key_bad);
+  }
   f32x16 dk[NB], dv[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) dk[b] = dv[b] = zero16();
@@ -581,15 +654,34 @@ window_bwd_dkdv_kernel(const WaArgs a) {
     for (int r = 0; r < 16; ++r)
       if (!wa_sees(a, i0 + acc_row(r, h), kj)) p[r] = 0.f;
   };
-  for (int t = part.begin, cur = -1, to = STAGES - 2; t < part.end; ++t) {
+  const int heads = TILES ? a.G : 1;  // lists one after the other
+  for (int g = 0; g < heads; ++g) {
+  if (TILES) {
+    // the head's queries; every wave is done with the head before
+    u32x4 parts[DP / 16][2];
+    const int bh = head0 + g;
+    if (g > 0) __syncthreads();
+    const LaneRow<DP, VEC> q = rows_of(a.q, wa_head(a.q, a, bh)), dO = rows_of(a.dout, wa_head(a.dout, a, bh));
+    const float stat = (h == 0 ? a.l2 : a.D)[((int64_t)bh * a.tiles + wave) * kTile + lr];
+    split_rows<DP, VEC>(q, lr, h, parts, qd[wave]);
+    split_rows<DP, VEC>(dO, lr, h, parts, qd[wave] + Tile::kBytes);
+    stats[wave][lane] = stat;
+    __syncthreads();
+    here = Place{bh, part.first};
+  }
+  for (int t = part.begin, cur = -1, to = STAGES - 2; t < (TILES ? part.count : part.end); ++t) {
     const int i0 = here.tile * kTile;
     here = next_of(here);
-    cur = cur + 1 < STAGES ? cur + 1 : 0;
-    to = to + 1 < STAGES ? to + 1 : 0;
-    ring_next<STAGES - 2, kStageDmas<DP, WAVES> + 1>(part.end - 1 - t);
-    if (t + STAGES - 1 < part.end) {
-      stage(ahead, to);
-      ahead = next_of(ahead);
+    if (TILES) {
+      cur = i0 / kTile;
+    } else {
+      cur = cur + 1 < STAGES ? cur + 1 : 0;
+      to = to + 1 < STAGES ? to + 1 : 0;
+      ring_next<STAGES - 2, kStageDmas<DP, WAVES> + 1>(part.end - 1 - t);
+      if (t + STAGES - 1 < part.end) {
+        stage(ahead, to);
+        ahead = next_of(ahead);
+      }
     }
     if (kw >= a.T || !wa_any(a, i0, kw)) continue;
     const uint32_t qt = top_of<DP>(qd[cur]), ot = top_of<DP>(qd[cur] + Tile::kBytes);
@@ -629,10 +721,13 @@ window_bwd_dkdv_kernel(const WaArgs a) {
     half_cols<DP>(qd[cur], x, f, 0, lane, dk);
     half_cols<DP>(qd[cur], x, f, 1, lane, dk);
   }
+  }
   fit_v.undo(dv);
   fit_k.undo(dk);
 
   if (kw < a.T && part.begin < part.end && __any(key_bad || (held & 1))) {
+    const float* K = key_ok ? wa_kv_head(a.k, a, bhk) + (int64_t)kj * a.k.st : nullptr;
+    const float* V = key_ok ? wa_kv_head(a.v, a, bhk) + (int64_t)kj * a.v.st : nullptr;
 #pragma unroll
     for (int b = 0; b < NB; ++b) dk[b] = dv[b] = zero16();
     for (int t = part.begin; t < part.end; ++t) {
@@ -742,6 +837,7 @@ WaArgs wa_args(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t d, int64_t 
   a.W = (int)std::min(window, T);
   a.S = (int)std::min(sinks, T);
   a.tiles = (int)ceil_div(T, kTile);
+  a.whole = a.tiles <= wa_whole(wa_dim(d));
   a.scale = scale;
   a.scale_log2 = scale * kLog2e;
   return a;
@@ -753,7 +849,7 @@ void wa_bwd_plan(WaArgs& a) {
   const int64_t near = std::min<int64_t>(a.T - 1, kBlock - 1 + (int64_t)a.W - 1) / kTile + 1, far = a.tiles - near;
   a.sink_tiles = (int)ceil_div(a.S, kTile);
   a.far_parts = a.far_chunk = 0;
-  if (a.sink_tiles == 0 || a.sink_tiles > 64 || far <= near) return;
+  if (a.whole || a.sink_tiles == 0 || a.sink_tiles > 64 || far <= near) return;
   // a wave a SIMD
   const int64_t waves = 4 * device_cu_count(), all = (int64_t)a.BHkv * a.sink_tiles * a.G * far;
   a.far_chunk = (int)std::max<int64_t>(8, ceil_div(all, waves));
@@ -763,7 +859,7 @@ void wa_bwd_plan(WaArgs& a) {
 // Where the workspace holds item i: K's and V's planes, then for the backward Q's and
 // dO's, l2, D, and the parts of dK and dV.
 size_t wa_bytes(const WaArgs& a, int i) {
-  const size_t pair = 2 * (wa_dim(a.d) == 64 ? HalfTile<64>::kBytes : HalfTile<128>::kBytes);
+  const size_t pair = a.whole ? 0 : 2 * (wa_dim(a.d) == 64 ? HalfTile<64>::kBytes : HalfTile<128>::kBytes);
   const size_t kv = (size_t)a.BHkv * a.tiles, q = (size_t)a.BH * a.tiles;
   const size_t part = (size_t)a.BHkv * a.sink_tiles * a.far_parts * kTile * wa_dim(a.d) * sizeof(float);
   const size_t size[6] = {kv * pair, q * pair, q * kTile * sizeof(float), q * kTile * sizeof(float), part, part};
@@ -774,6 +870,7 @@ size_t wa_bytes(const WaArgs& a, int i) {
 constexpr int kWaFwd = 1, kWaBwd = 6;  // items of a forward and of a backward
 
 bool wa_workspace(WaArgs& a, void* workspace, size_t bytes, int items) {
+  if (wa_bytes(a, items) == 0) return true;
   if (!workspace || !aligned16(workspace) || bytes < wa_bytes(a, items)) return false;
   char* ws = static_cast<char*>(workspace);
   a.kv_img = ws;
@@ -813,32 +910,57 @@ int launch_split(const WaArgs& a, hipStream_t st) {
   return launch_status();
 }
 
+// The forms for texts that LDS holds, by their tiles.
+template <int DP, bool VEC, int TILES>
+int launch_whole_fwd(const WaArgs& a, hipStream_t st) {
+  window_fwd_kernel<DP, VEC, 2, TILES><<<dim3((unsigned)a.BH), dim3(wa_threads(a.tiles)), 0, st>>>(a);
+  return launch_status();
+}
+template <int DP, bool VEC, int TILES>
+int launch_whole_bwd(const WaArgs& a, hipStream_t st) {
+  window_bwd_dq_kernel<DP, VEC, 2, TILES><<<dim3((unsigned)a.BH), dim3(wa_threads(a.tiles)), 0, st>>>(a);
+  const int rc = launch_status();
+  if (rc != AAR_OK) return rc;
+  window_bwd_dkdv_kernel<DP, VEC, 4, 2, TILES><<<dim3((unsigned)a.BHkv), dim3(wa_threads(a.tiles)), 0, st>>>(a);
+  return launch_status();
+}
+
 template <int DP, bool VEC>
 int launch_fwd(const WaArgs& a, hipStream_t st) {
+  if (a.whole) {
+    if (a.tiles <= 2) return launch_whole_fwd<DP, VEC, 2>(a, st);
+    if (a.tiles <= 4) return launch_whole_fwd<DP, VEC, 4>(a, st);
+    if constexpr (wa_whole(DP) > 4) return launch_whole_fwd<DP, VEC, wa_whole(DP)>(a, st);
+  }
   const int rc = launch_split<DP, VEC>(a, st);
   if (rc != AAR_OK) return rc;
   const dim3 grid((unsigned)(ceil_div(a.T, kBlock) * a.BH)), block(kFaThreads);
-  if ((int)grid.x <= device_cu_count()) window_fwd_kernel<DP, VEC, wa_deep(DP)><<<grid, block, 0, st>>>(a);
-  else window_fwd_kernel<DP, VEC, 2><<<grid, block, 0, st>>>(a);
+  if ((int)grid.x <= device_cu_count()) window_fwd_kernel<DP, VEC, wa_deep(DP), 0><<<grid, block, 0, st>>>(a);
+  else window_fwd_kernel<DP, VEC, 2, 0><<<grid, block, 0, st>>>(a);
   return launch_status();
 }
 
 template <int DP, bool VEC>
 int launch_bwd(const WaArgs& a, hipStream_t st) {
+  if (a.whole) {
+    if (a.tiles <= 2) return launch_whole_bwd<DP, VEC, 2>(a, st);
+    if (a.tiles <= 4) return launch_whole_bwd<DP, VEC, 4>(a, st);
+    if constexpr (wa_whole(DP) > 4) return launch_whole_bwd<DP, VEC, wa_whole(DP)>(a, st);
+  }
   int rc = launch_split<DP, VEC>(a, st);
   if (rc != AAR_OK) return rc;
   const int64_t blocks = ceil_div(a.T, kBlock);
   const dim3 rows((unsigned)(blocks * a.BH)), keys((unsigned)(blocks * a.BHkv)), block(kFaThreads);
-  if ((int)rows.x <= device_cu_count()) window_bwd_dq_kernel<DP, VEC, wa_deep(DP)><<<rows, block, 0, st>>>(a);
-  else window_bwd_dq_kernel<DP, VEC, 2><<<rows, block, 0, st>>>(a);
+  if ((int)rows.x <= device_cu_count()) window_bwd_dq_kernel<DP, VEC, wa_deep(DP), 0><<<rows, block, 0, st>>>(a);
+  else window_bwd_dq_kernel<DP, VEC, 2, 0><<<rows, block, 0, st>>>(a);
   rc = launch_status();
   if (rc != AAR_OK) return rc;
-  if ((int)keys.x <= device_cu_count()) window_bwd_dkdv_kernel<DP, VEC, 4, wa_deep(DP)><<<keys, block, 0, st>>>(a);
-  else window_bwd_dkdv_kernel<DP, VEC, 4, 2><<<keys, block, 0, st>>>(a);
+  if ((int)keys.x <= device_cu_count()) window_bwd_dkdv_kernel<DP, VEC, 4, wa_deep(DP), 0><<<keys, block, 0, st>>>(a);
+  else window_bwd_dkdv_kernel<DP, VEC, 4, 2, 0><<<keys, block, 0, st>>>(a);
   rc = launch_status();
   if (rc != AAR_OK || a.far_parts == 0) return rc;
   const int64_t far = (int64_t)a.BHkv * a.sink_tiles * a.far_parts;
-  window_bwd_dkdv_kernel<DP, VEC, 1, 2><<<dim3((unsigned)far), dim3(kWave), 0, st>>>(a);
+  window_bwd_dkdv_kernel<DP, VEC, 1, 2, 0><<<dim3((unsigned)far), dim3(kWave), 0, st>>>(a);
   rc = launch_status();
   if (rc != AAR_OK) return rc;
   window_bwd_sum_kernel<DP, VEC><<<dim3((unsigned)((int64_t)a.BHkv * a.S)), dim3(256), 0, st>>>(a);
