@@ -36,6 +36,7 @@ struct WaArgs {
   int T, d, H, G, Hkv, BH, BHkv;  // BH = B * H query heads, BHkv = B * Hkv
   int W, S, tiles;                // tiles of 32 rows
   bool whole;                     // a head's tiles fit in LDS
+  int turns;                      // workgroups that take its waves in turn, of 4
   int sink_tiles, far_parts, far_chunk;  // dK/dV: key tiles that hold sinks, parts of their far queries (0: none), tiles of one
   float scale, scale_log2;
 };
@@ -271,6 +272,8 @@ __device__ __forceinline__ void stage_pair(const char* src, char* lds, int wave,
 // Texts of up to TILES tiles are kept in LDS whole: a workgroup takes a head, a wave splits
 // a tile of K and of V (of Q and of dO) straight into LDS, and then its own 32 rows need
 // no barrier, no planes in HBM and no other workgroup's.  TILES = 0: longer texts.
+// Where half the CUs would have no head, two workgroups take one: both have its tiles, the
+// first the rows of waves 0 to 3 and the second those of waves 4 to 7, so that a SIMD has one.
 constexpr int wa_whole(int dp) { return dp == 64 ? 8 : 4; }
 constexpr int wa_threads(int tiles) { return tiles ? tiles * kWave : kFaThreads; }
 
@@ -301,8 +304,8 @@ window_fwd_kernel(const WaArgs a) {
   __shared__ __attribute__((aligned(16))) char kv[TILES ? TILES : STAGES][2 * Tile::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
-  const int bh = blockIdx.x % a.BH, qb = blockIdx.x / a.BH, bhk = wa_kv(a, bh);
-  const int q0 = qb * kBlock, w0 = q0 + wave * kTile, qi = w0 + lr;  // this lane's row
+  const int bh = blockIdx.x % a.BH, turn = blockIdx.x / a.BH, bhk = wa_kv(a, bh);
+  const int q0 = TILES ? 0 : turn * kBlock, w0 = q0 + wave * kTile, qi = w0 + lr;  // this lane's row
   const int wr = min(w0, a.T - 1);  // a row that is there
   auto rows_of = [&](const FaIn& x, const float* head) {
     return LaneRow<DP, VEC>(head + (int64_t)wr * x.st, x.st, w0, a.T, a.d, lr, h);
@@ -326,7 +329,10 @@ window_fwd_kernel(const WaArgs a) {
   bool row_bad = false;
   uint32_t held = 0;  // the lowest bit: a tile that is not
   const float qf = row.half(a.scale_log2, qp, row_bad);
-  if (TILES) __syncthreads();
+  if (TILES) {
+    __syncthreads();
+    if (a.turns > 1 && wave / 4 != turn) return;
+  }
   f32x16 o[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) o[b] = zero16();
@@ -443,8 +449,8 @@ window_bwd_dq_kernel(const WaArgs a) {
   __shared__ __attribute__((aligned(16))) char kv[TILES ? TILES : STAGES][2 * Tile::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
-  const int bh = blockIdx.x % a.BH, qb = blockIdx.x / a.BH, bhk = wa_kv(a, bh);
-  const int q0 = qb * kBlock, w0 = q0 + wave * kTile, qi = w0 + lr;
+  const int bh = blockIdx.x % a.BH, turn = blockIdx.x / a.BH, bhk = wa_kv(a, bh);
+  const int q0 = TILES ? 0 : turn * kBlock, w0 = q0 + wave * kTile, qi = w0 + lr;
   const bool row_ok = qi < a.T;
   const int wr = min(w0, a.T - 1);  // a row that is there
   auto rows_of = [&](const FaIn& x, const float* head) {
@@ -472,7 +478,8 @@ window_bwd_dq_kernel(const WaArgs a) {
   bool row_bad = false;
   uint32_t held = 0;
   float qf = 0.f, df = 0.f;
-  if (w0 < a.T) {
+  const bool mine = !TILES || a.turns == 1 || wave / 4 == turn;
+  if (w0 < a.T && mine) {
     const int64_t tile = (int64_t)bh * a.tiles + w0 / kTile;
     if (h == 0) {
       a.D[tile * kTile + lr] = dsum;
@@ -485,7 +492,10 @@ window_bwd_dq_kernel(const WaArgs a) {
     qf = lane_factor(top_bits(qt)) * a.scale_log2;
     df = lane_factor(top_bits(ot));
   }
-  if (TILES) __syncthreads();
+  if (TILES) {
+    __syncthreads();
+    if (!mine) return;
+  }
   f32x16 dq[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) dq[b] = zero16();
@@ -602,7 +612,8 @@ window_bwd_dkdv_kernel(const WaArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
   const int bhk = blockIdx.x % a.BHkv, item = blockIdx.x / a.BHkv;
-  const WaList<WAVES> part(a, item, TILES ? wave : 0);
+  const WaList<WAVES> part(a, TILES ? 0 : item, TILES ? wave : 0);
+  const bool mine = !TILES || a.turns == 1 || wave / 4 == item;
   const int kw = TILES ? wave * kTile : part.k0 + wave * kTile;  // the wave's first key
   const int kj = kw + lr;
   const bool key_ok = kj < a.T;
@@ -667,6 +678,7 @@ window_bwd_dkdv_kernel(const WaArgs a) {
     split_rows<DP, VEC>(dO, lr, h, parts, qd[wave] + Tile::kBytes);
     stats[wave][lane] = stat;
     __syncthreads();
+    if (!mine) continue;
     here = Place{bh, part.first};
   }
   for (int t = part.begin, cur = -1, to = STAGES - 2; t < (TILES ? part.count : part.end); ++t) {
@@ -722,6 +734,7 @@ window_bwd_dkdv_kernel(const WaArgs a) {
     half_cols<DP>(qd[cur], x, f, 1, lane, dk);
   }
   }
+  if (!mine) return;
   fit_v.undo(dv);
   fit_k.undo(dk);
 
@@ -838,6 +851,7 @@ WaArgs wa_args(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t d, int64_t 
   a.S = (int)std::min(sinks, T);
   a.tiles = (int)ceil_div(T, kTile);
   a.whole = a.tiles <= wa_whole(wa_dim(d));
+  a.turns = a.whole && a.tiles > 4 && 2 * a.BH <= device_cu_count() ? 2 : 1;
   a.scale = scale;
   a.scale_log2 = scale * kLog2e;
   return a;
@@ -913,15 +927,15 @@ int launch_split(const WaArgs& a, hipStream_t st) {
 // The forms for texts that LDS holds, by their tiles.
 template <int DP, bool VEC, int TILES>
 int launch_whole_fwd(const WaArgs& a, hipStream_t st) {
-  window_fwd_kernel<DP, VEC, 2, TILES><<<dim3((unsigned)a.BH), dim3(wa_threads(a.tiles)), 0, st>>>(a);
+  window_fwd_kernel<DP, VEC, 2, TILES><<<dim3((unsigned)(a.BH * a.turns)), dim3(wa_threads(a.tiles)), 0, st>>>(a);
   return launch_status();
 }
 template <int DP, bool VEC, int TILES>
 int launch_whole_bwd(const WaArgs& a, hipStream_t st) {
-  window_bwd_dq_kernel<DP, VEC, 2, TILES><<<dim3((unsigned)a.BH), dim3(wa_threads(a.tiles)), 0, st>>>(a);
+  window_bwd_dq_kernel<DP, VEC, 2, TILES><<<dim3((unsigned)(a.BH * a.turns)), dim3(wa_threads(a.tiles)), 0, st>>>(a);
   const int rc = launch_status();
   if (rc != AAR_OK) return rc;
-  window_bwd_dkdv_kernel<DP, VEC, 4, 2, TILES><<<dim3((unsigned)a.BHkv), dim3(wa_threads(a.tiles)), 0, st>>>(a);
+  window_bwd_dkdv_kernel<DP, VEC, 4, 2, TILES><<<dim3((unsigned)(a.BHkv * a.turns)), dim3(wa_threads(a.tiles)), 0, st>>>(a);
   return launch_status();
 }
 
