@@ -190,7 +190,7 @@ PYBIND11_MODULE(_core, m) {
       .def("extend", &KVCache::extend, py::arg("counts"), gil_release(),
            "counts[b] new tokens of sequence b: takes pages for them and gives back those that the window has left.")
       .def("append", &KVCache::append, py::arg("layer"), py::arg("k"), py::arg("v"), gil_release(),
-           "The new tokens' keys and values, [sequences, kv_heads, max(counts), d]; no gradient passes.")
+           "The new tokens' keys and values, [sequences, kv_heads, max(counts), d], once a step; no gradient passes.")
       .def("attend", &KVCache::attend, py::arg("layer"), py::arg("q"), gil_release(),
            "Attention of the new tokens' queries [sequences, H, max(counts), d] (a view of rows of all heads); rows from "
            "counts[b] on are zeros.")

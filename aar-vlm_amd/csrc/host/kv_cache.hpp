@@ -16,7 +16,9 @@ namespace aar {
 
 // Sequences are the rows of a batch.  A step of the model is `extend` (how many tokens
 // each sequence gets; pages are taken for them), then for every layer `append` with the
-// new tokens' keys and values and `attend` with their queries.  The page numbers are the
+// new tokens' keys and values, once, and `attend` with their queries, as often as wanted;
+// what breaks that order throws std::runtime_error and changes nothing.  A layer that has
+// missed tokens is not used again until all sequences are empty.  The page numbers are the
 // same in all layers.  A full page never changes, so a fork shares its parent's; the
 // pages a window has left are given back.
 class KVCache {
@@ -40,7 +42,8 @@ class KVCache {
   // kv_heads, n, d]; zeros where a sequence holds none.
   std::pair<Tensor, Tensor> read(int64_t layer, int64_t first, int64_t n);
 
-  // Sequence dst, which is emptied first, continues from what src holds.
+  // Sequence dst, which is emptied first, continues from what src holds: not between src's
+  // extend and the last layer's append.
   void fork(int64_t src, int64_t dst);
   // Empties a sequence.
   void free(int64_t sequence);
@@ -61,14 +64,17 @@ class KVCache {
   int64_t& entry(int64_t sequence, int64_t at) { return table_[sequence * width_ + at]; }
   void check_sequence(int64_t sequence, const char* op) const;
   void check_rows(const Tensor& t, int64_t heads, const char* op) const;
+  void check_whole(int64_t layer, const char* op) const;
   void drop(int64_t page);
   void clear(int64_t sequence);
   void upload();
 
-  std::mutex mu_;
+  mutable std::mutex mu_;
   int64_t B_, Hkv_, d_, P_, width_, n_pages_, window_, sinks_, T_ = 0;
   size_t page_bytes_ = 0;
   std::vector<Pool> pools_;
+  enum State : char { kMissed, kOpen, kAppended };  // a step's tokens, or some step's: not there; of this step not yet; there
+  std::vector<State> state_;  // of each layer
   std::vector<int64_t> table_, lens_, new_, refs_, free_;  // free_: the lowest last
   Tensor table_dev_, lens_dev_, new_dev_;
 };

@@ -218,6 +218,7 @@ KVCache::KVCache(int64_t layers, int64_t sequences, int64_t kv_heads, int64_t d_
                       std::make_shared<Storage>(n_pages_ * kv_heads * 2 * sizeof(float), device_allocator()),
                       std::make_shared<Storage>(sequences * kv_heads * 2 * page * d_head * sizeof(float), device_allocator())});
   }
+  state_.assign(layers, kAppended);
   table_.assign(sequences * width_, -1);
   lens_.assign(sequences, 0);
   new_.assign(sequences, 0);
@@ -253,6 +254,7 @@ void KVCache::clear(int64_t sequence) {
     entry(sequence, at) = -1;
   }
   lens_[sequence] = new_[sequence] = 0;
+  if (std::count(lens_.begin(), lens_.end(), 0) == B_) std::fill(state_.begin(), state_.end(), kAppended);
 }
 
 void KVCache::check_sequence(int64_t sequence, const char* op) const {
@@ -295,6 +297,9 @@ void KVCache::extend(const std::vector<int64_t>& counts) {
     lens_[b] += counts[b];
     new_[b] = counts[b];
   }
+  if (T_ > 0) {
+    for (State& s : state_) s = s == kAppended ? kOpen : kMissed;
+  }
   upload();
 }
 
@@ -319,11 +324,18 @@ void KVCache::check_rows(const Tensor& t, int64_t heads, const char* op) const {
   if (t.device == Device::CPU) throw_cpu_compute(name.c_str());
 }
 
+void KVCache::check_whole(int64_t layer, const char* op) const {
+  if (state_[layer] == kMissed) throw std::runtime_error(std::string("KVCache.") + op + ": the layer has missed tokens");
+}
+
 void KVCache::append(int64_t layer, const Tensor& k, const Tensor& v) {
   std::lock_guard<std::mutex> lock(mu_);
   const aar_kv_cache c = view(layer);
   check_rows(k, Hkv_, "append");
   check_rows(v, Hkv_, "append");
+  check_whole(layer, "append");
+  // twice, a page that the step has filled would take its first rows from the next page's
+  if (T_ > 0 && state_[layer] == kAppended) throw std::runtime_error("KVCache.append: the layer has this step's tokens");
   Tensor kv = head_view(k), vv = head_view(v);
   int64_t st[6];
   strides_of(st, kv);
@@ -331,12 +343,15 @@ void KVCache::append(int64_t layer, const Tensor& k, const Tensor& v) {
   check_status(aar_kv_cache_append_f32(&c, fp(kv), fp(vv), st, ip(lens_dev_), ip(new_dev_), T_,
                                        device_error_word(kErrCachePage), current_stream()),
                "KVCache.append");
+  state_[layer] = kAppended;
 }
 
 Tensor KVCache::attend(int64_t layer, const Tensor& q) {
   std::lock_guard<std::mutex> lock(mu_);
   const aar_kv_cache c = view(layer);
   check_rows(q, 0, "attend");
+  check_whole(layer, "attend");
+  if (state_[layer] == kOpen) throw std::runtime_error("KVCache.attend: append the layer's keys and values first");
   const int64_t H = q.shape[1], window = window_ > 0 ? window_ : int64_t(1) << 30;
   Tensor qv = head_view(q);
   // rows of all heads beside each other, as the next projection reads them
@@ -354,6 +369,7 @@ Tensor KVCache::attend(int64_t layer, const Tensor& q) {
 }
 
 Tensor KVCache::positions() const {
+  std::lock_guard<std::mutex> lock(mu_);
   Tensor host = Tensor::empty({B_, T_}, DType::Int64, Device::CPU);
   int64_t* p = static_cast<int64_t*>(host.data());
   for (int64_t b = 0; b < B_; ++b)
@@ -364,6 +380,8 @@ Tensor KVCache::positions() const {
 std::pair<Tensor, Tensor> KVCache::read(int64_t layer, int64_t first, int64_t n) {
   std::lock_guard<std::mutex> lock(mu_);
   const aar_kv_cache c = view(layer);
+  check_whole(layer, "read");
+  if (state_[layer] == kOpen) throw std::runtime_error("KVCache.read: append the layer's keys and values first");
   if (first < 0 || n < 0 || n > width_ * P_) throw std::invalid_argument("KVCache.read: need first >= 0, 0 <= n <= max_tokens");
   Tensor from = Tensor::empty({B_}, DType::Int64, Device::CPU);
   std::fill_n(static_cast<int64_t*>(from.data()), B_, first);
@@ -386,6 +404,9 @@ void KVCache::fork(int64_t src, int64_t dst) {
   check_sequence(src, "fork");
   check_sequence(dst, "fork");
   if (src == dst) return;
+  if (new_[src] > 0 && std::count(state_.begin(), state_.end(), kOpen) > 0) {
+    throw std::runtime_error("KVCache.fork: a layer has not appended this step's tokens");
+  }
   const int64_t full = lens_[src] / P_, rest = lens_[src] % P_;
   int64_t returned = 0;  // pages that dst holds alone
   for (int64_t at = 0; at < width_; ++at) {

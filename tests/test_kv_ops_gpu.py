@@ -228,3 +228,48 @@ def test_errors(ag):
     m = ag.nn.MultiHeadAttention(128, 2, causal=True, window=8).to(ag.Device.CUDA)
     with pytest.raises(ValueError):
         m.decode(dev(ag, randn(1, 2, 5, 128)), cache, 0)
+
+
+def test_the_order_of_a_step_is_kept(ag):
+    """Twice the same rows, attention before them, a fork between them and layers that miss
+    a step are refused, and change nothing."""
+    cache = ag.KVCache(2, 2, 2, 64, 128, page=32)
+    x, y = dev(ag, randn(1, 2, 2, 40, 64)), dev(ag, randn(2, 2, 2, 1, 64))
+    cache.extend([40, 33])
+    with pytest.raises(RuntimeError):
+        cache.attend(0, x)
+    with pytest.raises(RuntimeError):
+        cache.read(0, 0, 1)
+    cache.append(0, x, x)
+    with pytest.raises(RuntimeError):
+        cache.append(0, x, x)
+    with pytest.raises(RuntimeError):
+        cache.fork(0, 1)
+    cache.append(1, x, x)
+    before = [host(ag, t) for t in cache.read(1, 0, 64)]
+    out = host(ag, ag.contiguous(cache.attend(1, x)))
+    with pytest.raises(RuntimeError):
+        cache.append(1, x, x)
+    assert all(np.array_equal(a, host(ag, b)) for a, b in zip(before, cache.read(1, 0, 64)))
+    assert np.array_equal(out, host(ag, ag.contiguous(cache.attend(1, x))))
+    cache.extend([0, 0])  # no tokens: nothing is missed
+    cache.extend([1, 1])
+    cache.append(1, y, y)
+    cache.extend([0, 1])  # layer 0 has missed a step
+    cache.append(1, y, y)
+    with pytest.raises(RuntimeError):
+        cache.append(0, y, y)
+    with pytest.raises(RuntimeError):
+        cache.attend(0, y)
+    with pytest.raises(RuntimeError):
+        cache.read(0, 0, 1)
+    cache.fork(1, 0)
+    assert list(cache.lengths) == [35, 35]
+    rows = host(ag, cache.read(1, 0, 35)[0])
+    assert np.array_equal(rows[0], rows[1])
+    cache.free(0)
+    cache.free(1)
+    cache.extend([1, 0])
+    cache.append(0, y, y)
+    assert np.isfinite(host(ag, ag.contiguous(cache.attend(0, y)))).all()
+    ag.cuda_synchronize()
