@@ -259,8 +259,9 @@ kv_attn_kernel(const KvPages c, const KvAttn a) {
     }
     next_keys();
 
-    // positive, so that the largest product is the largest score
-    const float f = fmaxf(ldexpf(sk * fabsf(a.scale_log2), -ex), 0x1p-126f);
+    // positive, so that the largest product is the largest score; a scale that is not finite
+    // times its page's numbers, which are 0, is NaN
+    const float f = sk < INFINITY ? fmaxf(ldexpf(sk * fabsf(a.scale_log2), -ex), 0x1p-126f) : INFINITY;
     const bool all = key0 + kKeys - 1 <= span.first + t0 && (key0 > span.first + t1 - a.window || key0 + kKeys <= a.sinks);
     float mx = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -459,9 +460,9 @@ int kv_attn_check(const aar_kv_cache* c, int64_t H, int64_t T, int64_t window, i
   if (rc != AAR_OK) return rc;
   if (H <= 0 || H % c->kv_heads != 0 || T < 0 || window < 1 || sinks < 0) return AAR_EINVAL;
   if (T > (1 << 24) || H > (1 << 24) || H / c->kv_heads * T > (1 << 24)) return AAR_EUNSUPPORTED;
-  // a dispatch holds its work items in 32 bits
-  const int64_t blocks = ceil_div(H / c->kv_heads * T, 16) * c->sequences * c->kv_heads;
-  if (blocks > (int64_t)UINT32_MAX / (16 * 4 * kWave)) return AAR_EUNSUPPORTED;
+  // a dispatch holds its work items in 32 bits: 256 for a block of rows
+  const int64_t blocks = ceil_div(H / c->kv_heads * T, kRows) * c->sequences * c->kv_heads;
+  if (blocks >= (int64_t(1) << 22)) return AAR_EUNSUPPORTED;
   return AAR_OK;
 }
 

@@ -90,8 +90,8 @@ __device__ __forceinline__ void wa_store(float* row, const f32x16 (&x)[DP / 32],
 
 // A tile's exponent, by which its planes are scaled: half_exponent's of its largest element,
 // the lowest bit set where the planes do not hold it (elements that are not finite or
-// out of range, or rows whose largest elements are more than 2^12 apart: a row could
-// lose bits to one that a query does not see).
+// out of range, or rows whose largest elements are more than 2^16 apart: parts are off by up
+// to 2^-38 of the tile's largest element, which is then no more than 2^-22 of a row's).
 __device__ __forceinline__ uint32_t top_bits(uint32_t t) { return t & ~1u; }
 // log2 of row_factor: 2^14 over the scale.
 __device__ __forceinline__ int top_log(uint32_t t) { return (int)(t >> 23) - 126; }
@@ -108,7 +108,7 @@ __device__ __forceinline__ uint32_t top_of(const char* planes) {
 __device__ __forceinline__ uint32_t tile_top(uint32_t hi, uint32_t lo) {
   bool bad = false;
   const uint32_t ex = half_exponent(hi, bad);
-  return ex | (bad || (hi != 0 && (lo >> 23) + 12 < (hi >> 23)) ? 1u : 0u);
+  return ex | (bad || (hi != 0 && (lo >> 23) + 16 < (hi >> 23)) ? 1u : 0u);
 }
 
 // The planes of a tile's 32 rows of K or V, once for all the blocks that read them, as the
@@ -864,6 +864,7 @@ void wa_bwd_plan(WaArgs& a) {
   a.sink_tiles = (int)ceil_div(a.S, kTile);
   a.far_parts = a.far_chunk = 0;
   if (a.whole || a.sink_tiles == 0 || a.sink_tiles > 64 || far <= near) return;
+  if ((int64_t)a.BHkv * a.S > (1 << 23)) return;  // the summing dispatch's; such a grid has work enough
   // a wave a SIMD
   const int64_t waves = 4 * device_cu_count(), all = (int64_t)a.BHkv * a.sink_tiles * a.G * far;
   a.far_chunk = (int)std::max<int64_t>(8, ceil_div(all, waves));

@@ -677,11 +677,16 @@ int aar_distill_bwd_f32(const float* grad, const float* logits, const float* t_l
  * contiguous), as in aar_flash_fwd_strided_f32.  1 <= d <= 128 (AAR_EINVAL); row
  * strides st of q, k, v (and dout) from d to 2^23 (AAR_EUNSUPPORTED; of fewer than two
  * rows any).  16-byte aligned pointers, d and strides multiples of 4 read 128 bits at
- * once, others 32.  T at most 2^24, B, H at most 2^20, and fewer than 2^24 blocks of 128
- * rows over all heads (AAR_EUNSUPPORTED).
- * Products are formed from two fp16 parts of each operand, as in
- * aar_cross_attn_fwd_f32 with its bounds; rows whose largest element is not 0 and
- * outside [2^-99, 2^60) take the fp32 instruction. */
+ * once, others 32.  T at most 2^24, B, H at most 2^20, and over all B * H heads fewer
+ * than 2^20 blocks of 128 rows and 2^26 rows (AAR_EUNSUPPORTED).
+ * Products are formed from two fp16 parts of each operand: 22 bits of it, or 2^-38 of
+ * the largest element of its row or, of K and V (backward: of Q and dout too), of the
+ * 32 rows from a multiple of 32 on that it stands in; sums, softmax statistics and the
+ * bounds of P and dS are aar_cross_attn_fwd_f32's.  32 rows whose largest elements, where
+ * not 0, are more than 2^16 apart, or one outside [2^-99, 2^60), take the fp32
+ * instruction.
+ * The workspace holds K and V in parts where a head's text does not fit in LDS (0 bytes
+ * otherwise; 16-byte aligned, AAR_EWORKSPACE). */
 size_t aar_window_attn_fwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t d, int64_t window,
                                            int64_t sinks);
 int aar_window_attn_fwd_f32(const float* q, const float* k, const float* v, float* o, float* lse, int64_t B, int64_t H,
@@ -690,8 +695,8 @@ int aar_window_attn_fwd_f32(const float* q, const float* k, const float* v, floa
 /* dq, dk, dv (fully overwritten), summed over the query heads that share a
  * key/value head; no float atomics, the same bits on every run.  24 strides: q, k, v, o,
  * dout, dq, dk, dv.  The gradients overlap neither the inputs nor each other.  The
- * workspace holds dout . o of every query row, and parts of sums; 16-byte aligned
- * (AAR_EWORKSPACE). */
+ * workspace holds dout . o and lse of every query row, of longer texts K, V, Q and dout in
+ * parts, and parts of the sinks' sums; 16-byte aligned (AAR_EWORKSPACE). */
 size_t aar_window_attn_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t d, int64_t window,
                                            int64_t sinks);
 int aar_window_attn_bwd_f32(const float* q, const float* k, const float* v, const float* o, const float* lse,

@@ -153,6 +153,23 @@ def test_infinities_and_nan_in_a_page(L):
     assert (pool.read(L, ints(32), 32) == 0).all() and (pool.attend(L, q[:1, :1], ints(32)) == 0).all()
 
 
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("scale", [None, 0.0])
+def test_keys_that_are_not_finite(L, bad, scale):
+    """Queries that see the page are NaN, whatever the scale, others do not change."""
+    k, v, q = rand(1, 1, 1, 90, 64), rand(2, 1, 1, 90, 64), rand(3, 1, 2, 50, 64)
+    lens = ints(90)
+    pool = K.Pool(1, 1, 64, 32, 3)
+    pool.append(L, k, v, lens)
+    fine = pool.attend(L, q, lens, window=9, scale=scale)
+    k[0, 0, 40, 7] = bad
+    pool.append(L, k, v, lens)
+    o = pool.attend(L, q, lens, window=9, scale=scale)
+    sees = torch.arange(40, 90, device="cuda") - 9 < 63  # tokens 32 .. 63 share the page
+    assert torch.equal(torch.isnan(o).all(-1), sees.expand(1, 2, 50)) and torch.equal(torch.isnan(o).any(-1), torch.isnan(o).all(-1))
+    assert torch.equal(o[:, :, ~sees], fine[:, :, ~sees])
+
+
 @pytest.mark.parametrize("first", [None, (0, 5, 40), (-7, 33, 100), (64, 96, -200)])
 def test_reading_ranges(L, first):
     B, Hkv, T, d = 3, 2, 100, 36

@@ -138,6 +138,30 @@ def test_rows_of_any_magnitude(L, which, power, d):
         assert (off <= 16 * tol * top + 100 * 2.0 ** -149).all(), (name, (off / (top + 1e-300)).max().item())
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("T", [100, 600])
+@pytest.mark.parametrize("spread", [8, 30])
+def test_rows_of_mixed_magnitude(L, T, spread, d):
+    """Values and gradients whose rows lie up to 2^(2 spread) apart inside a tile: on both
+    sides of what a tile's parts hold."""
+    q, k, v, do = inputs(1, 4, 2, T, d)
+    power = torch.randint(-spread, spread + 1, (2, T), generator=torch.Generator().manual_seed(spread)).cuda()
+    v *= (2.0 ** power[0].double()).float()[:, None]
+    do *= (2.0 ** power[1].double()).float()[:, None]
+    got = K.window_run(L, q, k, v, do, 70, 2)
+    ref, mass = K.window_exact(q, k, v, do, 70, 2)
+    # each result's terms without their signs: cancelled or not, they are rounded
+    mass["o"] = K.window_exact(q, k, v.abs(), None, 70, 2)[0][0]
+    p = torch.matmul(q.double(), k.double().repeat_interleave(2, 1).transpose(2, 3).contiguous()) * d ** -0.5
+    p = torch.softmax(p.masked_fill(~K.window_mask(T, 70, 2).cuda(), -math.inf), -1)
+    mass["dv"] = torch.matmul(p.transpose(2, 3).contiguous(), do.double().abs()).view(1, 2, 2, T, d).sum(2)
+    tol = M.attn_tol(d, T)
+    for name, g, r in zip(NAMES, got, ref):
+        w = mass[name].amax(-1, keepdim=True) if r.dim() == 4 else mass[name]
+        off = (g.double() - r).abs()
+        assert (off <= 8 * tol * w).all(), (name, (off / w).max().item(), tol)
+
+
 @pytest.mark.parametrize("d", [64, 128, 36])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_what_is_not_finite_stays_where_it_is_seen(L, d, bad):
@@ -214,6 +238,31 @@ def test_same_bits_streams_and_graphs(L):
         torch.cuda.synchronize()
         for a, b in zip((o, lse, dq, dk, dv), K.window_run(L, q, k, v, do, 60, 4)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("shape", [
+    (43, 6, 3, 250, 64, 90, 3), (22, 6, 6, 200, 40, 200, 0), (5, 2, 2, 161, 64, 3, 170), (3, 4, 1, 128, 128, 40, 4),
+    (2, 6, 2, 1500, 64, 33, 700), (1, 4, 1, 2600, 128, 20, 2100), (1, 2, 2, 5000, 64, 64, 60), (70, 4, 4, 260, 36, 300, 2),
+    (9, 8, 8, 1100, 64, 200, 1)])
+def test_every_form_of_the_grid(L, shape):
+    """Texts in LDS with one and two workgroups a head, rings of both depths, the sinks' far
+    queries in parts and, of too many sinks, not."""
+    B, H, Hkv, T, d, window, sinks = shape
+    check(L, *inputs(B, H, Hkv, T, d), window, sinks)
+
+
+def test_the_forward_holds_to_its_workspace(L):
+    q, k, v, _ = inputs(1, 2, 1, 600, 64)
+    o, lse = torch.empty_like(q), torch.empty(1, 2, 600, device="cuda")
+    dims = (1, 2, 1, 600, 64)
+    nb = L.aar_window_attn_fwd_workspace_bytes(*dims, 30, 2)
+    assert nb > 0 and L.aar_window_attn_fwd_workspace_bytes(1, 2, 1, 64, 64, 30, 2) == 0
+    ws = torch.full((nb + 64,), 123, dtype=torch.uint8, device="cuda")
+    args, st = [t.data_ptr() for t in (q, k, v, o, lse)], M.strides3(q, k, v, o)
+    assert L.aar_window_attn_fwd_f32(*args, *dims, st, 30, 2, 0.125, ws.data_ptr(), nb, M.stream()) == 0
+    assert (ws[nb:] == 123).all()
+    for p, n in ((None, nb), (ws.data_ptr(), nb - 1), (ws.data_ptr() + 4, nb)):
+        assert L.aar_window_attn_fwd_f32(*args, *dims, st, 30, 2, 0.125, p, n, M.stream()) == M.EWORKSPACE
 
 
 def test_workspace_is_held_to(L):

@@ -45,6 +45,10 @@ def test_window_workspace(L):
     assert window(L, bwd=True, ws=(X, need - 1)) == M.EWORKSPACE
     assert window(L, bwd=True, ws=(X + 4, need)) == M.EWORKSPACE
     assert L.aar_window_attn_bwd_workspace_bytes(1, 2, 1, 4, 64, 0, 0) == 0
+    # a forward of a text that LDS holds needs none
+    assert L.aar_window_attn_fwd_workspace_bytes(1, 2, 1, 256, 64, 2, 0) == 0
+    assert L.aar_window_attn_fwd_workspace_bytes(1, 2, 1, 257, 64, 2, 0) > 0
+    assert window(L, T=300) == M.EWORKSPACE
     # sinks of any number: a few hundred parts at most
     for sinks in (1, 100, 5000, 1 << 40):
         assert L.aar_window_attn_bwd_workspace_bytes(1, 1, 1, 1 << 20, 64, 16, sinks) < 1 << 31
