@@ -447,8 +447,12 @@ KvPlan kv_plan(const aar_kv_cache& c, int64_t H, int64_t T, int64_t window, int6
   const int dt = kv_tile_dim(c.d), wide = 4 * kv_wide(dt);
   p.waves = 4;
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({kv_resident(dt) * cus / grid, tiles / (2 * p.waves), 64}));
-  // a workgroup that fills a CU, and no join
-  if (p.splits > 1 && grid <= cus && tiles <= (4 * grid >= 3 * cus ? 8 : 2) * wide) {
+  // A workgroup that fills a CU, and no join: where most CUs have one (256 heads' single rows,
+  // d 64, 500 tokens: 10.2 us, in parts 10.8; 4000: 23.1 and 26.0; d 128, 16000: 184 and 187),
+  // and for texts of two tiles a wave, where a second launch costs more (6 heads, 1000 tokens:
+  // 10.1 us a call and 11.6, though 9.7 and 9.2 from a graph).  Else in parts (48 heads, d 128,
+  // 4000 tokens: 17.4 us, whole 30.7).
+  if (p.splits > 1 && grid <= cus && tiles <= (4 * grid >= 3 * cus ? 16 : 2) * wide) {
     p.waves = wide;
     p.splits = 1;
   }

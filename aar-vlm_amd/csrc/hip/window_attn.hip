@@ -277,18 +277,12 @@ __device__ __forceinline__ void stage_pair(const char* src, char* lds, int wave,
 constexpr int wa_whole(int dp) { return dp == 64 ? 8 : 4; }
 constexpr int wa_threads(int tiles) { return tiles ? tiles * kWave : kFaThreads; }
 
-// Stages of the rings that longer texts' tiles arrive in: two where the grid fills the GPU, and where a
-// CU has one workgroup at most as many as its LDS holds, so that the first tiles of a
-// short list are all on their way at once.
-constexpr int wa_deep(int dp) { return dp == 64 ? 7 : 4; }
-
-// Until the next tile of a ring has arrived, with `behind` tiles of `dmas` DMAs a wave sent
-// for after it (of fewer than `most`, until all have): and every wave is done with the
-// tile before.
-template <int MOST, int DMAS>
-__device__ __forceinline__ void ring_next(int behind) {
-  if (MOST > 0 && behind >= MOST) wait_vm_lgkm0<MOST * DMAS>();
-  else wait_vm_lgkm0<0>();
+// Until the next of a longer text's tiles has arrived, in the other one of two buffers, and
+// every wave is done with the tile before.  More buffers where a CU has one workgroup gave
+// nothing (6 heads, 4096 tokens, window 1024, d 64, with gradients: 210 us with two, 217 with
+// seven).
+__device__ __forceinline__ void ring_next() {
+  wait_vm_lgkm0<0>();
   ring_barrier();
 }
 
@@ -296,12 +290,12 @@ __device__ __forceinline__ void ring_next(int behind) {
 // R, the row's, such that it stays below 2^15: the largest s + v so far, followed only when
 // it is passed by 2^4, so O is rarely rescaled.  So O is sum P V 2^(25 - R), and l is kept
 // as l 2^(-R - 29).
-template <int DP, bool VEC, int STAGES, int TILES>
-__global__ void __launch_bounds__(wa_threads(TILES), TILES ? (DP == 64 ? 2 : 1) : (STAGES > 2 ? 1 : (DP == 64 ? 3 : 2)))
+template <int DP, bool VEC, int TILES>
+__global__ void __launch_bounds__(wa_threads(TILES), TILES ? (DP == 64 ? 2 : 1) : (DP == 64 ? 3 : 2))
 window_fwd_kernel(const WaArgs a) {
   using Tile = HalfTile<DP>;
   constexpr int NB = DP / 32;
-  __shared__ __attribute__((aligned(16))) char kv[TILES ? TILES : STAGES][2 * Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) char kv[TILES ? TILES : 2][2 * Tile::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
   const int bh = blockIdx.x % a.BH, turn = blockIdx.x / a.BH, bhk = wa_kv(a, bh);
@@ -315,9 +309,7 @@ window_fwd_kernel(const WaArgs a) {
   auto stage = [&](int t, int buf) {
     stage_pair<DP, 4>(img + (int64_t)(tiles.key(t) / kTile) * 2 * Tile::kBytes, kv[buf], wave, lane);
   };
-#pragma unroll
-  for (int t = 0; t < STAGES - 1; ++t)
-    if (!TILES && t < tiles.count) stage(t, t);
+  if (!TILES) stage(0, 0);
 
   LaneRow<DP, VEC> row = rows_of(a.q, wa_head(a.q, a, bh));
   u32x4 qp[DP / 16][2];
@@ -359,15 +351,14 @@ window_fwd_kernel(const WaArgs a) {
       if (!wa_sees(a, qi, kv0 + acc_row(r, h))) s[r] = -INFINITY;
   };
 
-  for (int t = 0, buf = -1, to = STAGES - 2; t < tiles.count; ++t) {
+  for (int t = 0, buf = 1; t < tiles.count; ++t) {
     const int kv0 = tiles.key(t);
     if (TILES) {
       buf = kv0 / kTile;
     } else {
-      buf = buf + 1 < STAGES ? buf + 1 : 0;
-      to = to + 1 < STAGES ? to + 1 : 0;
-      ring_next<STAGES - 2, kStageDmas<DP, 4>>(tiles.count - 1 - t);
-      if (t + STAGES - 1 < tiles.count) stage(t + STAGES - 1, to);
+      buf ^= 1;
+      ring_next();
+      if (t + 1 < tiles.count) stage(t + 1, buf ^ 1);
     }
     if (w0 >= a.T || !wa_any(a, w0, kv0)) continue;
     const uint32_t kt = top_of<DP>(kv[buf]), vt = top_of<DP>(kv[buf] + Tile::kBytes);
@@ -441,12 +432,12 @@ window_fwd_kernel(const WaArgs a) {
 }
 
 // dQ, and what dK's and dV's pass reads of a query row: the planes of Q and dO, D and lse.
-template <int DP, bool VEC, int STAGES, int TILES>
-__global__ void __launch_bounds__(wa_threads(TILES), (TILES || STAGES == 2) && DP == 64 ? 2 : 1)
+template <int DP, bool VEC, int TILES>
+__global__ void __launch_bounds__(wa_threads(TILES), DP == 64 ? 2 : 1)
 window_bwd_dq_kernel(const WaArgs a) {
   constexpr int NB = DP / 32;
   using Tile = HalfTile<DP>;
-  __shared__ __attribute__((aligned(16))) char kv[TILES ? TILES : STAGES][2 * Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) char kv[TILES ? TILES : 2][2 * Tile::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
   const int bh = blockIdx.x % a.BH, turn = blockIdx.x / a.BH, bhk = wa_kv(a, bh);
@@ -461,9 +452,7 @@ window_bwd_dq_kernel(const WaArgs a) {
   auto stage = [&](int t, int buf) {
     stage_pair<DP, 4>(img + (int64_t)(tiles.key(t) / kTile) * 2 * Tile::kBytes, kv[buf], wave, lane);
   };
-#pragma unroll
-  for (int t = 0; t < STAGES - 1; ++t)
-    if (!TILES && t < tiles.count) stage(t, t);
+  if (!TILES) stage(0, 0);
 
   const LaneRow<DP, VEC> q = rows_of(a.q, wa_head(a.q, a, bh)), dO = rows_of(a.dout, wa_head(a.dout, a, bh));
   const LaneRow<DP, VEC> O = rows_of(a.o_in, wa_head(a.o_in, a, bh));
@@ -507,15 +496,14 @@ window_bwd_dq_kernel(const WaArgs a) {
     for (int r = 0; r < 16; ++r)
       if (!wa_sees(a, qi, kv0 + acc_row(r, h))) x[r] = 0.f;
   };
-  for (int t = 0, buf = -1, to = STAGES - 2; t < tiles.count; ++t) {
+  for (int t = 0, buf = 1; t < tiles.count; ++t) {
     const int kv0 = tiles.key(t);
     if (TILES) {
       buf = kv0 / kTile;
     } else {
-      buf = buf + 1 < STAGES ? buf + 1 : 0;
-      to = to + 1 < STAGES ? to + 1 : 0;
-      ring_next<STAGES - 2, kStageDmas<DP, 4>>(tiles.count - 1 - t);
-      if (t + STAGES - 1 < tiles.count) stage(t + STAGES - 1, to);
+      buf ^= 1;
+      ring_next();
+      if (t + 1 < tiles.count) stage(t + 1, buf ^ 1);
     }
     if (w0 >= a.T || !wa_any(a, w0, kv0)) continue;
     const uint32_t kt = top_of<DP>(kv[buf]), vt = top_of<DP>(kv[buf] + Tile::kBytes);
@@ -602,13 +590,13 @@ struct WaList {
 };
 
 // dK and dV: a wave takes 32 keys, a lane its key, and walks its workgroup's list.
-template <int DP, bool VEC, int WAVES, int STAGES, int TILES>
-__global__ void __launch_bounds__(TILES ? wa_threads(TILES) : WAVES * kWave, (TILES || STAGES == 2) && DP == 64 ? 2 : 1)
+template <int DP, bool VEC, int WAVES, int TILES>
+__global__ void __launch_bounds__(TILES ? wa_threads(TILES) : WAVES * kWave, DP == 64 ? 2 : 1)
 window_bwd_dkdv_kernel(const WaArgs a) {
   constexpr int NB = DP / 32;
   using Tile = HalfTile<DP>;
-  __shared__ __attribute__((aligned(16))) char qd[TILES ? TILES : STAGES][2 * Tile::kBytes];
-  __shared__ __attribute__((aligned(16))) float stats[TILES ? TILES : STAGES][2 * kTile];  // lse in log2, D
+  __shared__ __attribute__((aligned(16))) char qd[TILES ? TILES : 2][2 * Tile::kBytes];
+  __shared__ __attribute__((aligned(16))) float stats[TILES ? TILES : 2][2 * kTile];  // lse in log2, D
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
   const int bhk = blockIdx.x % a.BHkv, item = blockIdx.x / a.BHkv;
@@ -637,10 +625,8 @@ window_bwd_dkdv_kernel(const WaArgs a) {
     dma4_untracked((lane < kTile ? a.l2 : a.D) + at * kTile + lr, (lds_void_t*)stats[buf]);
   };
   Place here = part.begin < part.end ? place_of(part.begin) : Place{head0, part.first}, ahead = here;
-#pragma unroll
-  for (int n = 0; n < STAGES - 1; ++n) {
-    if (TILES || part.begin + n >= part.end) break;
-    stage(ahead, n);
+  if (!TILES && part.begin < part.end) {
+    stage(ahead, 0);
     ahead = next_of(ahead);
   }
 
@@ -681,17 +667,16 @@ window_bwd_dkdv_kernel(const WaArgs a) {
     if (!mine) continue;
     here = Place{bh, part.first};
   }
-  for (int t = part.begin, cur = -1, to = STAGES - 2; t < (TILES ? part.count : part.end); ++t) {
+  for (int t = part.begin, cur = 1; t < (TILES ? part.count : part.end); ++t) {
     const int i0 = here.tile * kTile;
     here = next_of(here);
     if (TILES) {
       cur = i0 / kTile;
     } else {
-      cur = cur + 1 < STAGES ? cur + 1 : 0;
-      to = to + 1 < STAGES ? to + 1 : 0;
-      ring_next<STAGES - 2, kStageDmas<DP, WAVES> + 1>(part.end - 1 - t);
-      if (t + STAGES - 1 < part.end) {
-        stage(ahead, to);
+      cur ^= 1;
+      ring_next();
+      if (t + 1 < part.end) {
+        stage(ahead, cur ^ 1);
         ahead = next_of(ahead);
       }
     }
@@ -928,15 +913,15 @@ int launch_split(const WaArgs& a, hipStream_t st) {
 // The forms for texts that LDS holds, by their tiles.
 template <int DP, bool VEC, int TILES>
 int launch_whole_fwd(const WaArgs& a, hipStream_t st) {
-  window_fwd_kernel<DP, VEC, 2, TILES><<<dim3((unsigned)(a.BH * a.turns)), dim3(wa_threads(a.tiles)), 0, st>>>(a);
+  window_fwd_kernel<DP, VEC, TILES><<<dim3((unsigned)(a.BH * a.turns)), dim3(wa_threads(a.tiles)), 0, st>>>(a);
   return launch_status();
 }
 template <int DP, bool VEC, int TILES>
 int launch_whole_bwd(const WaArgs& a, hipStream_t st) {
-  window_bwd_dq_kernel<DP, VEC, 2, TILES><<<dim3((unsigned)(a.BH * a.turns)), dim3(wa_threads(a.tiles)), 0, st>>>(a);
+  window_bwd_dq_kernel<DP, VEC, TILES><<<dim3((unsigned)(a.BH * a.turns)), dim3(wa_threads(a.tiles)), 0, st>>>(a);
   const int rc = launch_status();
   if (rc != AAR_OK) return rc;
-  window_bwd_dkdv_kernel<DP, VEC, 4, 2, TILES><<<dim3((unsigned)(a.BHkv * a.turns)), dim3(wa_threads(a.tiles)), 0, st>>>(a);
+  window_bwd_dkdv_kernel<DP, VEC, 4, TILES><<<dim3((unsigned)(a.BHkv * a.turns)), dim3(wa_threads(a.tiles)), 0, st>>>(a);
   return launch_status();
 }
 
@@ -950,8 +935,7 @@ int launch_fwd(const WaArgs& a, hipStream_t st) {
   const int rc = launch_split<DP, VEC>(a, st);
   if (rc != AAR_OK) return rc;
   const dim3 grid((unsigned)(ceil_div(a.T, kBlock) * a.BH)), block(kFaThreads);
-  if ((int)grid.x <= device_cu_count()) window_fwd_kernel<DP, VEC, wa_deep(DP), 0><<<grid, block, 0, st>>>(a);
-  else window_fwd_kernel<DP, VEC, 2, 0><<<grid, block, 0, st>>>(a);
+  window_fwd_kernel<DP, VEC, 0><<<grid, block, 0, st>>>(a);
   return launch_status();
 }
 
@@ -966,16 +950,14 @@ int launch_bwd(const WaArgs& a, hipStream_t st) {
   if (rc != AAR_OK) return rc;
   const int64_t blocks = ceil_div(a.T, kBlock);
   const dim3 rows((unsigned)(blocks * a.BH)), keys((unsigned)(blocks * a.BHkv)), block(kFaThreads);
-  if ((int)rows.x <= device_cu_count()) window_bwd_dq_kernel<DP, VEC, wa_deep(DP), 0><<<rows, block, 0, st>>>(a);
-  else window_bwd_dq_kernel<DP, VEC, 2, 0><<<rows, block, 0, st>>>(a);
+  window_bwd_dq_kernel<DP, VEC, 0><<<rows, block, 0, st>>>(a);
   rc = launch_status();
   if (rc != AAR_OK) return rc;
-  if ((int)keys.x <= device_cu_count()) window_bwd_dkdv_kernel<DP, VEC, 4, wa_deep(DP), 0><<<keys, block, 0, st>>>(a);
-  else window_bwd_dkdv_kernel<DP, VEC, 4, 2, 0><<<keys, block, 0, st>>>(a);
+  window_bwd_dkdv_kernel<DP, VEC, 4, 0><<<keys, block, 0, st>>>(a);
   rc = launch_status();
   if (rc != AAR_OK || a.far_parts == 0) return rc;
   const int64_t far = (int64_t)a.BHkv * a.sink_tiles * a.far_parts;
-  window_bwd_dkdv_kernel<DP, VEC, 1, 2, 0><<<dim3((unsigned)far), dim3(kWave), 0, st>>>(a);
+  window_bwd_dkdv_kernel<DP, VEC, 1, 0><<<dim3((unsigned)far), dim3(kWave), 0, st>>>(a);
   rc = launch_status();
   if (rc != AAR_OK) return rc;
   window_bwd_sum_kernel<DP, VEC><<<dim3((unsigned)((int64_t)a.BHkv * a.S)), dim3(256), 0, st>>>(a);
