@@ -5,8 +5,8 @@
 // matrix ops (lo hi, hi lo, hi hi; 16 steps each at 16 times the fp32 instruction's
 // rate) stand for one fp32 product.  An operand is off by at most 2^-22 of itself or,
 // where that is more, 2^-38 of its row's largest element, lo lo is at most 2^-22 of a
-// product and is left out; sums are in fp32.  e is a row's own, such that its largest
-// element is in [2^13, 2^14).  Over the head dim a row's factor is one of the output's
+// product and is left out; sums are in fp32.  e is a row's own (where a kernel says so, that of
+// a tile of 32 rows), such that its largest element is in [2^13, 2^14).  Over the head dim a row's factor is one of the output's
 // row or column.  Over a tile's rows it goes to the other operand, P or dS, which is
 // scaled by the lane's own power of two that follows the largest |P| 2^-e (|dS| 2^-e)
 // so far (HalfScale).  Rows whose largest element is not 0 and outside [2^-99, 2^60) are

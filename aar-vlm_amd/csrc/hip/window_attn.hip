@@ -12,6 +12,12 @@
 // sinks' and the window's.  A block of 128 keys visits the queries up to W - 1 behind
 // its last key, of all heads that share it; the later ones that see its sinks are visited
 // for the sinks' tiles alone, in parts that are summed at the end.
+//
+// Bound by the matrix unit for long windows: 24 heads on 8, 16384 tokens, window 1024, d 64:
+// forward 360 us (at 858 TFLOP/s of fp16 products; a large library product reaches 1095),
+// dQ 576 (836), dK and dV 870 (800), where the chip's clock falls to 1.6-1.8 GHz.  Short
+// texts are bound by the bytes and by a wave's chain of tiles (a tile some 1 us forward, 2 for
+// dK and dV): 384 heads, 256 tokens, window 128: 37, 52 and 63 us for 100, 150 and 150 MB.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -272,8 +278,13 @@ __device__ __forceinline__ void stage_pair(const char* src, char* lds, int wave,
 // Texts of up to TILES tiles are kept in LDS whole: a workgroup takes a head, a wave splits
 // a tile of K and of V (of Q and of dO) straight into LDS, and then its own 32 rows need
 // no barrier, no planes in HBM and no other workgroup's.  TILES = 0: longer texts.
+// With gradients, 384 heads of d 64: 128 tokens 89 us from HBM's planes and 65 so, 256 tokens
+// 179 and 146; d 128, 64 tokens 102 and 80, 128 tokens 167 and 153 (forward 33 and 34).  The
+// other side are few key/value heads of many query heads each, which dK and dV take in turn
+// (16 of 6, 256 tokens: 167 and 180).
 // Where half the CUs would have no head, two workgroups take one: both have its tiles, the
-// first the rows of waves 0 to 3 and the second those of waves 4 to 7, so that a SIMD has one.
+// first the rows of waves 0 to 3 and the second those of waves 4 to 7, so that a SIMD has one
+// (6 heads, 200 tokens: 54.5 and 52.0 us; 96 heads, 256 tokens: 70.1 and 68.4).
 constexpr int wa_whole(int dp) { return dp == 64 ? 8 : 4; }
 constexpr int wa_threads(int tiles) { return tiles ? tiles * kWave : kFaThreads; }
 
@@ -843,7 +854,9 @@ WaArgs wa_args(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t d, int64_t 
 }
 
 // Parts of the sinks' far queries: where the block that holds the first sinks would have
-// a list more than twice as long as the others', for up to 64 tiles of sinks.
+// a list more than twice as long as the others', for up to 64 tiles of sinks (24 heads on 8,
+// 16384 tokens, window 1024, 4 sinks, with the forward: 4558 us in one list, 1581 so; 6 heads,
+// 2048 tokens, window 64: 193 and 94; 600 tokens, the shortest: 86 and 84).
 void wa_bwd_plan(WaArgs& a) {
   const int64_t near = std::min<int64_t>(a.T - 1, kBlock - 1 + (int64_t)a.W - 1) / kTile + 1, far = a.tiles - near;
   a.sink_tiles = (int)ceil_div(a.S, kTile);
