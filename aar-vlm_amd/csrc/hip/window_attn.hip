@@ -310,7 +310,9 @@ window_fwd_kernel(const WaArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
   const int bh = blockIdx.x % a.BH, turn = blockIdx.x / a.BH, bhk = wa_kv(a, bh);
-  const int q0 = TILES ? 0 : turn * kBlock, w0 = q0 + wave * kTile, qi = w0 + lr;  // this lane's row
+  // the text's end first: the first rows' lists are short, and fill the end of the grid (64
+  // heads on 16, 1777 tokens, d 128, causal: 206 us in the text's order, 186 so)
+  const int q0 = TILES ? 0 : (a.tiles - 1) / 4 * kBlock - turn * kBlock, w0 = q0 + wave * kTile, qi = w0 + lr;  // this lane's row
   const int wr = min(w0, a.T - 1);  // a row that is there
   auto rows_of = [&](const FaIn& x, const float* head) {
     return LaneRow<DP, VEC>(head + (int64_t)wr * x.st, x.st, w0, a.T, a.d, lr, h);
@@ -452,7 +454,8 @@ window_bwd_dq_kernel(const WaArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, h = lane >> 5;
   const int bh = blockIdx.x % a.BH, turn = blockIdx.x / a.BH, bhk = wa_kv(a, bh);
-  const int q0 = TILES ? 0 : turn * kBlock, w0 = q0 + wave * kTile, qi = w0 + lr;
+  // the text's end first, as forward
+  const int q0 = TILES ? 0 : (a.tiles - 1) / 4 * kBlock - turn * kBlock, w0 = q0 + wave * kTile, qi = w0 + lr;
   const bool row_ok = qi < a.T;
   const int wr = min(w0, a.T - 1);  // a row that is there
   auto rows_of = [&](const FaIn& x, const float* head) {
