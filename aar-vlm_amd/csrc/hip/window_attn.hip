@@ -57,6 +57,22 @@ __device__ __forceinline__ bool wa_any(const WaArgs& a, int i, int j) {
   return j <= i + kTile - 1 && (i - (j + kTile - 1) < a.W || j < a.S);
 }
 
+// What a lane sees of a tile as bits, an accumulator's row (its offset without the lane's
+// half) a bit: two instructions an element then hide what it does not see, where comparing
+// takes five and as many on masks of lanes.
+__device__ __forceinline__ uint32_t bits_below(int n) {
+  n = min(max(n, 0), 32);
+  return n == 32 ? 0xffffffffu : (1u << n) - 1;
+}
+__device__ __forceinline__ uint32_t keys_seen(const WaArgs& a, int i, int j0) {  // of keys from j0 on, by query i
+  return bits_below(i + 1 - j0) & (~bits_below(i - a.W + 1 - j0) | bits_below(a.S - j0));
+}
+__device__ __forceinline__ uint32_t queries_that_see(const WaArgs& a, int i0, int j) {  // from i0 on, key j
+  return ~bits_below(j - i0) & (j < a.S ? 0xffffffffu : bits_below(j + a.W - i0));
+}
+// All bits set where element r of an accumulator is seen.
+__device__ __forceinline__ uint32_t seen(uint32_t bits, int r) { return (uint32_t)((int)(bits << (31 - acc_row(r, 0))) >> 31); }
+
 // The key tiles of queries [q0, q1]: sinks' tiles, then the window's.
 struct WaTiles {
   int sinks, near, count;
@@ -359,9 +375,12 @@ window_fwd_kernel(const WaArgs a) {
   };
   auto hide = [&](f32x16& s, int kv0) {
     if (wa_all(a, w0, kv0)) return;
+    const uint32_t bits = keys_seen(a, qi, kv0 + 4 * h), none = __float_as_uint(-INFINITY);
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-      if (!wa_sees(a, qi, kv0 + acc_row(r, h))) s[r] = -INFINITY;
+    for (int r = 0; r < 16; ++r) {
+      const uint32_t m = seen(bits, r);
+      s[r] = __uint_as_float((__float_as_uint(s[r]) & m) | (none & ~m));
+    }
   };
 
   for (int t = 0, buf = 1; t < tiles.count; ++t) {
@@ -506,9 +525,9 @@ window_bwd_dq_kernel(const WaArgs a) {
 
   auto hide = [&](f32x16& x, int kv0) {
     if (wa_all(a, w0, kv0)) return;
+    const uint32_t bits = keys_seen(a, qi, kv0 + 4 * h);
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-      if (!wa_sees(a, qi, kv0 + acc_row(r, h))) x[r] = 0.f;
+    for (int r = 0; r < 16; ++r) x[r] = __uint_as_float(__float_as_uint(x[r]) & seen(bits, r));
   };
   for (int t = 0, buf = 1; t < tiles.count; ++t) {
     const int kv0 = tiles.key(t);
@@ -661,9 +680,9 @@ window_bwd_dkdv_kernel(const WaArgs a) {
   // P or dS of the queries from i0 on that do not see the lane's key
   auto hide = [&](f32x16& p, int i0) {
     if (wa_all(a, i0, kw)) return;
+    const uint32_t bits = queries_that_see(a, i0 + 4 * h, kj);
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-      if (!wa_sees(a, i0 + acc_row(r, h), kj)) p[r] = 0.f;
+    for (int r = 0; r < 16; ++r) p[r] = __uint_as_float(__float_as_uint(p[r]) & seen(bits, r));
   };
   const int heads = TILES ? a.G : 1;  // lists one after the other
   for (int g = 0; g < heads; ++g) {
