@@ -14,10 +14,10 @@
 // for the sinks' tiles alone, in parts that are summed at the end.
 //
 // Bound by the matrix unit for long windows: 24 heads on 8, 16384 tokens, window 1024, d 64:
-// forward 360 us (at 858 TFLOP/s of fp16 products; a large library product reaches 1095),
-// dQ 576 (836), dK and dV 870 (800), where the chip's clock falls to 1.6-1.8 GHz.  Short
+// forward 351 us (at 880 TFLOP/s of fp16 products; a large library product reaches 1095),
+// dQ 567 (850), dK and dV 829 (840), where the chip's clock falls to 1.6-1.8 GHz.  Short
 // texts are bound by the bytes and by a wave's chain of tiles (a tile some 1 us forward, 2 for
-// dK and dV): 384 heads, 256 tokens, window 128: 37, 52 and 63 us for 100, 150 and 150 MB.
+// dK and dV): 384 heads, 256 tokens, window 128: 36, 52 and 60 us for 100, 150 and 150 MB.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -691,9 +691,14 @@ window_bwd_dkdv_kernel(const WaArgs a) {
     u32x4 parts[DP / 16][2];
     const int bh = head0 + g;
     if (g > 0) __syncthreads();
-    const LaneRow<DP, VEC> q = rows_of(a.q, wa_head(a.q, a, bh)), dO = rows_of(a.dout, wa_head(a.dout, a, bh));
     const float stat = (h == 0 ? a.l2 : a.D)[((int64_t)bh * a.tiles + wave) * kTile + lr];
-    split_rows<DP, VEC>(q, lr, h, parts, qd[wave]);
+    const LaneRow<DP, VEC> q = rows_of(a.q, wa_head(a.q, a, bh));
+    if (!VEC) {  // single floats' places fill the registers: one operand's at a time
+      split_rows<DP, VEC>(q, lr, h, parts, qd[wave]);
+      sched_fence();
+    }
+    const LaneRow<DP, VEC> dO = rows_of(a.dout, wa_head(a.dout, a, bh));
+    if (VEC) split_rows<DP, VEC>(q, lr, h, parts, qd[wave]);
     split_rows<DP, VEC>(dO, lr, h, parts, qd[wave] + Tile::kBytes);
     stats[wave][lane] = stat;
     __syncthreads();
