@@ -487,7 +487,10 @@ window_bwd_dq_kernel(const WaArgs a) {
   };
   if (!TILES) stage(0, 0);
 
-  const LaneRow<DP, VEC> q = rows_of(a.q, wa_head(a.q, a, bh)), dO = rows_of(a.dout, wa_head(a.dout, a, bh));
+  const LaneRow<DP, VEC> q = rows_of(a.q, wa_head(a.q, a, bh));
+  if (!VEC) sched_fence();  // single floats' places fill the registers: one operand's at a time
+  const LaneRow<DP, VEC> dO = rows_of(a.dout, wa_head(a.dout, a, bh));
+  if (!VEC) sched_fence();
   const LaneRow<DP, VEC> O = rows_of(a.o_in, wa_head(a.o_in, a, bh));
   const float lse = a.lse[(int64_t)bh * a.T + min(qi, a.T - 1)];
   u32x4 qp[DP / 16][2], dop[DP / 16][2];
@@ -647,17 +650,21 @@ window_bwd_dkdv_kernel(const WaArgs a) {
   struct Place {
     int head, tile;
   };
-  auto place_of = [&](int t) { return Place{head0 + t / part.count, part.first + t % part.count}; };
+  // (the same in all lanes, which the compiler does not see through the loop)
+  auto place = [&](int head, int tile) {
+    return Place{__builtin_amdgcn_readfirstlane(head), __builtin_amdgcn_readfirstlane(tile)};
+  };
+  auto place_of = [&](int t) { return place(head0 + t / part.count, part.first + t % part.count); };
   auto next_of = [&](Place p) {
-    return p.tile + 1 < part.first + part.count ? Place{p.head, p.tile + 1} : Place{p.head + 1, part.first};
+    const bool same = p.tile + 1 < part.first + part.count;
+    return place(same ? p.head : p.head + 1, same ? p.tile + 1 : part.first);
   };
   auto stage = [&](Place p, int buf) {
-    // the same in all lanes, which the compiler does not see through the loop
-    const int64_t at = (int64_t)__builtin_amdgcn_readfirstlane(p.head) * a.tiles + __builtin_amdgcn_readfirstlane(p.tile);
+    const int64_t at = (int64_t)p.head * a.tiles + p.tile;
     stage_pair<DP, WAVES>(a.qd_img + at * 2 * Tile::kBytes, qd[buf], wave, lane);
     dma4_untracked((lane < kTile ? a.l2 : a.D) + at * kTile + lr, (lds_void_t*)stats[buf]);
   };
-  Place here = part.begin < part.end ? place_of(part.begin) : Place{head0, part.first}, ahead = here;
+  Place here = part.begin < part.end ? place_of(part.begin) : place(head0, part.first), ahead = here;
   if (!TILES && part.begin < part.end) {
     stage(ahead, 0);
     ahead = next_of(ahead);
@@ -703,7 +710,7 @@ window_bwd_dkdv_kernel(const WaArgs a) {
     stats[wave][lane] = stat;
     __syncthreads();
     if (!mine) continue;
-    here = Place{bh, part.first};
+    here = place(bh, part.first);
   }
   for (int t = part.begin, cur = 1; t < (TILES ? part.count : part.end); ++t) {
     const int i0 = here.tile * kTile;
